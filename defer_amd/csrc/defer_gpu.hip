@@ -24,6 +24,7 @@
 
 #include "../../include/defer_gpu.h"
 #include "phases.h"
+#include "q8.h"
 
 using namespace dg;
 
@@ -45,13 +46,24 @@ DG_DECLARE_SPECIALISED(dg8b)
 
 static thread_local std::string g_last_error;
 
-static int fail(int code, const char* fmt, ...) {
+static int fail_with(int code, const char* fmt, va_list ap) {
   char buf[512];
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  g_last_error = buf;
+  return code;
+}
+static int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
+  fail_with(code, fmt, ap);
   va_end(ap);
-  g_last_error = buf;
+  return code;
+}
+int defer_gpu_fail_(int code, const char* fmt, ...) {  // for q8.hip
+  va_list ap;
+  va_start(ap, fmt);
+  fail_with(code, fmt, ap);
+  va_end(ap);
   return code;
 }
 

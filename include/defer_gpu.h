@@ -243,6 +243,109 @@ int defer_gpu_model_set_grid(defer_gpu_model* m, uint32_t workgroups, uint32_t g
 int defer_gpu_model_set_profiling(defer_gpu_model* m, uint32_t on);
 int defer_gpu_batch_stats(const defer_gpu_model* m, double* stats, uint32_t reset);
 
+/* -------------------------------------------------------- 8-bit operators
+ *
+ * What a decoder layer needs to run on 8-bit weights, activations and cache
+ * (no counterpart in the reference, which computes in f32). All pointers are
+ * device memory of the current device; `stream` is a hipStream_t (NULL: the
+ * null stream). A call checks its arguments, queues its kernels there and
+ * returns without waiting; it allocates nothing, keeps nothing and may be
+ * captured into a graph. Calls on different streams or threads share nothing
+ * but what the caller hands to both.
+ *
+ * A row of n values y is held as n codes and one f32 scale: scale =
+ * max |y| / 127 rounded to f32, code = y / scale rounded to the nearest (ties
+ * to even), in [-127, 127]. Under a maximum of 2^-100 scale and codes are 0. A
+ * row with an infinity or a NaN gets a NaN scale, codes 0, and whatever is
+ * computed from it is NaN. Quotients are formed in 64 bits, so codes do not
+ * depend on an order of summation.
+ *
+ * A row's results never depend on the other rows of the call, nor on how many
+ * there are: the same bits for a prompt fed at once or token by token.
+ *
+ * Value types of x, y, k, v, q and out: */
+#define DEFER_GPU_F32 0
+#define DEFER_GPU_BF16 1
+#define DEFER_GPU_F16 2
+
+/* codes [rows, n], scale [rows] of x [rows, n], rows x_stride values apart. */
+int defer_gpu_q8_quantize(uint32_t type, const void* x, int64_t x_stride, uint32_t rows, uint32_t n,
+                          int8_t* codes, float* scale, void* stream);
+
+/* Root-mean-square norm with the residual's addition, in 8 bits: sum = x +
+ * residual, rounded to the type (both nullable: without residual the sum is
+ * x; it may be x or residual itself), and the codes of
+ * sum * weight / sqrt(mean(sum^2) + eps). weight [n] is of the same type. */
+int defer_gpu_q8_rms_norm(uint32_t type, const void* x, int64_t x_stride, const void* residual,
+                          int64_t residual_stride, const void* weight, float eps, uint32_t rows,
+                          uint32_t n, void* sum, int64_t sum_stride, int8_t* codes, float* scale,
+                          void* stream);
+
+/* y[r, m] = x_scale[r] * w_scale[m] * sum_k x[r, k] * w[m, k] over codes, the
+ * sum exact: a scale per token and one per channel. Strides in codes and
+ * values. k < 131072. Any sizes, strides and alignments; k, the strides and the
+ * addresses as multiples of 16 are faster. */
+int defer_gpu_q8_linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w,
+                        int64_t w_stride, const float* w_scale, uint32_t rows, uint32_t m, uint32_t k,
+                        uint32_t type, void* y, int64_t y_stride, void* stream);
+
+/* A cache in 8 bits: a pool of pages of 64 positions, a scale for each position
+ * and head. D is head_dim rounded up to a multiple of 64; what the rest of a
+ * row and unwritten positions hold does not matter. Values lie transposed in
+ * their page, so that both attention products read 16 consecutive bytes a lane.
+ * Positions 64 j .. 64 j + 63 of sequence i are in page
+ * table[i * table_width + j]; an entry outside [0, pages) is a page that the
+ * sequence does not have: its positions are not written, read as zeros and
+ * are not attended to. Addresses are multiples of 16. */
+typedef struct defer_gpu_q8_pages {
+  int8_t* keys;          /* [pages, heads, 64, D] */
+  int8_t* values;        /* [pages, heads, D, 64] */
+  float* key_scale;      /* [pages, heads, 64] */
+  float* value_scale;    /* [pages, heads, 64] */
+  const int32_t* table;  /* [sequences, table_width] */
+  uint32_t pages, heads, head_dim, table_width;
+} defer_gpu_q8_pages;
+
+/* The rows of a call: rows row_start[i] .. row_start[i + 1] - 1 are the last
+ * positions of sequence i, which has kv_len[i] with them (row_start NULL: one
+ * row each). No sequence has more than most_rows. Rows of no sequence are left
+ * as they were; a row before its sequence's position 0 is not written, reads
+ * as zeros and attends to nothing. The arrays are device memory and not
+ * checked by the host: spans are clamped to the call's rows. */
+typedef struct defer_gpu_q8_rows {
+  const int32_t* row_start; /* [sequences + 1] or NULL */
+  const int32_t* kv_len;    /* [sequences] */
+  uint32_t sequences, rows, most_rows;
+} defer_gpu_q8_rows;
+
+/* Quantises k and v [rows, heads, head_dim] (rows a stride apart) into the
+ * cache. No two sequences of a call write the same position of a page. */
+int defer_gpu_q8_kv_write(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
+                          const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* stream);
+/* The values the codes stand for, k and v [rows, heads, head_dim] (either may
+ * be NULL). Rows of no sequence are zeros here. */
+int defer_gpu_q8_kv_read(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
+                         void* k, void* v, void* stream);
+
+/* out[r, h] = sum_t p_t v_t, p = softmax of scale * q[r, h] . k_t over the
+ * positions t of the row's sequence up to its own, q and out
+ * [rows, q_heads, head_dim], head h reading cache head
+ * h / (q_heads / heads). hidden (nullable) [sequences, hidden_len], rows
+ * hidden_stride bytes apart: non-zero hides a position (those behind
+ * hidden_len are not hidden), whatever it holds. A row that sees nothing is
+ * zeros. No sequence is longer than most_len: positions behind it are not
+ * attended to. Scores and sums have f32's accuracy. `workspace` (16-byte aligned) is
+ * scratch of the size that defer_gpu_q8_attention_workspace gives (which may
+ * be 0); calls that may overlap, captured ones among them, each need their
+ * own. */
+size_t defer_gpu_q8_attention_workspace(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
+                                        uint32_t q_heads, uint32_t most_len);
+int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
+                           const void* q, int64_t q_stride, uint32_t q_heads, uint32_t most_len,
+                           float scale, const uint8_t* hidden, int64_t hidden_stride,
+                           uint32_t hidden_len, void* out, int64_t out_stride, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 /* Thread-local description of the last failing call. */
 const char* defer_gpu_last_error(void);
 
