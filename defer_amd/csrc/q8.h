@@ -56,6 +56,7 @@ struct Attention {
   const uint8_t* hidden;  // [sequences][hidden_len], rows hidden_stride apart
   int64_t hidden_stride;
   uint32_t hidden_len;
+  bool clear;  // zeros for the rows of no sequence
 };
 size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len);
 int attention(const Pages& p, const Rows& r, const Attention& a, void* workspace, size_t workspace_bytes,

@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace q8 {
 
@@ -154,63 +155,362 @@ struct LinearArgs {
   uint32_t rows, m, k, type;
 };
 
-// 16 codes from p[k0 ..], zeros from k on.
+// 16 codes from p[k0 ..], zeros from k on. Unaligned rows are read by unaligned
+// 16-byte loads, their last codes one by one: nothing behind a row is read.
 template <bool ALIGNED>
 __device__ __forceinline__ v4i load16(const int8_t* p, uint32_t k0, uint32_t k) {
   v4i v = {0, 0, 0, 0};
   if (ALIGNED) {
     if (k0 < k) v = *reinterpret_cast<const v4i*>(p + k0);
+  } else if (k0 + 16 <= k) {
+    __builtin_memcpy(&v, p + k0, 16);
   } else {
-    union {
-      int8_t b[16];
-      v4i v;
-    } u;
-    u.v = v;
-    for (uint32_t i = 0; i < 16; ++i)
-      if (k0 + i < k) u.b[i] = p[k0 + i];
-    v = u.v;
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      uint32_t x = 0;
+      for (uint32_t i = 0; i < 4; ++i)
+        if (k0 + 4 * w + i < k) x |= (uint32_t)(uint8_t)p[k0 + 4 * w + i] << (8 * i);
+      v[w] = (int)x;
+    }
   }
   return v;
 }
 
-// Few rows: a workgroup owns 16 channels and 16 NT rows, its waves share k
+// Few rows: a workgroup owns 16 MT channels and 16 NT rows, its waves share k
 // in steps of 128 codes; a lane's 32 bytes of a step go straight into two
 // matrix instructions. The waves' sums meet in LDS.
-template <int NT, bool ALIGNED>
-__global__ __launch_bounds__(256) void k_linear_few(LinearArgs a) {
-  constexpr int NW = 4;
+template <int MT, int NT, int NW, bool ALIGNED>
+__global__ __launch_bounds__(NW * WAVE) void k_linear_few(LinearArgs a) {
   const uint32_t lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, r16 = lane % 16, kg = lane / 16;
-  const uint32_t m0 = blockIdx.x * 16, n0 = blockIdx.y * 16 * NT;
-  const int8_t* w = a.w + (int64_t)min(m0 + r16, a.m - 1) * a.wst;
-  const int8_t* x[NT];
+  const uint32_t m0 = blockIdx.x * 16 * MT, n0 = blockIdx.y * 16 * NT;
+  const int8_t *w[MT], *x[NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) w[t] = a.w + (int64_t)min(m0 + 16 * t + r16, a.m - 1) * a.wst;
 #pragma unroll
   for (int t = 0; t < NT; ++t) x[t] = a.x + (int64_t)min(n0 + 16 * t + r16, a.rows - 1) * a.xst;
-  v4i acc[NT];
+  v4i acc[MT][NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = v4i{0, 0, 0, 0};
-  for (uint32_t k0 = wave * 128 + kg * 32; k0 - kg * 32 < a.k; k0 += NW * 128) {
-    const v4i w0 = load16<ALIGNED>(w, k0, a.k), w1 = load16<ALIGNED>(w, k0 + 16, a.k);
+  for (int u = 0; u < MT; ++u)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w0, load16<ALIGNED>(x[t], k0, a.k), acc[t], 0, 0, 0);
-      acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w1, load16<ALIGNED>(x[t], k0 + 16, a.k), acc[t], 0, 0, 0);
-    }
+    for (int t = 0; t < NT; ++t) acc[u][t] = v4i{0, 0, 0, 0};
+  for (uint32_t s0 = wave * 128; s0 < a.k; s0 += NW * 128) {
+    const uint32_t k0 = s0 + kg * 32;
+    v4i wv[MT][2], xv[NT][2];
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) wv[u][h] = load16<ALIGNED>(w[u], k0 + 16 * h, a.k);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) xv[t][h] = load16<ALIGNED>(x[t], k0 + 16 * h, a.k);
+#pragma unroll
+    for (int u = 0; u < MT; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          acc[u][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][h], xv[t][h], acc[u][t], 0, 0, 0);
   }
-  __shared__ v4i part[NW][NT][WAVE];
+  __shared__ v4i part[NW][MT * NT][WAVE];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) part[wave][t][lane] = acc[t];
+  for (int u = 0; u < MT; ++u)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) part[wave][u * NT + t][lane] = acc[u][t];
   __syncthreads();
-  for (int t = wave; t < NT; t += NW) {
-    v4i s = part[0][t][lane];
-    for (int u = 1; u < NW; ++u) s += part[u][t][lane];
-    const uint32_t row = n0 + 16 * t + r16;
+  for (int f = wave; f < MT * NT; f += NW) {
+    v4i s = part[0][f][lane];
+#pragma unroll
+    for (int u = 1; u < NW; ++u) s += part[u][f][lane];
+    const uint32_t row = n0 + 16 * (f % NT) + r16, c0 = m0 + 16 * (f / NT) + 4 * kg;
     if (row >= a.rows) continue;
     const float xs = a.xs[row];
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t c = m0 + 4 * kg + i;
-      if (c < a.m) store_value(a.y, (int64_t)row * a.yst + c, a.type, (float)s[i] * (xs * a.ws[c]));
+    for (int i = 0; i < 4; ++i)
+      if (c0 + i < a.m) store_value(a.y, (int64_t)row * a.yst + c0 + i, a.type, (float)s[i] * (xs * a.ws[c0 + i]));
+  }
+}
+
+// Many rows: a workgroup of 2 x 2 waves owns BR = 64 TM rows and BC = 64 TN
+// channels and takes both operands through LDS, 128 codes of k a stage: a
+// copy instruction moves 8 whole 128-byte lines. A row's eight 16-byte chunks
+// lie in LDS in an order that depends on the row, so that the same chunk of
+// 8, or of 16, rows in turn lies in different banks. A wave's 32 x 32 products
+// take 16 bytes a lane of each side per 32 codes.
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+template <int TM, int TN>
+struct Tile {
+  static constexpr int BR = 64 * TM, BC = 64 * TN, BK = 128;
+  static constexpr int CHUNKS = BK / 16, ROWS = 64 / CHUNKS;  // of a row, rows of a copy instruction
+  static constexpr int NI = (BR + BC) / (4 * ROWS);           // copies of each wave
+  uint32_t r0, c0, xn, wn;                                    // the tile's first row and channel, and how many of each
+  uint32_t lane, wave, wr, wc, l32, half;
+
+  __device__ __forceinline__ Tile() {
+    lane = threadIdx.x % WAVE;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    wr = wave / 2 * 32 * TM;
+    wc = wave % 2 * 32 * TN;
+    l32 = lane % 32;
+    half = lane / 32;
+  }
+  __device__ __forceinline__ void at(const LinearArgs& a, uint32_t nrt, uint32_t id) {
+    r0 = id % nrt * BR;
+    c0 = id / nrt * BC;
+    xn = min((uint32_t)BR, a.rows - r0);
+    wn = min((uint32_t)BC, a.m - c0);
+  }
+  // the lane's row (of rows, then channels) and chunk in this wave's copy i
+  __device__ __forceinline__ uint32_t copy_row(int i) const { return ROWS * (4 * i + wave) + lane / CHUNKS; }
+  __device__ __forceinline__ uint32_t copy_chunk() const { return lane % CHUNKS ^ order(copy_row(0)); }  // any i: the same
+  __device__ __forceinline__ uint32_t copy_to(int i) const { return ROWS * (4 * i + wave) * BK; }
+  static constexpr bool copies_x(int i) { return ROWS * 4 * i < BR; }
+  // the place of a row's chunk c is c ^ order(row)
+  __device__ __forceinline__ static uint32_t order(uint32_t row) { return (row % 8) ^ (row / 8 % 2); }
+  // operands of the stage's ks-th 32 codes; wr and wc are multiples of 32, so
+  // the order of chunks goes by l32
+  __device__ __forceinline__ void read(const int8_t* stage, int ks, v4i* xv, v4i* wv) const {
+    const uint32_t at = ((2 * ks + half) ^ order(l32)) * 16;
+    const int8_t *xl = stage + (wr + l32) * BK + at, *wl = stage + (BR + wc + l32) * BK + at;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xv[i] = *reinterpret_cast<const v4i*>(xl + 32 * i * BK);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) wv[j] = *reinterpret_cast<const v4i*>(wl + 32 * j * BK);
+  }
+  // ... multiplied, with between(n) after the n-th product
+  template <class F>
+  __device__ __forceinline__ static void multiply(const v4i* xv, const v4i* wv, v16i (*acc)[TN], F between) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xv[i], wv[j], acc[i][j], 0, 0, 0);
+        between(i * TN + j);
+      }
+  }
+  // Register e of a product: row 8 (e / 4) + 4 half + e % 4, channel l32. Two
+  // neighbouring lanes exchange a register each, so that one stores row e's two
+  // channels and the other row e + 1's: half the stores, of twice the bytes.
+  template <class T>
+  __device__ __forceinline__ void store_as(const LinearArgs& a, const v16i (*acc)[TN], const float* xsl, const float* ws) const {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    T* y = static_cast<T*>(a.y);
+    const bool odd = lane & 1, pairs = (a.yst % 2 | (uintptr_t)a.y % sizeof(T2)) == 0;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const uint32_t r = wr + 32 * i + 4 * half + 8 * e4;
+        const v4f xs = *reinterpret_cast<const v4f*>(xsl + r);
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const uint32_t row = r0 + r + e, mine = row + odd;
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const uint32_t c = c0 + wc + 32 * j + l32;
+            const float v0 = (float)acc[i][j][4 * e4 + e] * (xs[e] * ws[j]);
+            const float v1 = (float)acc[i][j][4 * e4 + e + 1] * (xs[e + 1] * ws[j]);
+            const float got = dpp<0xb1>(odd ? v0 : v1);  // quad_perm 1 0 3 2
+            const uint32_t c2 = c - odd;
+            if (pairs && mine < a.rows && c2 + 1 < a.m) {
+              const T2 v = {(T)(odd ? got : v0), (T)(odd ? v1 : got)};
+              *reinterpret_cast<T2*>(y + (int64_t)mine * a.yst + c2) = v;
+            } else if (c < a.m && !(pairs && c2 + 1 < a.m)) {
+              if (row < a.rows) y[(int64_t)row * a.yst + c] = (T)v0;
+              if (row + 1 < a.rows) y[(int64_t)(row + 1) * a.yst + c] = (T)v1;
+            }
+          }
+        }
+      }
     }
   }
+  __device__ __forceinline__ void store(const LinearArgs& a, const v16i (*acc)[TN], const float* xsl, const float* ws) const {
+    if (a.type == DEFER_GPU_F32)
+      store_as<float>(a, acc, xsl, ws);
+    else if (a.type == DEFER_GPU_BF16)
+      store_as<__bf16>(a, acc, xsl, ws);
+    else
+      store_as<_Float16>(a, acc, xsl, ws);
+  }
+  // The tile's scales: this lane's channels', and a row's for each thread to
+  // leave in LDS (before a barrier).
+  __device__ __forceinline__ float scales(const LinearArgs& a, float* ws) const {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) ws[j] = a.ws[min(c0 + wc + 32 * j + l32, a.m - 1)];
+    return a.xs[min(r0 + threadIdx.x, a.rows - 1)];
+  }
+  static_assert(BR <= 256, "a row for each thread");
+};
+
+// The tile of a workgroup: an XCD (workgroups w % 8) takes a run of tiles, the
+// rows of one stripe of channels, then the next stripe.
+__device__ __forceinline__ bool tile_of_workgroup(uint32_t tiles, uint32_t* id) {
+  const uint32_t per = (tiles + 7) / 8;
+  *id = blockIdx.x % 8 * per + blockIdx.x / 8;
+  return blockIdx.x / 8 < per && *id < tiles;
+}
+
+// Aligned rows. Copies go memory -> LDS with no registers between (buffer
+// loads, which write zeros for what is outside the operand or behind k), two
+// stages ahead or more. They are issued one at a time between the products:
+// in a row they keep a wave from its next product for as long as the memory
+// pipeline takes them (2047 x 28672 x 4096: 320 us so, 269 now: 1,790 Tops/s; the
+// matrix cores alone reach 4,100, the library's i8 product of the same sizes
+// 236 us). Wider tiles (256 x 256: 310 us, half the LDS reads but one
+// stage of 64 codes less in flight), and one workgroup per CU that goes on to its
+// next tile's copies while it stores (312), were slower. A stage's last reads are waited for before the barrier in
+// it; behind that the next stage's first operands are read while its last
+// products run.
+template <int TM, int TN, int NBUF>
+__global__ __launch_bounds__(256) void k_linear_tile(LinearArgs a, uint32_t nrt, uint32_t tiles) {
+  typedef Tile<TM, TN> T;
+  constexpr int NI = T::NI, BK = T::BK, STAGE = (T::BR + T::BC) * BK, KS = BK / 32;
+  // one object: beside a second one the compiler waits for every copy before
+  // each read of LDS
+  __shared__ __align__(16) int8_t lds[NBUF * STAGE + 4 * T::BR];
+  float* xsl = reinterpret_cast<float*>(lds + NBUF * STAGE);
+  T t;
+  uint32_t id;
+  if (!tile_of_workgroup(tiles, &id)) return;
+  t.at(a, nrt, id);
+  float ws[TN];
+  const float xs = t.scales(a, ws);
+  auto* xb = const_cast<int8_t*>(a.x + (int64_t)t.r0 * a.xst);
+  auto* wb = const_cast<int8_t*>(a.w + (int64_t)t.c0 * a.wst);
+  auto xrs = __builtin_amdgcn_make_buffer_rsrc(xb, 0, (int)((t.xn - 1) * a.xst + a.k), 0x00020000);
+  auto wrs = __builtin_amdgcn_make_buffer_rsrc(wb, 0, (int)((t.wn - 1) * a.wst + a.k), 0x00020000);
+  constexpr uint32_t OUTSIDE = 0x80000000u;
+  uint32_t off[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const bool is_x = T::copies_x(i);
+    const uint32_t r = t.copy_row(i) - (is_x ? 0 : T::BR);
+    off[i] = r < (is_x ? t.xn : t.wn) ? (uint32_t)(r * (is_x ? a.xst : a.wst)) + t.copy_chunk() * 16 : OUTSIDE;
+  }
+  auto copy = [&](uint32_t k0, int buf, int i) {
+    const bool in = k0 + t.copy_chunk() * 16 < a.k;
+    auto* to = (__attribute__((address_space(3))) void*)(lds + buf * STAGE + t.copy_to(i));
+    const int from = (int)(in ? off[i] : OUTSIDE);
+    if (T::copies_x(i))
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xrs, to, 16, from, (int)k0, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wrs, to, 16, from, (int)k0, 0, 0);
+  };
+  v16i acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = v16i{};
+  v4i xv[2][TM], wv[2][TN];
+#pragma unroll
+  for (int b = 0; b < NBUF - 1; ++b)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) copy(b * BK, b, i);
+  if (threadIdx.x < T::BR) xsl[threadIdx.x] = xs;
+  // Every wave's copies of the oldest stage have arrived (the younger ones may
+  // be on their way), and what it has read so far is in its registers.
+#define Q8_STAGE_WAIT(YOUNGER)                                                                         \
+  do {                                                                                                 \
+    constexpr int n_ = (YOUNGER)*NI;                                                                   \
+    static_assert(n_ < 64, "vmcnt");                                                                   \
+    asm volatile("" ::: "memory");                                                                     \
+    __builtin_amdgcn_s_waitcnt((n_ & 15) | (n_ >> 4) << 14 | 0x0070); /* vmcnt(n_) lgkmcnt(0) */ \
+    __builtin_amdgcn_s_barrier();                                                                      \
+    asm volatile("" ::: "memory");                                                                     \
+    __builtin_amdgcn_sched_barrier(0);                                                                 \
+  } while (0)
+  Q8_STAGE_WAIT(NBUF - 2);
+  t.read(lds, 0, xv[0], wv[0]);
+  int buf = 0, free_buf = NBUF - 1;
+  for (uint32_t k0 = 0; k0 < a.k; k0 += BK) {
+    const int next = buf + 1 == NBUF ? 0 : buf + 1;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks < KS - 1) {
+        t.read(lds + buf * STAGE, ks + 1, xv[(ks + 1) % 2], wv[(ks + 1) % 2]);
+      } else {
+        Q8_STAGE_WAIT(NBUF - 2);
+        t.read(lds + next * STAGE, 0, xv[0], wv[0]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // this wave's copies of the stage NBUF - 1 on, evenly among the products
+      // before the barrier
+      constexpr int PRODUCTS = (KS - 1) * TM * TN;
+      T::multiply(xv[ks % 2], wv[ks % 2], acc, [&](int n) {
+        const int done = ks * TM * TN + n;
+        if (ks < KS - 1) {
+#pragma unroll
+          for (int i = done * NI / PRODUCTS; i < (done + 1) * NI / PRODUCTS; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            copy(k0 + (NBUF - 1) * BK, free_buf, i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    free_buf = buf;
+    buf = next;
+  }
+#undef Q8_STAGE_WAIT
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing may still be on its way into LDS at the end
+  t.store(a, acc, xsl, ws);
+}
+
+// Unaligned rows go through registers: the next stage is on its way there while
+// one is multiplied.
+template <int TM, int TN>
+__global__ __launch_bounds__(256) void k_linear_tile_odd(LinearArgs a, uint32_t nrt, uint32_t tiles) {
+  typedef Tile<TM, TN> T;
+  constexpr int NI = T::NI, STAGE = (T::BR + T::BC) * T::BK;
+  __shared__ __align__(16) int8_t lds[2 * STAGE];
+  __shared__ __align__(16) float xsl[T::BR];
+  T t;
+  uint32_t id;
+  if (!tile_of_workgroup(tiles, &id)) return;
+  t.at(a, nrt, id);
+  float ws[TN];
+  const float xs = t.scales(a, ws);
+  const int8_t* p[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const bool is_x = T::copies_x(i);
+    const uint32_t r = t.copy_row(i) - (is_x ? 0 : T::BR);
+    p[i] = is_x ? a.x + (int64_t)(t.r0 + min(r, t.xn - 1)) * a.xst : a.w + (int64_t)(t.c0 + min(r, t.wn - 1)) * a.wst;
+  }
+  v4i reg[NI];
+  auto fetch = [&](uint32_t k0) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) reg[i] = load16<false>(p[i], k0 + t.copy_chunk() * 16, a.k);
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      *reinterpret_cast<v4i*>(lds + buf * STAGE + t.copy_to(i) + t.lane * 16) = reg[i];
+  };
+  v16i acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = v16i{};
+  v4i xv[2][TM], wv[2][TN];
+  fetch(0);
+  put(0);
+  if (threadIdx.x < T::BR) xsl[threadIdx.x] = xs;
+  __syncthreads();
+  int buf = 0;
+  for (uint32_t k0 = 0; k0 < a.k; k0 += T::BK, buf ^= 1) {
+    const bool more = k0 + T::BK < a.k;
+    if (more) fetch(k0 + T::BK);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      t.read(lds + buf * STAGE, ks, xv[ks % 2], wv[ks % 2]);
+      T::multiply(xv[ks % 2], wv[ks % 2], acc, [](int) {});
+    }
+    if (more) put(buf ^ 1);
+    __syncthreads();
+  }
+  t.store(a, acc, xsl, ws);
 }
 
 // ------------------------------------------------------------- the cache
@@ -362,6 +662,8 @@ struct AttnArgs {
   void* out;
   int64_t qs, os;
   uint32_t type, nh, group, hd, tiles, units;
+  bool q_vec;  // a head's 16 values are 16-byte loads
+  bool clear;  // zeros for the rows of no sequence
   int64_t most_len;
   float scale2;  // scale * log2(e)
   const uint8_t* hidden;
@@ -379,15 +681,22 @@ __device__ __forceinline__ float undigit(v4i d) {
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
   return __builtin_amdgcn_perm(hi, lo, sel);
 }
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A running softmax: maximum (in the exponent of 2), sum, accumulators.
-// (M, L, A) joined with (m, l, acc) that follows it.
-__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.0f : m; }
+// A running softmax: maximum (as an exponent of 2), sum, accumulators. The
+// next part (m, l, acc) joins it with the weights x and y.
+__device__ __forceinline__ void join_weights(float& M, float m, float* x, float* y) {
+  const float mn = fmaxf(M, m), m0 = mn == -INFINITY ? 0.0f : mn;
+  *x = exp2_of(M - m0);
+  *y = exp2_of(m - m0);
+  M = mn;
+}
 
+enum AttnMode { DIRECT, SPLIT, GROUP };
 constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: rows of four heads on other banks
 
-// The attention of one wave: R tiles of four (row, head) pairs of one sequence
-// and cache head, over blocks of 64 positions.
+// What a wave does: the attention of R tiles of four (row, query head) pairs
+// of one sequence and cache head, over blocks of 64 positions.
 //
 // Scores: the four digits of a pair's query (31 bits, relative to the power of
 // two over its largest value: an exact scaling) are four rows of a 16-row
@@ -403,20 +712,41 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // scales are held in 30 bits relative to the largest such product: so one token
 // that takes nearly all of a softmax and has small values leaves the others'
 // contributions their accuracy.
-template <int KC, int R, bool SPLIT>
-__global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
+//
+// The next block's keys are on their way once this one's scores are formed, the
+// next values once this one's are used, or with the keys where registers
+// allow (R = 1: few rows, bound by memory).
+//
+// DIRECT: a wave goes through all its positions, unit after unit (many rows;
+// the four waves of a workgroup are neighbouring tiles and meet the same codes
+// in L1). SPLIT: a unit for each wave, left in the workspace for
+// k_attn_join. GROUP: the units of a tile are the waves of one workgroup, which
+// joins them through LDS.
+template <int KC, int R, AttnMode MODE>
+__global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R <= (KC < 3 ? 2 : 0) ? 2 : 1) void k_attn(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
-  __shared__ __align__(16) uint8_t lds[4][16 * P_ROW];
-  const uint32_t lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, n16 = lane % 16, quad = lane / 16;
-  uint8_t* pl = lds[wave];
+  constexpr bool AHEAD = R == 1 && KC <= 2;  // the next values wait in registers of their own
+  extern __shared__ __align__(16) uint8_t lds[];  // [waves][R][16][P_ROW], GROUP: then [4 R][units][2 + DP] floats
+  const uint32_t lane = threadIdx.x % WAVE, n16 = lane % 16, quad = lane / 16;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
+  uint8_t* pl = lds + wave * R * 16 * P_ROW;
 
-  // which wave does what: (tile or unit) slowest, (sequence, cache head) fastest
+  // which wave does what: (tile, unit) slowest, (sequence, cache head) fastest
   const uint32_t shs = a.r.sequences * a.p.heads;
-  const uint32_t sh = blockIdx.x % shs, item = blockIdx.x / shs * 4 + wave;
+  const uint32_t sh = blockIdx.x % shs, item = MODE == GROUP ? blockIdx.x / shs : blockIdx.x / shs * 4 + wave;
   const uint32_t seq = sh / a.p.heads, g = sh % a.p.heads;
-  const uint32_t tile = SPLIT ? item / a.units : a.tiles - 1 - min(item, a.tiles - 1);
-  const uint32_t unit = SPLIT ? item % a.units : 0;
-  if (SPLIT ? tile >= a.tiles : item >= a.tiles) return;
+  const uint32_t tile = MODE == SPLIT ? item / a.units : MODE == DIRECT ? a.tiles - 1 - min(item, a.tiles - 1) : item;
+  if (a.clear && blockIdx.x == 0) {
+    // rows of no sequence lie before the first span and behind the last
+    const Span none = span_of(a.r.row_start, a.r.kv_len, 0, a.r.rows);
+    const int64_t hi = max((int64_t)none.start, min((int64_t)a.r.row_start[a.r.sequences], (int64_t)a.r.rows));
+    for (int64_t row = wave; row < (int64_t)a.r.rows; row += waves) {
+      if (row == none.start) row += (hi - row + waves - 1) / waves * waves;
+      if (row < none.start || (row >= hi && row < (int64_t)a.r.rows))
+        for (uint32_t d = lane; d < a.nh * a.hd; d += WAVE) store_value(a.out, row * a.os + d, a.type, 0.0f);
+    }
+  }
+  if (MODE == SPLIT ? tile >= a.tiles : item >= a.tiles) return;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
   const uint32_t pair0 = tile * 4 * R;
   if (sp.n <= 0 || pair0 >= (uint32_t)sp.n * a.group) return;
@@ -426,7 +756,7 @@ __global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
   const uint8_t* hid = a.hidden ? a.hidden + (int64_t)seq * a.hs : nullptr;
 
   // pairs: (row j of the sequence, query head of the group)
-  int pos[R], max_pos = -1;
+  int pos[R], max_pos = -1, min_pos = 0x7fffffff;
   uint32_t orow[R], ohead[R];
   bool have[R];
 #pragma unroll
@@ -438,11 +768,34 @@ __global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
     orow[r] = sp.start + j;
     ohead[r] = g * a.group + pr % a.group;
     max_pos = max(max_pos, pos[r]);
+    min_pos = min(min_pos, pos[r] < 0 ? 0x7fffffff : pos[r]);
   }
   max_pos = max(max_pos, __shfl_xor(max_pos, 16));
-  max_pos = max(max_pos, __shfl_xor(max_pos, 32));
+  max_pos = __builtin_amdgcn_readfirstlane(max(max_pos, __shfl_xor(max_pos, 32)));
+  min_pos = min(min_pos, __shfl_xor(min_pos, 16));
+  min_pos = __builtin_amdgcn_readfirstlane(min(min_pos, __shfl_xor(min_pos, 32)));
 
-  // the queries' digits
+  v4i k[4][KC], v[DT], vn[AHEAD ? DT : 1];
+  v4f ks, vs, ksn, vsn;
+  const int8_t* k0 = q.keys + (size_t)g * PAGE * DP + 4 * n16 * DP + quad * 16;
+  const int8_t* v0 = q.values + (size_t)g * PAGE * DP + n16 * PAGE + quad * 16;
+  auto load_k = [&](int page) {
+    const int8_t* kb = k0 + (size_t)page * a.p.heads * PAGE * DP;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int kk = 0; kk < KC; ++kk) k[j][kk] = *reinterpret_cast<const v4i*>(kb + j * DP + kk * 64);
+    const size_t hp = ((size_t)page * a.p.heads + g) * PAGE + 4 * n16;
+    ksn = *reinterpret_cast<const v4f*>(q.key_scale + hp);
+    vsn = *reinterpret_cast<const v4f*>(q.value_scale + hp);
+  };
+  auto load_v = [&](int page, v4i* to) {
+    const int8_t* vb = v0 + (size_t)page * a.p.heads * PAGE * DP;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) to[t] = *reinterpret_cast<const v4i*>(vb + 16 * t * PAGE);
+  };
+
+  // the queries' digits; the scores' sign is the scale's, folded into them
   v4i aq[R][KC];
   float sq[R];
 #pragma unroll
@@ -452,14 +805,36 @@ __global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
     const int64_t q0 = (int64_t)(sp.start + (ok ? j : 0)) * a.qs + (int64_t)(g * a.group + pr % a.group) * a.hd;
     float x[KC][16], top = 0.0f, bad = 0.0f;
 #pragma unroll
-    for (int kk = 0; kk < KC; ++kk)
+    for (int kk = 0; kk < KC; ++kk) {
+      const uint32_t d0 = kk * 64 + quad * 16;
+      if (a.q_vec) {
+        const int64_t at = q0 + (d0 < a.hd ? d0 : 0);
+        if (a.type == DEFER_GPU_F32) {
+          const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(a.q) + at);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[kk][e] = p[e / 4][e % 4];
+        } else {
+          typedef uint16_t v8h __attribute__((ext_vector_type(8)));
+          const v8h* p = reinterpret_cast<const v8h*>(static_cast<const uint16_t*>(a.q) + at);
+          const bool bf = a.type == DEFER_GPU_BF16;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint16_t h = p[e / 8][e % 8];
+            x[kk][e] = bf ? __builtin_bit_cast(float, (uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[kk][e] = ok && d0 < a.hd ? x[kk][e] : 0.0f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[kk][e] = ok && d0 + e < a.hd ? load_value(a.q, q0 + d0 + e, a.type) : 0.0f;
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const uint32_t d = kk * 64 + quad * 16 + e;
-        x[kk][e] = ok && d < a.hd ? load_value(a.q, q0 + d, a.type) : 0.0f;
         top = fmaxf(top, fabsf(x[kk][e]));
         bad = fmaf(x[kk][e], 0.0f, bad);
       }
+    }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     bad += __shfl_xor(bad, 16);
@@ -468,35 +843,28 @@ __global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
     int ex = 0;
     (void)frexpf(top, &ex);
     ex = top > 0.0f ? max(ex, -96) : 0;
-    const float up = ldexpf(1.0f, 30 - ex);
-    const float s = isnan(bad) ? __builtin_nanf("") : ldexpf(1.0f, ex - 30) * a.scale2;
+    const float up = isnan(bad) ? 0.0f : a.scale2 < 0.0f ? -ldexpf(1.0f, 30 - ex) : ldexpf(1.0f, 30 - ex);
+    const float s = isnan(bad) ? __builtin_nanf("") : ldexpf(1.0f, ex - 30) * fabsf(a.scale2);
+    const uint32_t dg = n16 % 4, sel = dg | (4 + dg) << 8;
 #pragma unroll
     for (int kk = 0; kk < KC; ++kk)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        uint32_t v = 0;
+        uint32_t y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int xi = isnan(bad) ? 0 : (int)(x[kk][4 * w + e] * up);
-          v |= ((digits(xi) >> (8 * (n16 % 4))) & 0xffu) << (8 * e);
-        }
-        aq[r][kk][w] = (int)v;
+        for (int e = 0; e < 4; ++e) y[e] = digits((int)__builtin_amdgcn_fmed3f(x[kk][4 * w + e] * up, -0x1p30f, 0x1p30f));
+        aq[r][kk][w] = (int)perm(perm(y[3], y[2], sel), perm(y[1], y[0], sel), 0x05040100u);
       }
     sq[r] = __shfl(s, (int)quad * 4);
   }
 
-  // Rows whose units have another length (sequences over 8,192 positions, where a
-  // tile spans a multiple of that) go one length after the other.
+  // Units from u0 on, every `du`-th, of the rows whose units are `ul` long:
+  // rows of a tile that spans a multiple of 8,192 positions go one length
+  // after the other.
   const int ul_last = unit_len(max(max_pos, 0));
-  int lo = 0x7fffffff;
-#pragma unroll
-  for (int r = 0; r < R; ++r) lo = min(lo, pos[r] < 0 ? 0x7fffffff : pos[r]);
-  lo = min(lo, __shfl_xor(lo, 16));
-  lo = min(lo, __shfl_xor(lo, 32));
-  const int ul_first = lo == 0x7fffffff ? ul_last : unit_len(lo);
+  const int ul_first = max_pos < 0 ? ul_last : unit_len(min_pos);
   for (int ul = ul_first; ul <= ul_last; ul += UNIT) {
-    int ps[R];
-    int pmax = -1, pmin = 0x7fffffff;
+    int ps[R], pmax = -1, pmin = 0x7fffffff;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       ps[r] = pos[r] >= 0 && unit_len(pos[r]) == ul ? pos[r] : -1;
@@ -504,11 +872,9 @@ __global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
       pmin = min(pmin, ps[r]);
     }
     pmax = max(pmax, __shfl_xor(pmax, 16));
-    pmax = max(pmax, __shfl_xor(pmax, 32));
+    pmax = __builtin_amdgcn_readfirstlane(max(pmax, __shfl_xor(pmax, 32)));
     pmin = min(pmin, __shfl_xor(pmin, 16));
-    pmin = min(pmin, __shfl_xor(pmin, 32));
-    pmax = __builtin_amdgcn_readfirstlane(pmax);
-    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    pmin = __builtin_amdgcn_readfirstlane(min(pmin, __shfl_xor(pmin, 32)));
 
     float M[R], L[R], A[R][DT], m[R], l[R], acc[R][DT];
 #pragma unroll
@@ -518,123 +884,164 @@ __global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
 #pragma unroll
       for (int t = 0; t < DT; ++t) A[r][t] = acc[r][t] = 0.0f;
     }
-    const int bpu = ul / PAGE;
-    const int b0 = SPLIT ? (int)unit * bpu : 0;
-    const int b1 = min(pmax < 0 ? 0 : pmax / PAGE + 1, SPLIT ? b0 + bpu : 0x7fffffff);
-    for (int b = b0; b < b1; ++b) {
-      const int page = page_of(table, width, q.pages, b);
-      if (page >= 0) {
-        const size_t hp = (size_t)page * a.p.heads + g;
-        const int8_t* kb = q.keys + hp * PAGE * DP;
-        const int8_t* vb = q.values + hp * PAGE * DP;
-        v4i k[4][KC], v[DT];
+
+    // A block whose codes have been loaded: WHOLE if every row sees all of it.
+    // next: the page to load meanwhile, or -1.
+    auto block = [&](auto whole, int b, int next) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      ks = ksn;
+      vs = vsn;
+      const int tb = b * PAGE + 4 * n16;  // this lane's first position
+      bool hide[4] = {false, false, false, false};
+      if (!WHOLE && hid) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) hide[j] = (uint32_t)(tb + j) < a.hidden_len && hid[tb + j] != 0;
+      }
+      // a NaN value scale of a visible position reaches the sum, and with it
+      // every output (adding the zeros of the others changes nothing)
+      float vbad = 0.0f;
+      if (WHOLE) vbad = fmaf(vs[0], 0.0f, vs[1] * 0.0f) + fmaf(vs[2], 0.0f, vs[3] * 0.0f);
+      float lp[R], mb[R], down[R];
 #pragma unroll
-          for (int kk = 0; kk < KC; ++kk)
-            k[j][kk] = *reinterpret_cast<const v4i*>(kb + (4 * n16 + j) * DP + kk * 64 + quad * 16);
-        const v4f ks = *reinterpret_cast<const v4f*>(q.key_scale + hp * PAGE + 4 * n16);
-        const v4f vs = *reinterpret_cast<const v4f*>(q.value_scale + hp * PAGE + 4 * n16);
+      for (int r = 0; r < R; ++r) {
+        v4i d[4];
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-          v[t] = *reinterpret_cast<const v4i*>(vb + (16 * t + n16) * PAGE + quad * 16);
-        const int tb = b * PAGE + 4 * n16;  // this lane's first position
-        bool hide[4] = {false, false, false, false};
-        if (hid) {
+        for (int j = 0; j < 4; ++j) {
+          d[j] = v4i{0, 0, 0, 0};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) hide[j] = (uint32_t)(tb + j) < a.hidden_len && hid[tb + j] != 0;
+          for (int kk = 0; kk < KC; ++kk) d[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[r][kk], k[j][kk], d[j], 0, 0, 0);
         }
-        // every row sees the whole block
-        const bool whole = !hid && b * PAGE + PAGE - 1 <= pmin;
+        if (r == R - 1 && next >= 0) {
+          load_k(next);
+          if (AHEAD) load_v(next, vn);
+        }
+        float s[4], w[4];
+        bool see[4];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float s[4];
-          bool see[4];
+        for (int j = 0; j < 4; ++j) {
+          see[j] = WHOLE || (tb + j <= ps[r] && !hide[j]);
+          const float x = undigit(d[j]) * ks[j];
+          s[j] = see[j] ? x : -INFINITY;
+        }
+        const float top = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+        const bool none = !WHOLE && top == -INFINITY;
+        const float m0 = none ? 0.0f : top * sq[r];
+        mb[r] = none ? -INFINITY : m0;
+        lp[r] = vbad;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v4i d = {0, 0, 0, 0};
-#pragma unroll
-            for (int kk = 0; kk < KC; ++kk)
-              d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[r][kk], k[j][kk], d, 0, 0, 0);
-            see[j] = whole || (tb + j <= ps[r] && !hide[j]);
-            s[j] = see[j] ? undigit(d) * (sq[r] * ks[j]) : -INFINITY;
-          }
-          const float mb = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-          const float mb0 = finite_or_0(mb);
-          float lp = 0.0f, w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = see[j] ? __builtin_amdgcn_exp2f(s[j] - mb0) : 0.0f;
-            // a NaN value scale reaches the sum, and with it every output
-            lp += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
+        for (int j = 0; j < 4; ++j) {
+          float p = exp2_of(fmaf(s[j], sq[r], -m0));
+          if (!WHOLE) {
+            p = see[j] ? p : 0.0f;
+            lp[r] += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
             w[j] = see[j] ? p * vs[j] : 0.0f;
+          } else {
+            lp[r] += p;
+            w[j] = p * vs[j];
           }
-          int ex = 0;
-          (void)frexpf(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))), &ex);
-          const float down = ldexpf(1.0f, ex - 30);
-          uint32_t y[4];
+        }
+        int ex = 0;
+        (void)frexpf(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))), &ex);
+        ex = max(ex, -96);
+        const float up = ldexpf(1.0f, 30 - ex);
+        down[r] = ldexpf(1.0f, ex - 30);
+        uint32_t y[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = digits((int)fminf(fmaxf(ldexpf(w[j], 30 - ex), 0.0f), 0x1p30f));
-          const uint32_t t01l = perm(y[1], y[0], 0x05010400u), t23l = perm(y[3], y[2], 0x05010400u);
-          const uint32_t t01h = perm(y[1], y[0], 0x07030602u), t23h = perm(y[3], y[2], 0x07030602u);
-          uint32_t* pw = reinterpret_cast<uint32_t*>(pl + 4 * quad * P_ROW) + n16;
-          pw[0] = perm(t23l, t01l, 0x05040100u);
-          pw[P_ROW / 4] = perm(t23l, t01l, 0x07060302u);
-          pw[2 * P_ROW / 4] = perm(t23h, t01h, 0x05040100u);
-          pw[3 * P_ROW / 4] = perm(t23h, t01h, 0x07060302u);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          const v4i pa = *reinterpret_cast<const v4i*>(pl + n16 * P_ROW + quad * 16);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          const float mn = fmaxf(m[r], mb), mn0 = finite_or_0(mn);
-          const float al = __builtin_amdgcn_exp2f(m[r] - mn0), eb = __builtin_amdgcn_exp2f(mb - mn0);
-          const float be = eb * down;
+        for (int j = 0; j < 4; ++j) y[j] = digits((int)__builtin_amdgcn_fmed3f(w[j] * up, 0.0f, 0x1p30f));
+        const uint32_t t01l = perm(y[1], y[0], 0x05010400u), t23l = perm(y[3], y[2], 0x05010400u);
+        const uint32_t t01h = perm(y[1], y[0], 0x07030602u), t23h = perm(y[3], y[2], 0x07030602u);
+        uint32_t* pw = reinterpret_cast<uint32_t*>(pl + (16 * r + 4 * quad) * P_ROW) + n16;
+        pw[0] = perm(t23l, t01l, 0x05040100u);
+        pw[P_ROW / 4] = perm(t23l, t01l, 0x07060302u);
+        pw[2 * P_ROW / 4] = perm(t23h, t01h, 0x05040100u);
+        pw[3 * P_ROW / 4] = perm(t23h, t01h, 0x07060302u);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      v4i pa[R];
 #pragma unroll
-          for (int t = 0; t < DT; ++t) {
-            const v4i zero = {0, 0, 0, 0};
-            const v4i d = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa, v[t], zero, 0, 0, 0);
-            acc[r][t] = fmaf(undigit(d), be, acc[r][t] * al);
-          }
-          l[r] = fmaf(lp, eb, l[r] * al);
-          m[r] = mn;
+      for (int r = 0; r < R; ++r) pa[r] = *reinterpret_cast<const v4i*>(pl + (16 * r + n16) * P_ROW + quad * 16);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float x, y;
+        join_weights(m[r], mb[r], &x, &y);
+        const float be = y * down[r];
+        l[r] = fmaf(lp[r], y, l[r] * x);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          const v4i zero = {0, 0, 0, 0};
+          const v4i o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[r], v[t], zero, 0, 0, 0);
+          acc[r][t] = fmaf(undigit(o), be, acc[r][t] * x);
         }
       }
-      // the end of a unit, or of the row
-      if (!SPLIT && ((b + 1) % bpu == 0 || b + 1 == b1)) {
+      if (!AHEAD && next >= 0) load_v(next, v);
+      if (AHEAD) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) v[t] = vn[t];
+      }
+    };
+
+    const int bpu = ul / PAGE, blocks = pmax < 0 ? 0 : pmax / PAGE + 1;
+    const int du = MODE == GROUP ? (int)waves : 1;
+    int u = MODE == SPLIT ? (int)(item % a.units) : MODE == GROUP ? (int)wave : 0;
+    const int u_end = MODE == SPLIT ? u + 1 : (blocks + bpu - 1) / bpu;
+    int b = u * bpu;
+    int page = u < u_end && b < blocks ? page_of(table, width, q.pages, b) : -1;
+    if (page >= 0) {
+      load_k(page);
+      load_v(page, v);
+    }
+    while (u < u_end && b < blocks) {
+      const bool unit_ends = b + 1 == blocks || (b + 1) % bpu == 0;
+      const int bn = unit_ends ? (u + du) * bpu : b + 1;
+      const int next = bn < blocks && (!unit_ends || u + du < u_end) ? page_of(table, width, q.pages, bn) : -1;
+      if (page >= 0) {
+        if (!hid && b * PAGE + PAGE - 1 <= pmin)
+          block(std::true_type(), b, next);
+        else
+          block(std::false_type(), b, next);
+      } else if (next >= 0) {
+        load_k(next);
+        load_v(next, v);
+      }
+      if (unit_ends) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const float lu = row_sum(l[r]);
-          const float mn = fmaxf(M[r], m[r]), mn0 = finite_or_0(mn);
-          const float x = __builtin_amdgcn_exp2f(M[r] - mn0), y = __builtin_amdgcn_exp2f(m[r] - mn0);
+          if (MODE == DIRECT) {
+            float x, y;
+            join_weights(M[r], m[r], &x, &y);
 #pragma unroll
-          for (int t = 0; t < DT; ++t) {
-            A[r][t] = fmaf(acc[r][t], y, A[r][t] * x);
-            acc[r][t] = 0.0f;
+            for (int t = 0; t < DT; ++t) A[r][t] = fmaf(acc[r][t], y, A[r][t] * x);
+            L[r] = fmaf(lu, y, L[r] * x);
+          } else if (ps[r] >= 0 && u < unit_count(ps[r])) {
+            float* o = MODE == SPLIT ? a.part + (((size_t)orow[r] * a.nh + ohead[r]) * a.units + u) * (2 + DP)
+                                     : reinterpret_cast<float*>(lds + waves * R * 16 * P_ROW) +
+                                           ((4 * r + quad) * a.units + u) * (2 + DP);
+            if (n16 == 0) {
+              o[0] = m[r];
+              o[1] = lu;
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[2 + 16 * t + n16] = acc[r][t];
           }
-          L[r] = fmaf(lu, y, L[r] * x);
-          M[r] = mn;
           m[r] = -INFINITY;
           l[r] = 0.0f;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) acc[r][t] = 0.0f;
         }
+        u += du;
       }
+      b = bn;
+      page = next;
     }
+    if (MODE == DIRECT) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (SPLIT) {
-        if (ps[r] < 0 || (int)unit >= unit_count(ps[r])) continue;
-        const float lu = row_sum(l[r]);
-        float* o = a.part + (((size_t)orow[r] * a.nh + ohead[r]) * a.units + unit) * (2 + DP);
-        if (n16 == 0) {
-          o[0] = m[r];
-          o[1] = lu;
-        }
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[2 + 16 * t + n16] = acc[r][t];
-      } else {
+      for (int r = 0; r < R; ++r) {
         // a pair without a position is written in the first pass
-        const bool mine = have[r] && (ps[r] >= 0 || (pos[r] < 0 && ul == ul_first));
-        if (!mine) continue;
+        if (!have[r] || !(ps[r] >= 0 || (pos[r] < 0 && ul == ul_first))) continue;
         const float inv = L[r] == 0.0f ? 0.0f : 1.0f / L[r];
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
@@ -644,26 +1051,54 @@ __global__ __launch_bounds__(256) void k_attn(AttnArgs a) {
       }
     }
   }
+  if (MODE == GROUP) {
+    __syncthreads();
+    const float* parts = reinterpret_cast<const float*>(lds + waves * R * 16 * P_ROW);
+    for (uint32_t i = threadIdx.x; i < 4u * R * DP; i += blockDim.x) {
+      const uint32_t pr = pair0 + i / DP, j = pr / a.group, d = i % DP;
+      if (j >= (uint32_t)sp.n) continue;
+      const int n = unit_count(min(sp.pos((int)j), a.most_len - 1));
+      const float* p = parts + i / DP * a.units * (2 + DP);
+      float M = -INFINITY, L = 0.0f, A = 0.0f;
+      for (int u = 0; u < n; ++u, p += 2 + DP) {
+        float x, y;
+        join_weights(M, p[0], &x, &y);
+        A = fmaf(p[2 + d], y, A * x);
+        L = fmaf(p[1], y, L * x);
+      }
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      if (d < a.hd)
+        store_value(a.out, (int64_t)(sp.start + j) * a.os + (int64_t)(g * a.group + pr % a.group) * a.hd + d, a.type, A * inv);
+    }
+  }
 }
 
 // Joins a row's units in order, as the unsplit kernel does. One workgroup of
-// dp lanes per (row of a sequence, head).
+// dp lanes per (row of a sequence, head); a lane holds one unit's maximum and
+// sum, the accumulators of eight units are on their way at a time.
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   const uint32_t h = blockIdx.x % a.nh, j = blockIdx.x / a.nh % a.r.most_rows, seq = blockIdx.x / a.nh / a.r.most_rows;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
   if (j >= (uint32_t)sp.n) return;
   const int64_t pos = min(sp.pos((int)j), a.most_len - 1);
-  const uint32_t row = sp.start + j, d = threadIdx.x, dp = a.p.dp;
+  const uint32_t row = sp.start + j, d = threadIdx.x, dp = a.p.dp, lane = threadIdx.x % WAVE;
   const float* p = a.part + ((size_t)row * a.nh + h) * a.units * (2 + dp);
   const int n = unit_count(pos);
+  static_assert(MAX_UNITS <= WAVE, "a unit for each lane");
+  const float ml = (int)lane < n ? p[lane * (2 + dp)] : 0.0f, ll = (int)lane < n ? p[lane * (2 + dp) + 1] : 0.0f;
   float M = -INFINITY, L = 0.0f, A = 0.0f;
-  for (int u = 0; u < n; ++u, p += 2 + dp) {
-    const float m = p[0], l = p[1], acc = p[2 + d];
-    const float mn = fmaxf(M, m), mn0 = finite_or_0(mn);
-    const float x = __builtin_amdgcn_exp2f(M - mn0), y = __builtin_amdgcn_exp2f(m - mn0);
-    A = fmaf(acc, y, A * x);
-    L = fmaf(l, y, L * x);
-    M = mn;
+  for (int u0 = 0; u0 < n; u0 += 8) {
+    float acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = u0 + e < n ? p[(u0 + e) * (2 + dp) + 2 + d] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (u0 + e >= n) break;
+      float x, y;
+      join_weights(M, __shfl(ml, u0 + e), &x, &y);
+      A = fmaf(acc[e], y, A * x);
+      L = fmaf(__shfl(ll, u0 + e), y, L * x);
+    }
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   if (d < a.hd) store_value(a.out, (int64_t)row * a.os + (int64_t)h * a.hd + d, a.type, A * inv);
@@ -687,29 +1122,44 @@ int rows_launch(uint32_t type, const NormArgs& a, uint32_t rows, hipStream_t s) 
   return launched();
 }
 
-template <int R, bool SPLIT>
-void attn_launch(const AttnArgs& a, uint32_t blocks, hipStream_t s) {
-  switch (a.p.dp / 64) {
-    case 1: k_attn<1, R, SPLIT><<<blocks, 256, 0, s>>>(a); break;
-    case 2: k_attn<2, R, SPLIT><<<blocks, 256, 0, s>>>(a); break;
-    case 3: k_attn<3, R, SPLIT><<<blocks, 256, 0, s>>>(a); break;
-    default: k_attn<4, R, SPLIT><<<blocks, 256, 0, s>>>(a); break;
-  }
+template <int R, AttnMode MODE>
+void attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t lds, hipStream_t s) {
+  const uint32_t kc = a.p.dp / 64;
+  if (kc == 1)
+    k_attn<1, R, MODE><<<blocks, threads, lds, s>>>(a);
+  else if (kc == 2)
+    k_attn<2, R, MODE><<<blocks, threads, lds, s>>>(a);
+  if constexpr (MODE != GROUP && R <= 2)
+    if (kc == 3) k_attn<3, R, MODE><<<blocks, threads, lds, s>>>(a);
+  if constexpr (MODE != GROUP && R == 1)
+    if (kc == 4) k_attn<4, R, MODE><<<blocks, threads, lds, s>>>(a);
 }
 
-// How a call's pairs are dealt: tiles of 4 R pairs, units (0: unsplit).
+// How a call's pairs are dealt.
 struct Plan {
-  uint32_t R, tiles, units;
+  AttnMode mode;
+  uint32_t R, tiles, units, waves;  // tiles of 4 R pairs; units of a row at most; waves of a workgroup
+  size_t lds;
 };
 Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint32_t most_len) {
   const uint32_t pairs = r.most_rows * (heads / kv_heads);
   Plan p;
-  p.R = pairs <= 4 ? 1 : pairs <= 8 ? 2 : 4;
+  p.R = pairs <= 4 || dp > 192 ? 1 : pairs <= 8 || dp > 128 ? 2 : 4;  // as registers allow
   p.tiles = (pairs + 4 * p.R - 1) / (4 * p.R);
+  p.units = (uint32_t)most_units(most_len);
+  p.waves = 4;
   const uint64_t waves = (uint64_t)r.sequences * kv_heads * p.tiles;
-  const int u = most_units(most_len);
-  p.units = waves < 1024 && u > 1 ? (uint32_t)u : 0;
-  (void)dp;
+  const uint32_t w = std::min(p.units, 8u);
+  const size_t group_lds = w * p.R * 16 * P_ROW + 4 * (size_t)p.R * p.units * (2 + dp) * sizeof(float);
+  if (waves >= 1024 || p.units == 1) {
+    p.mode = DIRECT;
+  } else if (p.units <= 16 && p.R <= 2 && dp <= 128) {
+    p.mode = GROUP;
+    p.waves = w;
+  } else {
+    p.mode = SPLIT;
+  }
+  p.lds = p.mode == GROUP ? group_lds : 4 * p.R * 16 * P_ROW;
   return p;
 }
 
@@ -735,25 +1185,67 @@ int rms_norm(uint32_t type, const void* x, int64_t x_stride, const void* residua
   return rows_launch<true>(type, a, rows, s);
 }
 
+template <int MT, int NT, int NW>
+static int linear_few(const LinearArgs& a, bool aligned, hipStream_t s) {
+  const dim3 grid((a.m + 16 * MT - 1) / (16 * MT), (a.rows + 16 * NT - 1) / (16 * NT));
+  if (aligned)
+    k_linear_few<MT, NT, NW, true><<<grid, NW * WAVE, 0, s>>>(a);
+  else
+    k_linear_few<MT, NT, NW, false><<<grid, NW * WAVE, 0, s>>>(a);
+  return launched();
+}
+template <int TM, int TN, int NBUF>
+static int linear_tile(const LinearArgs& a, hipStream_t s) {
+  const uint32_t nrt = (a.rows + 64 * TM - 1) / (64 * TM), tiles = nrt * ((a.m + 64 * TN - 1) / (64 * TN));
+  k_linear_tile<TM, TN, NBUF><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(a, nrt, tiles);
+  return launched();
+}
+template <int TM, int TN>
+static int linear_tile_odd(const LinearArgs& a, hipStream_t s) {
+  const uint32_t nrt = (a.rows + 64 * TM - 1) / (64 * TM), tiles = nrt * ((a.m + 64 * TN - 1) / (64 * TN));
+  k_linear_tile_odd<TM, TN><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(a, nrt, tiles);
+  return launched();
+}
+
 int linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
            const float* w_scale, uint32_t rows, uint32_t m, uint32_t k, uint32_t type, void* y,
            int64_t y_stride, hipStream_t s) {
   if (!rows) return DEFER_GPU_OK;
   const LinearArgs a{x, w, x_scale, w_scale, x_stride, w_stride, y_stride, y, rows, m, k, type};
   const bool aligned = ((uintptr_t)x | (uintptr_t)w | (uintptr_t)x_stride | (uintptr_t)w_stride | k) % 16 == 0;
-  const dim3 grid((m + 15) / 16, (rows + 63) / 64);
-  if (rows <= 16) {
-    if (aligned)
-      k_linear_few<1, true><<<grid, 256, 0, s>>>(a);
-    else
-      k_linear_few<1, false><<<grid, 256, 0, s>>>(a);
-  } else {
-    if (aligned)
-      k_linear_few<4, true><<<grid, 256, 0, s>>>(a);
-    else
-      k_linear_few<4, false><<<grid, 256, 0, s>>>(a);
-  }
-  return launched();
+  // offsets within a tile's operand fit 31 bits
+  const bool near = std::max(x_stride, w_stride) <= (1 << 22);
+  // Few rows read every weight once, at the rate of memory: 16 channels a
+  // workgroup, whose waves share k; many waves of them where there are few
+  // channels (1 x 4096 x 14336: 26.8 us with 4, 13.1 with 16; 1 x 28672 x
+  // 4096: 26.0 and 28.4).
+  const uint64_t m16 = (m + 15) / 16;
+  if (rows <= 16)
+    return m16 <= 512 && k >= 2048 ? linear_few<1, 1, 16>(a, aligned, s) : linear_few<1, 1, 4>(a, aligned, s);
+  // Up to 64 rows and too few 64 x 64 tiles for the chip: k shared by eight
+  // waves (64 x 2048 x 8192: 14.5 us, 16.0 in tiles; 64 x 16384 x 2048: 27
+  // and 10.0), over 32 channels where 16 would be more than a workgroup per CU
+  // (64 x 4096 x 14336: 42.3 with 16, 29.5 with 32).
+  auto tiles_of = [&](uint32_t r, uint32_t c) { return (uint64_t)((rows + r - 1) / r) * ((m + c - 1) / c); };
+  if (rows <= 64 && (tiles_of(64, 64) < 192 || !aligned))
+    return m16 * ((rows + 31) / 32) <= 256 ? linear_few<1, 2, 8>(a, aligned, s) : linear_few<2, 2, 8>(a, aligned, s);
+  if (!near) return linear_few<2, 2, 8>(a, aligned, s);
+  // Unaligned: 301 x 577 x 1537 takes 21 us so and 27 in tiles, 130 x 9001 x
+  // 3001 takes 114 and 44.
+  if (!aligned)
+    return tiles_of(128, 128) < 32 ? linear_few<1, 2, 8>(a, aligned, s) : linear_tile_odd<2, 2>(a, s);
+  // The tile whose rounds over the chip take least: us a round and a stage as
+  // measured (2047 x 28672 x 4096: 269 us in 256 x 128, 350 in 128 x 128; 1000
+  // x 4096 x 4096: 31.1, 22.9, 32.1 in 64 x 64; 500 x 4096 x 4096: 29.7, 19.0,
+  // 17.7). Two 64 x 64 tiles share a CU.
+  const double stages = (k + 127) / 128;
+  auto rounds = [&](uint64_t tiles, uint64_t at_once) { return (double)((tiles + at_once - 1) / at_once); };
+  const uint64_t small = tiles_of(64, 64);
+  const double t256 = rounds(tiles_of(256, 128), 256) * (6.0 + 1.0 * stages);
+  const double t128 = rounds(tiles_of(128, 128), 256) * (3.0 + 0.7 * stages);
+  const double t64 = rounds(small, 512) * (2.0 + (small <= 256 ? 0.34 : 0.5) * stages);
+  if (t256 <= t128 && t256 <= t64) return linear_tile<4, 2, 3>(a, s);
+  return t128 <= t64 ? linear_tile<2, 2, 4>(a, s) : linear_tile<1, 1, 4>(a, s);
 }
 
 static uint32_t kv_grid(const Pages& p, const Rows& r) {
@@ -781,7 +1273,7 @@ size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uin
   if (!r.rows || !r.sequences || !r.most_rows) return 0;
   const uint32_t dp = padded(head_dim);
   const Plan pl = plan_of(r, heads, kv_heads, dp, most_len);
-  return (size_t)r.rows * heads * pl.units * (2 + dp) * sizeof(float);
+  return pl.mode == SPLIT ? (size_t)r.rows * heads * pl.units * (2 + dp) * sizeof(float) : 0;
 }
 
 int attention(const Pages& p, const Rows& r, const Attention& in, void* workspace, size_t workspace_bytes,
@@ -811,26 +1303,34 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   a.hs = in.hidden_stride;
   a.hidden_len = in.hidden_len;
   a.part = static_cast<float*>(workspace);
-  const uint64_t items = (uint64_t)pl.tiles * std::max(pl.units, 1u);
-  const uint64_t blocks = (items + 3) / 4 * r.sequences * p.heads;
+  a.clear = in.clear && r.row_start;
+  const size_t vs = in.type == DEFER_GPU_F32 ? 4 : 2;
+  a.q_vec = in.head_dim % 16 == 0 && ((uintptr_t)in.q | (uintptr_t)(in.q_stride * (int64_t)vs)) % 16 == 0;
+  const uint64_t items = (uint64_t)pl.tiles * (pl.mode == SPLIT ? pl.units : 1);
+  const uint64_t blocks = (pl.mode == GROUP ? items : (items + 3) / 4) * r.sequences * p.heads;
   if (blocks > 0x7fffffffu || (uint64_t)r.sequences * r.most_rows * in.heads > 0x7fffffffu)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
-  const uint32_t nb = (uint32_t)blocks;
-  if (pl.units) {
+  const uint32_t nb = (uint32_t)blocks, nt = pl.waves * WAVE;
+  if (pl.mode == SPLIT) {
     if (pl.R == 1)
-      attn_launch<1, true>(a, nb, s);
+      attn_launch<1, SPLIT>(a, nb, nt, pl.lds, s);
     else if (pl.R == 2)
-      attn_launch<2, true>(a, nb, s);
+      attn_launch<2, SPLIT>(a, nb, nt, pl.lds, s);
     else
-      attn_launch<4, true>(a, nb, s);
+      attn_launch<4, SPLIT>(a, nb, nt, pl.lds, s);
     k_attn_join<<<r.sequences * r.most_rows * in.heads, p.dp, 0, s>>>(a);
+  } else if (pl.mode == GROUP) {
+    if (pl.R == 1)
+      attn_launch<1, GROUP>(a, nb, nt, pl.lds, s);
+    else
+      attn_launch<2, GROUP>(a, nb, nt, pl.lds, s);
   } else {
     if (pl.R == 1)
-      attn_launch<1, false>(a, nb, s);
+      attn_launch<1, DIRECT>(a, nb, nt, pl.lds, s);
     else if (pl.R == 2)
-      attn_launch<2, false>(a, nb, s);
+      attn_launch<2, DIRECT>(a, nb, nt, pl.lds, s);
     else
-      attn_launch<4, false>(a, nb, s);
+      attn_launch<4, DIRECT>(a, nb, nt, pl.lds, s);
   }
   return launched();
 }
@@ -888,7 +1388,7 @@ extern "C" int defer_gpu_q8_linear(const int8_t* x, int64_t x_stride, const floa
   Q8_REQUIRE(k >= 1 && k < MAX_K, "k = %u: sums of code products are exact for 1 <= k < %u", k, MAX_K);
   int rc = check_rows_values(type, y, y_stride, rows, m, "y");
   if (rc) return rc;
-  Q8_REQUIRE((rows + 63) / 64 <= 65535, "%u rows: at most 4,194,240 in one call", rows);
+  Q8_REQUIRE((rows + 31) / 32 <= 65535, "%u rows: at most 2,097,120 in one call", rows);
   Q8_REQUIRE(rows == 0 || (x && x_scale), "null x");
   Q8_REQUIRE(w && w_scale, "null w");
   Q8_REQUIRE(rows <= 1 || x_stride >= (int64_t)k, "x: rows of %u codes %lld apart", k, (long long)x_stride);
@@ -963,8 +1463,8 @@ extern "C" size_t defer_gpu_q8_attention_workspace(const defer_gpu_q8_pages* pag
 extern "C" int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
                                       const void* q, int64_t q_stride, uint32_t q_heads, uint32_t most_len,
                                       float scale, const uint8_t* hidden, int64_t hidden_stride,
-                                      uint32_t hidden_len, void* out, int64_t out_stride, void* workspace,
-                                      size_t workspace_bytes, void* stream) {
+                                      uint32_t hidden_len, void* out, int64_t out_stride, uint32_t clear,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
   Pages p;
   Rows r;
   int rc = check_pages(pages, rows, &p, &r);
@@ -978,6 +1478,6 @@ extern "C" int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const def
              hidden_len, (long long)hidden_stride);
   Q8_REQUIRE(aligned16(workspace), "workspace is not 16-byte aligned");
   Attention a{type, q, q_stride, out, out_stride, q_heads, pages->head_dim, scale, most_len, hidden, hidden_stride,
-              hidden_len};
+              hidden_len, clear != 0};
   return attention(p, r, a, workspace, workspace_bytes, (hipStream_t)stream);
 }

@@ -334,7 +334,8 @@ int defer_gpu_q8_kv_read(const defer_gpu_q8_pages* pages, const defer_gpu_q8_row
  * hidden_stride bytes apart: non-zero hides a position (those behind
  * hidden_len are not hidden), whatever it holds. A row that sees nothing is
  * zeros. No sequence is longer than most_len: positions behind it are not
- * attended to. Scores and sums have f32's accuracy. `workspace` (16-byte aligned) is
+ * attended to. clear != 0: rows of no sequence become zeros. Scores and sums
+ * have f32's accuracy. `workspace` (16-byte aligned) is
  * scratch of the size that defer_gpu_q8_attention_workspace gives (which may
  * be 0); calls that may overlap, captured ones among them, each need their
  * own. */
@@ -343,8 +344,8 @@ size_t defer_gpu_q8_attention_workspace(const defer_gpu_q8_pages* pages, const d
 int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
                            const void* q, int64_t q_stride, uint32_t q_heads, uint32_t most_len,
                            float scale, const uint8_t* hidden, int64_t hidden_stride,
-                           uint32_t hidden_len, void* out, int64_t out_stride, void* workspace,
-                           size_t workspace_bytes, void* stream);
+                           uint32_t hidden_len, void* out, int64_t out_stride, uint32_t clear,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 /* Thread-local description of the last failing call. */
 const char* defer_gpu_last_error(void);

@@ -152,7 +152,7 @@ def test_cache_and_attention_refuse_pages_and_rows(pages, rows):
     p, r = _cache(**pages), _rows(**rows)
     refused("kv_write", p, r, 0, P, 128, P, 128, None)
     refused("kv_read", p, r, 0, P, P, None)
-    refused("attention", p, r, 0, P, 256, 4, 128, 1.0, None, 0, 0, P, 256, P, 1 << 20, None)
+    refused("attention", p, r, 0, P, 256, 4, 128, 1.0, None, 0, 0, P, 256, 0, P, 1 << 20, None)
 
 
 def test_cache_and_attention_refuse_arguments():
@@ -162,16 +162,16 @@ def test_cache_and_attention_refuse_arguments():
     refused("kv_read", p, r, 5, P, P, None)
     refused("kv_read", p, r, 5, None, None, None)
     refused("kv_read", p, r, 0, P + 2, P, None)
-    ok = [0, P, 256, 4, 128, 1.0, None, 0, 0, P, 256, P, 1 << 20, None]
-    for i, bad in ((0, 3), (1, None), (2, 255), (3, 0), (3, 3), (3, 1 << 17), (4, 1 << 31), (9, None), (10, 255), (11, P + 8)):
+    ok = [0, P, 256, 4, 128, 1.0, None, 0, 0, P, 256, 1, P, 1 << 20, None]
+    for i, bad in ((0, 3), (1, None), (2, 255), (3, 0), (3, 3), (3, 1 << 17), (4, 1 << 31), (9, None), (10, 255), (12, P + 8)):
         refused("attention", p, r, *[bad if j == i else a for j, a in enumerate(ok)])
-    refused("attention", p, r, 0, P, 256, 4, 128, 1.0, P, 99, 100, P, 256, P, 1 << 20, None)
-    need = q8._lib().defer_gpu_q8_attention_workspace(p, _rows(), 4, 1000)
+    refused("attention", p, r, 0, P, 256, 4, 128, 1.0, P, 99, 100, P, 256, 0, P, 1 << 20, None)
+    need = q8._lib().defer_gpu_q8_attention_workspace(p, _rows(), 4, 10000)
     assert need > 0
-    assert "workspace" in refused("attention", p, r, 0, P, 256, 4, 1000, 1.0, None, 0, 0, P, 256, P, need - 1, None)
-    refused("attention", p, r, 0, P, 256, 4, 1000, 1.0, None, 0, 0, P, 256, None, need, None)
+    assert "workspace" in refused("attention", p, r, 0, P, 256, 4, 10000, 1.0, None, 0, 0, P, 256, 0, P, need - 1, None)
+    refused("attention", p, r, 0, P, 256, 4, 10000, 1.0, None, 0, 0, P, 256, 0, None, need, None)
     none = _rows(sequences=0, rows=0, most_rows=0, row_start=None, kv_len=None)
-    assert q8._lib().defer_gpu_q8_attention(p, none, 0, None, 256, 4, 128, 1.0, None, 0, 0, None, 256, None, 0, None) == G.OK
+    assert q8._lib().defer_gpu_q8_attention(p, none, 0, None, 256, 4, 128, 1.0, None, 0, 0, None, 256, 0, None, 0, None) == G.OK
     assert q8._lib().defer_gpu_q8_kv_write(p, none, 0, None, 128, None, 128, None) == G.OK
     assert q8._lib().defer_gpu_q8_attention_workspace(None, r, 4, 10) == 0
 
