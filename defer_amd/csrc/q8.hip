@@ -75,11 +75,21 @@ __device__ __forceinline__ float scale_of(double top, bool nan) {
   const float s = top < TINY ? 0.0f : (float)(top / 127.0);
   return nan || !(s < INFINITY) ? __builtin_nanf("") : s;
 }
-// The code of y at a scale: in 64 bits, so that a quotient next to a half is
-// on the side it belongs to. `scale` is 0 or NaN for a row of zeros.
-__device__ __forceinline__ int code_of(double y, double scale) {
-  return scale > 0.0 ? (int)rint(y / scale) : 0;
-}
+// The code of x at a scale, rint(x / s) with ties to even. x and s are 24-bit
+// values: what the product with 1 / s leaves is exact in 64 bits and says
+// where the quotient is on the wrong side of a half (a division takes three
+// times the instructions). `scale` is 0 or NaN for a row of zeros.
+struct Coder {
+  double s, r;
+  __device__ __forceinline__ explicit Coder(float scale) : s(scale > 0.0f ? (double)scale : 0.0), r(s > 0.0 ? 1.0 / s : 0.0) {}
+  __device__ __forceinline__ int operator()(float v) const {
+    const double x = s > 0.0 ? (double)v : 0.0;
+    int c = (int)rint(x * r);
+    const double left = fma(-(double)c, s, x), over = 2.0 * fabs(left) - s;
+    if (over > 0.0 || (over == 0.0 && (c & 1))) c += left > 0.0 ? 1 : -1;
+    return c;
+  }
+};
 
 struct NormArgs {
   const void *x, *r, *w;
@@ -93,55 +103,126 @@ struct NormArgs {
 
 // One workgroup per row: z = x + r, sum z^2, max |z w|, then the codes. The
 // squares and products are formed in 64 bits (24 + 24 bits: the products
-// exactly), which a kernel bound by memory does not notice, so that codes are
-// those of the formula and not of a rounding.
+// exactly), so that codes are those of the formula and not of a rounding;
+// memory hides that. Bound by memory: 2048 x 4096 bf16 with residual, 58.7 MB.
+struct RowSum {
+  double ss = 0.0, top = 0.0;
+  float bad = 0.0f;  // NaN once a value is not finite
+  template <bool NORM>
+  __device__ __forceinline__ double add(float v, float w) {
+    const double d = (double)v, y = NORM ? d * (double)w : d;
+    if (NORM) ss = fma(d, d, ss);
+    top = fmax(top, fabs(y));
+    bad = fmaf(v, 0.0f, bad);
+    if (NORM) bad = fmaf(w, 0.0f, bad);
+    return y;
+  }
+  // over the workgroup: lanes by halves, waves in order
+  __device__ __forceinline__ void join() {
+    __shared__ double s_ss[16], s_top[16];
+    __shared__ float s_bad[16];
+    ss = wave_add(ss);
+    top = wave_max(top);
+    bad = wave_add(bad);
+    const uint32_t w = threadIdx.x / WAVE, waves = blockDim.x / WAVE;
+    if (threadIdx.x % WAVE == 0) {
+      s_ss[w] = ss;
+      s_top[w] = top;
+      s_bad[w] = bad;
+    }
+    __syncthreads();
+    ss = s_ss[0];
+    top = s_top[0];
+    bad = s_bad[0];
+    for (uint32_t i = 1; i < waves; ++i) {
+      ss += s_ss[i];
+      top = fmax(top, s_top[i]);
+      bad += s_bad[i];
+    }
+  }
+};
+
 template <class T, bool NORM>
 __global__ __launch_bounds__(256) void k_rows(NormArgs a) {
   const size_t row = blockIdx.x;
-  const uint32_t tid = threadIdx.x, n = a.n;
+  const uint32_t n = a.n;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
   const T* r = a.r ? static_cast<const T*>(a.r) + row * a.rs : nullptr;
   const T* w = static_cast<const T*>(a.w);
   T* z = a.z ? static_cast<T*>(a.z) + row * a.zs : nullptr;
-  auto value = [&](uint32_t i) {
-    T v = x[i];
-    if (NORM && r) v = (T)((float)v + (float)r[i]);
-    return v;
-  };
-  double ss = 0.0, top = 0.0;
-  float bad = 0.0f;  // NaN once a value is not finite
-  for (uint32_t i = tid; i < n; i += 256) {
-    const T v = value(i);
-    const double d = (double)(float)v;
-    const double y = NORM ? d * (double)(float)w[i] : d;
-    if (NORM) ss = fma(d, d, ss);
-    top = fmax(top, fabs(y));
-    bad = fmaf((float)v, 0.0f, bad);
-    if (NORM) bad = fmaf((float)w[i], 0.0f, bad);
-  }
-  __shared__ double s_ss[4], s_top[4];
-  __shared__ float s_bad[4];
-  ss = wave_add(ss);
-  top = wave_max(top);
-  bad = wave_add(bad);
-  if (tid % WAVE == 0) {
-    s_ss[tid / WAVE] = ss;
-    s_top[tid / WAVE] = top;
-    s_bad[tid / WAVE] = bad;
-  }
-  __syncthreads();
-  ss = (s_ss[0] + s_ss[1]) + (s_ss[2] + s_ss[3]);
-  top = fmax(fmax(s_top[0], s_top[1]), fmax(s_top[2], s_top[3]));
-  bad = (s_bad[0] + s_bad[1]) + (s_bad[2] + s_bad[3]);
-  const double inv = NORM ? 1.0 / sqrt(ss / n + (double)a.eps) : 1.0;
-  const float scale = scale_of(top * inv, isnan(bad));
-  if (tid == 0) a.scale[row] = scale;
+  auto value = [&](uint32_t i) { return NORM && r ? (T)((float)x[i] + (float)r[i]) : x[i]; };
+  RowSum s;
+  for (uint32_t i = threadIdx.x; i < n; i += 256) s.add<NORM>((float)value(i), NORM ? (float)w[i] : 1.0f);
+  s.join();
+  const double inv = NORM ? 1.0 / sqrt(s.ss / n + (double)a.eps) : 1.0;
+  const float scale = scale_of(s.top * inv, isnan(s.bad));
+  if (threadIdx.x == 0) a.scale[row] = scale;
+  const double f = NORM && scale > 0.0f ? inv / (double)scale : 0.0;
+  const Coder code(scale);
   int8_t* c = a.codes + row * (size_t)n;
-  for (uint32_t i = tid; i < n; i += 256) {
+  for (uint32_t i = threadIdx.x; i < n; i += 256) {
     const T v = value(i);
-    const double d = (double)(float)v;
-    c[i] = (int8_t)code_of(NORM ? d * (double)(float)w[i] * inv : d, (double)scale);
+    c[i] = (int8_t)(NORM ? (f > 0.0 ? (int)rint((double)(float)v * (double)(float)w[i] * f) : 0) : code((float)v));
     if (NORM && z) z[i] = v;
+  }
+}
+
+// The same where every row is a multiple of 16 bytes apart and long: 16-byte
+// loads, and the row stays in registers between its two passes. The sum of
+// squares goes by thread in another order than k_rows': which of the two runs
+// depends on n, the strides and the addresses only.
+template <class T, bool NORM, int BLOCK, int C>
+__global__ __launch_bounds__(BLOCK) void k_rows_vec(NormArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T vt __attribute__((ext_vector_type(V)));
+  typedef int8_t vc __attribute__((ext_vector_type(V)));
+  const size_t row = blockIdx.x;
+  const uint32_t n = a.n;
+  const vt* x = reinterpret_cast<const vt*>(static_cast<const T*>(a.x) + row * a.xs);
+  const vt* r = a.r ? reinterpret_cast<const vt*>(static_cast<const T*>(a.r) + row * a.rs) : nullptr;
+  const vt* w = static_cast<const vt*>(a.w);
+  vt* z = a.z ? reinterpret_cast<vt*>(static_cast<T*>(a.z) + row * a.zs) : nullptr;
+  const uint32_t nv = n / V;
+  vt v[C], rv[C], wv[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const uint32_t i = c * BLOCK + threadIdx.x;
+    if (i < nv) {
+      v[c] = x[i];
+      if (NORM && r) rv[c] = r[i];
+      if (NORM) wv[c] = w[i];
+    }
+  }
+  RowSum s;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const uint32_t i = c * BLOCK + threadIdx.x;
+    if (i >= nv) continue;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (NORM && r) v[c][e] = (T)((float)v[c][e] + (float)rv[c][e]);
+      s.add<NORM>((float)v[c][e], NORM ? (float)wv[c][e] : 1.0f);
+    }
+    if (NORM && z) z[i] = v[c];
+  }
+  s.join();
+  const double inv = NORM ? 1.0 / sqrt(s.ss / n + (double)a.eps) : 1.0;
+  const float scale = scale_of(s.top * inv, isnan(s.bad));
+  if (threadIdx.x == 0) a.scale[row] = scale;
+  const double f = NORM && scale > 0.0f ? inv / (double)scale : 0.0;
+  const Coder code(scale);
+  vc* codes = reinterpret_cast<vc*>(a.codes + row * (size_t)n);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const uint32_t i = c * BLOCK + threadIdx.x;
+    if (i >= nv) continue;
+    vc o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float y = (float)v[c][e];
+      o[e] = (int8_t)(NORM ? (f > 0.0 ? (int)rint((double)y * (double)(float)wv[c][e] * f) : 0) : code(y));
+    }
+    codes[i] = o;
   }
 }
 
@@ -538,22 +619,89 @@ struct KvArgs {
   void *k, *v;
   int64_t ks, vs;
   uint32_t type, hd;
+  bool vec;  // eight values of a row are 16-byte loads and stores
 };
 
-constexpr int KV_ROW = 256 + 4;  // bytes of a token's codes in LDS, apart by an odd number of words
+// Runs that rows of neighbouring positions may lie in.
+Q8_HD uint32_t kv_runs(uint32_t rows) { return (rows + 14) / 16 + 1; }
+constexpr int KV_ROW = 256 + 8;  // bytes of a token's codes in LDS
+constexpr int KV_RUN = 16;       // positions a workgroup takes: a quarter of a page
 
-// A workgroup owns the new rows of one block of 64 positions, one head. A wave
-// takes a row: maximum, scale, codes; keys go out as they are, values through
-// LDS into their transposed page. No other workgroup of the call writes
-// this block of the sequence, and bytes of rows that are not the call's are
-// not touched.
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+  return __builtin_amdgcn_perm(hi, lo, sel);
+}
+// 4 x 4 bytes, rows to columns.
+__device__ __forceinline__ void transpose4(const uint32_t* in, uint32_t* out) {
+  const uint32_t l01 = perm(in[1], in[0], 0x05010400u), l23 = perm(in[3], in[2], 0x05010400u);
+  const uint32_t h01 = perm(in[1], in[0], 0x07030602u), h23 = perm(in[3], in[2], 0x07030602u);
+  out[0] = perm(l23, l01, 0x05040100u);
+  out[1] = perm(l23, l01, 0x07060302u);
+  out[2] = perm(h23, h01, 0x05040100u);
+  out[3] = perm(h23, h01, 0x07060302u);
+}
+
+// 8 values of a row from d on, zeros from hd on; vec: 16-byte loads.
+__device__ __forceinline__ void load8(const void* p, int64_t i0, uint32_t d, uint32_t hd, uint32_t type, bool vec, float* y) {
+  if (vec && d < hd) {
+    if (type == DEFER_GPU_F32) {
+      const v4f* q = reinterpret_cast<const v4f*>(static_cast<const float*>(p) + i0 + d);
+      const v4f a = q[0], b = q[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[e] = a[e];
+        y[4 + e] = b[e];
+      }
+    } else {
+      const v4i w = *reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(p) + i0 + d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t h = (uint16_t)((uint32_t)w[e / 2] >> (16 * (e % 2)));
+        y[e] = type == DEFER_GPU_BF16 ? __builtin_bit_cast(float, (uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < 8; ++e) y[e] = d + e < hd ? load_value(p, i0 + d + e, type) : 0.0f;
+}
+__device__ __forceinline__ void store8(void* p, int64_t i0, uint32_t d, uint32_t hd, uint32_t type, bool vec, const float* y) {
+  if (vec && d < hd) {
+    if (type == DEFER_GPU_F32) {
+      v4f* q = reinterpret_cast<v4f*>(static_cast<float*>(p) + i0 + d);
+      q[0] = v4f{y[0], y[1], y[2], y[3]};
+      q[1] = v4f{y[4], y[5], y[6], y[7]};
+    } else {
+      v4i w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint16_t lo = type == DEFER_GPU_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[2 * e]) : __builtin_bit_cast(uint16_t, (_Float16)y[2 * e]);
+        const uint16_t hi = type == DEFER_GPU_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[2 * e + 1]) : __builtin_bit_cast(uint16_t, (_Float16)y[2 * e + 1]);
+        w[e] = (int)((uint32_t)lo | (uint32_t)hi << 16);
+      }
+      *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p) + i0 + d) = w;
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < 8; ++e)
+    if (d + e < hd) store_value(p, i0 + d + e, type, y[e]);
+}
+
+// A workgroup owns the new rows of 16 positions of a page, one head. 16 lanes
+// take a row, 8 values each: maximum, scale, codes; keys go out as they are,
+// values through LDS into their transposed page, 16 positions (16 bytes) a store.
+// No other workgroup of the call writes these positions of the sequence, and
+// bytes of rows that are not the call's are not touched. (2000 rows of 8 heads of
+// 128 in bf16: 40 us with a wave per row and a whole page per workgroup, 14.6
+// with 16 lanes per row.)
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs a) {
-  const uint32_t per = (a.r.most_rows + PAGE - 2) / PAGE + 1;
+  const uint32_t per = kv_runs(a.r.most_rows);
   const uint32_t g = blockIdx.x % a.p.heads, b = blockIdx.x / a.p.heads % per, seq = blockIdx.x / a.p.heads / per;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
   const int64_t first = max((int64_t)0, sp.pos(0)), end = sp.len;  // positions [first, end)
-  const int64_t block = first / PAGE + b, t0 = max(first, block * PAGE), t1 = min(end, (block + 1) * PAGE);
+  const int64_t run = first / KV_RUN + b, t0 = max(first, run * KV_RUN), t1 = min(end, (run + 1) * KV_RUN);
   if (t0 >= t1) return;
+  const int64_t block = run * KV_RUN / PAGE;
   const int32_t* table;
   uint32_t width;
   const SeqPages q = pool_of(a.p, seq, table, width);
@@ -562,74 +710,97 @@ __global__ __launch_bounds__(256) void k_kv_write(KvArgs a) {
   const size_t hp = (size_t)page * a.p.heads + g;
   int8_t* kc = q.keys + hp * PAGE * a.p.dp;
   int8_t* vc = q.values + hp * PAGE * a.p.dp;
-  const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, hd = a.hd;
-  __shared__ int8_t tile[PAGE * KV_ROW];
-  for (int64_t t = t0 + wave; t < t1; t += 4) {
-    const int64_t row = sp.start + (t - sp.pos(0));
-    const int at = (int)(t - block * PAGE);
+  const uint32_t n16 = threadIdx.x % 16, quad = threadIdx.x / 16, quads = blockDim.x / 16, hd = a.hd;
+  const int a0 = (int)(t0 - block * PAGE), a1 = (int)(t1 - block * PAGE);
+  const int64_t row0 = sp.start + (block * PAGE - sp.pos(0));  // the row of the block's first position
+  __shared__ __align__(16) int8_t tile[KV_RUN * KV_ROW];
+  const int tr = (int)(run * KV_RUN - block * PAGE);  // the run's first place in its page
+  for (int at = a0 + (int)quad; at < a1; at += (int)quads) {
+    const int64_t row = row0 + at;
+    float y[2][2][8];
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h)
+        if (h == 0 || hd > 128)
+          load8(which ? a.v : a.k, row * (which ? a.vs : a.ks) + (int64_t)g * hd, 128 * h + 8 * n16, hd, a.type, a.vec, y[which][h]);
+#pragma unroll
     for (int which = 0; which < 2; ++which) {
-      const void* src = which ? a.v : a.k;
-      const int64_t i0 = row * (which ? a.vs : a.ks) + (int64_t)g * hd;
-      float y[4];
       float top = 0.0f, bad = 0.0f;
-      for (uint32_t e = 0; e < 4; ++e) {
-        const uint32_t d = lane + WAVE * e;
-        y[e] = d < hd ? load_value(src, i0 + d, a.type) : 0.0f;
-        top = fmaxf(top, fabsf(y[e]));
-        bad = fmaf(y[e], 0.0f, bad);
-      }
-      top = wave_max(top);
-      const float scale = scale_of(top, isnan(wave_add(bad)));
-      for (uint32_t e = 0; e < 4; ++e) {
-        const uint32_t d = lane + WAVE * e;
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h)
+        if (h == 0 || hd > 128)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            top = fmaxf(top, fabsf(y[which][h][e]));
+            bad = fmaf(y[which][h][e], 0.0f, bad);
+          }
+      const float scale = scale_of(row_max(top), isnan(row_sum(bad)));
+      const Coder code(scale);
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t d = 128 * h + 8 * n16;
         if (d >= hd) continue;
-        const int8_t c = (int8_t)code_of(y[e], scale);
-        if (which)
-          tile[at * KV_ROW + d] = c;
-        else
-          kc[at * a.p.dp + d] = c;
+        uint64_t c = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c |= (uint64_t)(uint8_t)code(y[which][h][e]) << (8 * e);
+        // a page's row is a multiple of 64 codes: those behind hd are zeros
+        *reinterpret_cast<uint64_t*>(which ? tile + (at - tr) * KV_ROW + d : kc + at * a.p.dp + d) = c;
       }
-      if (lane == 0) (which ? q.value_scale : q.key_scale)[hp * PAGE + at] = scale;
+      if (n16 == 0) (which ? q.value_scale : q.key_scale)[hp * PAGE + at] = scale;
     }
   }
   __syncthreads();
-  const int a0 = (int)(t0 - block * PAGE), a1 = (int)(t1 - block * PAGE);
-  for (uint32_t i = threadIdx.x; i < hd * (PAGE / 4); i += 256) {
-    const uint32_t d = i / (PAGE / 4);
-    const int t = 4 * (int)(i % (PAGE / 4));
-    if (t >= a0 && t + 4 <= a1) {
-      uint32_t w = 0;
-      for (int e = 0; e < 4; ++e) w |= (uint32_t)(uint8_t)tile[(t + e) * KV_ROW + d] << (8 * e);
-      *reinterpret_cast<uint32_t*>(vc + d * PAGE + t) = w;
-    } else {
-      for (int e = 0; e < 4; ++e)
-        if (t + e >= a0 && t + e < a1) vc[d * PAGE + t + e] = tile[(t + e) * KV_ROW + d];
+  if (a1 - a0 < KV_RUN) {  // some of the run: byte by byte
+    for (uint32_t i = threadIdx.x; i < (uint32_t)(a1 - a0) * hd; i += blockDim.x) {
+      const uint32_t d = i % hd, t = a0 + i / hd;
+      vc[d * PAGE + t] = tile[(t - tr) * KV_ROW + d];
     }
+    return;
+  }
+  for (uint32_t d = 4 * threadIdx.x; d < hd; d += 4 * blockDim.x) {  // four channels a thread
+    uint32_t w[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t in[4], out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in[e] = *reinterpret_cast<const uint32_t*>(tile + (4 * u + e) * KV_ROW + d);
+      transpose4(in, out);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[c][u] = out[c];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (d + c < hd)
+        *reinterpret_cast<v4i*>(vc + (d + c) * PAGE + tr) = v4i{(int)w[c][0], (int)w[c][1], (int)w[c][2], (int)w[c][3]};
   }
 }
 
-// The same blocks back: codes times scales. What would be the blocks of one
-// more sequence clear the rows of none.
+// The same runs back: codes times scales. What would be the runs of one more
+// sequence clear the rows of none.
 __global__ __launch_bounds__(256) void k_kv_read(KvArgs a) {
-  const uint32_t per = (a.r.most_rows + PAGE - 2) / PAGE + 1;
+  const uint32_t per = kv_runs(a.r.most_rows);
   const uint32_t g = blockIdx.x % a.p.heads, b = blockIdx.x / a.p.heads % per, seq = blockIdx.x / a.p.heads / per;
+  const uint32_t n16 = threadIdx.x % 16, quad = threadIdx.x / 16, quads = blockDim.x / 16, hd = a.hd;
   if (seq == a.r.sequences) {
     const int64_t lo = min((int64_t)max(a.r.row_start[0], 0), (int64_t)a.r.rows);
     const int64_t hi = min((int64_t)max(a.r.row_start[seq], (int)lo), (int64_t)a.r.rows);
-    for (int64_t row = b; row < (int64_t)a.r.rows; row += per) {
-      if (row >= lo && row < hi) continue;
-      for (uint32_t d = threadIdx.x; d < a.hd; d += 256) {
-        if (a.k) store_value(a.k, (row * a.p.heads + g) * a.hd + d, a.type, 0.0f);
-        if (a.v) store_value(a.v, (row * a.p.heads + g) * a.hd + d, a.type, 0.0f);
+    for (int64_t i = b; i < lo + ((int64_t)a.r.rows - hi); i += per) {
+      const int64_t row = i < lo ? i : hi + (i - lo);
+      for (uint32_t d = threadIdx.x; d < hd; d += blockDim.x) {
+        if (a.k) store_value(a.k, (row * a.p.heads + g) * hd + d, a.type, 0.0f);
+        if (a.v) store_value(a.v, (row * a.p.heads + g) * hd + d, a.type, 0.0f);
       }
     }
     return;
   }
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
-  // blocks from the one of the first row on, which may be before position 0
-  const int64_t p0 = sp.pos(0), base = p0 >= 0 ? p0 / PAGE : -((-p0 + PAGE - 1) / PAGE);
-  const int64_t block = base + b, t0 = max(p0, block * PAGE), t1 = min((int64_t)sp.len, (block + 1) * PAGE);
+  // runs from the one of the first row on, which may be before position 0
+  auto down = [](int64_t t, int n) { return t >= 0 ? t / n : -((-t + n - 1) / n); };
+  const int64_t p0 = sp.pos(0), run = down(p0, KV_RUN) + b;
+  const int64_t t0 = max(p0, run * KV_RUN), t1 = min((int64_t)sp.len, (run + 1) * KV_RUN);
   if (t0 >= t1) return;
+  const int64_t block = down(run, PAGE / KV_RUN);
   const int32_t* table;
   uint32_t width;
   const SeqPages q = pool_of(a.p, seq, table, width);
@@ -637,19 +808,42 @@ __global__ __launch_bounds__(256) void k_kv_read(KvArgs a) {
   const size_t hp = (size_t)max(page, 0) * a.p.heads + g;
   const int8_t* kc = q.keys + hp * PAGE * a.p.dp;
   const int8_t* vc = q.values + hp * PAGE * a.p.dp;
-  const uint32_t hd = a.hd;
-  for (uint32_t i = threadIdx.x; i < (uint32_t)(t1 - t0) * hd; i += 256) {
-    const int at = (int)(t0 - block * PAGE) + (int)(i / hd);
-    const uint32_t d = i % hd;
-    const int64_t row = sp.start + (block * PAGE + at - p0);
-    float k = 0.0f, v = 0.0f;
-    if (page >= 0) {
-      k = (float)kc[at * a.p.dp + d] * q.key_scale[hp * PAGE + at];
-      v = (float)vc[d * PAGE + at] * q.value_scale[hp * PAGE + at];
+  const int a0 = (int)(t0 - block * PAGE), a1 = (int)(t1 - block * PAGE);
+  const int64_t row0 = sp.start + (block * PAGE - p0);
+  __shared__ __align__(16) int8_t tile[KV_RUN * KV_ROW];
+  const int tr = (int)(run * KV_RUN - block * PAGE);  // the run's first place in its page
+  if (page >= 0 && a.v) {
+    for (uint32_t d = 4 * threadIdx.x; d < hd; d += 4 * blockDim.x) {  // rows up to a multiple of 64 are there
+      v4i w[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const v4i*>(vc + (d + c) * PAGE + tr);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t in[4], out[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) in[c] = (uint32_t)w[c][u];
+        transpose4(in, out);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(tile + (4 * u + e) * KV_ROW + d) = out[e];
+      }
     }
-    const int64_t o = (row * a.p.heads + g) * hd + d;
-    if (a.k) store_value(a.k, o, a.type, k);
-    if (a.v) store_value(a.v, o, a.type, v);
+  }
+  __syncthreads();
+  for (int at = a0 + (int)quad; at < a1; at += (int)quads) {
+    const float ks = page >= 0 ? q.key_scale[hp * PAGE + at] : 0.0f, vs = page >= 0 ? q.value_scale[hp * PAGE + at] : 0.0f;
+    const int64_t o = ((row0 + at) * a.p.heads + g) * hd;
+    for (uint32_t d = 8 * n16; d < hd; d += 128) {
+      float k[8], v[8];
+      const uint64_t ck = page >= 0 ? *reinterpret_cast<const uint64_t*>(kc + at * a.p.dp + d) : 0;
+      const uint64_t cv = page >= 0 ? *reinterpret_cast<const uint64_t*>(tile + (at - tr) * KV_ROW + d) : 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        k[e] = page >= 0 ? (float)(int8_t)(ck >> (8 * e)) * ks : 0.0f;
+        v[e] = page >= 0 ? (float)(int8_t)(cv >> (8 * e)) * vs : 0.0f;
+      }
+      if (a.k) store8(a.k, o, d, hd, a.type, a.vec, k);
+      if (a.v) store8(a.v, o, d, hd, a.type, a.vec, v);
+    }
   }
 }
 
@@ -677,9 +871,6 @@ __device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x0080
 // ... and back, from sums of products of each digit with codes.
 __device__ __forceinline__ float undigit(v4i d) {
   return fmaf((float)((d[3] << 8) + d[2]), 65536.0f, (float)((d[1] << 8) + d[0]));
-}
-__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
-  return __builtin_amdgcn_perm(hi, lo, sel);
 }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -948,13 +1139,11 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
         uint32_t y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = digits((int)__builtin_amdgcn_fmed3f(w[j] * up, 0.0f, 0x1p30f));
-        const uint32_t t01l = perm(y[1], y[0], 0x05010400u), t23l = perm(y[3], y[2], 0x05010400u);
-        const uint32_t t01h = perm(y[1], y[0], 0x07030602u), t23h = perm(y[3], y[2], 0x07030602u);
         uint32_t* pw = reinterpret_cast<uint32_t*>(pl + (16 * r + 4 * quad) * P_ROW) + n16;
-        pw[0] = perm(t23l, t01l, 0x05040100u);
-        pw[P_ROW / 4] = perm(t23l, t01l, 0x07060302u);
-        pw[2 * P_ROW / 4] = perm(t23h, t01h, 0x05040100u);
-        pw[3 * P_ROW / 4] = perm(t23h, t01h, 0x07060302u);
+        uint32_t by_digit[4];
+        transpose4(y, by_digit);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pw[e * P_ROW / 4] = by_digit[e];
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -1111,15 +1300,30 @@ int launched() {
   return e == hipSuccess ? DEFER_GPU_OK : defer_gpu_fail_(DEFER_GPU_E_HIP, "launch: %s", hipGetErrorString(e));
 }
 
+template <class T, bool NORM>
+int rows_launch_as(const NormArgs& a, uint32_t rows, hipStream_t s) {
+  constexpr uint32_t V = 16 / sizeof(T);
+  auto fits = [](const void* p, int64_t stride) { return ((uintptr_t)p | (uintptr_t)(stride * (int64_t)sizeof(T))) % 16 == 0; };
+  const bool vec = a.n % V == 0 && fits(a.x, a.xs) && fits(a.w, 0) && (!a.r || fits(a.r, a.rs)) && (!a.z || fits(a.z, a.zs)) &&
+                   ((uintptr_t)a.codes | a.n) % V == 0;
+  const uint32_t nv = a.n / V;
+  if (vec && nv <= 256)
+    k_rows_vec<T, NORM, 256, 1><<<rows, 256, 0, s>>>(a);
+  else if (vec && nv <= 512)
+    k_rows_vec<T, NORM, 256, 2><<<rows, 256, 0, s>>>(a);
+  else if (vec && nv <= 1024)
+    k_rows_vec<T, NORM, 256, 4><<<rows, 256, 0, s>>>(a);
+  else if (vec && nv <= 4096)
+    k_rows_vec<T, NORM, 1024, 4><<<rows, 1024, 0, s>>>(a);
+  else
+    k_rows<T, NORM><<<rows, 256, 0, s>>>(a);
+  return launched();
+}
 template <bool NORM>
 int rows_launch(uint32_t type, const NormArgs& a, uint32_t rows, hipStream_t s) {
-  if (type == DEFER_GPU_F32)
-    k_rows<float, NORM><<<rows, 256, 0, s>>>(a);
-  else if (type == DEFER_GPU_BF16)
-    k_rows<__bf16, NORM><<<rows, 256, 0, s>>>(a);
-  else
-    k_rows<_Float16, NORM><<<rows, 256, 0, s>>>(a);
-  return launched();
+  if (type == DEFER_GPU_F32) return rows_launch_as<float, NORM>(a, rows, s);
+  if (type == DEFER_GPU_BF16) return rows_launch_as<__bf16, NORM>(a, rows, s);
+  return rows_launch_as<_Float16, NORM>(a, rows, s);
 }
 
 template <int R, AttnMode MODE>
@@ -1249,23 +1453,26 @@ int linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t
 }
 
 static uint32_t kv_grid(const Pages& p, const Rows& r) {
-  return r.sequences * p.heads * ((r.most_rows + PAGE - 2) / PAGE + 1);
+  return r.sequences * p.heads * kv_runs(r.most_rows);
 }
 
 int kv_write(const Pages& p, const Rows& r, uint32_t type, const void* k, int64_t k_stride, const void* v,
              int64_t v_stride, uint32_t head_dim, hipStream_t s) {
   if (!r.rows || !r.sequences || !r.most_rows) return DEFER_GPU_OK;
-  const KvArgs a{p, r, const_cast<void*>(k), const_cast<void*>(v), k_stride, v_stride, type, head_dim};
-  k_kv_write<<<kv_grid(p, r), 256, 0, s>>>(a);
+  const int64_t vs = type == DEFER_GPU_F32 ? 4 : 2;
+  const bool vec = head_dim % 8 == 0 && ((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * vs) | (uintptr_t)(v_stride * vs)) % 16 == 0;
+  const KvArgs a{p, r, const_cast<void*>(k), const_cast<void*>(v), k_stride, v_stride, type, head_dim, vec};
+  k_kv_write<<<kv_grid(p, r), r.most_rows <= 4 ? 64 : 256, 0, s>>>(a);
   return launched();
 }
 
 int kv_read(const Pages& p, const Rows& r, uint32_t type, void* k, void* v, uint32_t head_dim, hipStream_t s) {
   if (!r.rows || !r.sequences || !r.most_rows) return DEFER_GPU_OK;
-  const KvArgs a{p, r, k, v, 0, 0, type, head_dim};
+  const bool vec = head_dim % 8 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
+  const KvArgs a{p, r, k, v, 0, 0, type, head_dim, vec};
   Rows and_one = r;
   and_one.sequences += r.row_start != nullptr;
-  k_kv_read<<<kv_grid(p, and_one), 256, 0, s>>>(a);
+  k_kv_read<<<kv_grid(p, and_one), r.most_rows <= 8 ? 64 : 256, 0, s>>>(a);
   return launched();
 }
 
@@ -1414,7 +1621,7 @@ static int check_pages(const defer_gpu_q8_pages* p, const defer_gpu_q8_rows* r, 
   Q8_REQUIRE(p->pages == 0 || (p->keys && p->values && p->key_scale && p->value_scale), "null pages");
   Q8_REQUIRE(aligned16(p->keys) && aligned16(p->values) && aligned16(p->key_scale) && aligned16(p->value_scale),
              "pages are not 16-byte aligned");
-  Q8_REQUIRE(((uint64_t)r->sequences + 1) * p->heads * ((r->most_rows + PAGE - 2) / PAGE + 1) <= 0x7fffffffu,
+  Q8_REQUIRE(((uint64_t)r->sequences + 1) * p->heads * kv_runs(r->most_rows) <= 0x7fffffffu,
              "too many rows for one call");
   return DEFER_GPU_OK;
 }
