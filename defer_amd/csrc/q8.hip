@@ -45,11 +45,26 @@ template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
 }
+// (Written out: the compiler moves each lane's value, quiets it, then takes the
+// maximum: three instructions a step. A lane reads another's register two wait
+// states after it was written.)
 __device__ __forceinline__ float row_max(float v) {
-  v = fmaxf(v, dpp<0x128>(v));
-  v = fmaxf(v, dpp<0x124>(v));
-  v = fmaxf(v, dpp<0x122>(v));
-  return fmaxf(v, dpp<0x121>(v));
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:4 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:2 row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:1 row_mask:0xf bank_mask:0xf\n\ts_nop 1"
+      : "+v"(v));
+#endif
+  return v;
+}
+// Towards zero; what is not a number is 0, what is out of range the nearest.
+__device__ __forceinline__ int to_int(float v) {
+  int i = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("v_cvt_i32_f32 %0, %1" : "=v"(i) : "v"(v));
+#endif
+  return i;
 }
 __device__ __forceinline__ float row_sum(float v) {
   v += dpp<0x128>(v);
@@ -856,6 +871,7 @@ struct AttnArgs {
   void* out;
   int64_t qs, os;
   uint32_t type, nh, group, hd, tiles, units;
+  uint32_t per_wave;  // units a wave takes (SPLIT)
   bool q_vec;  // a head's 16 values are 16-byte loads
   bool clear;  // zeros for the rows of no sequence
   int64_t most_len;
@@ -884,6 +900,7 @@ __device__ __forceinline__ void join_weights(float& M, float m, float* x, float*
 }
 
 enum AttnMode { DIRECT, SPLIT, GROUP };
+constexpr uint32_t SPLIT_WAVES = 4096;
 constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: rows of four heads on other banks
 
 // What a wave does: the attention of R tiles of four (row, query head) pairs
@@ -910,13 +927,13 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 //
 // DIRECT: a wave goes through all its positions, unit after unit (many rows;
 // the four waves of a workgroup are neighbouring tiles and meet the same codes
-// in L1). SPLIT: a unit for each wave, left in the workspace for
+// in L1). SPLIT: a few units for each wave, left in the workspace for
 // k_attn_join. GROUP: the units of a tile are the waves of one workgroup, which
 // joins them through LDS.
 template <int KC, int R, AttnMode MODE>
-__global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R <= (KC < 3 ? 2 : 0) ? 2 : 1) void k_attn(AttnArgs a) {
+__global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && (KC == 1 || (KC == 2 && R == 1)) ? 2 : 1) void k_attn(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
-  constexpr bool AHEAD = R == 1 && KC <= 2;  // the next values wait in registers of their own
+  constexpr bool AHEAD = R == 1 && KC <= 2 && MODE != GROUP;  // the next values wait in registers of their own
   extern __shared__ __align__(16) uint8_t lds[];  // [waves][R][16][P_ROW], GROUP: then [4 R][units][2 + DP] floats
   const uint32_t lane = threadIdx.x % WAVE, n16 = lane % 16, quad = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
@@ -926,7 +943,8 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
   const uint32_t shs = a.r.sequences * a.p.heads;
   const uint32_t sh = blockIdx.x % shs, item = MODE == GROUP ? blockIdx.x / shs : blockIdx.x / shs * 4 + wave;
   const uint32_t seq = sh / a.p.heads, g = sh % a.p.heads;
-  const uint32_t tile = MODE == SPLIT ? item / a.units : MODE == DIRECT ? a.tiles - 1 - min(item, a.tiles - 1) : item;
+  const uint32_t chunks = (a.units + a.per_wave - 1) / a.per_wave;  // of a row's units (SPLIT)
+  const uint32_t tile = MODE == SPLIT ? item / chunks : MODE == DIRECT ? a.tiles - 1 - min(item, a.tiles - 1) : item;
   if (a.clear && blockIdx.x == 0) {
     // rows of no sequence lie before the first span and behind the last
     const Span none = span_of(a.r.row_start, a.r.kv_len, 0, a.r.rows);
@@ -948,16 +966,11 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
 
   // pairs: (row j of the sequence, query head of the group)
   int pos[R], max_pos = -1, min_pos = 0x7fffffff;
-  uint32_t orow[R], ohead[R];
-  bool have[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const uint32_t pr = pair0 + 4 * r + quad, j = pr / a.group;
-    have[r] = j < (uint32_t)sp.n;
-    const int64_t t = have[r] ? min(sp.pos((int)j), a.most_len - 1) : -1;
+    const uint32_t j = (pair0 + 4 * r + quad) / a.group;
+    const int64_t t = j < (uint32_t)sp.n ? min(sp.pos((int)j), a.most_len - 1) : -1;
     pos[r] = t < 0 ? -1 : (int)t;
-    orow[r] = sp.start + j;
-    ohead[r] = g * a.group + pr % a.group;
     max_pos = max(max_pos, pos[r]);
     min_pos = min(min_pos, pos[r] < 0 ? 0x7fffffff : pos[r]);
   }
@@ -1043,7 +1056,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
       for (int w = 0; w < 4; ++w) {
         uint32_t y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = digits((int)__builtin_amdgcn_fmed3f(x[kk][4 * w + e] * up, -0x1p30f, 0x1p30f));
+        for (int e = 0; e < 4; ++e) y[e] = digits(to_int(x[kk][4 * w + e] * up));
         aq[r][kk][w] = (int)perm(perm(y[3], y[2], sel), perm(y[1], y[0], sel), 0x05040100u);
       }
     sq[r] = __shfl(s, (int)quad * 4);
@@ -1092,7 +1105,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
       // every output (adding the zeros of the others changes nothing)
       float vbad = 0.0f;
       if (WHOLE) vbad = fmaf(vs[0], 0.0f, vs[1] * 0.0f) + fmaf(vs[2], 0.0f, vs[3] * 0.0f);
-      float lp[R], mb[R], down[R];
+      float xw[R], be[R];  // the weights of what came before and of this block
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         v4i d[4];
@@ -1117,17 +1130,16 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
         const float top = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
         const bool none = !WHOLE && top == -INFINITY;
         const float m0 = none ? 0.0f : top * sq[r];
-        mb[r] = none ? -INFINITY : m0;
-        lp[r] = vbad;
+        float lp = vbad;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float p = exp2_of(fmaf(s[j], sq[r], -m0));
           if (!WHOLE) {
             p = see[j] ? p : 0.0f;
-            lp[r] += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
+            lp += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
             w[j] = see[j] ? p * vs[j] : 0.0f;
           } else {
-            lp[r] += p;
+            lp += p;
             w[j] = p * vs[j];
           }
         }
@@ -1135,10 +1147,13 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
         (void)frexpf(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))), &ex);
         ex = max(ex, -96);
         const float up = ldexpf(1.0f, 30 - ex);
-        down[r] = ldexpf(1.0f, ex - 30);
+        float yw;
+        join_weights(m[r], none ? -INFINITY : m0, &xw[r], &yw);
+        be[r] = yw * ldexpf(1.0f, ex - 30);
+        l[r] = fmaf(lp, yw, l[r] * xw[r]);
         uint32_t y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = digits((int)__builtin_amdgcn_fmed3f(w[j] * up, 0.0f, 0x1p30f));
+        for (int j = 0; j < 4; ++j) y[j] = digits(to_int(w[j] * up));
         uint32_t* pw = reinterpret_cast<uint32_t*>(pl + (16 * r + 4 * quad) * P_ROW) + n16;
         uint32_t by_digit[4];
         transpose4(y, by_digit);
@@ -1147,24 +1162,18 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      v4i pa[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) pa[r] = *reinterpret_cast<const v4i*>(pl + (16 * r + n16) * P_ROW + quad * 16);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        float x, y;
-        join_weights(m[r], mb[r], &x, &y);
-        const float be = y * down[r];
-        l[r] = fmaf(lp[r], y, l[r] * x);
+        const v4i pa = *reinterpret_cast<const v4i*>(pl + (16 * r + n16) * P_ROW + quad * 16);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
           const v4i zero = {0, 0, 0, 0};
-          const v4i o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[r], v[t], zero, 0, 0, 0);
-          acc[r][t] = fmaf(undigit(o), be, acc[r][t] * x);
+          const v4i o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa, v[t], zero, 0, 0, 0);
+          acc[r][t] = fmaf(undigit(o), be[r], acc[r][t] * xw[r]);
         }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
       if (!AHEAD && next >= 0) load_v(next, v);
       if (AHEAD) {
 #pragma unroll
@@ -1174,10 +1183,20 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
 
     const int bpu = ul / PAGE, blocks = pmax < 0 ? 0 : pmax / PAGE + 1;
     const int du = MODE == GROUP ? (int)waves : 1;
-    int u = MODE == SPLIT ? (int)(item % a.units) : MODE == GROUP ? (int)wave : 0;
-    const int u_end = MODE == SPLIT ? u + 1 : (blocks + bpu - 1) / bpu;
+    int u = MODE == SPLIT ? (int)(item % chunks * a.per_wave) : MODE == GROUP ? (int)wave : 0;
+    const int u_end = MODE == SPLIT ? u + (int)a.per_wave : (blocks + bpu - 1) / bpu;
     int b = u * bpu;
-    int page = u < u_end && b < blocks ? page_of(table, width, q.pages, b) : -1;
+    // pages of 64 blocks at a time, one a lane: a load for each block would have
+    // to arrive before the block's own loads can go out
+    int window = -1, window_page = -1;
+    auto page_at = [&](int block) {
+      if (block / WAVE != window) {
+        window = block / WAVE;
+        window_page = page_of(table, width, q.pages, (int64_t)window * WAVE + lane);
+      }
+      return __builtin_amdgcn_readlane(window_page, block % WAVE);
+    };
+    int page = u < u_end && b < blocks ? page_at(b) : -1;
     if (page >= 0) {
       load_k(page);
       load_v(page, v);
@@ -1185,7 +1204,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
     while (u < u_end && b < blocks) {
       const bool unit_ends = b + 1 == blocks || (b + 1) % bpu == 0;
       const int bn = unit_ends ? (u + du) * bpu : b + 1;
-      const int next = bn < blocks && (!unit_ends || u + du < u_end) ? page_of(table, width, q.pages, bn) : -1;
+      const int next = bn < blocks && (!unit_ends || u + du < u_end) ? page_at(bn) : -1;
       if (page >= 0) {
         if (!hid && b * PAGE + PAGE - 1 <= pmin)
           block(std::true_type(), b, next);
@@ -1206,7 +1225,8 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
             for (int t = 0; t < DT; ++t) A[r][t] = fmaf(acc[r][t], y, A[r][t] * x);
             L[r] = fmaf(lu, y, L[r] * x);
           } else if (ps[r] >= 0 && u < unit_count(ps[r])) {
-            float* o = MODE == SPLIT ? a.part + (((size_t)orow[r] * a.nh + ohead[r]) * a.units + u) * (2 + DP)
+            const uint32_t pr = pair0 + 4 * r + quad;
+            float* o = MODE == SPLIT ? a.part + (((size_t)(sp.start + pr / a.group) * a.nh + g * a.group + pr % a.group) * a.units + u) * (2 + DP)
                                      : reinterpret_cast<float*>(lds + waves * R * 16 * P_ROW) +
                                            ((4 * r + quad) * a.units + u) * (2 + DP);
             if (n16 == 0) {
@@ -1230,12 +1250,14 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         // a pair without a position is written in the first pass
-        if (!have[r] || !(ps[r] >= 0 || (pos[r] < 0 && ul == ul_first))) continue;
+        const uint32_t pr = pair0 + 4 * r + quad, j = pr / a.group;
+        if (j >= (uint32_t)sp.n || !(ps[r] >= 0 || (pos[r] < 0 && ul == ul_first))) continue;
+        const int64_t o = (int64_t)(sp.start + j) * a.os + (int64_t)(g * a.group + pr % a.group) * a.hd;
         const float inv = L[r] == 0.0f ? 0.0f : 1.0f / L[r];
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
           const uint32_t d = 16 * t + n16;
-          if (d < a.hd) store_value(a.out, (int64_t)orow[r] * a.os + (int64_t)ohead[r] * a.hd + d, a.type, A[r][t] * inv);
+          if (d < a.hd) store_value(a.out, o + d, a.type, A[r][t] * inv);
         }
       }
     }
@@ -1264,7 +1286,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC * R 
 
 // Joins a row's units in order, as the unsplit kernel does. One workgroup of
 // dp lanes per (row of a sequence, head); a lane holds one unit's maximum and
-// sum, the accumulators of eight units are on their way at a time.
+// sum, the accumulators of 32 units are on their way at a time.
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   const uint32_t h = blockIdx.x % a.nh, j = blockIdx.x / a.nh % a.r.most_rows, seq = blockIdx.x / a.nh / a.r.most_rows;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
@@ -1276,17 +1298,19 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   static_assert(MAX_UNITS <= WAVE, "a unit for each lane");
   const float ml = (int)lane < n ? p[lane * (2 + dp)] : 0.0f, ll = (int)lane < n ? p[lane * (2 + dp) + 1] : 0.0f;
   float M = -INFINITY, L = 0.0f, A = 0.0f;
-  for (int u0 = 0; u0 < n; u0 += 8) {
-    float acc[8];
+  constexpr int AT_ONCE = 32;
+  for (int u0 = 0; u0 < n; u0 += AT_ONCE) {
+    float acc[AT_ONCE];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = u0 + e < n ? p[(u0 + e) * (2 + dp) + 2 + d] : 0.0f;
+    for (int e = 0; e < AT_ONCE; ++e) acc[e] = u0 + e < n ? p[(u0 + e) * (2 + dp) + 2 + d] : 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (u0 + e >= n) break;
-      float x, y;
-      join_weights(M, __shfl(ml, u0 + e), &x, &y);
-      A = fmaf(acc[e], y, A * x);
-      L = fmaf(__shfl(ll, u0 + e), y, L * x);
+    for (int e = 0; e < AT_ONCE; ++e) {
+      if (u0 + e < n) {
+        float x, y;
+        join_weights(M, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ml), u0 + e)), &x, &y);
+        A = fmaf(acc[e], y, A * x);
+        L = fmaf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ll), u0 + e)), y, L * x);
+      }
     }
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -1342,28 +1366,38 @@ void attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t ld
 // How a call's pairs are dealt.
 struct Plan {
   AttnMode mode;
-  uint32_t R, tiles, units, waves;  // tiles of 4 R pairs; units of a row at most; waves of a workgroup
-  size_t lds;
+  uint32_t R, tiles, units, per_wave, waves;  // tiles of 4 R pairs; units of a row at most, of a wave; waves of a workgroup
+  size_t lds, workspace;
 };
 Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint32_t most_len) {
   const uint32_t pairs = r.most_rows * (heads / kv_heads);
   Plan p;
-  p.R = pairs <= 4 || dp > 192 ? 1 : pairs <= 8 || dp > 128 ? 2 : 4;  // as registers allow
+  // Tiles share the codes a wave has loaded, so the more the better, as far as
+  // registers allow and waves are left for the chip: a prompt of 2048 8B rows
+  // takes 394, 338 and 275 us with 1, 2 and 4, one of 301 135M rows 13.3, 14.5
+  // and 18.8.
+  auto waves_of = [&](uint32_t R) { return (uint64_t)r.sequences * kv_heads * ((pairs + 4 * R - 1) / (4 * R)); };
+  p.R = pairs <= 4 || dp > 192 ? 1 : pairs > 8 && dp <= 128 && waves_of(4) >= 2048 ? 4 : pairs <= 8 || waves_of(2) >= 1024 ? 2 : 1;
   p.tiles = (pairs + 4 * p.R - 1) / (4 * p.R);
   p.units = (uint32_t)most_units(most_len);
   p.waves = 4;
-  const uint64_t waves = (uint64_t)r.sequences * kv_heads * p.tiles;
+  p.per_wave = 1;
+  p.workspace = 0;
+  const uint64_t waves = waves_of(p.R);
+  const size_t partials = (size_t)r.rows * heads * p.units * (2 + dp) * sizeof(float);
   const uint32_t w = std::min(p.units, 8u);
-  const size_t group_lds = w * p.R * 16 * P_ROW + 4 * (size_t)p.R * p.units * (2 + dp) * sizeof(float);
-  if (waves >= 1024 || p.units == 1) {
-    p.mode = DIRECT;
-  } else if (p.units <= 16 && p.R <= 2 && dp <= 128) {
+  if (p.units > 1 && p.units <= 16 && p.R <= 2 && dp <= 128 && waves < 2048) {
     p.mode = GROUP;
     p.waves = w;
-  } else {
+  } else if (p.units > 1 && waves < 4096 && partials <= ((size_t)128 << 20)) {
+    // about as many waves as the chip holds: each has its rows' digits to form
     p.mode = SPLIT;
+    p.per_wave = (uint32_t)std::max<uint64_t>(1, waves * p.units / SPLIT_WAVES);
+    p.workspace = partials;
+  } else {
+    p.mode = DIRECT;
   }
-  p.lds = p.mode == GROUP ? group_lds : 4 * p.R * 16 * P_ROW;
+  p.lds = p.waves * p.R * 16 * P_ROW + (p.mode == GROUP ? 4 * (size_t)p.R * p.units * (2 + dp) * sizeof(float) : 0);
   return p;
 }
 
@@ -1480,7 +1514,7 @@ size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uin
   if (!r.rows || !r.sequences || !r.most_rows) return 0;
   const uint32_t dp = padded(head_dim);
   const Plan pl = plan_of(r, heads, kv_heads, dp, most_len);
-  return pl.mode == SPLIT ? (size_t)r.rows * heads * pl.units * (2 + dp) * sizeof(float) : 0;
+  return pl.workspace;
 }
 
 int attention(const Pages& p, const Rows& r, const Attention& in, void* workspace, size_t workspace_bytes,
@@ -1504,6 +1538,7 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   a.hd = in.head_dim;
   a.tiles = pl.tiles;
   a.units = pl.units;
+  a.per_wave = pl.per_wave;
   a.most_len = in.most_len;
   a.scale2 = in.scale * 1.44269504088896340736f;
   a.hidden = in.hidden;
@@ -1513,7 +1548,7 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   a.clear = in.clear && r.row_start;
   const size_t vs = in.type == DEFER_GPU_F32 ? 4 : 2;
   a.q_vec = in.head_dim % 16 == 0 && ((uintptr_t)in.q | (uintptr_t)(in.q_stride * (int64_t)vs)) % 16 == 0;
-  const uint64_t items = (uint64_t)pl.tiles * (pl.mode == SPLIT ? pl.units : 1);
+  const uint64_t items = (uint64_t)pl.tiles * (pl.mode == SPLIT ? (pl.units + pl.per_wave - 1) / pl.per_wave : 1);
   const uint64_t blocks = (pl.mode == GROUP ? items : (items + 3) / 4) * r.sequences * p.heads;
   if (blocks > 0x7fffffffu || (uint64_t)r.sequences * r.most_rows * in.heads > 0x7fffffffu)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
