@@ -462,6 +462,13 @@ struct defer_gpu_model {
   std::vector<double> pflop;     // algorithmic flop of each pair
   size_t pused = 0;
   double pstat[6] = {0, 0, 0, 0, 0, 0};
+  struct Q8Model* q8 = nullptr;  // set: weights and caches in 8 bits (q8_model.h)
+};
+
+// What a call on one cache in 8 bits hands to the operators.
+struct Q8CacheArgs {
+  q8::SeqPages view;
+  int32_t row_start[2], kv_len;
 };
 
 // k_b_sample's LDS: the rows layout, with the sampler's region (stage A's
@@ -517,6 +524,9 @@ struct defer_gpu_cache {
   float* d_logits = nullptr;
   float* d_tmp = nullptr;  // kv gather staging
   float* d_trace = nullptr;   // a traced forward: probabilities [L][nh][cap], then queries [L][q]
+  int8_t* q8buf = nullptr;    // a cache in 8 bits, in place of kc and vc
+  Q8CacheArgs* d_q8args = nullptr;
+  uint8_t* d_hidden = nullptr;  // masked positions of a forward in 8 bits
   float* d_norms = nullptr;   // staging of defer_gpu_value_norms
   size_t norms_cap = 0;
   uint32_t pos = 0;        // host mirror of st->pos
@@ -736,13 +746,27 @@ static int apply_layout(defer_gpu_model* m, uint32_t G) {
   return DEFER_GPU_OK;
 }
 
+static void q8_free(Q8Model* q);
+static hipError_t q8_alloc(defer_gpu_model* m);
+static size_t q8_cache_bytes(const defer_gpu_cache* c);
+static int q8_cache_read(defer_gpu_cache* c, uint32_t layer, float* keys, float* values);
+static int q8_forward(defer_gpu_model* m, defer_gpu_cache* c, uint32_t token, const uint32_t* masked, size_t n_masked,
+                      float* logits_out);
+static int q8_generate(defer_gpu_model* m, defer_gpu_cache* c, uint32_t n, uint32_t max_tokens, float T,
+                       const uint32_t* words, const uint32_t* stop, size_t n_stop, uint32_t* out, uint32_t* n_out,
+                       defer_gpu_token_fn on_token, void* user);
+struct Q8Matrix;
+static Q8Matrix* q8_matrix(Q8Model* q, uint32_t l, uint32_t which);
+static hipError_t q8_upload(const Q8Matrix& to, size_t at, const float* src, size_t rows, float* stage, size_t cap);
+
 extern "C" int defer_gpu_model_create(const defer_gpu_config* cfg, const float* const* tensors,
                                       size_t n_tensors, uint32_t flags, defer_gpu_model** out) {
   if (!out) return fail(DEFER_GPU_E_INVALID, "null output handle");
   *out = nullptr;
   int rc = validate(cfg);
   if (rc) return rc;
-  (void)flags;
+  if (flags & ~DEFER_GPU_MODEL_8BIT) return fail(DEFER_GPU_E_INVALID, "unknown model flags 0x%x", flags);
+  const bool in8 = flags & DEFER_GPU_MODEL_8BIT;
   if (!tensors || n_tensors != defer_gpu_model_tensor_count(cfg))
     return fail(DEFER_GPU_E_INVALID, "expected %zu tensors, got %zu",
                 defer_gpu_model_tensor_count(cfg), n_tensors);
@@ -805,16 +829,16 @@ extern "C" int defer_gpu_model_create(const defer_gpu_config* cfg, const float* 
   std::vector<LOff> lo(d.L);
   for (uint32_t l = 0; l < d.L; ++l) {
     lo[l].an = take(h);
-    lo[l].qkv = take((q + 2 * kv) * h);
+    lo[l].qkv = in8 ? 0 : take((q + 2 * kv) * h);
     lo[l].b = d.has_bias ? take(q + 2 * kv) : 0;
-    lo[l].wo = take(h * q);
+    lo[l].wo = in8 ? 0 : take(h * q);
     lo[l].fn = take(h);
-    lo[l].wg = take(ff * h);
-    lo[l].wu = take(ff * h);
-    lo[l].wd = take(h * ff);
+    lo[l].wg = in8 ? 0 : take(ff * h);
+    lo[l].wu = in8 ? 0 : take(ff * h);
+    lo[l].wd = in8 ? 0 : take(h * ff);
   }
   const size_t o_norm = take(h);
-  const size_t o_head = d.tied ? o_embed : take(V * h);
+  const size_t o_head = d.tied ? o_embed : in8 ? 0 : take(V * h);
   const size_t total = off;
 
   e = hipStreamCreateWithFlags(&m->stream, hipStreamNonBlocking);
@@ -847,6 +871,21 @@ extern "C" int defer_gpu_model_create(const defer_gpu_config* cfg, const float* 
     }
     return hipSuccess;
   };
+  // In 8 bits: a scale per output row, the norms' weights left to the norms. A
+  // matrix passes through `q8_stage` a stretch of rows at a time.
+  constexpr size_t Q8_STAGE = (size_t)16 << 20;
+  float* q8_stage = nullptr;
+  if (in8) {
+    e = q8_alloc(m);
+    if (e == hipSuccess) e = counted_malloc(&q8_stage, Q8_STAGE * sizeof(float));
+    if (e != hipSuccess) return cleanup(fail(DEFER_GPU_E_HIP, "hipMalloc for weights: %s", hipGetErrorString(e)));
+  }
+  enum { QKV, WO, GU, DOWN, LM };
+  auto up_matrix = [&](uint32_t l, uint32_t which, size_t row0, size_t o, const float* src, size_t rows, size_t cols,
+                       const float* wn) {
+    if (in8) return q8_upload(*q8_matrix(m->q8, l, which), row0, src, rows, q8_stage, Q8_STAGE);
+    return wn ? up_folded(o, src, rows, wn) : up(o, src, rows * cols);
+  };
   size_t k = 0;
   e = up(o_embed, tensors[k++], V * h);
   for (uint32_t l = 0; l < d.L && e == hipSuccess; ++l) {
@@ -858,23 +897,27 @@ extern "C" int defer_gpu_model_create(const defer_gpu_config* cfg, const float* 
     const float* bk = d.has_bias ? tensors[k++] : nullptr;
     const float* wv = tensors[k++];
     const float* bv = d.has_bias ? tensors[k++] : nullptr;
-    if (e == hipSuccess) e = up_folded(lo[l].qkv, wq, q, an);
-    if (e == hipSuccess) e = up_folded(lo[l].qkv + q * h * sizeof(float), wk, kv, an);
-    if (e == hipSuccess) e = up_folded(lo[l].qkv + (q + kv) * h * sizeof(float), wv, kv, an);
+    if (e == hipSuccess) e = up_matrix(l, QKV, 0, lo[l].qkv, wq, q, h, an);
+    if (e == hipSuccess) e = up_matrix(l, QKV, q, lo[l].qkv + q * h * sizeof(float), wk, kv, h, an);
+    if (e == hipSuccess) e = up_matrix(l, QKV, q + kv, lo[l].qkv + (q + kv) * h * sizeof(float), wv, kv, h, an);
     if (d.has_bias) {
       if (e == hipSuccess) e = up(lo[l].b, bq, q);
       if (e == hipSuccess) e = up(lo[l].b + q * sizeof(float), bk, kv);
       if (e == hipSuccess) e = up(lo[l].b + (q + kv) * sizeof(float), bv, kv);
     }
-    if (e == hipSuccess) e = up(lo[l].wo, tensors[k++], h * q);
+    const float* wo = tensors[k++];
+    if (e == hipSuccess) e = up_matrix(l, WO, 0, lo[l].wo, wo, h, q, nullptr);
     const float* fnw = tensors[k++];
     if (e == hipSuccess) e = up(lo[l].fn, fnw, h);
-    if (e == hipSuccess) e = up_folded(lo[l].wg, tensors[k++], ff, fnw);
-    if (e == hipSuccess) e = up_folded(lo[l].wu, tensors[k++], ff, fnw);
-    if (e == hipSuccess) e = up(lo[l].wd, tensors[k++], h * ff);
+    const float *wg = tensors[k++], *wu = tensors[k++], *wd = tensors[k++];
+    if (e == hipSuccess) e = up_matrix(l, GU, 0, lo[l].wg, wg, ff, h, fnw);
+    if (e == hipSuccess) e = up_matrix(l, GU, ff, lo[l].wu, wu, ff, h, fnw);
+    if (e == hipSuccess) e = up_matrix(l, DOWN, 0, lo[l].wd, wd, h, ff, nullptr);
   }
   if (e == hipSuccess) e = up(o_norm, tensors[k++], h);
-  if (e == hipSuccess && !d.tied) e = up(o_head, tensors[k++], V * h);
+  const float* head = d.tied ? tensors[0] : tensors[n_tensors - 1];
+  if (e == hipSuccess && (in8 || !d.tied)) e = up_matrix(0, LM, 0, o_head, head, V, h, nullptr);
+  (void)hipFree(q8_stage);  // waits for what reads it
   if (e != hipSuccess)
     return cleanup(fail(DEFER_GPU_E_HIP, "weight upload: %s", hipGetErrorString(e)));
 
@@ -940,6 +983,7 @@ extern "C" void defer_gpu_model_destroy(defer_gpu_model* m) {
   if (!m) return;
   if (m->stream) (void)hipStreamSynchronize(m->stream);
   batch_ws_free(m);
+  q8_free(m->q8);
   for (hipEvent_t e : m->pev) (void)hipEventDestroy(e);
   for (DevState* slab : m->state_slabs) (void)hipHostFree(slab);
   (void)hipFree(m->panels);
@@ -997,8 +1041,12 @@ static int cache_alloc(const defer_gpu_model* m, uint32_t cap, defer_gpu_cache* 
   ++g_live_caches;
   c->cap = cap;
   const size_t kvn = (size_t)d.L * d.nkv * cap * d.kvs;
-  HIP_TRY(counted_malloc(&c->kc, kvn * sizeof(float)));
-  HIP_TRY(counted_malloc(&c->vc, kvn * sizeof(float)));
+  if (m->q8) {
+    HIP_TRY(counted_malloc(&c->q8buf, q8_cache_bytes(c)));
+  } else {
+    HIP_TRY(counted_malloc(&c->kc, kvn * sizeof(float)));
+    HIP_TRY(counted_malloc(&c->vc, kvn * sizeof(float)));
+  }
   const size_t hs = d.hd + 2;
   // xo, xd, g: MB_REPS replicas of one block, each on its own 32 KB boundary
   const size_t rep_words = ((size_t)2 * d.h + d.ff + 4095) / 4096 * 4096;
@@ -1059,6 +1107,9 @@ static void cache_free(defer_gpu_cache* c) {
   if (c->graph) (void)hipGraphExecDestroy(c->graph);
   (void)hipFree(c->kc);
   (void)hipFree(c->vc);
+  (void)hipFree(c->q8buf);
+  (void)hipFree(c->d_q8args);
+  (void)hipFree(c->d_hidden);
   (void)hipFree(c->mb);
   (void)hipFree(c->d_run);
   (void)hipFree(c->d_mask);
@@ -1133,8 +1184,8 @@ extern "C" int defer_gpu_cache_clone(const defer_gpu_cache* src, defer_gpu_cache
   auto copy = [&](void* to, const void* from, size_t n) {
     return hipMemcpyAsync(to, from, n, hipMemcpyDeviceToDevice, s);
   };
-  hipError_t e = copy(c->kc, src->kc, kvn * sizeof(float));
-  if (e == hipSuccess) e = copy(c->vc, src->vc, kvn * sizeof(float));
+  hipError_t e = src->q8buf ? copy(c->q8buf, src->q8buf, q8_cache_bytes(src)) : copy(c->kc, src->kc, kvn * sizeof(float));
+  if (e == hipSuccess && !src->q8buf) e = copy(c->vc, src->vc, kvn * sizeof(float));
   if (e == hipSuccess) e = copy(c->mb, src->mb, src->mb_words * sizeof(u64) + sizeof(DevState));
   if (e == hipSuccess) e = hipStreamSynchronize(s);
   if (e != hipSuccess) {
@@ -1158,6 +1209,7 @@ extern "C" int defer_gpu_cache_read(const defer_gpu_cache* cc, uint32_t layer, f
   if (layer >= d.L) return fail(DEFER_GPU_E_INVALID, "layer %u out of range", layer);
   const size_t n = (size_t)c->pos * d.kv;
   if (n == 0) return DEFER_GPU_OK;
+  if (c->q8buf) return q8_cache_read(c, layer, keys, values);
   if (!c->d_tmp) HIP_TRY(counted_malloc(&c->d_tmp, (size_t)c->cap * d.kv * sizeof(float)));
   const hipStream_t s = c->m->stream;
   const size_t per_layer = (size_t)d.nkv * c->cap * d.kvs;
@@ -1188,6 +1240,7 @@ extern "C" int defer_gpu_value_norms(const defer_gpu_cache* cc, uint32_t t0, uin
   if (t0 > t1 || t1 > c->pos)
     return fail(DEFER_GPU_E_INVALID, "positions [%u, %u) outside the cache's %u", t0, t1, c->pos);
   const defer_gpu_model* m = c->m;
+  if (m->q8) return fail(DEFER_GPU_E_INVALID, "value norms need a model in f32");
   const Dims& d = m->d;
   const uint32_t nt = t1 - t0;
   if (nt == 0) return DEFER_GPU_OK;
@@ -1471,6 +1524,10 @@ extern "C" int defer_gpu_forward(const defer_gpu_model* m, defer_gpu_cache* c, u
   if (token >= m->d.V) return fail(DEFER_GPU_E_TOKEN, "token id %u out of range", token);
   if (c->pos >= c->cap)
     return fail(DEFER_GPU_E_CONTEXT, "context length %u exceeded", m->cfg.max_seq_len);
+  if (m->q8) {
+    if (trace_out) return fail(DEFER_GPU_E_INVALID, "attention probabilities need a model in f32");
+    return q8_forward(const_cast<defer_gpu_model*>(m), c, token, masked, n_masked, logits_out);
+  }
   const uint32_t pos0 = c->pos;
   const hipStream_t s = m->stream;
   const size_t n_probs = (size_t)m->d.L * m->d.nh * c->cap;
@@ -1553,7 +1610,9 @@ extern "C" int defer_gpu_prompt(const defer_gpu_model* m, defer_gpu_cache* c,
       break;
     }
   }
-  if (use_batch(m, n_ok))
+  if (m->q8 && !n_ok)
+    rc = DEFER_GPU_OK;
+  else if (use_batch(m, n_ok))
     rc = timed(m, [&] { return feed_batched(const_cast<defer_gpu_model*>(m), c, tokens, n_ok); });
   else
     rc = feed_tokens(m, c, tokens, n_ok);
@@ -1588,6 +1647,11 @@ extern "C" int defer_gpu_generate(const defer_gpu_model* m, defer_gpu_cache* c, 
   if (n == 0) return fail(DEFER_GPU_E_CONTEXT, "context length %u exceeded", m->cfg.max_seq_len);
   if (temperature != 0.0f && !rng_words) return fail(DEFER_GPU_E_INVALID, "null rng words");
   if (!tokens_out) return fail(DEFER_GPU_E_INVALID, "null tokens_out");
+  if (m->q8) {
+    if (n_stop && !stop) return fail(DEFER_GPU_E_INVALID, "null stop tokens");
+    return q8_generate(const_cast<defer_gpu_model*>(m), c, n, max_tokens, temperature, rng_words, stop, n_stop, tokens_out,
+                       n_out, nullptr, nullptr);
+  }
   rc = ensure_run_buffers(c, n, n_stop);
   if (rc) return rc;
   RunInput in;
@@ -1655,6 +1719,9 @@ extern "C" int defer_gpu_generate_cb(const defer_gpu_model* m, defer_gpu_cache* 
   if (temperature != 0.0f && !rng_words) return fail(DEFER_GPU_E_INVALID, "null rng words");
   if (n_stop && !stop) return fail(DEFER_GPU_E_INVALID, "null stop tokens");
   if (!tokens_out) return fail(DEFER_GPU_E_INVALID, "null tokens_out");
+  if (m->q8)
+    return q8_generate(const_cast<defer_gpu_model*>(m), c, n, max_tokens, temperature, rng_words, stop, n_stop, tokens_out,
+                       n_out, on_token, user);
   rc = ensure_run_buffers(c, n, n_stop);
   if (rc) return rc;
   rc = ensure_ring(c, n);
@@ -1806,6 +1873,7 @@ extern "C" int defer_gpu_generate_static(const defer_gpu_model* m, defer_gpu_cac
   int rc = check_pair(m, c);
   if (rc) return rc;
   if (n_out) *n_out = 0;
+  if (m->q8) return fail(DEFER_GPU_E_INVALID, "defer_gpu_generate_static needs a model in f32");
   rc = check_temperature(temperature);
   if (rc) return rc;
   if (max_tokens > STATIC_MAX_TOKENS)
@@ -1932,6 +2000,7 @@ extern "C" int defer_gpu_replay(const defer_gpu_model* m, defer_gpu_cache* c,
     if (history[i] >= m->d.V) return fail(DEFER_GPU_E_TOKEN, "token id %u out of range", history[i]);
   if (n_history > c->cap)
     return fail(DEFER_GPU_E_CONTEXT, "context length %u exceeded", m->cfg.max_seq_len);
+  if (m->q8 && !n_history) return DEFER_GPU_OK;
   if (use_batch(m, n_history))
     return timed(m, [&] {
       return replay_batched(const_cast<defer_gpu_model*>(m), c, history, n_history, prompt_len,
@@ -2026,13 +2095,15 @@ static int ensure_ws(defer_gpu_model* m, uint32_t rows, uint32_t lm) {
   const uint32_t kmax = std::max({d.h, d.q, d.ff});
   HIP_TRY(counted_malloc(&w.X, (size_t)R * d.h * sizeof(float)));
   HIP_TRY(counted_malloc(&w.Y, (size_t)R * batch_ldy(d) * sizeof(float)));
-  HIP_TRY(counted_malloc(&w.INV, (size_t)R * sizeof(float)));
-  HIP_TRY(counted_malloc(&w.XP, panel_floats(R, d.h) * sizeof(float)));
-  HIP_TRY(counted_malloc(&w.QKVT, (size_t)R * d.qkv_rows * sizeof(u64)));
-  HIP_TRY(counted_malloc(&w.PART, (size_t)R * part_words(d) * sizeof(u64)));
   const uint32_t L1 = std::max(Lm, 1u);
-  HIP_TRY(counted_malloc(&w.XQ, panel_floats(std::max(R, L1), kmax) * sizeof(float)));
-  HIP_TRY(counted_malloc(&w.LINV, (size_t)L1 * sizeof(float)));
+  if (!m->q8) {  // rows in 8 bits have a workspace of their own beside this one
+    HIP_TRY(counted_malloc(&w.INV, (size_t)R * sizeof(float)));
+    HIP_TRY(counted_malloc(&w.XP, panel_floats(R, d.h) * sizeof(float)));
+    HIP_TRY(counted_malloc(&w.QKVT, (size_t)R * d.qkv_rows * sizeof(u64)));
+    HIP_TRY(counted_malloc(&w.PART, (size_t)R * part_words(d) * sizeof(u64)));
+    HIP_TRY(counted_malloc(&w.XQ, panel_floats(std::max(R, L1), kmax) * sizeof(float)));
+    HIP_TRY(counted_malloc(&w.LINV, (size_t)L1 * sizeof(float)));
+  }
   HIP_TRY(counted_malloc(&w.LOGT, (size_t)L1 * d.V * sizeof(u64)));
   HIP_TRY(counted_malloc(&w.VMAX, (size_t)L1 * d.nvc * sizeof(u64)));
   HIP_TRY(counted_malloc(&w.VARG, (size_t)L1 * d.nvc * sizeof(u64)));
@@ -2255,6 +2326,9 @@ static void launch_attn_tile(defer_gpu_model* m, uint32_t nb, const uint32_t* it
                         attn_tile_lds(d.hd, nb, nj), m->stream);
 }
 
+static int q8_run(defer_gpu_model* m, const BRow* rows, defer_gpu_cache* const* rcache, uint32_t n, const uint32_t* sel,
+                  uint32_t nl, const uint32_t* dtok, bool deferred);
+
 // Runs n rows (n <= BATCH_MAX_ROWS) through every layer; logits rows
 // sel[0..nl) (batch row indices) get tagged logits and chunk maxima in the
 // workspace. Rows must already be validated (tokens, capacity).
@@ -2263,6 +2337,7 @@ static void launch_attn_tile(defer_gpu_model* m, uint32_t nb, const uint32_t* it
 static int batch_run(defer_gpu_model* m, const BRow* rows, defer_gpu_cache* const* rcache,
                      uint32_t n, const uint32_t* sel, uint32_t nl,
                      const uint32_t* dtok = nullptr, bool deferred = false) {
+  if (m->q8) return q8_run(m, rows, rcache, n, sel, nl, dtok, deferred);
   const Dims& d = m->d;
   const hipStream_t s = m->stream;
   int rc = ensure_panels(m);
@@ -2609,7 +2684,8 @@ static BRow make_row(const defer_gpu_cache* c, uint32_t pos, uint32_t tick, uint
   return r;
 }
 
-static bool use_batch(const defer_gpu_model* m, size_t n) { return m->batch_min && n >= m->batch_min; }
+// (A model in 8 bits has no other path.)
+static bool use_batch(const defer_gpu_model* m, size_t n) { return m->q8 || (m->batch_min && n >= m->batch_min); }
 
 extern "C" int defer_gpu_model_set_batching(defer_gpu_model* m, uint32_t min_rows) {
   if (!m) return fail(DEFER_GPU_E_INVALID, "null model");
@@ -2851,3 +2927,7 @@ static int replay_batched(defer_gpu_model* m, defer_gpu_cache* c, const uint32_t
   }
   return DEFER_GPU_OK;
 }
+
+// ------------------------------------------------------------------ 8 bits
+
+#include "q8_model.h"

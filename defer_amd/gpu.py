@@ -20,6 +20,7 @@ LIB_PATH = os.path.join(_HERE, "libdefer_gpu.so")
 EXEC_PERSISTENT = 0
 EXEC_GRAPH = 1
 EXEC_EAGER = 2
+MODEL_8BIT = 1
 
 OK = 0
 E_INVALID = 1
@@ -188,14 +189,18 @@ def tensor_count(cfg: Config) -> int:
 
 
 class GpuModel:
-    """Weights resident in HBM (Model::from_safetensors, model.rs:301-363)."""
+    """Weights resident in HBM (Model::from_safetensors, model.rs:301-363).
+    bits=8: weights, activations and caches in 8 bits (DEFER_GPU_MODEL_8BIT)."""
 
-    def __init__(self, cfg: Config, tensors: Sequence[np.ndarray]):
+    def __init__(self, cfg: Config, tensors: Sequence[np.ndarray], bits: int = 32):
+        if bits not in (8, 32):
+            raise ValueError(f"bits: 8 or 32, not {bits}")
         self.cfg = cfg
         arrs = [np.ascontiguousarray(t, dtype=np.float32) for t in tensors]
         ptrs = (ctypes.c_void_p * len(arrs))(*[a.ctypes.data for a in arrs])
         h = ctypes.c_void_p()
-        _check(lib().defer_gpu_model_create(ctypes.byref(cfg), ptrs, len(arrs), 0, ctypes.byref(h)))
+        _check(lib().defer_gpu_model_create(ctypes.byref(cfg), ptrs, len(arrs), MODEL_8BIT if bits == 8 else 0,
+                                             ctypes.byref(h)))
         self._h = h
 
     def close(self) -> None:

@@ -66,12 +66,23 @@ typedef struct defer_gpu_cache defer_gpu_cache;
 #define DEFER_GPU_EXEC_GRAPH 1      /* one captured hipGraph of phase kernels per token */
 #define DEFER_GPU_EXEC_EAGER 2      /* phase kernels launched one by one */
 
+/* A model in 8 bits (no counterpart in the reference): weights as codes with a
+ * scale per output row, the products' inputs with one per row, caches with one
+ * per position and head; embedding, norms, residuals and softmax in f32. It runs
+ * on the 8-bit operators below and answers every call of this header in its own
+ * arithmetic, bit-identical however rows are grouped into calls, except
+ * probabilities (trace_out), defer_gpu_value_norms and
+ * defer_gpu_generate_static, which are DEFER_GPU_E_INVALID. Execution mode,
+ * batching and grid change nothing; generate runs a step at a time. */
+#define DEFER_GPU_MODEL_8BIT 1
+
 /* Model::from_safetensors (model.rs:301-363). `tensors` holds host pointers in
  * the order of model.rs:322-347: embed [V,h]; per layer attn_norm [h],
  * wq [q,h], (bq [q]), wk [kv,h], (bk [kv]), wv [kv,h], (bv [kv]), wo [h,q],
  * ffn_norm [h], w_gate [ff,h], w_up [ff,h], w_down [h,ff]; norm [h];
  * (lm_head [V,h] when untied). The library copies them to HBM and computes
- * RoPE tables on the host as model.rs:348-353 and 438-445 do. `flags` is 0. */
+ * RoPE tables on the host as model.rs:348-353 and 438-445 do. `flags` is 0 or
+ * DEFER_GPU_MODEL_8BIT. */
 int defer_gpu_model_create(const defer_gpu_config* cfg, const float* const* tensors,
                            size_t n_tensors, uint32_t flags, defer_gpu_model** out);
 void defer_gpu_model_destroy(defer_gpu_model* m);
