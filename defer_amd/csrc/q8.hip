@@ -931,7 +931,7 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // k_attn_join. GROUP: the units of a tile are the waves of one workgroup, which
 // joins them through LDS.
 template <int KC, int R, AttnMode MODE>
-__global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && (KC == 1 || (KC == 2 && R == 1)) ? 2 : 1) void k_attn(AttnArgs a) {
+__global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 1 ? 3 : MODE != GROUP && (KC == 1 || (KC == 2 && R == 1)) ? 2 : 1) void k_attn(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
   constexpr bool AHEAD = R == 1 && KC <= 2 && MODE != GROUP;  // the next values wait in registers of their own
   extern __shared__ __align__(16) uint8_t lds[];  // [waves][R][16][P_ROW], GROUP: then [4 R][units][2 + DP] floats
@@ -1353,10 +1353,9 @@ int rows_launch(uint32_t type, const NormArgs& a, uint32_t rows, hipStream_t s) 
 template <int R, AttnMode MODE>
 void attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t lds, hipStream_t s) {
   const uint32_t kc = a.p.dp / 64;
-  if (kc == 1)
-    k_attn<1, R, MODE><<<blocks, threads, lds, s>>>(a);
-  else if (kc == 2)
-    k_attn<2, R, MODE><<<blocks, threads, lds, s>>>(a);
+  if constexpr (R <= 2)
+    if (kc == 1) k_attn<1, R, MODE><<<blocks, threads, lds, s>>>(a);
+  if (kc == 2) k_attn<2, R, MODE><<<blocks, threads, lds, s>>>(a);
   if constexpr (MODE != GROUP && R <= 2)
     if (kc == 3) k_attn<3, R, MODE><<<blocks, threads, lds, s>>>(a);
   if constexpr (MODE != GROUP && R == 1)
@@ -1374,10 +1373,11 @@ Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint
   Plan p;
   // Tiles share the codes a wave has loaded, so the more the better, as far as
   // registers allow and waves are left for the chip: a prompt of 2048 8B rows
-  // takes 394, 338 and 275 us with 1, 2 and 4, one of 301 135M rows 13.3, 14.5
-  // and 18.8.
+  // takes 394, 338 and 262 us with 1, 2 and 4, one of 301 135M rows 13.3, 14.5
+  // and 18.8. Heads of 64 fit three waves of R = 2 a SIMD, which hide more than
+  // sharing between four saves (3500 360M rows: 206 us with 4, 191 with 2).
   auto waves_of = [&](uint32_t R) { return (uint64_t)r.sequences * kv_heads * ((pairs + 4 * R - 1) / (4 * R)); };
-  p.R = pairs <= 4 || dp > 192 ? 1 : pairs > 8 && dp <= 128 && waves_of(4) >= 2048 ? 4 : pairs <= 8 || waves_of(2) >= 1024 ? 2 : 1;
+  p.R = pairs <= 4 || dp > 192 ? 1 : pairs > 8 && dp == 128 && waves_of(4) >= 2048 ? 4 : pairs <= 8 || waves_of(2) >= 1024 ? 2 : 1;
   p.tiles = (pairs + 4 * p.R - 1) / (4 * p.R);
   p.units = (uint32_t)most_units(most_len);
   p.waves = 4;
@@ -1386,11 +1386,16 @@ Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint
   const uint64_t waves = waves_of(p.R);
   const size_t partials = (size_t)r.rows * heads * p.units * (2 + dp) * sizeof(float);
   const uint32_t w = std::min(p.units, 8u);
-  if (p.units > 1 && p.units <= 16 && p.R <= 2 && dp <= 128 && waves < 2048) {
+  // A wave for each of the chip's 1,024 SIMDs, and a row's units need no
+  // dealing: 128 8B rows of 2000 positions take 116 us in one piece and 146 as
+  // a workgroup's units; the 512 waves of 64 1B rows of 4000 take 98 in one piece
+  // and 68 split.
+  if (p.units > 1 && p.units <= 16 && p.R <= 2 && dp <= 128 && waves < 1024) {
     p.mode = GROUP;
     p.waves = w;
-  } else if (p.units > 1 && waves < 4096 && partials <= ((size_t)128 << 20)) {
-    // about as many waves as the chip holds: each has its rows' digits to form
+  } else if (p.units > 1 && waves < 1024 && partials <= ((size_t)128 << 20)) {
+    // about four waves a SIMD: each has its rows' digits to form, so not more (11
+    // 8B rows of 6000 positions: 42.8 us; 16 of 8000: 66 us, 74 with half as many)
     p.mode = SPLIT;
     p.per_wave = (uint32_t)std::max<uint64_t>(1, waves * p.units / SPLIT_WAVES);
     p.workspace = partials;
@@ -1556,10 +1561,8 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   if (pl.mode == SPLIT) {
     if (pl.R == 1)
       attn_launch<1, SPLIT>(a, nb, nt, pl.lds, s);
-    else if (pl.R == 2)
-      attn_launch<2, SPLIT>(a, nb, nt, pl.lds, s);
     else
-      attn_launch<4, SPLIT>(a, nb, nt, pl.lds, s);
+      attn_launch<2, SPLIT>(a, nb, nt, pl.lds, s);
     k_attn_join<<<r.sequences * r.most_rows * in.heads, p.dp, 0, s>>>(a);
   } else if (pl.mode == GROUP) {
     if (pl.R == 1)

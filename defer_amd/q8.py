@@ -157,8 +157,7 @@ def quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _need(x.dim() == 2 and x.shape[1] > 0, "x: need [rows, n]")
     rows, n = x.shape
     st = _row_stride(x, "x", dev, x.dtype, x.shape)
-    codes = torch.empty((rows, n), dtype=_I8, device=x.device)
-    scale = torch.empty(rows, dtype=_F32, device=x.device)
+    codes, scale = x.new_empty((rows, n), dtype=_I8), x.new_empty(rows, dtype=_F32)
     _call(dev, _lib().defer_gpu_q8_quantize, ty, x.data_ptr(), st, rows, n, codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
@@ -171,7 +170,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Option
     dev = _gpu_of(x, "x")
     ty = _type(x, "x")
     _need(x.dim() == 2 and x.shape[1] > 0, "x: need [rows, n]")
-    shape, dtype, device = x.shape, x.dtype, x.device
+    shape, dtype = x.shape, x.dtype
     rows, n = shape
     xs = _row_stride(x, "x", dev, dtype, shape)
     wp = _take(weight, "weight", dev, dtype, (n,))
@@ -181,13 +180,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Option
         rs = _row_stride(residual, "residual", dev, dtype, shape)
         rp = residual.data_ptr()
         if out is None:
-            z = torch.empty((rows, n), dtype=dtype, device=device)
+            z = x.new_empty((rows, n))
             zp, zs = z.data_ptr(), n
     if out is not None:
         zs = _row_stride(z, "out", dev, dtype, shape)
         zp = z.data_ptr()
-    codes = torch.empty((rows, n), dtype=_I8, device=device)
-    scale = torch.empty(rows, dtype=_F32, device=device)
+    codes, scale = x.new_empty((rows, n), dtype=_I8), x.new_empty(rows, dtype=_F32)
     _call(dev, _lib().defer_gpu_q8_rms_norm, ty, x.data_ptr(), xs, rp, rs, wp, eps, rows, n, zp, zs,
           codes.data_ptr(), scale.data_ptr())
     return z, codes, scale
@@ -206,7 +204,7 @@ def linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     xs = _row_stride(x, "x", dev, _I8, x.shape)
     ws = _row_stride(w, "w", dev, _I8, (m, k))
     xp, wp = _take(x_scale, "x_scale", dev, _F32, (rows,)), _take(w_scale, "w_scale", dev, _F32, (m,))
-    y = torch.empty((rows, m), dtype=dtype, device=x.device)
+    y = x_scale.new_empty((rows, m), dtype=dtype)
     _call(dev, _lib().defer_gpu_q8_linear, x.data_ptr(), xs, xp, w.data_ptr(), ws, wp, rows, m, k, ty, y.data_ptr(), m)
     return y
 
@@ -265,8 +263,8 @@ def kv_read(pages: Pages, kv_len: torch.Tensor, row_start: Optional[torch.Tensor
     _need(ty is not None, f"dtype: float32, bfloat16 or float16, not {dtype}")
     cp = _pages(pages, head_dim, dev)
     cr = _rows(pages, kv_len, row_start, rows, most_rows, dev)
-    k = torch.empty((rows, cp.heads, head_dim), dtype=dtype, device=kv_len.device)
-    v = torch.empty((rows, cp.heads, head_dim), dtype=dtype, device=kv_len.device)
+    k = kv_len.new_empty((rows, cp.heads, head_dim), dtype=dtype)
+    v = torch.empty_like(k)
     _call(dev, _lib().defer_gpu_q8_kv_read, cp, cr, ty, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -301,12 +299,12 @@ def attention(q: torch.Tensor, pages: Pages, kv_len: torch.Tensor, row_start: Op
         hs, hp = _row_stride(hidden, "hidden", dev, hidden.dtype, (pages.table.shape[0], hn)), hidden.data_ptr()
     clear = out is None
     if clear:
-        out, os_ = torch.empty(shape, dtype=dtype, device=q.device), heads * hd
+        out, os_ = q.new_empty(shape), heads * hd
     else:
         os_ = _row_stride(out, "out", dev, dtype, shape)
     L = _lib()
     need = L.defer_gpu_q8_attention_workspace(cp, cr, heads, most_len)
-    ws = torch.empty(need, dtype=_U8, device=q.device) if need else None
+    ws = q.new_empty(need, dtype=_U8) if need else None
     _call(dev, L.defer_gpu_q8_attention, cp, cr, ty, q.data_ptr(), qs, heads, most_len,
           hd ** -0.5 if scale is None else scale, hp, hs, hn, out.data_ptr(), os_, clear,
           None if ws is None else ws.data_ptr(), need)
