@@ -19,6 +19,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int WAVE = 64;
+constexpr uint32_t MAX_THREADS = 0xffffffffu;  // of a launch in one dimension
 constexpr double TINY = 0x1p-100;  // rows with a smaller maximum are held as zeros
 
 // ------------------------------------------------------------- value types
@@ -157,8 +158,11 @@ struct RowSum {
   }
 };
 
-template <class T, bool NORM>
-__global__ __launch_bounds__(256) void k_rows(NormArgs a) {
+// Threads take 16 bytes of values in turn, as k_rows_vec's do, so that the sum
+// of squares has the same order in both.
+template <class T, bool NORM, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void k_rows(NormArgs a) {
+  constexpr uint32_t V = 16 / sizeof(T);
   const size_t row = blockIdx.x;
   const uint32_t n = a.n;
   const T* x = static_cast<const T*>(a.x) + row * a.xs;
@@ -167,7 +171,10 @@ __global__ __launch_bounds__(256) void k_rows(NormArgs a) {
   T* z = a.z ? static_cast<T*>(a.z) + row * a.zs : nullptr;
   auto value = [&](uint32_t i) { return NORM && r ? (T)((float)x[i] + (float)r[i]) : x[i]; };
   RowSum s;
-  for (uint32_t i = threadIdx.x; i < n; i += 256) s.add<NORM>((float)value(i), NORM ? (float)w[i] : 1.0f);
+  for (uint64_t i0 = V * threadIdx.x; i0 < n; i0 += V * BLOCK)
+#pragma unroll
+    for (uint32_t e = 0; e < V; ++e)
+      if (i0 + e < n) s.add<NORM>((float)value((uint32_t)i0 + e), NORM ? (float)w[i0 + e] : 1.0f);
   s.join();
   const double inv = NORM ? 1.0 / sqrt(s.ss / n + (double)a.eps) : 1.0;
   const float scale = scale_of(s.top * inv, isnan(s.bad));
@@ -175,17 +182,15 @@ __global__ __launch_bounds__(256) void k_rows(NormArgs a) {
   const double f = NORM && scale > 0.0f ? inv / (double)scale : 0.0;
   const Coder code(scale);
   int8_t* c = a.codes + row * (size_t)n;
-  for (uint32_t i = threadIdx.x; i < n; i += 256) {
-    const T v = value(i);
+  for (uint64_t i = threadIdx.x; i < n; i += BLOCK) {
+    const T v = value((uint32_t)i);
     c[i] = (int8_t)(NORM ? (f > 0.0 ? (int)rint((double)(float)v * (double)(float)w[i] * f) : 0) : code((float)v));
     if (NORM && z) z[i] = v;
   }
 }
 
 // The same where every row is a multiple of 16 bytes apart and long: 16-byte
-// loads, and the row stays in registers between its two passes. The sum of
-// squares goes by thread in another order than k_rows': which of the two runs
-// depends on n, the strides and the addresses only.
+// loads, and the row stays in registers between its two passes.
 template <class T, bool NORM, int BLOCK, int C>
 __global__ __launch_bounds__(BLOCK) void k_rows_vec(NormArgs a) {
   constexpr int V = 16 / sizeof(T);
@@ -1317,6 +1322,11 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   if (d < a.hd) store_value(a.out, (int64_t)row * a.os + (int64_t)h * a.hd + d, a.type, A * inv);
 }
 
+// Zeros for the rows of a call without sequences.
+__global__ __launch_bounds__(256) void k_zero_rows(void* out, int64_t stride, uint32_t n, uint32_t type) {
+  for (uint32_t i = threadIdx.x; i < n; i += 256) store_value(out, (int64_t)blockIdx.x * stride + i, type, 0.0f);
+}
+
 // ------------------------------------------------------------- launches
 
 int launched() {
@@ -1330,7 +1340,7 @@ int rows_launch_as(const NormArgs& a, uint32_t rows, hipStream_t s) {
   auto fits = [](const void* p, int64_t stride) { return ((uintptr_t)p | (uintptr_t)(stride * (int64_t)sizeof(T))) % 16 == 0; };
   const bool vec = a.n % V == 0 && fits(a.x, a.xs) && fits(a.w, 0) && (!a.r || fits(a.r, a.rs)) && (!a.z || fits(a.z, a.zs)) &&
                    ((uintptr_t)a.codes | a.n) % V == 0;
-  const uint32_t nv = a.n / V;
+  const uint32_t nv = a.n / V;  // threads by n alone: they make the order of the sums
   if (vec && nv <= 256)
     k_rows_vec<T, NORM, 256, 1><<<rows, 256, 0, s>>>(a);
   else if (vec && nv <= 512)
@@ -1339,8 +1349,10 @@ int rows_launch_as(const NormArgs& a, uint32_t rows, hipStream_t s) {
     k_rows_vec<T, NORM, 256, 4><<<rows, 256, 0, s>>>(a);
   else if (vec && nv <= 4096)
     k_rows_vec<T, NORM, 1024, 4><<<rows, 1024, 0, s>>>(a);
+  else if (nv <= 1024)
+    k_rows<T, NORM, 256><<<rows, 256, 0, s>>>(a);
   else
-    k_rows<T, NORM><<<rows, 256, 0, s>>>(a);
+    k_rows<T, NORM, 1024><<<rows, 1024, 0, s>>>(a);
   return launched();
 }
 template <bool NORM>
@@ -1506,7 +1518,13 @@ int kv_write(const Pages& p, const Rows& r, uint32_t type, const void* k, int64_
 }
 
 int kv_read(const Pages& p, const Rows& r, uint32_t type, void* k, void* v, uint32_t head_dim, hipStream_t s) {
-  if (!r.rows || !r.sequences || !r.most_rows) return DEFER_GPU_OK;
+  if (!r.rows) return DEFER_GPU_OK;
+  if (!r.sequences || !r.most_rows) {
+    const uint32_t n = p.heads * head_dim;
+    if (k) k_zero_rows<<<r.rows, 256, 0, s>>>(k, n, n, type);
+    if (v) k_zero_rows<<<r.rows, 256, 0, s>>>(v, n, n, type);
+    return launched();
+  }
   const bool vec = head_dim % 8 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
   const KvArgs a{p, r, k, v, 0, 0, type, head_dim, vec};
   Rows and_one = r;
@@ -1524,7 +1542,11 @@ size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uin
 
 int attention(const Pages& p, const Rows& r, const Attention& in, void* workspace, size_t workspace_bytes,
               hipStream_t s) {
-  if (!r.rows || !r.sequences || !r.most_rows) return DEFER_GPU_OK;
+  if (!r.rows) return DEFER_GPU_OK;
+  if (!r.sequences || !r.most_rows) {
+    if (in.clear) k_zero_rows<<<r.rows, 256, 0, s>>>(in.out, in.out_stride, in.heads * in.head_dim, in.type);
+    return launched();
+  }
   const Plan pl = plan_of(r, in.heads, p.heads, p.dp, in.most_len);
   const size_t need = attention_workspace(r, in.heads, p.heads, in.head_dim, in.most_len);
   if (need && (!workspace || workspace_bytes < need))
@@ -1555,7 +1577,7 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   a.q_vec = in.head_dim % 16 == 0 && ((uintptr_t)in.q | (uintptr_t)(in.q_stride * (int64_t)vs)) % 16 == 0;
   const uint64_t items = (uint64_t)pl.tiles * (pl.mode == SPLIT ? (pl.units + pl.per_wave - 1) / pl.per_wave : 1);
   const uint64_t blocks = (pl.mode == GROUP ? items : (items + 3) / 4) * r.sequences * p.heads;
-  if (blocks > 0x7fffffffu || (uint64_t)r.sequences * r.most_rows * in.heads > 0x7fffffffu)
+  if (blocks * pl.waves * WAVE > MAX_THREADS)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
   const uint32_t nb = (uint32_t)blocks, nt = pl.waves * WAVE;
   if (pl.mode == SPLIT) {
@@ -1597,7 +1619,7 @@ static bool aligned_to(const void* p, size_t n) { return (uintptr_t)p % n == 0; 
 
 static int check_rows_values(uint32_t type, const void* x, int64_t stride, uint32_t rows, uint32_t n, const char* what) {
   Q8_REQUIRE(type <= DEFER_GPU_F16, "value type %u", type);
-  Q8_REQUIRE(n >= 1 && n <= 0x7fffffffu && rows <= 0x7fffffffu, "%s: %u rows of %u values", what, rows, n);
+  Q8_REQUIRE(n >= 1 && n <= 0x7fffffffu && rows <= MAX_THREADS / 1024, "%s: %u rows of %u values", what, rows, n);
   Q8_REQUIRE(rows == 0 || x, "%s is null", what);
   Q8_REQUIRE(rows <= 1 || stride >= (int64_t)n, "%s: rows of %u values %lld apart", what, n, (long long)stride);
   Q8_REQUIRE(aligned_to(x, value_size(type)), "%s is not aligned to its type", what);
@@ -1635,6 +1657,7 @@ extern "C" int defer_gpu_q8_linear(const int8_t* x, int64_t x_stride, const floa
   if (rc) return rc;
   Q8_REQUIRE((rows + 31) / 32 <= 65535, "%u rows: at most 2,097,120 in one call", rows);
   Q8_REQUIRE(rows == 0 || (x && x_scale), "null x");
+  Q8_REQUIRE(m <= MAX_THREADS / 16, "%u channels: at most %u in one call", m, MAX_THREADS / 16);
   Q8_REQUIRE(w && w_scale, "null w");
   Q8_REQUIRE(rows <= 1 || x_stride >= (int64_t)k, "x: rows of %u codes %lld apart", k, (long long)x_stride);
   Q8_REQUIRE(m <= 1 || w_stride >= (int64_t)k, "w: rows of %u codes %lld apart", k, (long long)w_stride);
@@ -1647,7 +1670,7 @@ static int check_pages(const defer_gpu_q8_pages* p, const defer_gpu_q8_rows* r, 
   Q8_REQUIRE(p->heads >= 1 && p->heads <= 65535, "%u cache heads", p->heads);
   Q8_REQUIRE(p->pages <= 0x7fffffffu && p->table_width <= 0x7fffffffu / PAGE, "%u pages, %u a sequence", p->pages,
              p->table_width);
-  Q8_REQUIRE(r->rows <= 0x7fffffffu && r->sequences <= 0x7fffffffu, "%u rows of %u sequences", r->rows, r->sequences);
+  Q8_REQUIRE(r->rows <= MAX_THREADS / 1024 && r->sequences <= MAX_THREADS / 1024, "%u rows of %u sequences", r->rows, r->sequences);
   Q8_REQUIRE(r->most_rows <= r->rows, "most_rows %u of %u rows", r->most_rows, r->rows);
   *rows = Rows{r->row_start, r->kv_len, r->sequences, r->rows, r->most_rows};
   *pages = Pages{p->keys, p->values, p->key_scale, p->value_scale, p->table, p->pages, p->heads,
@@ -1659,7 +1682,7 @@ static int check_pages(const defer_gpu_q8_pages* p, const defer_gpu_q8_rows* r, 
   Q8_REQUIRE(p->pages == 0 || (p->keys && p->values && p->key_scale && p->value_scale), "null pages");
   Q8_REQUIRE(aligned16(p->keys) && aligned16(p->values) && aligned16(p->key_scale) && aligned16(p->value_scale),
              "pages are not 16-byte aligned");
-  Q8_REQUIRE(((uint64_t)r->sequences + 1) * p->heads * kv_runs(r->most_rows) <= 0x7fffffffu,
+  Q8_REQUIRE(((uint64_t)r->sequences + 1) * p->heads * kv_runs(r->most_rows) <= MAX_THREADS / 256,
              "too many rows for one call");
   return DEFER_GPU_OK;
 }

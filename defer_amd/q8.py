@@ -8,7 +8,8 @@ float32 scale (max / 127); the header says what is rounded where.
 Every call is queued on torch's current stream of its tensors' device, returns
 without waiting and may be captured into a graph. Tensors that the kernels
 cannot take as they are (another device, type or layout) are refused with a
-ValueError, never copied. Values are float32, bfloat16 or float16.
+ValueError, never copied. Values are float32, bfloat16 or float16. There is no
+backward: results carry no gradient.
 """
 from __future__ import annotations
 

@@ -143,6 +143,21 @@ def test_a_row_is_the_same_in_every_call():
             assert torch.equal(zi, z[i:i + 1]) and torch.equal(ci, c[i:i + 1]) and torch.equal(si, s[i:i + 1])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_row_is_the_same_at_every_stride_and_alignment(dtype):
+    for n in (64, 1000, 4096, 9000, 20000):
+        x, r, w = (rnd(*shape, seed=i, dtype=dtype).to(DEV) for i, shape in enumerate([(7, n), (7, n), (n,)]))
+        want = q8.rms_norm(x, w, 1e-5, residual=r)
+        for pad in (1, 3, 16):  # rows an odd distance apart, from an odd address on
+            wide = torch.zeros(7, n + pad, dtype=dtype, device=DEV)
+            wide[:, pad:] = x
+            odd = torch.zeros(n + 1, dtype=dtype, device=DEV)
+            odd[1:] = w
+            for weight in (w, odd[1:]):
+                assert all(torch.equal(a, b) for a, b in zip(q8.rms_norm(wide[:, pad:], weight, 1e-5, residual=r), want))
+            assert all(torch.equal(a, b) for a, b in zip(q8.quantize(wide[:, pad:]), q8.quantize(x)))
+
+
 # ------------------------------------------------------------------ the product
 
 def i8(*shape, seed=0):
@@ -604,6 +619,45 @@ def test_attention_long_rows_are_the_same_split_or_not():
         assert torch.equal(one, out[i:i + 1]), i
     rows = q8.attention(q[:150], pages, i32([n]), starts([150]), 150, n)
     assert torch.equal(rows, out[:150])
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 128), (16, 2, 64), (8, 2, 128)])
+def test_attention_units_of_a_workgroup_are_the_same_in_one_piece(nh, nkv, hd):
+    """Few sequences of 16 units, which share a workgroup, and many."""
+    lens = [2048, 1921, 700]
+    q, pages, out = run_attention(lens, [1, 1, 1], nh, nkv, hd, seed=2)
+    rep = 400
+    many = q8.Pages(*pages[:4], pages.table.repeat(rep, 1))
+    got = q8.attention(q.repeat(rep, 1, 1).to(DEV), many, i32(lens * rep), most_len=2048)
+    assert torch.equal(got, out.repeat(rep, 1, 1))
+
+
+def test_attention_of_a_long_prompt_is_its_rows():
+    n, nh, nkv, hd = 1100, 32, 8, 128
+    pages = make_cache([n], nkv, hd)
+    fill(pages, [n], nkv, hd)
+    q = rnd(n, nh, hd, seed=4).to(DEV)
+    out = q8.attention(q, pages, i32([n]), starts([n]), n, n)
+    for a, b in ((0, 3), (500, 540), (1024, 1025), (n - 1, n)):
+        assert torch.equal(q8.attention(q[a:b], pages, i32([b]), starts([b - a]), b - a, b), out[a:b])
+
+
+def test_rows_of_a_call_without_sequences_are_zeros():
+    pages = make_cache([100], 2, 40)
+    q = rnd(5, 4, 40).to(DEV)
+    none = pages._replace(table=torch.zeros(0, 3, dtype=torch.int32, device=DEV))
+    for p, n, start in ((none, i32([]), i32([0])), (pages, i32([100]), i32([2, 2]))):
+        for dtype in TYPES:
+            junk = torch.full((5, 4, 40), math.nan, dtype=dtype, device=DEV)  # what a fresh output may hold
+            del junk
+            assert not q8.attention(q.to(dtype), p, n, start, 0).any()
+            assert not q8.attention(q.to(dtype), p, n, start, 5).any()
+            for most in (0, 5):
+                k, v = q8.kv_read(p, n, start, 5, 40, most, dtype)
+                assert not k.any() and not v.any()
+        keep = q.clone()
+        q8.attention(q, p, n, start, 0, out=keep)
+        assert torch.equal(keep, q)
 
 
 def test_attention_refuses():

@@ -176,6 +176,20 @@ def test_cache_and_attention_refuse_arguments():
     assert q8._lib().defer_gpu_q8_attention_workspace(None, r, 4, 10) == 0
 
 
+def test_calls_too_large_for_a_launch_are_refused():
+    big = 1 << 22
+    refused("quantize", 0, P, 8, big, 8, P, P, None)
+    refused("rms_norm", 1, P, 8, P, 8, P, 1e-5, big, 8, P, 8, P, P, None)
+    refused("linear", P, 32, P, P, 32, P, 2, 1 << 28, 32, 0, P, 1 << 28, None)
+    refused("linear", P, 32, P, P, 32, P, 2097121, 4, 32, 0, P, 4, None)
+    p, r = _cache(heads=64), _rows(rows=big - 1, most_rows=big - 1)
+    refused("kv_write", p, r, 0, P, 64 * 64, P, 64 * 64, None)
+    refused("kv_read", p, r, 0, P, P, None)
+    refused("attention", p, r, 0, P, 1 << 20, 64, 128, 1.0, None, 0, 0, P, 1 << 20, 0, P, 1 << 20, None)
+    p, r = _cache(heads=1), _rows(rows=big - 1, most_rows=big - 1)
+    refused("attention", p, r, 0, P, 1 << 22, 65535, 128, 1.0, None, 0, 0, P, 1 << 22, 0, P, 1 << 20, None)
+
+
 def test_python_refuses_what_is_not_on_a_gpu():
     x = torch.zeros(2, 64)
     c = torch.zeros(2, 64, dtype=torch.int8)
