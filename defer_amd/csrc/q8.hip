@@ -277,6 +277,11 @@ __device__ __forceinline__ v4i load16(const int8_t* p, uint32_t k0, uint32_t k) 
   return v;
 }
 
+// A sum of code products as the value it stands for. The scales are 2^-107 or
+// more: sum and row scale first, so that no factor is lost below f32's range
+// (the scales' own product would be) where the value is not.
+__device__ __forceinline__ float scaled(int sum, float xs, float ws) { return (float)sum * xs * ws; }
+
 // Few rows: a workgroup owns 16 MT channels and 16 NT rows, its waves share k
 // in steps of 128 codes; a lane's 32 bytes of a step go straight into two
 // matrix instructions. The waves' sums meet in LDS.
@@ -327,7 +332,7 @@ __global__ __launch_bounds__(NW * WAVE) void k_linear_few(LinearArgs a) {
     if (row >= a.rows) continue;
     const float xs = a.xs[row];
     for (int i = 0; i < 4; ++i)
-      if (c0 + i < a.m) store_value(a.y, (int64_t)row * a.yst + c0 + i, a.type, (float)s[i] * (xs * a.ws[c0 + i]));
+      if (c0 + i < a.m) store_value(a.y, (int64_t)row * a.yst + c0 + i, a.type, scaled(s[i], xs, a.ws[c0 + i]));
   }
 }
 
@@ -409,8 +414,8 @@ struct Tile {
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
             const uint32_t c = c0 + wc + 32 * j + l32;
-            const float v0 = (float)acc[i][j][4 * e4 + e] * (xs[e] * ws[j]);
-            const float v1 = (float)acc[i][j][4 * e4 + e + 1] * (xs[e + 1] * ws[j]);
+            const float v0 = scaled(acc[i][j][4 * e4 + e], xs[e], ws[j]);
+            const float v1 = scaled(acc[i][j][4 * e4 + e + 1], xs[e + 1], ws[j]);
             const float got = dpp<0xb1>(odd ? v0 : v1);  // quad_perm 1 0 3 2
             const uint32_t c2 = c - odd;
             if (pairs && mine < a.rows && c2 + 1 < a.m) {

@@ -220,6 +220,21 @@ def test_linear_strides_alignment_and_scales():
         q8.linear(big, xs, wig, ws, dtype=torch.int32)
 
 
+@pytest.mark.parametrize("rows,m", [(1, 40), (33, 100), (130, 200)])
+def test_linear_scales_whose_product_is_below_the_type(rows, m):
+    x, w = i8(rows, 4096, seed=1), i8(m, 4096, seed=2)
+    x[0] = 0
+    for a, b in ((2.0 ** -105, 1.3 * 2.0 ** -30), (1.7 * 2.0 ** -30, 2.0 ** -100), (1e20, 1e19)):
+        xs, ws = torch.full((rows,), a), torch.full((m,), b)
+        y = q8.linear(x.to(DEV), xs.to(DEV), w.to(DEV), ws.to(DEV)).cpu().double()
+        assert not y[0].any()
+        want = (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
+        # the sum to f32 and two products: half a step each, or half the least number of the type
+        far = (y - want).abs() - torch.clamp(3.03 * HALF[torch.float32] * want.abs(), min=2.0 ** -149)
+        fits = want.abs() < 3.4e38
+        assert (far[fits] <= 0).all() and torch.isinf(y[~fits]).all()
+
+
 def test_linear_rows_are_the_same_in_every_call():
     for m, k in ((200, 640), (130, 1000)):
         x, w = i8(300, k, seed=1).to(DEV), i8(m, k, seed=2).to(DEV)
