@@ -120,7 +120,8 @@ struct NormArgs {
 // One workgroup per row: z = x + r, sum z^2, max |z w|, then the codes. The
 // squares and products are formed in 64 bits (24 + 24 bits: the products
 // exactly), so that codes are those of the formula and not of a rounding;
-// memory hides that. Bound by memory: 2048 x 4096 bf16 with residual, 58.7 MB.
+// memory hides that. Bound by memory: 2048 x 4096 bf16 with residual, 58.7 MB in
+// 16.0 us (3.7 TB/s; a large copy moves 4.75); 1 x 576: 2.6 us, all latency.
 struct RowSum {
   double ss = 0.0, top = 0.0;
   float bad = 0.0f;  // NaN once a value is not finite
@@ -190,7 +191,8 @@ __global__ __launch_bounds__(BLOCK) void k_rows(NormArgs a) {
 }
 
 // The same where every row is a multiple of 16 bytes apart and long: 16-byte
-// loads, and the row stays in registers between its two passes.
+// loads, and the row stays in registers between its two passes (2048 x 4096:
+// 34 us through k_rows, 16.0 so).
 template <class T, bool NORM, int BLOCK, int C>
 __global__ __launch_bounds__(BLOCK) void k_rows_vec(NormArgs a) {
   constexpr int V = 16 / sizeof(T);
@@ -284,7 +286,9 @@ __device__ __forceinline__ float scaled(int sum, float xs, float ws) { return (f
 
 // Few rows: a workgroup owns 16 MT channels and 16 NT rows, its waves share k
 // in steps of 128 codes; a lane's 32 bytes of a step go straight into two
-// matrix instructions. The waves' sums meet in LDS.
+// matrix instructions. The waves' sums meet in LDS. Bound by memory, which reads
+// every weight once: 1 x 28672 x 4096 in 22.3 us (5.3 TB/s of the 6.1 that a large
+// read reaches); 1 x 960 x 576 in 3.3 us, latency.
 template <int MT, int NT, int NW, bool ALIGNED>
 __global__ __launch_bounds__(NW * WAVE) void k_linear_few(LinearArgs a) {
   const uint32_t lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, r16 = lane % 16, kg = lane / 16;
@@ -460,7 +464,7 @@ __device__ __forceinline__ bool tile_of_workgroup(uint32_t tiles, uint32_t* id) 
 // loads, which write zeros for what is outside the operand or behind k), two
 // stages ahead or more. They are issued one at a time between the products:
 // in a row they keep a wave from its next product for as long as the memory
-// pipeline takes them (2047 x 28672 x 4096: 320 us so, 269 now: 1,790 Tops/s; the
+// pipeline takes them (2047 x 28672 x 4096: 320 us so, 257 now: 1,870 Tops/s; the
 // matrix cores alone reach 4,100, the library's i8 product of the same sizes
 // 236 us). Wider tiles (256 x 256: 310 us, half the LDS reads but one
 // stage of 64 codes less in flight), and one workgroup per CU that goes on to its
@@ -717,8 +721,9 @@ __device__ __forceinline__ void store8(void* p, int64_t i0, uint32_t d, uint32_t
 // values through LDS into their transposed page, 16 positions (16 bytes) a store.
 // No other workgroup of the call writes these positions of the sequence, and
 // bytes of rows that are not the call's are not touched. (2000 rows of 8 heads of
-// 128 in bf16: 40 us with a wave per row and a whole page per workgroup, 14.6
-// with 16 lanes per row.)
+// 128 in bf16, 12.4 MB: 40 us with a wave per row and a whole page per workgroup,
+// 14.6 with 16 lanes per row, 9.6 with a quarter page. Bound by the latency of
+// one load, a reduction and one store.)
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs a) {
   const uint32_t per = kv_runs(a.r.most_rows);
   const uint32_t g = blockIdx.x % a.p.heads, b = blockIdx.x / a.p.heads % per, seq = blockIdx.x / a.p.heads / per;
@@ -801,8 +806,9 @@ __global__ __launch_bounds__(256) void k_kv_write(KvArgs a) {
   }
 }
 
-// The same runs back: codes times scales. What would be the runs of one more
-// sequence clear the rows of none.
+// The same runs back: codes times scales (5001 rows of 8 heads of 128 to bf16,
+// 31 MB in 10.1 us). What would be the runs of one more sequence clear the rows
+// of none.
 __global__ __launch_bounds__(256) void k_kv_read(KvArgs a) {
   const uint32_t per = kv_runs(a.r.most_rows);
   const uint32_t g = blockIdx.x % a.p.heads, b = blockIdx.x / a.p.heads % per, seq = blockIdx.x / a.p.heads / per;
@@ -934,6 +940,12 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // The next block's keys are on their way once this one's scores are formed, the
 // next values once this one's are used, or with the keys where registers
 // allow (R = 1: few rows, bound by memory).
+//
+// A long cache is bound by memory (11 8B rows of 6000 positions: 140 MB in 34.5
+// us; 512 of 2000: 2.2 GB in 400 us, 5.4 TB/s), a prompt by vector instructions
+// (3500 360M rows: 180 us, 138 of them the vector unit's; a tile and block takes
+// about 190 of them beside 8 matrix products), a short step by its chain of
+// dependent loads (64 1B rows of 385 positions: 10.9 us).
 //
 // DIRECT: a wave goes through all its positions, unit after unit (many rows;
 // the four waves of a workgroup are neighbouring tiles and meet the same codes
@@ -1296,7 +1308,9 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 
 // Joins a row's units in order, as the unsplit kernel does. One workgroup of
 // dp lanes per (row of a sequence, head); a lane holds one unit's maximum and
-// sum, the accumulators of 32 units are on their way at a time.
+// sum, the accumulators of 32 units are on their way at a time. Three dependent
+// reads of what other XCDs wrote: 9.7 us for 11 x 32 heads of 47 units (8.6 MB);
+// 64 units at a time changed nothing.
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   const uint32_t h = blockIdx.x % a.nh, j = blockIdx.x / a.nh % a.r.most_rows, seq = blockIdx.x / a.nh / a.r.most_rows;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
@@ -1495,7 +1509,7 @@ int linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t
   if (!aligned)
     return tiles_of(128, 128) < 32 ? linear_few<1, 2, 8>(a, aligned, s) : linear_tile_odd<2, 2>(a, s);
   // The tile whose rounds over the chip take least: us a round and a stage as
-  // measured (2047 x 28672 x 4096: 269 us in 256 x 128, 350 in 128 x 128; 1000
+  // measured (2047 x 28672 x 4096: 257 us in 256 x 128, 350 in 128 x 128; 1000
   // x 4096 x 4096: 31.1, 22.9, 32.1 in 64 x 64; 500 x 4096 x 4096: 29.7, 19.0,
   // 17.7). Two 64 x 64 tiles share a CU.
   const double stages = (k + 127) / 128;
