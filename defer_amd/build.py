@@ -8,6 +8,7 @@
                        its checker) that the GPU tests run.
 * tests/probe/libexact_probe.so -- test-only entry points into the exact
                        sampler's device code (tests/test_exact.py).
+* _q8_torch.so      -- the 8-bit operators on torch tensors (C++, torch's headers).
 * libdefer_host.so  -- the C++ host side (session, WAL, checkpoint, ChaCha8,
                        SHA-256, safetensors) of include/defer_host.h.
 
@@ -116,8 +117,29 @@ def build_host() -> str:
     return out
 
 
+def build_torch() -> str:
+    """defer_amd/_q8_torch.so: the 8-bit operators on torch tensors, C++ against
+    the installed torch."""
+    import sysconfig
+
+    import torch
+
+    t = os.path.dirname(torch.__file__)
+    out = os.path.join(PKG, "_q8_torch.so")
+    tmp = out + ".tmp"
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-isystem", os.path.join(t, "include"),
+          "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+          "-I", sysconfig.get_paths()["include"], "-o", tmp, os.path.join(CSRC, "q8_torch.cpp"),
+          "-L", os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl"])
+    os.replace(tmp, out)
+    return out
+
+
 def build_all() -> None:
     build_gpu()
+    build_torch()
     if os.path.isdir(os.path.join(CSRC, "host")):
         build_host()
     build_c_abi_test()
@@ -127,5 +149,5 @@ def build_all() -> None:
 if __name__ == "__main__":
     which = sys.argv[1:] or ["all"]
     for w in which:
-        {"gpu": build_gpu, "host": build_host, "c_abi": build_c_abi_test, "probe": build_probe,
+        {"gpu": build_gpu, "torch": build_torch, "host": build_host, "c_abi": build_c_abi_test, "probe": build_probe,
          "all": build_all}[w]()

@@ -2,6 +2,7 @@
 64-bit implementations on the CPU: types, sizes, strides, ragged rows, masks
 that leave nothing, values that are not finite, pages that are not there."""
 import math
+import sys
 
 import numpy as np
 import pytest
@@ -787,6 +788,71 @@ def test_a_layer_in_a_graph_and_on_streams():
                 outs[i] = eager(caches[i], x * (1.0 if i == 0 else 0.5))
     torch.cuda.synchronize()
     assert torch.equal(outs[0][1], want[1.0][1]) and torch.equal(outs[1][1], want[0.5][1])
+
+
+def test_calls_return_the_callers_tensors_and_keep_nothing():
+    nh, nkv, hd = 4, 2, 64
+    lens = [3000, 40]
+    pages = make_cache(lens, nkv, hd)
+    k, v = (t.to(DEV) for t in fill(pages, lens, nkv, hd))
+    x, w, q = rnd(2, 64).to(DEV), rnd(64).to(DEV), rnd(2, nh, hd).to(DEV)
+    n, start = i32(lens), starts([1, 1])
+    refs = (x, w, q, n, start, k, v, *pages)
+
+    def calls():
+        z, c, s = q8.rms_norm(x, w, 1e-5)
+        assert z is x
+        into = torch.empty_like(x)
+        assert q8.rms_norm(x, w, 1e-5, residual=x, out=into)[0] is into
+        out = torch.empty_like(q)
+        assert q8.attention(q, pages, n, start, 1, out=out) is out
+        q8.attention(q, pages, n, start, 1, 3000)
+        q8.linear(c, s, c, s, torch.float16)
+        q8.kv_write(pages, k, v, n, starts(lens), 3000)
+        q8.kv_read(pages, n, start, 2, hd, 1)
+        for bad in (lambda: q8.attention(q, pages, n, start, 7), lambda: q8.attention(q, pages, n, start, 1, 1 << 31),
+                    lambda: q8.attention(q, pages, n, start, 1, hidden=x), lambda: q8.kv_read(pages, n, start, 2, 65),
+                    lambda: q8.kv_read(pages, n, start, -1, hd), lambda: q8.kv_read(pages[:4], n, start, 2, hd),
+                    lambda: q8.linear(c, s, c, s, torch.int8), lambda: q8.linear(c, s, c, s, "float32")):
+            with pytest.raises(ValueError):
+                bad()
+        with pytest.raises(TypeError):
+            q8.attention(q, pages, n, start, 1.5)
+        with pytest.raises(G.DeferGpuError):
+            q8.rms_norm(x, w, float("nan"))
+
+    calls()
+    torch.cuda.synchronize()
+    held, counts = torch.cuda.memory_allocated(), [sys.getrefcount(t) for t in refs]
+    for _ in range(20):
+        calls()
+    assert torch.cuda.memory_allocated() == held and [sys.getrefcount(t) for t in refs] == counts
+
+
+def test_calls_from_two_threads_on_two_streams():
+    import threading
+
+    x, w = rnd(64, 512, seed=1).to(DEV), rnd(300, 512, seed=2).to(DEV)
+    wc, ws = q8.quantize(w)
+    want = q8.linear(*q8.quantize(x), wc, ws)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(stream):
+        with torch.cuda.stream(stream):
+            for _ in range(200):
+                y = q8.linear(*q8.quantize(x), wc, ws)
+            stream.synchronize()
+            if not torch.equal(y, want):
+                bad.append(stream)
+
+    ts = [threading.Thread(target=work, args=(torch.cuda.Stream(),)) for _ in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
+
 
 
 def test_large_offsets():

@@ -5,6 +5,7 @@ import ctypes
 import os
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
@@ -201,3 +202,22 @@ def test_python_refuses_what_is_not_on_a_gpu():
                  lambda: q8.attention(x[:1, None], pages, n), lambda: q8.quantize([1.0])):
         with pytest.raises(ValueError):
             call()
+
+
+def test_python_refuses_what_is_no_tensor():
+    x, n = torch.zeros(2, 64), torch.ones(1, dtype=torch.int32)
+    pages = q8.Pages(*[None] * 5)
+    for bad in (None, 3, "x", [1.0], np.zeros((2, 64))):
+        for call in (lambda: q8.quantize(bad), lambda: q8.rms_norm(bad, x[0], 1e-5), lambda: q8.linear(bad, x, x, x),
+                     lambda: q8.kv_write(pages, bad, x, n), lambda: q8.kv_read(pages, bad, n, 1, 64),
+                     lambda: q8.attention(bad, pages, n)):
+            with pytest.raises(ValueError):
+                call()
+    for call in (lambda: q8.linear(x, x, x), lambda: q8._native().quantize(), lambda: q8._native().attention(1)):
+        with pytest.raises(TypeError):
+            call()
+    for bad in ("no such library", q8.__file__):
+        with pytest.raises(ImportError):
+            q8._native().bind(bad, None, None, None)
+    with pytest.raises(ValueError):
+        q8.quantize(x)  # what was bound stays bound
