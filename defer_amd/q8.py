@@ -21,8 +21,6 @@ import torch
 from .gpu import _check, lib
 
 PAGE = 64
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_I8, _I32, _F32, _U8 = torch.int8, torch.int32, torch.float32, torch.uint8
 
 
 class Pages(NamedTuple):
@@ -44,10 +42,10 @@ def new_pages(pages: int, heads: int, head_dim: int, table: torch.Tensor) -> Pag
     """An empty pool on the table's device."""
     d = padded(head_dim)
     dev = table.device
-    return Pages(torch.zeros(pages, heads, PAGE, d, dtype=_I8, device=dev),
-                 torch.zeros(pages, heads, d, PAGE, dtype=_I8, device=dev),
-                 torch.zeros(pages, heads, PAGE, dtype=_F32, device=dev),
-                 torch.zeros(pages, heads, PAGE, dtype=_F32, device=dev), table)
+    return Pages(torch.zeros(pages, heads, PAGE, d, dtype=torch.int8, device=dev),
+                 torch.zeros(pages, heads, d, PAGE, dtype=torch.int8, device=dev),
+                 torch.zeros(pages, heads, PAGE, dtype=torch.float32, device=dev),
+                 torch.zeros(pages, heads, PAGE, dtype=torch.float32, device=dev), table)
 
 
 def padded(head_dim: int) -> int:
