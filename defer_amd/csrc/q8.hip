@@ -717,13 +717,14 @@ __device__ __forceinline__ void store8(void* p, int64_t i0, uint32_t d, uint32_t
 }
 
 // A workgroup owns the new rows of 16 positions of a page, one head. 16 lanes
-// take a row, 8 values each: maximum, scale, codes; keys go out as they are,
+// take a row's key or value, 8 values each: maximum, scale, codes; keys go out as they are,
 // values through LDS into their transposed page, 16 positions (16 bytes) a store.
 // No other workgroup of the call writes these positions of the sequence, and
 // bytes of rows that are not the call's are not touched. (2000 rows of 8 heads of
 // 128 in bf16, 12.4 MB: 40 us with a wave per row and a whole page per workgroup,
-// 14.6 with 16 lanes per row, 9.6 with a quarter page. Bound by the latency of
-// one load, a reduction and one store.)
+// 14.6 with 16 lanes per row, 9.4 with a quarter page. Bound by the latency of
+// one load, a reduction and one store; so a row's key and value go side by side:
+// 64 sequences' single rows 4.8 us, 6.5 one after the other.)
 __global__ __launch_bounds__(256) void k_kv_write(KvArgs a) {
   const uint32_t per = kv_runs(a.r.most_rows);
   const uint32_t g = blockIdx.x % a.p.heads, b = blockIdx.x / a.p.heads % per, seq = blockIdx.x / a.p.heads / per;
@@ -745,40 +746,36 @@ __global__ __launch_bounds__(256) void k_kv_write(KvArgs a) {
   const int64_t row0 = sp.start + (block * PAGE - sp.pos(0));  // the row of the block's first position
   __shared__ __align__(16) int8_t tile[KV_RUN * KV_ROW];
   const int tr = (int)(run * KV_RUN - block * PAGE);  // the run's first place in its page
-  for (int at = a0 + (int)quad; at < a1; at += (int)quads) {
+  // every other 16 lanes a key, those between its value
+  const bool which = quad % 2;
+  for (int at = a0 + (int)quad / 2; at < a1; at += (int)quads / 2) {
     const int64_t row = row0 + at;
-    float y[2][2][8];
+    float y[2][8], top = 0.0f, bad = 0.0f;
 #pragma unroll
-    for (int which = 0; which < 2; ++which)
+    for (uint32_t h = 0; h < 2; ++h)
+      if (h == 0 || hd > 128)
+        load8(which ? a.v : a.k, row * (which ? a.vs : a.ks) + (int64_t)g * hd, 128 * h + 8 * n16, hd, a.type, a.vec, y[h]);
 #pragma unroll
-      for (uint32_t h = 0; h < 2; ++h)
-        if (h == 0 || hd > 128)
-          load8(which ? a.v : a.k, row * (which ? a.vs : a.ks) + (int64_t)g * hd, 128 * h + 8 * n16, hd, a.type, a.vec, y[which][h]);
+    for (uint32_t h = 0; h < 2; ++h)
+      if (h == 0 || hd > 128)
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      float top = 0.0f, bad = 0.0f;
+        for (int e = 0; e < 8; ++e) {
+          top = fmaxf(top, fabsf(y[h][e]));
+          bad = fmaf(y[h][e], 0.0f, bad);
+        }
+    const float scale = scale_of(row_max(top), isnan(row_sum(bad)));
+    const Coder code(scale);
 #pragma unroll
-      for (uint32_t h = 0; h < 2; ++h)
-        if (h == 0 || hd > 128)
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t d = 128 * h + 8 * n16;
+      if (d >= hd) continue;
+      uint64_t c = 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            top = fmaxf(top, fabsf(y[which][h][e]));
-            bad = fmaf(y[which][h][e], 0.0f, bad);
-          }
-      const float scale = scale_of(row_max(top), isnan(row_sum(bad)));
-      const Coder code(scale);
-#pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t d = 128 * h + 8 * n16;
-        if (d >= hd) continue;
-        uint64_t c = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c |= (uint64_t)(uint8_t)code(y[which][h][e]) << (8 * e);
-        // a page's row is a multiple of 64 codes: those behind hd are zeros
-        *reinterpret_cast<uint64_t*>(which ? tile + (at - tr) * KV_ROW + d : kc + at * a.p.dp + d) = c;
-      }
-      if (n16 == 0) (which ? q.value_scale : q.key_scale)[hp * PAGE + at] = scale;
+      for (int e = 0; e < 8; ++e) c |= (uint64_t)(uint8_t)code(y[h][e]) << (8 * e);
+      // a page's row is a multiple of 64 codes: those behind hd are zeros
+      *reinterpret_cast<uint64_t*>(which ? tile + (at - tr) * KV_ROW + d : kc + at * a.p.dp + d) = c;
     }
+    if (n16 == 0) (which ? q.value_scale : q.key_scale)[hp * PAGE + at] = scale;
   }
   __syncthreads();
   if (a1 - a0 < KV_RUN) {  // some of the run: byte by byte
@@ -1532,7 +1529,7 @@ int kv_write(const Pages& p, const Rows& r, uint32_t type, const void* k, int64_
   const int64_t vs = type == DEFER_GPU_F32 ? 4 : 2;
   const bool vec = head_dim % 8 == 0 && ((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * vs) | (uintptr_t)(v_stride * vs)) % 16 == 0;
   const KvArgs a{p, r, const_cast<void*>(k), const_cast<void*>(v), k_stride, v_stride, type, head_dim, vec};
-  k_kv_write<<<kv_grid(p, r), r.most_rows <= 4 ? 64 : 256, 0, s>>>(a);
+  k_kv_write<<<kv_grid(p, r), r.most_rows <= 2 ? 64 : 256, 0, s>>>(a);
   return launched();
 }
 
