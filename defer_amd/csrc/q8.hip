@@ -283,6 +283,14 @@ __device__ __forceinline__ v4i load16(const int8_t* p, uint32_t k0, uint32_t k) 
 // more: sum and row scale first, so that no factor is lost below f32's range
 // (the scales' own product would be) where the value is not.
 __device__ __forceinline__ float scaled(int sum, float xs, float ws) { return (float)sum * xs * ws; }
+// ... of a row whose scale may be over 2^64, where the sum would pass f32's range
+// above it and the value does not: the scale is taken 2^64 times smaller until
+// the channel's is in. Powers of two are exact: in range the bits are the same.
+__device__ __forceinline__ bool large_scale(float xs) { return xs > 0x1p64f; }
+__device__ __forceinline__ float scaled_any(int sum, float xs, float ws) {
+  const bool large = large_scale(xs);
+  return scaled(sum, large ? xs * 0x1p-64f : xs, ws) * (large ? 0x1p64f : 1.0f);
+}
 
 // Few rows: a workgroup owns 16 MT channels and 16 NT rows, its waves share k
 // in steps of 128 codes; a lane's 32 bytes of a step go straight into two
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(NW * WAVE) void k_linear_few(LinearArgs a) {
     if (row >= a.rows) continue;
     const float xs = a.xs[row];
     for (int i = 0; i < 4; ++i)
-      if (c0 + i < a.m) store_value(a.y, (int64_t)row * a.yst + c0 + i, a.type, scaled(s[i], xs, a.ws[c0 + i]));
+      if (c0 + i < a.m) store_value(a.y, (int64_t)row * a.yst + c0 + i, a.type, scaled_any(s[i], xs, a.ws[c0 + i]));
   }
 }
 
@@ -401,8 +409,9 @@ struct Tile {
   // Register e of a product: row 8 (e / 4) + 4 half + e % 4, channel l32. Two
   // neighbouring lanes exchange a register each, so that one stores row e's two
   // channels and the other row e + 1's: half the stores, of twice the bytes.
-  template <class T>
+  template <class T, bool LARGE>
   __device__ __forceinline__ void store_as(const LinearArgs& a, const v16i (*acc)[TN], const float* xsl, const float* ws) const {
+    auto value = [](int sum, float x, float w) { return LARGE ? scaled_any(sum, x, w) : scaled(sum, x, w); };
     typedef T T2 __attribute__((ext_vector_type(2)));
     T* y = static_cast<T*>(a.y);
     const bool odd = lane & 1, pairs = (a.yst % 2 | (uintptr_t)a.y % sizeof(T2)) == 0;
@@ -418,8 +427,8 @@ struct Tile {
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
             const uint32_t c = c0 + wc + 32 * j + l32;
-            const float v0 = scaled(acc[i][j][4 * e4 + e], xs[e], ws[j]);
-            const float v1 = scaled(acc[i][j][4 * e4 + e + 1], xs[e + 1], ws[j]);
+            const float v0 = value(acc[i][j][4 * e4 + e], xs[e], ws[j]);
+            const float v1 = value(acc[i][j][4 * e4 + e + 1], xs[e + 1], ws[j]);
             const float got = dpp<0xb1>(odd ? v0 : v1);  // quad_perm 1 0 3 2
             const uint32_t c2 = c - odd;
             if (pairs && mine < a.rows && c2 + 1 < a.m) {
@@ -434,13 +443,23 @@ struct Tile {
       }
     }
   }
-  __device__ __forceinline__ void store(const LinearArgs& a, const v16i (*acc)[TN], const float* xsl, const float* ws) const {
+  // (Apart: the factors in every value are 8 of 260 us at 2047 x 28672 x 4096.)
+  template <bool LARGE>
+  __device__ __forceinline__ void store_typed(const LinearArgs& a, const v16i (*acc)[TN], const float* xsl, const float* ws) const {
     if (a.type == DEFER_GPU_F32)
-      store_as<float>(a, acc, xsl, ws);
+      store_as<float, LARGE>(a, acc, xsl, ws);
     else if (a.type == DEFER_GPU_BF16)
-      store_as<__bf16>(a, acc, xsl, ws);
+      store_as<__bf16, LARGE>(a, acc, xsl, ws);
     else
-      store_as<_Float16>(a, acc, xsl, ws);
+      store_as<_Float16, LARGE>(a, acc, xsl, ws);
+  }
+  __device__ __forceinline__ void store(const LinearArgs& a, const v16i (*acc)[TN], const float* xsl, const float* ws) const {
+    bool large = false;
+    for (int i = 0; i < TM; ++i) large = large || large_scale(xsl[wr + 32 * i + l32]);
+    if (__any(large))
+      store_typed<true>(a, acc, xsl, ws);
+    else
+      store_typed<false>(a, acc, xsl, ws);
   }
   // The tile's scales: this lane's channels', and a row's for each thread to
   // leave in LDS (before a barrier).
