@@ -920,6 +920,10 @@ __device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x0080
 __device__ __forceinline__ float undigit(v4i d) {
   return fmaf((float)((d[3] << 8) + d[2]), 65536.0f, (float)((d[1] << 8) + d[0]));
 }
+// ... times 2^-45, so that it is less than 1 and times any key scale in range.
+__device__ __forceinline__ float undigit_small(v4i d) {
+  return fmaf((float)((d[3] << 8) + d[2]), 0x1p-29f, (float)((d[1] << 8) + d[0]) * 0x1p-45f);
+}
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A running softmax: maximum (as an exponent of 2), sum, accumulators. The
@@ -952,6 +956,13 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // scales are held in 30 bits relative to the largest such product: so one token
 // that takes nearly all of a softmax and has small values leaves the others'
 // contributions their accuracy.
+//
+// A score is digit sum * key scale * the query's factor. The sum counts the
+// query as some 2^30 and the codes as 2^15 more, so that its product with a large
+// key scale would pass f32's range where the score does not, and the factor of a
+// small query would lie below it: 2^45 goes from the sum to the factor, exactly.
+// (For a query over 2^64 the factor would then pass the range: there the products
+// are raised again, in a wave that has one.)
 //
 // The next block's keys are on their way once this one's scores are formed, the
 // next values once this one's are used, or with the keys where registers
@@ -1039,7 +1050,8 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 
   // the queries' digits; the scores' sign is the scale's, folded into them
   v4i aq[R][KC];
-  float sq[R];
+  float sq[R];  // queries' factors; negative: 2^45 times too small
+  bool any_huge = false;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint32_t pr = pair0 + 4 * r + n16 / 4, j = pr / a.group;
@@ -1081,12 +1093,22 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
     top = fmaxf(top, __shfl_xor(top, 32));
     bad += __shfl_xor(bad, 16);
     bad += __shfl_xor(bad, 32);
-    // top < 2^ex; values of rows under 2^-96 keep fewer digits
-    int ex = 0;
+    const bool tiny = top > 0.0f && top < 0x1p-64f;
+    if (__any(tiny)) {
+      const float lift = tiny ? 0x1p80f : 1.0f;
+      top *= lift;
+#pragma unroll
+      for (int kk = 0; kk < KC; ++kk)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[kk][e] *= lift;
+    }
+    int ex = 0;  // top < 2^ex
     (void)frexpf(top, &ex);
-    ex = top > 0.0f ? max(ex, -96) : 0;
+    ex = top > 0.0f ? ex : 0;
     const float up = isnan(bad) ? 0.0f : a.scale2 < 0.0f ? -ldexpf(1.0f, 30 - ex) : ldexpf(1.0f, 30 - ex);
-    const float s = isnan(bad) ? __builtin_nanf("") : ldexpf(1.0f, ex - 30) * fabsf(a.scale2);
+    const bool huge = ex > 64;
+    const float s = isnan(bad) ? __builtin_nanf("") : huge ? ldexpf(-1.0f, ex - 30) * fabsf(a.scale2) : ldexpf(1.0f, ex - (tiny ? 80 : 0) - 30 + 45) * fabsf(a.scale2);
+    any_huge = any_huge || __any(huge);
     const uint32_t dg = n16 % 4, sel = dg | (4 + dg) << 8;
 #pragma unroll
     for (int kk = 0; kk < KC; ++kk)
@@ -1162,16 +1184,20 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           see[j] = WHOLE || (tb + j <= ps[r] && !hide[j]);
-          const float x = undigit(d[j]) * ks[j];
+          const float x = undigit_small(d[j]) * ks[j];
           s[j] = see[j] ? x : -INFINITY;
+        }
+        if (any_huge) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[j] *= sq[r] < 0.0f ? 0x1p45f : 1.0f;
         }
         const float top = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
         const bool none = !WHOLE && top == -INFINITY;
-        const float m0 = none ? 0.0f : top * sq[r];
+        const float m0 = none ? 0.0f : top * fabsf(sq[r]);
         float lp = vbad;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float p = exp2_of(fmaf(s[j], sq[r], -m0));
+          float p = exp2_of(fmaf(s[j], fabsf(sq[r]), -m0));
           if (!WHOLE) {
             p = see[j] ? p : 0.0f;
             lp += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;

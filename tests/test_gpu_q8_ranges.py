@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from defer_amd import q8
+from test_gpu_q8 import i32, make_cache, ref_attention, rnd, starts, tolerance, values
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +66,59 @@ def test_linear_large_row_scales_in_every_type(rows, m, k, dtype):
     assert ((y.cpu().double() - want).abs() <= tol).all()
     for i in range(0, rows, 7):
         assert torch.equal(q8.linear(x[i:i + 1].to(DEV), xs[i:i + 1].to(DEV), w.to(DEV), ws.to(DEV), dtype=dtype), y[i:i + 1])
+
+
+# ------------------------------------------------------------------ attention
+
+def attend(lens, counts, nh, nkv, hd, dtype, kscale, qscale, hidden=None, loud=None):
+    """Rows of each sequence's end against the formula; the queries, the pages and what came out."""
+    pages = make_cache(lens, nkv, hd, seed=hd)
+    k = (rnd(sum(lens), nkv, hd, seed=1) * kscale).to(dtype)
+    if loud is not None:  # a few keys of their own size
+        at, size = loud
+        k[at] = (rnd(len(at), nkv, hd, seed=4) * size).to(dtype)
+    v = rnd(sum(lens), nkv, hd, seed=2, dtype=dtype)
+    q = (rnd(sum(counts), nh, hd, seed=3) * qscale).to(dtype)
+    q8.kv_write(pages, k.to(DEV), v.to(DEV), i32(lens), starts(lens), max(lens))
+    out = q8.attention(q.to(DEV), pages, i32(lens), starts(counts), max(counts), max(lens),
+                       hidden=None if hidden is None else hidden.to(DEV))
+    kd, vd, at = values(k), values(v), 0
+    for i, (n, c) in enumerate(zip(lens, counts)):
+        k0 = sum(lens[:i])
+        want, big, mass = ref_attention(q[at:at + c], kd[k0:k0 + n], vd[k0:k0 + n], list(range(n - c, n)),
+                                        None if hidden is None else hidden[i], hd ** -0.5)
+        got = out[at:at + c].cpu().double()
+        assert torch.isfinite(got).all()
+        far = (got - want).abs() - tolerance(dtype, n, big, mass, want)
+        assert (far <= 0).all(), (i, float(far.max()))
+        at += c
+    return q, pages, out
+
+
+# one row in one piece, in a workgroup's units, split over workgroups; a prompt
+SPREAD = [([60, 100], [1, 1]), ([777], [1]), ([3000], [1]), ([200, 70], [200, 33])]
+# keys' size, queries' size: products of some 1 to 10, the ends of f32's and bf16's range
+FAR = [(1e32, 1e-32), (5e37, 2e-38), (1e26, 1e-25), (1e-26, 1e26), (2e-30, 1e30), (1.0, 1e-40), (1e-20, 1e-20)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nh,nkv,hd", [(6, 2, 64), (16, 2, 128), (3, 1, 40)])
+@pytest.mark.parametrize("lens,counts", SPREAD)
+def test_attention_of_large_and_small_keys(lens, counts, nh, nkv, hd, dtype):
+    for kscale, qscale in FAR:
+        attend(lens, counts, nh, nkv, hd, dtype, kscale, qscale)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(6, 2, 64), (16, 2, 128), (2, 1, 256)])
+def test_attention_of_a_few_large_keys_among_small_ones(nh, nkv, hd):
+    """Rows before and behind them, hidden or not; each the same bits in any call."""
+    n, at = 300, torch.tensor([3, 70, 131, 255])
+    shown = torch.zeros(1, n, dtype=torch.bool)
+    shown[0, 131] = True
+    for hidden in (None, shown):
+        for size, qscale in ((1e33, 1e-33), (1e37, 1e-36)):
+            q, pages, out = attend([n], [n], nh, nkv, hd, torch.float32, 1e25, qscale, hidden, (at, size))
+            h = None if hidden is None else hidden.to(DEV)
+            for a, b in ((0, 3), (3, 4), (60, 80), (130, 133), (299, 300)):
+                got = q8.attention(q[a:b].to(DEV), pages, i32([b]), starts([b - a]), b - a, b, hidden=h)
+                assert torch.equal(got, out[a:b]), (a, b)
