@@ -122,3 +122,60 @@ def test_attention_of_a_few_large_keys_among_small_ones(nh, nkv, hd):
             for a, b in ((0, 3), (3, 4), (60, 80), (130, 133), (299, 300)):
                 got = q8.attention(q[a:b].to(DEV), pages, i32([b]), starts([b - a]), b - a, b, hidden=h)
                 assert torch.equal(got, out[a:b]), (a, b)
+
+
+def test_attention_of_queries_of_every_size_in_a_tile():
+    """One row large, one small, one not finite, one of zeros: each as if it were alone."""
+    n, nh, nkv, hd = 130, 8, 2, 64
+    pages = make_cache([n], nkv, hd)
+    k, v = rnd(n, nkv, hd, seed=1), rnd(n, nkv, hd, seed=2)
+    q8.kv_write(pages, k.to(DEV), v.to(DEV), i32([n]), starts([n]), n)
+    q = rnd(12, nh, hd, seed=3)
+    for i, size in enumerate((1e30, 1e-30, 1e37, 1e-38, 1e20, 1e-20, 2.0 ** 64, 2.0 ** -64, 1.0, 0.0)):
+        q[i] *= size
+    q[10, 0, 0], q[11, 3, 5] = float("inf"), float("nan")
+    out = q8.attention(q.to(DEV), pages, i32([n]), starts([12]), 12, n)
+    for i in range(12):
+        one = q8.attention(q[i:i + 1].to(DEV), pages, i32([n - 11 + i]))
+        assert torch.equal(torch.isnan(one), torch.isnan(out[i:i + 1]))
+        assert torch.equal(one.nan_to_num(), out[i:i + 1].nan_to_num()), i
+    assert torch.isnan(out[10, 0]).all() and torch.isnan(out[11, 3]).all() and torch.isfinite(out[:10]).all()
+    assert torch.isfinite(out[10, 1:]).all() and torch.isfinite(out[11, :3]).all()
+    kd, vd = values(k), values(v)
+    for i in (1, 3, 5, 7, 8, 9):
+        want, big, mass = ref_attention(q[i:i + 1], kd[:n - 11 + i], vd[:n - 11 + i], [n - 12 + i], None, hd ** -0.5)
+        assert ((out[i:i + 1].cpu().double() - want).abs() <= tolerance(torch.float32, n, big, mass, want)).all(), i
+
+
+@pytest.mark.parametrize("lens,counts", SPREAD)
+def test_attention_of_scores_too_large_for_a_softmax(lens, counts):
+    """Scores of 1e9 and more: the row's largest one takes all, on any size of either."""
+    nh, nkv, hd = 6, 2, 64
+    for kscale, qscale in ((1.0, 1e10), (1.0, 1e25), (1e15, 1e5), (1e15, 1e20), (1e-15, 1e30)):
+        pages = make_cache(lens, nkv, hd, seed=1)
+        k, v = rnd(sum(lens), nkv, hd, seed=1) * kscale, rnd(sum(lens), nkv, hd, seed=2)
+        q = rnd(sum(counts), nh, hd, seed=3) * qscale
+        q8.kv_write(pages, k.to(DEV), v.to(DEV), i32(lens), starts(lens), max(lens))
+        out = q8.attention(q.to(DEV), pages, i32(lens), starts(counts), max(counts), max(lens)).cpu().double()
+        kd, vd, at, sure = values(k), values(v), 0, 0
+        for i, (n, c) in enumerate(zip(lens, counts)):
+            k0 = sum(lens[:i])
+            for j in range(c):
+                m = n - c + j + 1
+                for h in range(nh):
+                    s = kd[k0:k0 + m, h // 3] @ q[at + j, h].double() * hd ** -0.5
+                    s, order = s.sort(descending=True)
+                    # a score is off by some 10 half steps of the largest, and by 2^-30 of each product's factors
+                    if m == 1 or s[0] - s[1] > 100 + 2.0 ** -18 * s.abs().max():
+                        want = vd[k0 + order[0], h // 3]
+                        assert ((out[at + j, h] - want).abs() <= 2.0 ** -20 * want.abs().max()).all(), (kscale, qscale, i, j, h)
+                        sure += 1
+            at += c
+        assert sure >= 0.9 * sum(counts) * nh
+
+
+@pytest.mark.parametrize("nh,nkv,hd,lens,counts", [(4, 1, 64, [8200], [20]), (8, 2, 128, [8200], [9]), (8, 2, 192, [300, 70], [300, 70]),
+                                                   (6, 3, 192, [700], [2]), (4, 1, 256, [300], [300]), (16, 2, 128, [1100], [1100])])
+def test_attention_at_both_ends_across_units_and_head_sizes(nh, nkv, hd, lens, counts):
+    for kscale, qscale in ((1e32, 1e-32), (1e-26, 1e26)):
+        attend(lens, counts, nh, nkv, hd, torch.float32, kscale, qscale)
