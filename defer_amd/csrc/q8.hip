@@ -994,14 +994,13 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
   const uint32_t seq = sh / a.p.heads, g = sh % a.p.heads;
   const uint32_t chunks = (a.units + a.per_wave - 1) / a.per_wave;  // of a row's units (SPLIT)
   const uint32_t tile = MODE == SPLIT ? item / chunks : MODE == DIRECT ? a.tiles - 1 - min(item, a.tiles - 1) : item;
-  if (a.clear && blockIdx.x == 0) {
+  if (a.clear && blockIdx.x == gridDim.x - 1) {  // the first ones have the longest rows
     // rows of no sequence lie before the first span and behind the last
-    const Span none = span_of(a.r.row_start, a.r.kv_len, 0, a.r.rows);
-    const int64_t hi = max((int64_t)none.start, min((int64_t)a.r.row_start[a.r.sequences], (int64_t)a.r.rows));
-    for (int64_t row = wave; row < (int64_t)a.r.rows; row += waves) {
-      if (row == none.start) row += (hi - row + waves - 1) / waves * waves;
-      if (row < none.start || (row >= hi && row < (int64_t)a.r.rows))
-        for (uint32_t d = lane; d < a.nh * a.hd; d += WAVE) store_value(a.out, row * a.os + d, a.type, 0.0f);
+    const int64_t lo = span_of(a.r.row_start, a.r.kv_len, 0, a.r.rows).start;
+    const int64_t hi = max(lo, min((int64_t)a.r.row_start[a.r.sequences], (int64_t)a.r.rows));
+    for (int64_t i = wave; i < lo + ((int64_t)a.r.rows - hi); i += waves) {
+      const int64_t row = i < lo ? i : hi + (i - lo);
+      for (uint32_t d = lane; d < a.nh * a.hd; d += WAVE) store_value(a.out, row * a.os + d, a.type, 0.0f);
     }
   }
   if (MODE == SPLIT ? tile >= a.tiles : item >= a.tiles) return;
