@@ -1739,6 +1739,12 @@ extern "C" int defer_gpu_q8_rms_norm(uint32_t type, const void* x, int64_t x_str
   if (!rc && sum) rc = check_rows_values(type, sum, sum_stride, rows, n, "sum");
   if (!rc) rc = check_rows_values(type, weight, n, 1, n, "weight");
   if (rc) return rc;
+  if (sum) {
+    const int64_t v = (int64_t)value_size(type);
+    Q8_REQUIRE(!overlap(sum, sum_stride * v, rows, x, x_stride * v, rows, n * v), "sum overlaps x");
+    Q8_REQUIRE(!residual || !overlap(sum, sum_stride * v, rows, residual, residual_stride * v, rows, n * v), "sum overlaps residual");
+    Q8_REQUIRE(rows == 0 || (sum != weight && !overlap(sum, sum_stride * v, rows, weight, 0, 1, n * v)), "sum overlaps weight");
+  }
   Q8_REQUIRE(eps >= 0.0f && eps < INFINITY, "eps %g", (double)eps);
   Q8_REQUIRE(rows == 0 || (codes && scale), "null output");
   return rms_norm(type, x, x_stride, residual, residual_stride, weight, eps, rows, n, sum, sum_stride, codes, scale,
@@ -1838,6 +1844,8 @@ extern "C" int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const def
   rc = check_rows_values(type, q, q_stride, r.rows, n, "q");
   if (!rc) rc = check_rows_values(type, out, out_stride, r.rows, n, "out");
   if (rc) return rc;
+  const int64_t v = (int64_t)value_size(type);
+  Q8_REQUIRE(!overlap(out, out_stride * v, r.rows, q, q_stride * v, r.rows, n * v), "out overlaps q");
   Q8_REQUIRE(!hidden || r.sequences <= 1 || hidden_stride >= (int64_t)hidden_len, "hidden: rows of %u, %lld apart",
              hidden_len, (long long)hidden_stride);
   Q8_REQUIRE(aligned16(workspace), "workspace is not 16-byte aligned");

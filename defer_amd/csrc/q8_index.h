@@ -60,4 +60,31 @@ Q8_HD int most_units(int64_t len) {
   return n < 1 ? 1 : n > MAX_UNITS ? MAX_UNITS : (int)n;
 }
 
+// Whether two sets of rows share memory other than row by row, each row the
+// same in both: rows of `row` bytes from a and b on, as and bs bytes apart (at
+// least `row`; any number where there is one row).
+inline bool overlap(const void* a, int64_t as, uint32_t a_rows, const void* b, int64_t bs, uint32_t b_rows, int64_t row) {
+  const int64_t x = (int64_t)(uintptr_t)a, y = (int64_t)(uintptr_t)b;
+  const int64_t na = a_rows, nb = b_rows;
+  if (!na || !nb) return false;
+  if (na == 1) as = row;
+  if (nb == 1) bs = row;
+  if (x == y && na == nb && as == bs) return false;
+  if (x + (na - 1) * as + row <= y || y + (nb - 1) * bs + row <= x) return false;
+  if (as == bs) {  // columns of one matrix: the later one's first row lies between two of the other's
+    const int64_t d = x < y ? y - x : x - y, n = x < y ? na : nb, k = d / as, left = d % as;
+    return (k < n && left < row) || (k + 1 < n && as - left < row);
+  }
+  for (int64_t i = 0, j = 0; i < na && j < nb;) {
+    const int64_t p = x + i * as, q = y + j * bs;
+    if (p + row <= q)
+      ++i;
+    else if (q + row <= p)
+      ++j;
+    else
+      return true;
+  }
+  return false;
+}
+
 }  // namespace q8

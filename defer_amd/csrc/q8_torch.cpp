@@ -20,6 +20,7 @@
 #include <string>
 
 #include "../../include/defer_gpu.h"
+#include "q8_index.h"
 
 namespace {
 
@@ -97,6 +98,13 @@ int64_t row_stride(const Tensor& t, const char* what, at::Device dev, ScalarType
   if (shape[0] <= 1) return n;
   if (t.stride(0) < n) throw Refused(std::string(what) + ": rows overlap");
   return t.stride(0);
+}
+
+// Rows that a call writes lie apart from those it reads, or are the same rows.
+void apart(const Tensor& out, int64_t os, const Tensor& in, int64_t is, const char* what) {
+  const int64_t rows = out.size(0), v = out.element_size(), n = rows ? out.numel() / rows * v : 0;
+  if (rows <= 0xffffffffll && q8::overlap(out.data_ptr(), os * v, (uint32_t)rows, in.data_ptr(), is * v, (uint32_t)rows, n))
+    throw Refused(std::string("out overlaps ") + what);
 }
 
 uint32_t u32(int64_t n, const char* what) {
@@ -241,6 +249,8 @@ PyObject* rms_norm(PyObject* const* a) {  // x, weight, eps, residual, out
     z = tensor(a[4], "out");
     zs = row_stride(z, "out", dev, type, x.sizes());
     store = true;
+    apart(z, zs, x, xs, "x");
+    if (r) apart(z, zs, tensor(a[3], "residual"), rs, "residual");
   } else if (a[3] != Py_None) {
     z = fresh(x.sizes(), type, dev);
     zs = n;
@@ -336,6 +346,7 @@ PyObject* attention(PyObject* const* a) {  // q, pages, kv_len, row_start, most_
   } else {
     out = tensor(a[8], "out");
     os = row_stride(out, "out", dev, type, q.sizes());
+    apart(out, os, q, qs, "q");
   }
   const size_t need_bytes = lib.attention_workspace(&c.p, &c.r, heads, (uint32_t)most_len);
   Tensor work;

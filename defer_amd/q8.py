@@ -113,8 +113,8 @@ def quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor] = None,
              out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(z, codes, scales): z = x + residual rounded to the type (into ``out``,
-    which may be x or residual itself; x where there is no residual), and
-    z * weight / sqrt(mean(z^2) + eps) in 8 bits."""
+    which may be x or residual itself, or rows apart from both; x where there is
+    no residual), and z * weight / sqrt(mean(z^2) + eps) in 8 bits."""
     return _native().rms_norm(x, weight, eps, residual, out)
 
 
@@ -150,5 +150,6 @@ def attention(q: torch.Tensor, pages: Pages, kv_len: torch.Tensor, row_start: Op
     ``scale``: 1 / sqrt(head_dim) without. ``hidden`` [sequences, n] uint8 or
     bool: non-zero hides a position. ``most_len``: no sequence is longer
     (without: what the table holds). A row that sees nothing is zeros; rows of
-    no sequence are left as ``out`` has them (without ``out``: zeros)."""
+    no sequence are left as ``out`` has them (without ``out``: zeros). ``out`` may
+    be q itself, or rows apart from it."""
     return _native().attention(q, pages, kv_len, row_start, most_rows, most_len, scale, hidden, out)

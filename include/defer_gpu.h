@@ -274,7 +274,8 @@ int defer_gpu_batch_stats(const defer_gpu_model* m, double* stats, uint32_t rese
  * A row's results never depend on the other rows of the call, nor on how many
  * there are, nor on strides and alignments: the same bits for a prompt fed at
  * once or token by token. A call takes at most 4,194,303 rows or sequences (the
- * product 2,097,120 rows and 268,435,455 channels); more is refused.
+ * product 2,097,120 rows and 268,435,455 channels); more is refused. What a call
+ * writes shares no memory with what it reads, but where it says so.
  *
  * Value types of x, y, k, v, q and out: */
 #define DEFER_GPU_F32 0
@@ -287,7 +288,8 @@ int defer_gpu_q8_quantize(uint32_t type, const void* x, int64_t x_stride, uint32
 
 /* Root-mean-square norm with the residual's addition, in 8 bits: sum = x +
  * residual, rounded to the type (both nullable: without residual the sum is
- * x; it may be x or residual itself), and the codes of
+ * x; it may be x or residual itself, no other rows that share memory with
+ * them or weight), and the codes of
  * sum * weight / sqrt(mean(sum^2) + eps). weight [n] is of the same type. */
 int defer_gpu_q8_rms_norm(uint32_t type, const void* x, int64_t x_stride, const void* residual,
                           int64_t residual_stride, const void* weight, float eps, uint32_t rows,
@@ -342,7 +344,7 @@ int defer_gpu_q8_kv_read(const defer_gpu_q8_pages* pages, const defer_gpu_q8_row
 
 /* out[r, h] = sum_t p_t v_t, p = softmax of scale * q[r, h] . k_t over the
  * positions t of the row's sequence up to its own, q and out
- * [rows, q_heads, head_dim], head h reading cache head
+ * [rows, q_heads, head_dim] (out may be q itself), head h reading cache head
  * h / (q_heads / heads). hidden (nullable) [sequences, hidden_len], rows
  * hidden_stride bytes apart: non-zero hides a position (those behind
  * hidden_len are not hidden), whatever it holds. A row that sees nothing is
