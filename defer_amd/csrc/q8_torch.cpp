@@ -9,7 +9,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <dlfcn.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -60,7 +62,15 @@ std::string shape_of(IntArrayRef s) {
 
 const Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) throw Refused(std::string(what) + " is not a tensor but " + Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (c10::GradMode::is_enabled() && t.requires_grad())  // its gradient would be lost without a word
+    throw Refused(std::string(what) + " requires a gradient, and there is no backward: detach it or call under torch.no_grad()");
+  return t;
+}
+
+// The call has written this tensor: autograd sees that what it may have saved is gone.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 const Tensor& on_gpu(PyObject* o, const char* what) {
@@ -261,6 +271,7 @@ PyObject* rms_norm(PyObject* const* a) {  // x, weight, eps, residual, out
     return lib.rms_norm(ty, x.data_ptr(), xs, r, rs, w, eps, rows, n, store ? z.data_ptr() : nullptr, zs,
                         codes.data_ptr<int8_t>(), scale.data_ptr<float>(), s);
   });
+  if (store) written(z);
   PyObject* const zo = a[4] != Py_None ? a[4] : store ? nullptr : a[0];  // the caller's own tensor comes back as it is
   Py_XINCREF(zo);
   return Py_BuildValue("(NNN)", zo ? zo : THPVariable_Wrap(z), THPVariable_Wrap(codes), THPVariable_Wrap(scale));
@@ -299,6 +310,7 @@ PyObject* kv_write(PyObject* const* a) {  // pages, k, v, kv_len, row_start, mos
   const int64_t vs = row_stride(v, "v", dev, k.scalar_type(), k.sizes());
   c.rows(a[3], a[4], k.size(0), a[5], dev);
   call(dev, [&](void* s) { return lib.kv_write(&c.p, &c.r, ty, k.data_ptr(), ks, v.data_ptr(), vs, s); });
+  for (Py_ssize_t i = 0; i < 4; ++i) written(THPVariable_Unpack(PyTuple_GET_ITEM(a[0], i)));
   Py_RETURN_NONE;
 }
 
@@ -356,6 +368,7 @@ PyObject* attention(PyObject* const* a) {  // q, pages, kv_len, row_start, most_
                          os, clear, need_bytes ? work.data_ptr() : nullptr, need_bytes, s);
   });
   if (clear) return THPVariable_Wrap(out);
+  written(out);
   Py_INCREF(a[8]);
   return a[8];
 }
@@ -366,6 +379,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != N) return PyErr_Format(PyExc_TypeError, "expected %d arguments, got %zd", N, n);
   if (!lib.attention) return PyErr_Format(PyExc_RuntimeError, "bind() first");
   try {
+    need(!at::tracer::impl::is_dispatch_enabled(), "torch.jit.trace would keep what this call returns as constants");
     return F(args);
   } catch (const PythonError&) {
     return nullptr;

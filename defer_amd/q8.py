@@ -9,7 +9,8 @@ Every call is queued on torch's current stream of its tensors' device, returns
 without waiting and may be captured into a graph. Tensors that the kernels
 cannot take as they are (another device, type or layout) are refused with a
 ValueError, never copied. Values are float32, bfloat16 or float16. There is no
-backward: results carry no gradient.
+backward: results carry no gradient, and a tensor that requires one is refused
+where gradients are on, as is any call under torch.jit.trace.
 """
 from __future__ import annotations
 
