@@ -1470,6 +1470,11 @@ void attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t ld
     if (kc == 4) k_attn<4, R, MODE><<<blocks, threads, lds, s>>>(a);
 }
 
+// (Row, query head) pairs of a sequence and cache head. A call of more than
+// MOST_PAIRS has too many workgroups anyway.
+uint64_t pairs_of(const Rows& r, uint32_t heads, uint32_t kv_heads) { return (uint64_t)r.most_rows * (heads / kv_heads); }
+constexpr uint64_t MOST_PAIRS = 0x7fffffff;
+
 // How a call's pairs are dealt.
 struct Plan {
   AttnMode mode;
@@ -1477,7 +1482,7 @@ struct Plan {
   size_t lds, workspace;
 };
 Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint32_t most_len) {
-  const uint32_t pairs = r.most_rows * (heads / kv_heads);
+  const uint32_t pairs = (uint32_t)pairs_of(r, heads, kv_heads);
   Plan p;
   // Tiles share the codes a wave has loaded, so the more the better, as far as
   // registers allow and waves are left for the chip: a prompt of 2048 8B rows
@@ -1630,7 +1635,7 @@ int kv_read(const Pages& p, const Rows& r, uint32_t type, void* k, void* v, uint
 }
 
 size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len) {
-  if (!r.rows || !r.sequences || !r.most_rows) return 0;
+  if (!r.rows || !r.sequences || !r.most_rows || pairs_of(r, heads, kv_heads) > MOST_PAIRS) return 0;
   const uint32_t dp = padded(head_dim);
   const Plan pl = plan_of(r, heads, kv_heads, dp, most_len);
   return pl.workspace;
@@ -1643,6 +1648,8 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
     if (in.clear) k_zero_rows<<<r.rows, 256, 0, s>>>(in.out, in.out_stride, in.heads * in.head_dim, in.type);
     return launched();
   }
+  if (pairs_of(r, in.heads, p.heads) > MOST_PAIRS)
+    return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
   const Plan pl = plan_of(r, in.heads, p.heads, p.dp, in.most_len);
   const size_t need = attention_workspace(r, in.heads, p.heads, in.head_dim, in.most_len);
   if (need && (!workspace || workspace_bytes < need))
