@@ -1766,7 +1766,8 @@ extern "C" int defer_gpu_q8_linear(const int8_t* x, int64_t x_stride, const floa
   if (rc) return rc;
   Q8_REQUIRE((rows + 31) / 32 <= 65535, "%u rows: at most 2,097,120 in one call", rows);
   Q8_REQUIRE(rows == 0 || (x && x_scale), "null x");
-  Q8_REQUIRE(m <= MAX_THREADS / 16, "%u channels: at most %u in one call", m, MAX_THREADS / 16);
+  constexpr uint32_t MOST_M = MAX_THREADS / 512 * 32;  // 512 threads for 32 channels, 256 for 16
+  Q8_REQUIRE(m <= MOST_M, "%u channels: at most %u in one call", m, MOST_M);
   Q8_REQUIRE(w && w_scale, "null w");
   Q8_REQUIRE(rows <= 1 || x_stride >= (int64_t)k, "x: rows of %u codes %lld apart", k, (long long)x_stride);
   Q8_REQUIRE(m <= 1 || w_stride >= (int64_t)k, "w: rows of %u codes %lld apart", k, (long long)w_stride);

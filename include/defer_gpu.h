@@ -274,7 +274,7 @@ int defer_gpu_batch_stats(const defer_gpu_model* m, double* stats, uint32_t rese
  * A row's results never depend on the other rows of the call, nor on how many
  * there are, nor on strides and alignments: the same bits for a prompt fed at
  * once or token by token. A call takes at most 4,194,303 rows or sequences (the
- * product 2,097,120 rows and 268,435,455 channels); more is refused. What a call
+ * product 2,097,120 rows and 268,435,424 channels); more is refused. What a call
  * writes shares no memory with what it reads, but where it says so.
  *
  * Value types of x, y, k, v, q and out: */

@@ -19,3 +19,10 @@ def test_attention_of_more_pairs_than_32_bits_count():
         assert "too many rows" in refused("attention", pages, r, 1, 1 << 40, heads, heads, 128, 1.0, None, 0, 0, 1 << 41, heads, 0, P,
                                           1 << 20, None), (rows, heads)
         assert q8._lib().defer_gpu_q8_attention_workspace(pages, r, heads, 128) == 0
+
+
+def test_linear_of_more_channels_than_a_launch_has_threads_for():
+    """16 channels are 256 threads, 32 channels 512, and a launch has fewer than 2^32."""
+    for rows in (1, 17, 100):
+        for m in (268435425, 268435441, 268435455):
+            assert "268435424" in refused("linear", P, 32, P, P, 32, P, rows, m, 32, 0, P, m, None)
