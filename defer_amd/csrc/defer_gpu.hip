@@ -50,6 +50,8 @@ static int fail_with(int code, const char* fmt, va_list ap) {
   char buf[512];
   vsnprintf(buf, sizeof(buf), fmt, ap);
   g_last_error = buf;
+  // told here: not again by the next launch that asks for the runtime's last error
+  if (code == DEFER_GPU_E_HIP) (void)hipGetLastError();
   return code;
 }
 static int fail(int code, const char* fmt, ...) {

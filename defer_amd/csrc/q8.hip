@@ -1425,8 +1425,16 @@ __global__ __launch_bounds__(256) void k_zero_rows(void* out, int64_t stride, ui
 
 // ------------------------------------------------------------- launches
 
-int launched() {
-  const hipError_t e = hipGetLastError();
+// (The launch's own status: the runtime's last error may be that of an earlier
+// call of the program's, and stays there for it.)
+template <class A>
+struct Same {
+  typedef A type;
+};
+template <class... A>
+int launch(void (*kernel)(A...), dim3 grid, dim3 block, size_t lds, hipStream_t s, typename Same<A>::type... args) {
+  void* p[] = {&args...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, p, lds, s);
   return e == hipSuccess ? DEFER_GPU_OK : defer_gpu_fail_(DEFER_GPU_E_HIP, "launch: %s", hipGetErrorString(e));
 }
 
@@ -1438,18 +1446,16 @@ int rows_launch_as(const NormArgs& a, uint32_t rows, hipStream_t s) {
                    ((uintptr_t)a.codes | a.n) % V == 0;
   const uint32_t nv = a.n / V;  // threads by n alone: they make the order of the sums
   if (vec && nv <= 256)
-    k_rows_vec<T, NORM, 256, 1><<<rows, 256, 0, s>>>(a);
-  else if (vec && nv <= 512)
-    k_rows_vec<T, NORM, 256, 2><<<rows, 256, 0, s>>>(a);
-  else if (vec && nv <= 1024)
-    k_rows_vec<T, NORM, 256, 4><<<rows, 256, 0, s>>>(a);
-  else if (vec && nv <= 4096)
-    k_rows_vec<T, NORM, 1024, 4><<<rows, 1024, 0, s>>>(a);
-  else if (nv <= 1024)
-    k_rows<T, NORM, 256><<<rows, 256, 0, s>>>(a);
-  else
-    k_rows<T, NORM, 1024><<<rows, 1024, 0, s>>>(a);
-  return launched();
+    return launch(k_rows_vec<T, NORM, 256, 1>, rows, 256, 0, s, a);
+  if (vec && nv <= 512)
+    return launch(k_rows_vec<T, NORM, 256, 2>, rows, 256, 0, s, a);
+  if (vec && nv <= 1024)
+    return launch(k_rows_vec<T, NORM, 256, 4>, rows, 256, 0, s, a);
+  if (vec && nv <= 4096)
+    return launch(k_rows_vec<T, NORM, 1024, 4>, rows, 1024, 0, s, a);
+  if (nv <= 1024)
+    return launch(k_rows<T, NORM, 256>, rows, 256, 0, s, a);
+  return launch(k_rows<T, NORM, 1024>, rows, 1024, 0, s, a);
 }
 template <bool NORM>
 int rows_launch(uint32_t type, const NormArgs& a, uint32_t rows, hipStream_t s) {
@@ -1459,15 +1465,16 @@ int rows_launch(uint32_t type, const NormArgs& a, uint32_t rows, hipStream_t s) 
 }
 
 template <int R, AttnMode MODE>
-void attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t lds, hipStream_t s) {
+int attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t lds, hipStream_t s) {
   const uint32_t kc = a.p.dp / 64;
   if constexpr (R <= 2)
-    if (kc == 1) k_attn<1, R, MODE><<<blocks, threads, lds, s>>>(a);
-  if (kc == 2) k_attn<2, R, MODE><<<blocks, threads, lds, s>>>(a);
+    if (kc == 1) return launch(k_attn<1, R, MODE>, blocks, threads, lds, s, a);
+  if (kc == 2) return launch(k_attn<2, R, MODE>, blocks, threads, lds, s, a);
   if constexpr (MODE != GROUP && R <= 2)
-    if (kc == 3) k_attn<3, R, MODE><<<blocks, threads, lds, s>>>(a);
+    if (kc == 3) return launch(k_attn<3, R, MODE>, blocks, threads, lds, s, a);
   if constexpr (MODE != GROUP && R == 1)
-    if (kc == 4) k_attn<4, R, MODE><<<blocks, threads, lds, s>>>(a);
+    if (kc == 4) return launch(k_attn<4, R, MODE>, blocks, threads, lds, s, a);
+  return defer_gpu_fail_(DEFER_GPU_E_INVALID, "no attention kernel for head_dim %u", a.hd);
 }
 
 // (Row, query head) pairs of a sequence and cache head. A call of more than
@@ -1544,23 +1551,17 @@ int rms_norm(uint32_t type, const void* x, int64_t x_stride, const void* residua
 template <int MT, int NT, int NW>
 static int linear_few(const LinearArgs& a, bool aligned, hipStream_t s) {
   const dim3 grid((a.m + 16 * MT - 1) / (16 * MT), (a.rows + 16 * NT - 1) / (16 * NT));
-  if (aligned)
-    k_linear_few<MT, NT, NW, true><<<grid, NW * WAVE, 0, s>>>(a);
-  else
-    k_linear_few<MT, NT, NW, false><<<grid, NW * WAVE, 0, s>>>(a);
-  return launched();
+  return launch(aligned ? k_linear_few<MT, NT, NW, true> : k_linear_few<MT, NT, NW, false>, grid, NW * WAVE, 0, s, a);
 }
 template <int TM, int TN, int NBUF>
 static int linear_tile(const LinearArgs& a, hipStream_t s) {
   const uint32_t nrt = (a.rows + 64 * TM - 1) / (64 * TM), tiles = nrt * ((a.m + 64 * TN - 1) / (64 * TN));
-  k_linear_tile<TM, TN, NBUF><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(a, nrt, tiles);
-  return launched();
+  return launch(k_linear_tile<TM, TN, NBUF>, (tiles + 7) / 8 * 8, 256, 0, s, a, nrt, tiles);
 }
 template <int TM, int TN>
 static int linear_tile_odd(const LinearArgs& a, hipStream_t s) {
   const uint32_t nrt = (a.rows + 64 * TM - 1) / (64 * TM), tiles = nrt * ((a.m + 64 * TN - 1) / (64 * TN));
-  k_linear_tile_odd<TM, TN><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(a, nrt, tiles);
-  return launched();
+  return launch(k_linear_tile_odd<TM, TN>, (tiles + 7) / 8 * 8, 256, 0, s, a, nrt, tiles);
 }
 
 int linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
@@ -1614,24 +1615,21 @@ int kv_write(const Pages& p, const Rows& r, uint32_t type, const void* k, int64_
   const int64_t vs = type == DEFER_GPU_F32 ? 4 : 2;
   const bool vec = head_dim % 8 == 0 && ((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * vs) | (uintptr_t)(v_stride * vs)) % 16 == 0;
   const KvArgs a{p, r, const_cast<void*>(k), const_cast<void*>(v), k_stride, v_stride, type, head_dim, vec};
-  k_kv_write<<<kv_grid(p, r), r.most_rows <= 2 ? 64 : 256, 0, s>>>(a);
-  return launched();
+  return launch(k_kv_write, kv_grid(p, r), r.most_rows <= 2 ? 64 : 256, 0, s, a);
 }
 
 int kv_read(const Pages& p, const Rows& r, uint32_t type, void* k, void* v, uint32_t head_dim, hipStream_t s) {
   if (!r.rows) return DEFER_GPU_OK;
   if (!r.sequences || !r.most_rows) {
     const uint32_t n = p.heads * head_dim;
-    if (k) k_zero_rows<<<r.rows, 256, 0, s>>>(k, n, n, type);
-    if (v) k_zero_rows<<<r.rows, 256, 0, s>>>(v, n, n, type);
-    return launched();
+    const int rc = k ? launch(k_zero_rows, r.rows, 256, 0, s, k, n, n, type) : DEFER_GPU_OK;
+    return rc || !v ? rc : launch(k_zero_rows, r.rows, 256, 0, s, v, n, n, type);
   }
   const bool vec = head_dim % 8 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
   const KvArgs a{p, r, k, v, 0, 0, type, head_dim, vec};
   Rows and_one = r;
   and_one.sequences += r.row_start != nullptr;
-  k_kv_read<<<kv_grid(p, and_one), r.most_rows <= 8 ? 64 : 256, 0, s>>>(a);
-  return launched();
+  return launch(k_kv_read, kv_grid(p, and_one), r.most_rows <= 8 ? 64 : 256, 0, s, a);
 }
 
 size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len) {
@@ -1645,8 +1643,7 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
               hipStream_t s) {
   if (!r.rows) return DEFER_GPU_OK;
   if (!r.sequences || !r.most_rows) {
-    if (in.clear) k_zero_rows<<<r.rows, 256, 0, s>>>(in.out, in.out_stride, in.heads * in.head_dim, in.type);
-    return launched();
+    return in.clear ? launch(k_zero_rows, r.rows, 256, 0, s, in.out, in.out_stride, in.heads * in.head_dim, in.type) : DEFER_GPU_OK;
   }
   if (pairs_of(r, in.heads, p.heads) > MOST_PAIRS)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
@@ -1684,25 +1681,13 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
   const uint32_t nb = (uint32_t)blocks, nt = pl.waves * WAVE;
   if (pl.mode == SPLIT) {
-    if (pl.R == 1)
-      attn_launch<1, SPLIT>(a, nb, nt, pl.lds, s);
-    else
-      attn_launch<2, SPLIT>(a, nb, nt, pl.lds, s);
-    k_attn_join<<<r.sequences * r.most_rows * in.heads, p.dp, 0, s>>>(a);
-  } else if (pl.mode == GROUP) {
-    if (pl.R == 1)
-      attn_launch<1, GROUP>(a, nb, nt, pl.lds, s);
-    else
-      attn_launch<2, GROUP>(a, nb, nt, pl.lds, s);
-  } else {
-    if (pl.R == 1)
-      attn_launch<1, DIRECT>(a, nb, nt, pl.lds, s);
-    else if (pl.R == 2)
-      attn_launch<2, DIRECT>(a, nb, nt, pl.lds, s);
-    else
-      attn_launch<4, DIRECT>(a, nb, nt, pl.lds, s);
+    const int rc = pl.R == 1 ? attn_launch<1, SPLIT>(a, nb, nt, pl.lds, s) : attn_launch<2, SPLIT>(a, nb, nt, pl.lds, s);
+    return rc ? rc : launch(k_attn_join, r.sequences * r.most_rows * in.heads, p.dp, 0, s, a);
   }
-  return launched();
+  if (pl.mode == GROUP)
+    return pl.R == 1 ? attn_launch<1, GROUP>(a, nb, nt, pl.lds, s) : attn_launch<2, GROUP>(a, nb, nt, pl.lds, s);
+  if (pl.R == 1) return attn_launch<1, DIRECT>(a, nb, nt, pl.lds, s);
+  return pl.R == 2 ? attn_launch<2, DIRECT>(a, nb, nt, pl.lds, s) : attn_launch<4, DIRECT>(a, nb, nt, pl.lds, s);
 }
 
 }  // namespace q8
