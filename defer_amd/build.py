@@ -8,7 +8,8 @@
                        its checker) that the GPU tests run.
 * tests/probe/libexact_probe.so -- test-only entry points into the exact
                        sampler's device code (tests/test_exact.py).
-* _q8_torch.so      -- the 8-bit operators on torch tensors (C++, torch's headers).
+* _q8_torch.so      -- the 8-bit operators on torch tensors (C++, torch's headers;
+                       where torch is installed).
 * libdefer_host.so  -- the C++ host side (session, WAL, checkpoint, ChaCha8,
                        SHA-256, safetensors) of include/defer_host.h.
 
@@ -117,6 +118,12 @@ def build_host() -> str:
     return out
 
 
+def has_torch() -> bool:
+    import importlib.util
+
+    return importlib.util.find_spec("torch") is not None
+
+
 def build_torch() -> str:
     """defer_amd/_q8_torch.so: the 8-bit operators on torch tensors, C++ against
     the installed torch."""
@@ -139,11 +146,14 @@ def build_torch() -> str:
 
 def build_all() -> None:
     build_gpu()
-    build_torch()
     if os.path.isdir(os.path.join(CSRC, "host")):
         build_host()
     build_c_abi_test()
     build_probe()
+    if has_torch():  # nothing else here needs it
+        build_torch()
+    else:
+        print("torch is not installed: _q8_torch.so (defer_amd.q8) is not built", flush=True)
 
 
 if __name__ == "__main__":
