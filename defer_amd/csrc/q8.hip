@@ -954,15 +954,18 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // contributions their accuracy.
 //
 // A score is digit sum * key scale * the query's factor. The sum counts the
-// query as some 2^30 and the codes as up to 2^15 more, so that times a key scale
-// over 2^80 it may pass f32's range where the score does not, and the factor of a
-// query under 2^-64 may lie below it: such a row (for keys: in such a block) takes
-// the sum 2^45 times smaller and the factor larger, exactly. Scores over 2^26 are
-// rounded before the largest is taken off. What makes a row do either is its own
-// and what it sees of the block, so its bits are its own, too. Blocks that every
-// row of a tile sees all of go without; where the largest key scale of them says that a
-// row may have had to, the wave starts again with care (a check in every block
-// makes it wait: 2048 8B rows 235 -> 247 us).
+// query as some 2^30 and the codes as up to 2^15 more, so that its product with a large
+// key scale would pass f32's range where the score does not, and the factor of a
+// small query would lie below it: 2^45 goes from the sum to the factor, exactly
+// (not for a query over 2^64, whose factor would pass the range). Scores over 2^26
+// have the largest taken off before they are multiplied by the factor: behind it
+// the largest is rounded and a fused product is not, which could put a block's
+// probabilities above or below f32's range. Both by selects: 11 of a block's and
+// tile's 200 instructions (2048 8B rows 234 -> 242 us, 272 -> 282 with hidden
+// positions; sessions' single rows as before). Branches around what is seldom needed
+// hold more registers (251 us); a wave that starts again once its key scales say
+// that it must takes 233 us, but 301 with hidden positions, and 64 1B rows 15.5 in
+// place of 11.5.
 //
 // The next block's keys are on their way once this one's scores are formed, the
 // next values once this one's are used, or with the keys where registers
@@ -980,7 +983,7 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // k_attn_join. GROUP: the units of a tile are the waves of one workgroup, which
 // joins them through LDS.
 template <int KC, int R, AttnMode MODE>
-__global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1 ? 3 : MODE != GROUP && KC == 2 && R == 1 ? 2 : 1) void k_attn(AttnArgs a) {
+__global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 1 ? 3 : MODE != GROUP && (KC == 1 || (KC == 2 && R == 1)) ? 2 : 1) void k_attn(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
   constexpr bool AHEAD = R == 1 && KC <= 2 && MODE != GROUP;  // the next values wait in registers of their own
   extern __shared__ __align__(16) uint8_t lds[];  // [waves][R][16][P_ROW], GROUP: then [4 R][units][2 + DP] floats
@@ -1049,7 +1052,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
 
   // the queries' digits; the scores' sign is the scale's, folded into them
   v4i aq[R][KC];
-  float sq[R];  // queries' factors; negative: 2^45 times as large
+  float sq[R];  // queries' factors for digit sums times 2^-45; negative: for the sums as they are
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint32_t pr = pair0 + 4 * r + n16 / 4, j = pr / a.group;
@@ -1104,7 +1107,8 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
     (void)frexpf(top, &ex);
     ex = top > 0.0f ? ex : 0;
     const float up = isnan(bad) ? 0.0f : a.scale2 < 0.0f ? -ldexpf(1.0f, 30 - ex) : ldexpf(1.0f, 30 - ex);
-    const float s = isnan(bad) ? __builtin_nanf("") : (tiny ? -ldexpf(1.0f, ex - 80 - 30 + 45) : ldexpf(1.0f, ex - 30)) * fabsf(a.scale2);
+    const int unit = (tiny ? ex - 80 : ex) - 30;  // of the digit sums
+    const float s = isnan(bad) ? __builtin_nanf("") : (ex > 64 ? -ldexpf(1.0f, unit) : ldexpf(1.0f, unit + 45)) * fabsf(a.scale2);
     const uint32_t dg = n16 % 4, sel = dg | (4 + dg) << 8;
 #pragma unroll
     for (int kk = 0; kk < KC; ++kk)
@@ -1123,9 +1127,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
   // after the other.
   const int ul_last = unit_len(max(max_pos, 0));
   const int ul_first = max_pos < 0 ? ul_last : unit_len(min_pos);
-  bool plain = !hid;  // blocks that every row sees all of need no care for ranges
   for (int ul = ul_first; ul <= ul_last; ul += UNIT) {
-    float largest = 0.0f;  // key scale of such a block
     int ps[R], pmax = -1, pmin = 0x7fffffff;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -1147,8 +1149,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
       for (int t = 0; t < DT; ++t) A[r][t] = acc[r][t] = 0.0f;
     }
 
-    // A block whose codes have been loaded: WHOLE if every row sees all of it and no
-    // product leaves the range.
+    // A block whose codes have been loaded: WHOLE if every row sees all of it.
     // next: the page to load meanwhile, or -1.
     auto block = [&](auto whole, int b, int next) {
       constexpr bool WHOLE = decltype(whole)::value;
@@ -1164,7 +1165,6 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
       // every output (adding the zeros of the others changes nothing)
       float vbad = 0.0f;
       if (WHOLE) vbad = fmaf(vs[0], 0.0f, vs[1] * 0.0f) + fmaf(vs[2], 0.0f, vs[3] * 0.0f);
-      if (WHOLE) largest = fmaxf(largest, fmaxf(fmaxf(ks[0], ks[1]), fmaxf(ks[2], ks[3])));
       float xw[R], be[R];  // the weights of what came before and of this block
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -1179,45 +1179,24 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
           load_k(next);
           if (AHEAD) load_v(next, vn);
         }
-        float s[4], w[4], factor = sq[r];
+        float s[4], w[4];
         bool see[4];
+        const float unit = sq[r] < 0.0f ? 1.0f : 0x1p-45f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           see[j] = WHOLE || (tb + j <= ps[r] && !hide[j]);
-          const float x = undigit(d[j]) * ks[j];
+          const float x = undigit(d[j]) * unit * ks[j];
           s[j] = see[j] ? x : -INFINITY;
-        }
-        if (!WHOLE) {
-          float seen = 0.0f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) seen = fmaxf(seen, see[j] ? ks[j] : 0.0f);
-          if (__builtin_expect(__any(factor < 0.0f || seen > 0x1p80f), 0)) {
-            const bool lift = factor < 0.0f || row_max(seen) > 0x1p80f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (lift && see[j]) s[j] = undigit(d[j]) * 0x1p-45f * ks[j];
-            // (a factor past the range is one of scores past it, or of 0)
-            factor = factor < 0.0f ? -factor : !lift ? factor : factor > 0x1p82f ? __FLT_MAX__ : factor * 0x1p45f;
-          }
         }
         const float top = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
         const bool none = !WHOLE && top == -INFINITY;
-        const float m0 = none ? 0.0f : top * factor;
-        float lp = vbad, e[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = fmaf(s[j], factor, -m0);
-        if (!WHOLE) {
-          // m0 is rounded and the fused product is not: that could put a block's
-          // probabilities above or below f32's range
-          const bool sharp = fabsf(m0) > 0x1p26f;
-          if (__builtin_expect(__any(sharp), 0)) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = sharp ? s[j] * factor - m0 : e[j];
-          }
-        }
+        const float m0 = none ? 0.0f : top * fabsf(sq[r]);
+        const bool sharp = fabsf(m0) > 0x1p26f;
+        const float before = sharp ? top : 0.0f, behind = sharp ? 0.0f : m0;
+        float lp = vbad;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float p = exp2_of(e[j]);
+          float p = exp2_of(fmaf(s[j] - before, fabsf(sq[r]), -behind));
           if (!WHOLE) {
             p = see[j] ? p : 0.0f;
             lp += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
@@ -1290,7 +1269,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
       const int bn = unit_ends ? (u + du) * bpu : b + 1;
       const int next = bn < blocks && (!unit_ends || u + du < u_end) ? page_at(bn) : -1;
       if (page >= 0) {
-        if (plain && b * PAGE + PAGE - 1 <= pmin)
+        if (!hid && b * PAGE + PAGE - 1 <= pmin)
           block(std::true_type(), b, next);
         else
           block(std::false_type(), b, next);
@@ -1329,21 +1308,6 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE != GROUP && KC == 1
       }
       b = bn;
       page = next;
-    }
-    if (plain) {
-      // scores of at most 2^26, whatever the digit sums (2^37 DP at most)
-      float top = 0.0f;
-      bool in_range = largest <= 0x1p80f;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        top = fmaxf(top, sq[r]);
-        in_range = in_range && !(sq[r] < 0.0f);
-      }
-      if (__builtin_expect(__any(!in_range || largest * top > 0x1p-11f / DP), 0)) {
-        plain = false;
-        ul -= UNIT;  // once more
-        continue;
-      }
     }
     if (MODE == DIRECT) {
 #pragma unroll
