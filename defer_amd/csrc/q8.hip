@@ -120,8 +120,10 @@ struct NormArgs {
 // One workgroup per row: z = x + r, sum z^2, max |z w|, then the codes. The
 // squares and products are formed in 64 bits (24 + 24 bits: the products
 // exactly), so that codes are those of the formula and not of a rounding;
-// memory hides that. Bound by memory: 2048 x 4096 bf16 with residual, 58.7 MB in
-// 16.0 us (3.7 TB/s; a large copy moves 4.75); 1 x 576: 2.6 us, all latency.
+// memory hides that (2048 x 4096: 5.0 M vector instructions, 8 of the 15.6 us at 4
+// cycles each). Bound by memory: 2048 x 4096 bf16 with residual, 58.7 MB in
+// 15.6 us (3.8 TB/s; a large copy moves 4.7); codes alone of 2047 x 14336 f32, 147
+// MB in 37.0 us (4.0 TB/s); 1 x 576: 2.6 us, all latency.
 struct RowSum {
   double ss = 0.0, top = 0.0;
   float bad = 0.0f;  // NaN once a value is not finite
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(BLOCK) void k_rows(NormArgs a) {
 
 // The same where every row is a multiple of 16 bytes apart and long: 16-byte
 // loads, and the row stays in registers between its two passes (2048 x 4096:
-// 34 us through k_rows, 16.0 so).
+// 34 us through k_rows, 15.6 so).
 template <class T, bool NORM, int BLOCK, int C>
 __global__ __launch_bounds__(BLOCK) void k_rows_vec(NormArgs a) {
   constexpr int V = 16 / sizeof(T);
@@ -295,8 +297,8 @@ __device__ __forceinline__ float scaled_any(int sum, float xs, float ws) {
 // Few rows: a workgroup owns 16 MT channels and 16 NT rows, its waves share k
 // in steps of 128 codes; a lane's 32 bytes of a step go straight into two
 // matrix instructions. The waves' sums meet in LDS. Bound by memory, which reads
-// every weight once: 1 x 28672 x 4096 in 22.3 us (5.3 TB/s of the 6.1 that a large
-// read reaches); 1 x 960 x 576 in 3.3 us, latency.
+// every weight once: 1 x 28672 x 4096 in 21.8 us (5.4 TB/s of the 6.0 that a large
+// read reaches); 1 x 960 x 576 in 3.2 us, latency.
 template <int MT, int NT, int NW, bool ALIGNED>
 __global__ __launch_bounds__(NW * WAVE) void k_linear_few(LinearArgs a) {
   const uint32_t lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, r16 = lane % 16, kg = lane / 16;
@@ -483,9 +485,9 @@ __device__ __forceinline__ bool tile_of_workgroup(uint32_t tiles, uint32_t* id) 
 // loads, which write zeros for what is outside the operand or behind k), two
 // stages ahead or more. They are issued one at a time between the products:
 // in a row they keep a wave from its next product for as long as the memory
-// pipeline takes them (2047 x 28672 x 4096: 320 us so, 257 now: 1,870 Tops/s; the
-// matrix cores alone reach 4,100, the library's i8 product of the same sizes
-// 236 us). Wider tiles (256 x 256: 310 us, half the LDS reads but one
+// pipeline takes them (2047 x 28672 x 4096: 320 us so, 257 now: 1,870 Tops/s, and
+// 268 on operands that were not there a call before; the matrix cores alone reach
+// 4,100, the library's i8 product of the same sizes takes 243 us). Wider tiles (256 x 256: 310 us, half the LDS reads but one
 // stage of 64 codes less in flight), and one workgroup per CU that goes on to its
 // next tile's copies while it stores (312), were slower. A stage's last reads are waited for before the barrier in
 // it; behind that the next stage's first operands are read while its last
@@ -971,11 +973,12 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // next values once this one's are used, or with the keys where registers
 // allow (R = 1: few rows, bound by memory).
 //
-// A long cache is bound by memory (11 8B rows of 6000 positions: 140 MB in 34.5
-// us; 512 of 2000: 2.2 GB in 400 us, 5.4 TB/s), a prompt by vector instructions
-// (3500 360M rows: 180 us, 138 of them the vector unit's; a tile and block takes
-// about 190 of them beside 8 matrix products), a short step by its chain of
-// dependent loads (64 1B rows of 385 positions: 10.9 us).
+// A long cache is bound by memory (11 8B rows of 6000 positions: 140 MB in 36.7
+// us; 512 of 2000: 2.2 GB in 403 us, 5.4 TB/s), a prompt by vector instructions
+// (3500 360M rows: 180 us, 146 of them the vector unit's; a tile and block takes
+// about 200 of them beside 8 matrix products), a short step by its chain of
+// dependent loads (64 1B rows of 385 positions: 10.7 us with hidden ones, 8.6
+// without: four byte loads more a block).
 //
 // DIRECT: a wave goes through all its positions, unit after unit (many rows;
 // the four waves of a workgroup are neighbouring tiles and meet the same codes
@@ -1350,7 +1353,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 // Joins a row's units in order, as the unsplit kernel does. One workgroup of
 // dp lanes per (row of a sequence, head); a lane holds one unit's maximum and
 // sum, the accumulators of 32 units are on their way at a time. Three dependent
-// reads of what other XCDs wrote: 9.7 us for 11 x 32 heads of 47 units (8.6 MB);
+// reads of what other XCDs wrote: 10 us for 11 x 32 heads of 47 units (8.6 MB);
 // 64 units at a time changed nothing.
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   const uint32_t h = blockIdx.x % a.nh, j = blockIdx.x / a.nh % a.r.most_rows, seq = blockIdx.x / a.nh / a.r.most_rows;
@@ -1457,9 +1460,10 @@ Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint
   Plan p;
   // Tiles share the codes a wave has loaded, so the more the better, as far as
   // registers allow and waves are left for the chip: a prompt of 2048 8B rows
-  // takes 394, 338 and 262 us with 1, 2 and 4, one of 301 135M rows 13.3, 14.5
-  // and 18.8. Heads of 64 fit three waves of R = 2 a SIMD, which hide more than
-  // sharing between four saves (3500 360M rows: 206 us with 4, 191 with 2).
+  // takes 372, 276 and 242 us with 1, 2 and 4, one of 301 135M rows 9.0 and 12.5
+  // with 1 and 2 (3500 360M rows: 307 and 180). Heads of 64 take three waves of R =
+  // 2 a SIMD with 13 registers of each spilled, which hides more than sharing
+  // between four rows saved at two waves (206 us with 4 where 2 took 191).
   auto waves_of = [&](uint32_t R) { return (uint64_t)r.sequences * kv_heads * ((pairs + 4 * R - 1) / (4 * R)); };
   p.R = pairs <= 4 || dp > 192 ? 1 : pairs > 8 && dp == 128 && waves_of(4) >= 2048 ? 4 : pairs <= 8 || waves_of(2) >= 1024 ? 2 : 1;
   p.tiles = (pairs + 4 * p.R - 1) / (4 * p.R);
@@ -1471,15 +1475,16 @@ Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint
   const size_t partials = (size_t)r.rows * heads * p.units * (2 + dp) * sizeof(float);
   const uint32_t w = std::min(p.units, 8u);
   // A wave for each of the chip's 1,024 SIMDs, and a row's units need no
-  // dealing: 128 8B rows of 2000 positions take 116 us in one piece and 146 as
-  // a workgroup's units; the 512 waves of 64 1B rows of 4000 take 98 in one piece
-  // and 68 split.
+  // dealing: 128 8B rows of 2000 positions take 98 us in one piece and 116 as
+  // a workgroup's units; the 512 waves of 64 1B rows of 4000 take 70 in one piece
+  // and 59 split.
   if (p.units > 1 && p.units <= 16 && p.R <= 2 && dp <= 128 && waves < 1024) {
     p.mode = GROUP;
     p.waves = w;
   } else if (p.units > 1 && waves < 1024 && partials <= ((size_t)128 << 20)) {
     // about four waves a SIMD: each has its rows' digits to form, so not more (11
-    // 8B rows of 6000 positions: 42.8 us; 16 of 8000: 66 us, 74 with half as many)
+    // 8B rows of 6000 positions: 37 us with the join, 101 in one piece; 16 of 8000:
+    // 59, 158 in one piece, an eighth more with half as many waves)
     p.mode = SPLIT;
     p.per_wave = (uint32_t)std::max<uint64_t>(1, waves * p.units / SPLIT_WAVES);
     p.workspace = partials;
@@ -1538,27 +1543,29 @@ int linear(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t
   const bool near = std::max(x_stride, w_stride) <= (1 << 22);
   // Few rows read every weight once, at the rate of memory: 16 channels a
   // workgroup, whose waves share k; many waves of them where there are few
-  // channels (1 x 4096 x 14336: 26.8 us with 4, 13.1 with 16; 1 x 28672 x
-  // 4096: 26.0 and 28.4).
+  // channels (1 x 4096 x 14336: 19.4 us with 4, 10.9 with 16; 1 x 28672 x
+  // 4096: 21.8 and 25.9).
   const uint64_t m16 = (m + 15) / 16;
   if (rows <= 16)
     return m16 <= 512 && k >= 2048 ? linear_few<1, 1, 16>(a, aligned, s) : linear_few<1, 1, 4>(a, aligned, s);
   // Up to 64 rows and too few 64 x 64 tiles for the chip: k shared by eight
-  // waves (64 x 2048 x 8192: 14.5 us, 16.0 in tiles; 64 x 16384 x 2048: 27
-  // and 10.0), over 32 channels where 16 would be more than a workgroup per CU
-  // (64 x 4096 x 14336: 42.3 with 16, 29.5 with 32).
+  // waves (64 x 2048 x 8192: 13.7 us, 14.5 in tiles; 64 x 16384 x 2048: 18.4
+  // and 7.4), over 32 channels where 16 would be more than a workgroup per CU
+  // (64 x 4096 x 14336: 39.7 with 16, 27.8 with 32). Between the two the tiles are
+  // already ahead: 64 x 4096 x 14336 would take 24.3 in them, 64 x 8192 x 2048 6.6
+  // where this takes 10.7.
   auto tiles_of = [&](uint32_t r, uint32_t c) { return (uint64_t)((rows + r - 1) / r) * ((m + c - 1) / c); };
   if (rows <= 64 && (tiles_of(64, 64) < 192 || !aligned))
     return m16 * ((rows + 31) / 32) <= 256 ? linear_few<1, 2, 8>(a, aligned, s) : linear_few<2, 2, 8>(a, aligned, s);
   if (!near) return linear_few<2, 2, 8>(a, aligned, s);
-  // Unaligned: 301 x 577 x 1537 takes 21 us so and 27 in tiles, 130 x 9001 x
-  // 3001 takes 114 and 44.
+  // Unaligned: 301 x 577 x 1537 takes 20.5 us so and 23.8 in tiles, 130 x 9001 x
+  // 3001 takes 113 and 42.
   if (!aligned)
     return tiles_of(128, 128) < 32 ? linear_few<1, 2, 8>(a, aligned, s) : linear_tile_odd<2, 2>(a, s);
   // The tile whose rounds over the chip take least: us a round and a stage as
-  // measured (2047 x 28672 x 4096: 257 us in 256 x 128, 350 in 128 x 128; 1000
-  // x 4096 x 4096: 31.1, 22.9, 32.1 in 64 x 64; 500 x 4096 x 4096: 29.7, 19.0,
-  // 17.7). Two 64 x 64 tiles share a CU.
+  // measured (2047 x 28672 x 4096: 257 us in 256 x 128, 303 in 128 x 128; 1000
+  // x 4096 x 4096: 32.2, 24.5, 31.7 in 64 x 64; 500 x 4096 x 4096: 29.3, 19.0,
+  // 17.1). Two 64 x 64 tiles share a CU.
   const double stages = (k + 127) / 128;
   auto rounds = [&](uint64_t tiles, uint64_t at_once) { return (double)((tiles + at_once - 1) / at_once); };
   const uint64_t small = tiles_of(64, 64);

@@ -352,7 +352,7 @@ int defer_gpu_q8_kv_read(const defer_gpu_q8_pages* pages, const defer_gpu_q8_row
  * attended to. clear != 0: rows of no sequence become zeros. Scores and sums
  * have f32's accuracy, also where keys lie at one end of its range and queries at the
  * other; the sum of p_t |v_t| with the row's largest p_t as 1 has to be in
- * the range. `workspace` (16-byte aligned) is
+ * the range, and values under 1e-27 have fewer digits. `workspace` (16-byte aligned) is
  * scratch of the size that defer_gpu_q8_attention_workspace gives (which may
  * be 0); calls that may overlap, captured ones among them, each need their
  * own. */
