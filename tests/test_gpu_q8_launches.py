@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from defer_amd import q8
-from test_gpu_q8 import DEV, HALF, TYPES, check_linear, fill, i8, i32, make_cache, ref_attention, rnd, starts, values
+from test_gpu_q8 import DEV, TYPES, check_linear, fill, i8, i32, make_cache, ref_attention, rnd, starts, values
 
 pytestmark = pytest.mark.gpu
 
