@@ -57,6 +57,7 @@ struct Attention {
   int64_t hidden_stride;
   uint32_t hidden_len;
   bool clear;  // zeros for the rows of no sequence
+  const int32_t* parent;  // [rows], or NULL: rows are no tree
 };
 size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len);
 int attention(const Pages& p, const Rows& r, const Attention& a, void* workspace, size_t workspace_bytes,

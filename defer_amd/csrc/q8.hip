@@ -4,9 +4,7 @@
 // Sums of code products are exact in 32-bit integers (v_mfma_i32_16x16x64_i8),
 // so they have no order; every other sum has one that depends on its own row
 // only. Nothing here keeps state, allocates or waits.
-#include "q8.h"
-
-#include <math.h>
+#include "q8_common.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -14,98 +12,6 @@
 namespace q8 {
 
 namespace {
-
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-
-constexpr int WAVE = 64;
-constexpr uint32_t MAX_THREADS = 0xffffffffu;  // of a launch in one dimension
-constexpr double TINY = 0x1p-100;  // rows with a smaller maximum are held as zeros
-
-// ------------------------------------------------------------- value types
-
-__device__ __forceinline__ float load_value(const void* p, int64_t i, uint32_t type) {
-  if (type == DEFER_GPU_F32) return static_cast<const float*>(p)[i];
-  if (type == DEFER_GPU_BF16) return (float)static_cast<const __bf16*>(p)[i];
-  return (float)static_cast<const _Float16*>(p)[i];
-}
-__device__ __forceinline__ void store_value(void* p, int64_t i, uint32_t type, float v) {
-  if (type == DEFER_GPU_F32)
-    static_cast<float*>(p)[i] = v;
-  else if (type == DEFER_GPU_BF16)
-    static_cast<__bf16*>(p)[i] = (__bf16)v;
-  else
-    static_cast<_Float16*>(p)[i] = (_Float16)v;
-}
-
-// ------------------------------------------------------------- reductions
-
-// Over the 16 lanes of a DPP row; every lane gets the result. Each step adds
-// the same two numbers in both lanes of a pair, so all 16 hold the same bits.
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
-}
-// (Written out: the compiler moves each lane's value, quiets it, then takes the
-// maximum: three instructions a step. A lane reads another's register two wait
-// states after it was written.)
-__device__ __forceinline__ float row_max(float v) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
-      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:4 row_mask:0xf bank_mask:0xf\n\t"
-      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:2 row_mask:0xf bank_mask:0xf\n\t"
-      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_ror:1 row_mask:0xf bank_mask:0xf\n\ts_nop 1"
-      : "+v"(v));
-#endif
-  return v;
-}
-// Towards zero; what is not a number is 0, what is out of range the nearest.
-__device__ __forceinline__ int to_int(float v) {
-  int i = 0;
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm("v_cvt_i32_f32 %0, %1" : "=v"(i) : "v"(v));
-#endif
-  return i;
-}
-__device__ __forceinline__ float row_sum(float v) {
-  v += dpp<0x128>(v);
-  v += dpp<0x124>(v);
-  v += dpp<0x122>(v);
-  return v + dpp<0x121>(v);
-}
-template <class V>
-__device__ __forceinline__ V wave_max(V v) {
-  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
-  return v;
-}
-template <class V>
-__device__ __forceinline__ V wave_add(V v) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-
-// ------------------------------------------------------------- rows to codes
-
-// Scale of a row with maximum `top`; nan: the row holds no finite values only.
-__device__ __forceinline__ float scale_of(double top, bool nan) {
-  const float s = top < TINY ? 0.0f : (float)(top / 127.0);
-  return nan || !(s < INFINITY) ? __builtin_nanf("") : s;
-}
-// The code of x at a scale, rint(x / s) with ties to even. x and s are 24-bit
-// values: what the product with 1 / s leaves is exact in 64 bits and says
-// where the quotient is on the wrong side of a half (a division takes three
-// times the instructions). `scale` is 0 or NaN for a row of zeros.
-struct Coder {
-  double s, r;
-  __device__ __forceinline__ explicit Coder(float scale) : s(scale > 0.0f ? (double)scale : 0.0), r(s > 0.0 ? 1.0 / s : 0.0) {}
-  __device__ __forceinline__ int operator()(float v) const {
-    const double x = s > 0.0 ? (double)v : 0.0;
-    int c = (int)rint(x * r);
-    const double left = fma(-(double)c, s, x), over = 2.0 * fabs(left) - s;
-    if (over > 0.0 || (over == 0.0 && (c & 1))) c += left > 0.0 ? 1 : -1;
-    return c;
-  }
-};
 
 struct NormArgs {
   const void *x, *r, *w;
@@ -646,23 +552,6 @@ __global__ __launch_bounds__(256) void k_linear_tile_odd(LinearArgs a, uint32_t 
 
 // ------------------------------------------------------------- the cache
 
-__device__ __forceinline__ SeqPages pool_of(const Pages& p, uint32_t seq, const int32_t*& table, uint32_t& width) {
-  if (p.seqs) {
-    SeqPages s = p.seqs[seq];
-    table = nullptr;
-    width = s.pages;
-    const int64_t off = p.seq_layer * s.pages * p.heads * PAGE;
-    s.keys += off * p.dp;
-    s.values += off * p.dp;
-    s.key_scale += off;
-    s.value_scale += off;
-    return s;
-  }
-  table = p.table + (size_t)seq * p.width;
-  width = p.width;
-  return SeqPages{p.keys, p.values, p.key_scale, p.value_scale, p.pages};
-}
-
 struct KvArgs {
   Pages p;
   Rows r;
@@ -671,71 +560,6 @@ struct KvArgs {
   uint32_t type, hd;
   bool vec;  // eight values of a row are 16-byte loads and stores
 };
-
-// Runs that rows of neighbouring positions may lie in.
-Q8_HD uint32_t kv_runs(uint32_t rows) { return (rows + 14) / 16 + 1; }
-constexpr int KV_ROW = 256 + 8;  // bytes of a token's codes in LDS
-constexpr int KV_RUN = 16;       // positions a workgroup takes: a quarter of a page
-
-__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
-  return __builtin_amdgcn_perm(hi, lo, sel);
-}
-// 4 x 4 bytes, rows to columns.
-__device__ __forceinline__ void transpose4(const uint32_t* in, uint32_t* out) {
-  const uint32_t l01 = perm(in[1], in[0], 0x05010400u), l23 = perm(in[3], in[2], 0x05010400u);
-  const uint32_t h01 = perm(in[1], in[0], 0x07030602u), h23 = perm(in[3], in[2], 0x07030602u);
-  out[0] = perm(l23, l01, 0x05040100u);
-  out[1] = perm(l23, l01, 0x07060302u);
-  out[2] = perm(h23, h01, 0x05040100u);
-  out[3] = perm(h23, h01, 0x07060302u);
-}
-
-// 8 values of a row from d on, zeros from hd on; vec: 16-byte loads.
-__device__ __forceinline__ void load8(const void* p, int64_t i0, uint32_t d, uint32_t hd, uint32_t type, bool vec, float* y) {
-  if (vec && d < hd) {
-    if (type == DEFER_GPU_F32) {
-      const v4f* q = reinterpret_cast<const v4f*>(static_cast<const float*>(p) + i0 + d);
-      const v4f a = q[0], b = q[1];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = a[e];
-        y[4 + e] = b[e];
-      }
-    } else {
-      const v4i w = *reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(p) + i0 + d);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint16_t h = (uint16_t)((uint32_t)w[e / 2] >> (16 * (e % 2)));
-        y[e] = type == DEFER_GPU_BF16 ? __builtin_bit_cast(float, (uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (uint32_t e = 0; e < 8; ++e) y[e] = d + e < hd ? load_value(p, i0 + d + e, type) : 0.0f;
-}
-__device__ __forceinline__ void store8(void* p, int64_t i0, uint32_t d, uint32_t hd, uint32_t type, bool vec, const float* y) {
-  if (vec && d < hd) {
-    if (type == DEFER_GPU_F32) {
-      v4f* q = reinterpret_cast<v4f*>(static_cast<float*>(p) + i0 + d);
-      q[0] = v4f{y[0], y[1], y[2], y[3]};
-      q[1] = v4f{y[4], y[5], y[6], y[7]};
-    } else {
-      v4i w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint16_t lo = type == DEFER_GPU_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[2 * e]) : __builtin_bit_cast(uint16_t, (_Float16)y[2 * e]);
-        const uint16_t hi = type == DEFER_GPU_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y[2 * e + 1]) : __builtin_bit_cast(uint16_t, (_Float16)y[2 * e + 1]);
-        w[e] = (int)((uint32_t)lo | (uint32_t)hi << 16);
-      }
-      *reinterpret_cast<v4i*>(static_cast<uint16_t*>(p) + i0 + d) = w;
-    }
-    return;
-  }
-#pragma unroll
-  for (uint32_t e = 0; e < 8; ++e)
-    if (d + e < hd) store_value(p, i0 + d + e, type, y[e]);
-}
 
 // A workgroup owns the new rows of 16 positions of a page, one head. 16 lanes
 // take a row's key or value, 8 values each: maximum, scale, codes; keys go out as they are,
@@ -914,6 +738,7 @@ struct AttnArgs {
   int64_t hs;
   uint32_t hidden_len;
   float* part;  // [rows][nh][units][2 + dp]: maximum, sum, accumulators
+  const int32_t* parent;  // [rows] (TREE)
 };
 
 // Four signed base-256 digits of x, one a byte: x = sum of byte_i 256^i.
@@ -933,9 +758,44 @@ __device__ __forceinline__ void join_weights(float& M, float m, float* x, float*
   M = mn;
 }
 
+// A sequence's drafted rows as a tree, a row each lane: the rows that are its
+// own or above it. A parent that is no earlier row is none: the row hangs on the
+// history. Each step doubles how far up a row has looked.
+struct Tree {
+  uint64_t path;
+  __device__ __forceinline__ Tree(const int32_t* parent, const Span& sp) {
+    const int lane = threadIdx.x % WAVE;
+    int up = lane < sp.n ? parent[sp.start + lane] : -1;
+    up = up < lane ? up : -1;
+    path = 1ull << lane;
+    while (__any(up >= 0)) {
+      const int from = max(up, 0), above = __shfl(up, from);
+      const uint64_t more = __shfl((unsigned long long)path, from);
+      if (up >= 0) {
+        path |= more;
+        up = above;
+      }
+    }
+  }
+  // how many rows are above the lane's own
+  __device__ __forceinline__ int depth() const { return __popcll(path) - 1; }
+  // the position of row j, which is as far behind the history as the row is deep; -1: it has none
+  __device__ __forceinline__ int64_t pos(const Span& sp, uint32_t j) const {
+    const int64_t history = (int64_t)sp.len - sp.n, d = __shfl(depth(), (int)j);
+    return history < 0 || j >= MAX_TREE ? -1 : history + d;
+  }
+};
+struct NoTree {
+  __device__ __forceinline__ NoTree(const int32_t*, const Span&) {}
+  __device__ __forceinline__ int64_t pos(const Span& sp, uint32_t j) const { return sp.pos((int)j); }
+};
+
 enum AttnMode { DIRECT, SPLIT, GROUP };
 constexpr uint32_t SPLIT_WAVES = 4096;
 constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: rows of four heads on other banks
+constexpr int PATH_LDS = 3 * 4 * PAGE * 4;  // a tile's scores, value scales and marks by position (TREE)
+// Bytes of LDS of a wave's probabilities.
+constexpr size_t attn_lds(uint32_t R, bool tree) { return R * 16 * P_ROW * (tree ? 2 : 1) + (tree ? PATH_LDS : 0); }
 
 // What a wave does: the attention of R tiles of four (row, query head) pairs
 // of one sequence and cache head, over blocks of 64 positions.
@@ -985,14 +845,22 @@ constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: r
 // in L1). SPLIT: a few units for each wave, left in the workspace for
 // k_attn_join. GROUP: the units of a tile are the waves of one workgroup, which
 // joins them through LDS.
-template <int KC, int R, AttnMode MODE>
+//
+// TREE: rows are nodes of a tree. Each has the history and the path from there
+// down to itself, which it meets at the positions that the path would have alone:
+// blocks before the history's end are those of every row; in the others the
+// scores of the nodes' own places go through LDS to the path's positions, the
+// probabilities back from there. Sums over a block's positions of digits times
+// codes are exact, so the places' order changes nothing: the bits are those of
+// the path alone.
+template <int KC, int R, AttnMode MODE, bool TREE>
 __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 1 ? 3 : MODE != GROUP && (KC == 1 || (KC == 2 && R == 1)) ? 2 : 1) void k_attn(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
   constexpr bool AHEAD = R == 1 && KC <= 2 && MODE != GROUP;  // the next values wait in registers of their own
   extern __shared__ __align__(16) uint8_t lds[];  // [waves][R][16][P_ROW], GROUP: then [4 R][units][2 + DP] floats
   const uint32_t lane = threadIdx.x % WAVE, n16 = lane % 16, quad = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
-  uint8_t* pl = lds + wave * R * 16 * P_ROW;
+  uint8_t* pl = lds + wave * attn_lds(R, TREE);
 
   // which wave does what: (tile, unit) slowest, (sequence, cache head) fastest
   const uint32_t shs = a.r.sequences * a.p.heads;
@@ -1011,6 +879,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
   }
   if (MODE == SPLIT ? tile >= a.tiles : item >= a.tiles) return;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
+  const typename std::conditional<TREE, Tree, NoTree>::type tree(a.parent, sp);
   const uint32_t pair0 = tile * 4 * R;
   if (sp.n <= 0 || pair0 >= (uint32_t)sp.n * a.group) return;
   const int32_t* table;
@@ -1023,7 +892,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint32_t j = (pair0 + 4 * r + quad) / a.group;
-    const int64_t t = j < (uint32_t)sp.n ? min(sp.pos((int)j), a.most_len - 1) : -1;
+    const int64_t at = tree.pos(sp, j), t = j < (uint32_t)sp.n ? min(at, a.most_len - 1) : -1;  // (by all lanes)
     pos[r] = t < 0 ? -1 : (int)t;
     max_pos = max(max_pos, pos[r]);
     min_pos = min(min_pos, pos[r] < 0 ? 0x7fffffff : pos[r]);
@@ -1152,6 +1021,42 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
       for (int t = 0; t < DT; ++t) A[r][t] = acc[r][t] = 0.0f;
     }
 
+    // A block's scores s of the positions that a lane sees, with their value scales,
+    // as the digits of their probabilities; xw and be: the weights of what came
+    // before and of this block. vbad: what makes the sum NaN (WHOLE).
+    auto weigh = [&](auto whole, int r, const float* s, const bool* see, const v4f& vs, float vbad, float* xw, float* be, uint32_t* y) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      float w[4];
+      const float top = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+      const bool none = !WHOLE && top == -INFINITY;
+      const float m0 = none ? 0.0f : top * fabsf(sq[r]);
+      const bool sharp = fabsf(m0) > 0x1p26f;
+      const float before = sharp ? top : 0.0f, behind = sharp ? 0.0f : m0;
+      float lp = vbad;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float p = exp2_of(fmaf(s[j] - before, fabsf(sq[r]), -behind));
+        if (!WHOLE) {
+          p = see[j] ? p : 0.0f;
+          lp += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
+          w[j] = see[j] ? p * vs[j] : 0.0f;
+        } else {
+          lp += p;
+          w[j] = p * vs[j];
+        }
+      }
+      int ex = 0;
+      (void)frexpf(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))), &ex);
+      ex = max(ex, -96);
+      const float up = ldexpf(1.0f, 30 - ex);
+      float yw;
+      join_weights(m[r], none ? -INFINITY : m0, xw, &yw);
+      *be = yw * ldexpf(1.0f, ex - 30);
+      l[r] = fmaf(lp, yw, l[r] * *xw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = digits(to_int(w[j] * up));
+    };
+
     // A block whose codes have been loaded: WHOLE if every row sees all of it.
     // next: the page to load meanwhile, or -1.
     auto block = [&](auto whole, int b, int next) {
@@ -1182,7 +1087,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
           load_k(next);
           if (AHEAD) load_v(next, vn);
         }
-        float s[4], w[4];
+        float s[4];
         bool see[4];
         const float unit = sq[r] < 0.0f ? 1.0f : 0x1p-45f;
 #pragma unroll
@@ -1191,35 +1096,8 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
           const float x = undigit(d[j]) * unit * ks[j];
           s[j] = see[j] ? x : -INFINITY;
         }
-        const float top = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-        const bool none = !WHOLE && top == -INFINITY;
-        const float m0 = none ? 0.0f : top * fabsf(sq[r]);
-        const bool sharp = fabsf(m0) > 0x1p26f;
-        const float before = sharp ? top : 0.0f, behind = sharp ? 0.0f : m0;
-        float lp = vbad;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float p = exp2_of(fmaf(s[j] - before, fabsf(sq[r]), -behind));
-          if (!WHOLE) {
-            p = see[j] ? p : 0.0f;
-            lp += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
-            w[j] = see[j] ? p * vs[j] : 0.0f;
-          } else {
-            lp += p;
-            w[j] = p * vs[j];
-          }
-        }
-        int ex = 0;
-        (void)frexpf(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))), &ex);
-        ex = max(ex, -96);
-        const float up = ldexpf(1.0f, 30 - ex);
-        float yw;
-        join_weights(m[r], none ? -INFINITY : m0, &xw[r], &yw);
-        be[r] = yw * ldexpf(1.0f, ex - 30);
-        l[r] = fmaf(lp, yw, l[r] * xw[r]);
         uint32_t y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = digits(to_int(w[j] * up));
+        weigh(whole, r, s, see, vs, vbad, &xw[r], &be[r], y);
         uint32_t* pw = reinterpret_cast<uint32_t*>(pl + (16 * r + 4 * quad) * P_ROW) + n16;
         uint32_t by_digit[4];
         transpose4(y, by_digit);
@@ -1247,6 +1125,128 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
       }
     };
 
+    // A block of a path's positions, behind the history's end or around it. The nodes
+    // on it are in this place's page or the next (a tree has no more than 64 rows).
+    const int history = (int)min((int64_t)sp.len - sp.n, (int64_t)0x7fffffff), first_path = TREE ? history / PAGE : 0x7fffffff;
+    auto path_block = [&](int b, int page, int page_behind, int next) {
+      if constexpr (TREE) {
+        float x[2][R][4];
+        int at[2][4];  // the position within the block of a place's node
+        uint32_t seen[2][R];
+        v4f vsp[2];
+        const int depth = tree.depth();
+#pragma unroll
+        for (int pb = 0; pb < 2; ++pb) {
+          if (pb) {
+            if (page_behind >= 0) load_k(page_behind);
+          }
+          vsp[pb] = vsn;
+          const v4f kp = ksn;
+          const bool there = (pb ? page_behind : page) >= 0;
+          bool on[4];
+          int node[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = (b + pb) * PAGE + 4 * n16 + j;
+            node[j] = t - history;
+            const int d = __shfl(depth, node[j] & (WAVE - 1));
+            at[pb][j] = (node[j] < 0 ? t : history + d) - b * PAGE;
+            on[j] = there && node[j] < min(sp.n, (int)MAX_TREE) && at[pb][j] >= 0 && at[pb][j] < PAGE;
+            if (hid && on[j]) on[j] = !((uint32_t)t < a.hidden_len && hid[t] != 0);
+          }
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float unit = sq[r] < 0.0f ? 1.0f : 0x1p-45f;
+            const uint64_t path = __shfl((unsigned long long)tree.path, (int)((pair0 + 4 * r + quad) / a.group) & (WAVE - 1));
+            seen[pb][r] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              v4i d = {0, 0, 0, 0};
+              if (there) {
+#pragma unroll
+                for (int kk = 0; kk < KC; ++kk) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[r][kk], k[j][kk], d, 0, 0, 0);
+              }
+              x[pb][r][j] = undigit(d) * unit * kp[j];
+              const bool see = on[j] && b * PAGE + at[pb][j] <= ps[r] && (node[j] < 0 || (path >> (node[j] & (WAVE - 1)) & 1));
+              seen[pb][r] |= (uint32_t)see << j;
+            }
+          }
+        }
+        float* const sl = reinterpret_cast<float*>(pl + 2 * R * 16 * P_ROW) + quad * PAGE;  // this quad's pair
+        float* const vl = sl + 4 * PAGE;
+        uint32_t* const ml = reinterpret_cast<uint32_t*>(vl + 4 * PAGE);
+        float xw[R], be[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          *reinterpret_cast<v4i*>(ml + 4 * n16) = v4i{0, 0, 0, 0};
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int pb = 0; pb < 2; ++pb)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (seen[pb][r] >> j & 1) {
+                sl[at[pb][j]] = x[pb][r][j];
+                vl[at[pb][j]] = vsp[pb][j];
+                ml[at[pb][j]] = 1;
+              }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          const v4f sv = *reinterpret_cast<const v4f*>(sl + 4 * n16), vv = *reinterpret_cast<const v4f*>(vl + 4 * n16);
+          const v4i mv = *reinterpret_cast<const v4i*>(ml + 4 * n16);
+          float s[4];
+          bool see[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            see[j] = mv[j] != 0;
+            s[j] = see[j] ? sv[j] : -INFINITY;
+          }
+          uint32_t y[4];
+          weigh(std::false_type(), r, s, see, vv, 0.0f, &xw[r], &be[r], y);
+          *reinterpret_cast<v4i*>(ml + 4 * n16) = v4i{(int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int pb = 0; pb < 2; ++pb) {
+            uint32_t p[4], by_digit[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = seen[pb][r] >> j & 1 ? ml[at[pb][j]] : 0;
+            transpose4(p, by_digit);
+            uint32_t* pw = reinterpret_cast<uint32_t*>(pl + (16 * (2 * r + pb) + 4 * quad) * P_ROW) + n16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pw[i * P_ROW / 4] = by_digit[i];
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        }
+        v4i pa[R][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int pb = 0; pb < 2; ++pb)
+            pa[r][pb] = *reinterpret_cast<const v4i*>(pl + (16 * (2 * r + pb) + n16) * P_ROW + quad * 16);
+        const int8_t* const vb = v0 + (size_t)max(page_behind, 0) * a.p.heads * PAGE * DP;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          v4i vt = {0, 0, 0, 0};
+          if (page_behind >= 0) vt = *reinterpret_cast<const v4i*>(vb + 16 * t * PAGE);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            v4i o = {0, 0, 0, 0};
+            if (page >= 0) o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[r][0], v[t], o, 0, 0, 0);
+            if (page_behind >= 0) o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[r][1], vt, o, 0, 0, 0);
+            acc[r][t] = fmaf(undigit(o), be[r], acc[r][t] * xw[r]);
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (next >= 0) {
+          load_k(next);
+          load_v(next, v);
+        }
+      }
+    };
+
     const int bpu = ul / PAGE, blocks = pmax < 0 ? 0 : pmax / PAGE + 1;
     const int du = MODE == GROUP ? (int)waves : 1;
     int u = MODE == SPLIT ? (int)(item % chunks * a.per_wave) : MODE == GROUP ? (int)wave : 0;
@@ -1271,7 +1271,10 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
       const bool unit_ends = b + 1 == blocks || (b + 1) % bpu == 0;
       const int bn = unit_ends ? (u + du) * bpu : b + 1;
       const int next = bn < blocks && (!unit_ends || u + du < u_end) ? page_at(bn) : -1;
-      if (page >= 0) {
+      if (TREE && b >= first_path) {
+        const int last = (history + min(sp.n, (int)MAX_TREE) - 1) / PAGE;  // the last place's page
+        path_block(b, page, b < last ? page_at(b + 1) : -1, next);
+      } else if (page >= 0) {
         if (!hid && b * PAGE + PAGE - 1 <= pmin)
           block(std::true_type(), b, next);
         else
@@ -1293,7 +1296,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
           } else if (ps[r] >= 0 && u < unit_count(ps[r])) {
             const uint32_t pr = pair0 + 4 * r + quad;
             float* o = MODE == SPLIT ? a.part + (((size_t)(sp.start + pr / a.group) * a.nh + g * a.group + pr % a.group) * a.units + u) * (2 + DP)
-                                     : reinterpret_cast<float*>(lds + waves * R * 16 * P_ROW) +
+                                     : reinterpret_cast<float*>(lds + waves * attn_lds(R, TREE)) +
                                            ((4 * r + quad) * a.units + u) * (2 + DP);
             if (n16 == 0) {
               o[0] = m[r];
@@ -1330,11 +1333,11 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
   }
   if (MODE == GROUP) {
     __syncthreads();
-    const float* parts = reinterpret_cast<const float*>(lds + waves * R * 16 * P_ROW);
+    const float* parts = reinterpret_cast<const float*>(lds + waves * attn_lds(R, TREE));
     for (uint32_t i = threadIdx.x; i < 4u * R * DP; i += blockDim.x) {
-      const uint32_t pr = pair0 + i / DP, j = pr / a.group, d = i % DP;
+      const uint32_t pr = pair0 + i / DP, j = pr / a.group, d = i % DP;  // (pr: the same in all lanes)
       if (j >= (uint32_t)sp.n) continue;
-      const int n = unit_count(min(sp.pos((int)j), a.most_len - 1));
+      const int n = unit_count(min(tree.pos(sp, j), a.most_len - 1));
       const float* p = parts + i / DP * a.units * (2 + DP);
       float M = -INFINITY, L = 0.0f, A = 0.0f;
       for (int u = 0; u < n; ++u, p += 2 + DP) {
@@ -1355,11 +1358,13 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 // sum, the accumulators of 32 units are on their way at a time. Three dependent
 // reads of what other XCDs wrote: 10 us for 11 x 32 heads of 47 units (8.6 MB);
 // 64 units at a time changed nothing.
+template <bool TREE>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   const uint32_t h = blockIdx.x % a.nh, j = blockIdx.x / a.nh % a.r.most_rows, seq = blockIdx.x / a.nh / a.r.most_rows;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
   if (j >= (uint32_t)sp.n) return;
-  const int64_t pos = min(sp.pos((int)j), a.most_len - 1);
+  const typename std::conditional<TREE, Tree, NoTree>::type tree(a.parent, sp);
+  const int64_t pos = min(tree.pos(sp, j), a.most_len - 1);
   const uint32_t row = sp.start + j, d = threadIdx.x, dp = a.p.dp, lane = threadIdx.x % WAVE;
   const float* p = a.part + ((size_t)row * a.nh + h) * a.units * (2 + dp);
   const int n = unit_count(pos);
@@ -1385,25 +1390,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   if (d < a.hd) store_value(a.out, (int64_t)row * a.os + (int64_t)h * a.hd + d, a.type, A * inv);
 }
 
-// Zeros for the rows of a call without sequences.
-__global__ __launch_bounds__(256) void k_zero_rows(void* out, int64_t stride, uint32_t n, uint32_t type) {
-  for (uint32_t i = threadIdx.x; i < n; i += 256) store_value(out, (int64_t)blockIdx.x * stride + i, type, 0.0f);
-}
-
 // ------------------------------------------------------------- launches
-
-// (The launch's own status: the runtime's last error may be that of an earlier
-// call of the program's, and stays there for it.)
-template <class A>
-struct Same {
-  typedef A type;
-};
-template <class... A>
-int launch(void (*kernel)(A...), dim3 grid, dim3 block, size_t lds, hipStream_t s, typename Same<A>::type... args) {
-  void* p[] = {&args...};
-  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, p, lds, s);
-  return e == hipSuccess ? DEFER_GPU_OK : defer_gpu_fail_(DEFER_GPU_E_HIP, "launch: %s", hipGetErrorString(e));
-}
 
 template <class T, bool NORM>
 int rows_launch_as(const NormArgs& a, uint32_t rows, hipStream_t s) {
@@ -1431,16 +1418,16 @@ int rows_launch(uint32_t type, const NormArgs& a, uint32_t rows, hipStream_t s) 
   return rows_launch_as<_Float16, NORM>(a, rows, s);
 }
 
-template <int R, AttnMode MODE>
+template <int R, AttnMode MODE, bool TREE>
 int attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t lds, hipStream_t s) {
   const uint32_t kc = a.p.dp / 64;
   if constexpr (R <= 2)
-    if (kc == 1) return launch(k_attn<1, R, MODE>, blocks, threads, lds, s, a);
-  if (kc == 2) return launch(k_attn<2, R, MODE>, blocks, threads, lds, s, a);
+    if (kc == 1) return launch(k_attn<1, R, MODE, TREE>, blocks, threads, lds, s, a);
+  if (kc == 2) return launch(k_attn<2, R, MODE, TREE>, blocks, threads, lds, s, a);
   if constexpr (MODE != GROUP && R <= 2)
-    if (kc == 3) return launch(k_attn<3, R, MODE>, blocks, threads, lds, s, a);
+    if (kc == 3) return launch(k_attn<3, R, MODE, TREE>, blocks, threads, lds, s, a);
   if constexpr (MODE != GROUP && R == 1)
-    if (kc == 4) return launch(k_attn<4, R, MODE>, blocks, threads, lds, s, a);
+    if (kc == 4) return launch(k_attn<4, R, MODE, TREE>, blocks, threads, lds, s, a);
   return defer_gpu_fail_(DEFER_GPU_E_INVALID, "no attention kernel for head_dim %u", a.hd);
 }
 
@@ -1455,7 +1442,7 @@ struct Plan {
   uint32_t R, tiles, units, per_wave, waves;  // tiles of 4 R pairs; units of a row at most, of a wave; waves of a workgroup
   size_t lds, workspace;
 };
-Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint32_t most_len) {
+Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint32_t most_len, bool tree) {
   const uint32_t pairs = (uint32_t)pairs_of(r, heads, kv_heads);
   Plan p;
   // Tiles share the codes a wave has loaded, so the more the better, as far as
@@ -1491,7 +1478,7 @@ Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint
   } else {
     p.mode = DIRECT;
   }
-  p.lds = p.waves * p.R * 16 * P_ROW + (p.mode == GROUP ? 4 * (size_t)p.R * p.units * (2 + dp) * sizeof(float) : 0);
+  p.lds = p.waves * attn_lds(p.R, tree) + (p.mode == GROUP ? 4 * (size_t)p.R * p.units * (2 + dp) * sizeof(float) : 0);
   return p;
 }
 
@@ -1603,11 +1590,22 @@ int kv_read(const Pages& p, const Rows& r, uint32_t type, void* k, void* v, uint
   return launch(k_kv_read, kv_grid(p, and_one), r.most_rows <= 8 ? 64 : 256, 0, s, a);
 }
 
+template <bool TREE>
+static int attn_dispatch(const AttnArgs& a, const Plan& pl, uint32_t nb, uint32_t nt, hipStream_t s) {
+  if (pl.mode == SPLIT) {
+    const int rc = pl.R == 1 ? attn_launch<1, SPLIT, TREE>(a, nb, nt, pl.lds, s) : attn_launch<2, SPLIT, TREE>(a, nb, nt, pl.lds, s);
+    return rc ? rc : launch(k_attn_join<TREE>, a.r.sequences * a.r.most_rows * a.nh, a.p.dp, 0, s, a);
+  }
+  if (pl.mode == GROUP)
+    return pl.R == 1 ? attn_launch<1, GROUP, TREE>(a, nb, nt, pl.lds, s) : attn_launch<2, GROUP, TREE>(a, nb, nt, pl.lds, s);
+  if (pl.R == 1) return attn_launch<1, DIRECT, TREE>(a, nb, nt, pl.lds, s);
+  return pl.R == 2 ? attn_launch<2, DIRECT, TREE>(a, nb, nt, pl.lds, s) : attn_launch<4, DIRECT, TREE>(a, nb, nt, pl.lds, s);
+}
+
 size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len) {
   if (!r.rows || !r.sequences || !r.most_rows || pairs_of(r, heads, kv_heads) > MOST_PAIRS) return 0;
   const uint32_t dp = padded(head_dim);
-  const Plan pl = plan_of(r, heads, kv_heads, dp, most_len);
-  return pl.workspace;
+  return plan_of(r, heads, kv_heads, dp, most_len, false).workspace;
 }
 
 int attention(const Pages& p, const Rows& r, const Attention& in, void* workspace, size_t workspace_bytes,
@@ -1618,7 +1616,7 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   }
   if (pairs_of(r, in.heads, p.heads) > MOST_PAIRS)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
-  const Plan pl = plan_of(r, in.heads, p.heads, p.dp, in.most_len);
+  const Plan pl = plan_of(r, in.heads, p.heads, p.dp, in.most_len, in.parent != nullptr);
   const size_t need = attention_workspace(r, in.heads, p.heads, in.head_dim, in.most_len);
   if (need && (!workspace || workspace_bytes < need))
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "attention needs a workspace of %zu bytes, got %zu", need,
@@ -1643,6 +1641,7 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   a.hs = in.hidden_stride;
   a.hidden_len = in.hidden_len;
   a.part = static_cast<float*>(workspace);
+  a.parent = in.parent;
   a.clear = in.clear && r.row_start;
   const size_t vs = in.type == DEFER_GPU_F32 ? 4 : 2;
   a.q_vec = in.head_dim % 16 == 0 && ((uintptr_t)in.q | (uintptr_t)(in.q_stride * (int64_t)vs)) % 16 == 0;
@@ -1651,14 +1650,7 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   if (blocks * pl.waves * WAVE > MAX_THREADS)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
   const uint32_t nb = (uint32_t)blocks, nt = pl.waves * WAVE;
-  if (pl.mode == SPLIT) {
-    const int rc = pl.R == 1 ? attn_launch<1, SPLIT>(a, nb, nt, pl.lds, s) : attn_launch<2, SPLIT>(a, nb, nt, pl.lds, s);
-    return rc ? rc : launch(k_attn_join, r.sequences * r.most_rows * in.heads, p.dp, 0, s, a);
-  }
-  if (pl.mode == GROUP)
-    return pl.R == 1 ? attn_launch<1, GROUP>(a, nb, nt, pl.lds, s) : attn_launch<2, GROUP>(a, nb, nt, pl.lds, s);
-  if (pl.R == 1) return attn_launch<1, DIRECT>(a, nb, nt, pl.lds, s);
-  return pl.R == 2 ? attn_launch<2, DIRECT>(a, nb, nt, pl.lds, s) : attn_launch<4, DIRECT>(a, nb, nt, pl.lds, s);
+  return in.parent ? attn_dispatch<true>(a, pl, nb, nt, s) : attn_dispatch<false>(a, pl, nb, nt, s);
 }
 
 }  // namespace q8
@@ -1666,24 +1658,6 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
 // ------------------------------------------------------------- C entry points
 
 using namespace q8;
-
-#define Q8_REQUIRE(cond, ...)                                              \
-  do {                                                                     \
-    if (!(cond)) return defer_gpu_fail_(DEFER_GPU_E_INVALID, __VA_ARGS__); \
-  } while (0)
-
-static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
-static size_t value_size(uint32_t type) { return type == DEFER_GPU_F32 ? 4 : 2; }
-static bool aligned_to(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
-
-static int check_rows_values(uint32_t type, const void* x, int64_t stride, uint32_t rows, uint32_t n, const char* what) {
-  Q8_REQUIRE(type <= DEFER_GPU_F16, "value type %u", type);
-  Q8_REQUIRE(n >= 1 && n <= 0x7fffffffu && rows <= MAX_THREADS / 1024, "%s: %u rows of %u values", what, rows, n);
-  Q8_REQUIRE(rows == 0 || x, "%s is null", what);
-  Q8_REQUIRE(rows <= 1 || stride >= (int64_t)n, "%s: rows of %u values %lld apart", what, n, (long long)stride);
-  Q8_REQUIRE(aligned_to(x, value_size(type)), "%s is not aligned to its type", what);
-  return DEFER_GPU_OK;
-}
 
 extern "C" int defer_gpu_q8_quantize(uint32_t type, const void* x, int64_t x_stride, uint32_t rows, uint32_t n,
                                      int8_t* codes, float* scale, void* stream) {
@@ -1730,29 +1704,6 @@ extern "C" int defer_gpu_q8_linear(const int8_t* x, int64_t x_stride, const floa
   return linear(x, x_stride, x_scale, w, w_stride, w_scale, rows, m, k, type, y, y_stride, (hipStream_t)stream);
 }
 
-static int check_pages(const defer_gpu_q8_pages* p, const defer_gpu_q8_rows* r, Pages* pages, Rows* rows) {
-  Q8_REQUIRE(p && r, "null argument");
-  Q8_REQUIRE(p->head_dim >= 1 && p->head_dim <= MAX_HEAD_DIM, "head_dim %u: 1 to %u", p->head_dim, MAX_HEAD_DIM);
-  Q8_REQUIRE(p->heads >= 1 && p->heads <= 65535, "%u cache heads", p->heads);
-  Q8_REQUIRE(p->pages <= 0x7fffffffu && p->table_width <= 0x7fffffffu / PAGE, "%u pages, %u a sequence", p->pages,
-             p->table_width);
-  Q8_REQUIRE(r->rows <= MAX_THREADS / 1024 && r->sequences <= MAX_THREADS / 1024, "%u rows of %u sequences", r->rows, r->sequences);
-  Q8_REQUIRE(r->most_rows <= r->rows, "most_rows %u of %u rows", r->most_rows, r->rows);
-  *rows = Rows{r->row_start, r->kv_len, r->sequences, r->rows, r->most_rows};
-  *pages = Pages{p->keys, p->values, p->key_scale, p->value_scale, p->table, p->pages, p->heads,
-                 padded(p->head_dim), p->table_width, nullptr, 0};
-  if (!r->rows || !r->sequences || !r->most_rows) return DEFER_GPU_OK;
-  Q8_REQUIRE(r->row_start || r->rows == r->sequences, "%u rows of %u sequences without row_start", r->rows, r->sequences);
-  Q8_REQUIRE(r->kv_len, "kv_len is null");
-  Q8_REQUIRE(p->table_width == 0 || p->table, "table is null");
-  Q8_REQUIRE(p->pages == 0 || (p->keys && p->values && p->key_scale && p->value_scale), "null pages");
-  Q8_REQUIRE(aligned16(p->keys) && aligned16(p->values) && aligned16(p->key_scale) && aligned16(p->value_scale),
-             "pages are not 16-byte aligned");
-  Q8_REQUIRE(((uint64_t)r->sequences + 1) * p->heads * kv_runs(r->most_rows) <= MAX_THREADS / 256,
-             "too many rows for one call");
-  return DEFER_GPU_OK;
-}
-
 extern "C" int defer_gpu_q8_kv_write(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
                                      const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* stream) {
   Pages p;
@@ -1780,13 +1731,6 @@ extern "C" int defer_gpu_q8_kv_read(const defer_gpu_q8_pages* pages, const defer
   return kv_read(p, r, type, k, v, pages->head_dim, (hipStream_t)stream);
 }
 
-static int check_heads(const defer_gpu_q8_pages* p, uint32_t q_heads, uint32_t most_len) {
-  Q8_REQUIRE(q_heads >= 1 && q_heads <= 65535 && q_heads % p->heads == 0, "%u query heads on %u cache heads", q_heads,
-             p->heads);
-  Q8_REQUIRE(most_len <= 0x7fffffffu, "most_len %u", most_len);
-  return DEFER_GPU_OK;
-}
-
 extern "C" size_t defer_gpu_q8_attention_workspace(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
                                                    uint32_t q_heads, uint32_t most_len) {
   if (!pages || !rows || !pages->heads || !q_heads || pages->head_dim > MAX_HEAD_DIM) return 0;
@@ -1794,11 +1738,10 @@ extern "C" size_t defer_gpu_q8_attention_workspace(const defer_gpu_q8_pages* pag
   return attention_workspace(r, q_heads, pages->heads, pages->head_dim, most_len);
 }
 
-extern "C" int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
-                                      const void* q, int64_t q_stride, uint32_t q_heads, uint32_t most_len,
-                                      float scale, const uint8_t* hidden, int64_t hidden_stride,
-                                      uint32_t hidden_len, void* out, int64_t out_stride, uint32_t clear,
-                                      void* workspace, size_t workspace_bytes, void* stream) {
+static int attend(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type, const void* q,
+                  int64_t q_stride, uint32_t q_heads, const int32_t* parent, uint32_t most_len, float scale,
+                  const uint8_t* hidden, int64_t hidden_stride, uint32_t hidden_len, void* out, int64_t out_stride,
+                  uint32_t clear, void* workspace, size_t workspace_bytes, void* stream) {
   Pages p;
   Rows r;
   int rc = check_pages(pages, rows, &p, &r);
@@ -1814,6 +1757,27 @@ extern "C" int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const def
              hidden_len, (long long)hidden_stride);
   Q8_REQUIRE(aligned16(workspace), "workspace is not 16-byte aligned");
   Attention a{type, q, q_stride, out, out_stride, q_heads, pages->head_dim, scale, most_len, hidden, hidden_stride,
-              hidden_len, clear != 0};
+              hidden_len, clear != 0, parent};
   return attention(p, r, a, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
+                                      const void* q, int64_t q_stride, uint32_t q_heads, uint32_t most_len,
+                                      float scale, const uint8_t* hidden, int64_t hidden_stride,
+                                      uint32_t hidden_len, void* out, int64_t out_stride, uint32_t clear,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  return attend(pages, rows, type, q, q_stride, q_heads, nullptr, most_len, scale, hidden, hidden_stride, hidden_len, out,
+                out_stride, clear, workspace, workspace_bytes, stream);
+}
+
+extern "C" int defer_gpu_q8_tree_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
+                                           const void* q, int64_t q_stride, uint32_t q_heads, const int32_t* parent,
+                                           uint32_t most_len, float scale, const uint8_t* hidden, int64_t hidden_stride,
+                                           uint32_t hidden_len, void* out, int64_t out_stride, uint32_t clear,
+                                           void* workspace, size_t workspace_bytes, void* stream) {
+  Q8_REQUIRE(!rows || rows->most_rows <= MAX_TREE, "%u rows of a sequence: at most %u", rows->most_rows, MAX_TREE);
+  Q8_REQUIRE(!rows || rows->rows == 0 || parent, "parent is null");
+  Q8_REQUIRE(aligned_to(parent, 4), "parent is not aligned to its type");
+  return attend(pages, rows, type, q, q_stride, q_heads, parent, most_len, scale, hidden, hidden_stride, hidden_len, out,
+                out_stride, clear, workspace, workspace_bytes, stream);
 }

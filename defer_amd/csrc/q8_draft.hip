@@ -1,0 +1,698 @@
+// q8_draft.hip -- what a program that drafts tokens and verifies them needs
+// around the attention: rows normed, rotated and appended to the cache in one
+// launch, the log probabilities of given tokens, and the accepted path moved
+// together in the cache. (The attention of a tree of drafts is in q8.hip, beside
+// the one whose bits it has.)
+#include "q8_common.h"
+
+#include <algorithm>
+
+namespace q8 {
+
+namespace {
+
+// ------------------------------------------------------------- append
+
+struct AppendArgs {
+  Pages p;
+  Rows r;
+  const void *q, *k, *v;
+  void* out;
+  int64_t qs, ks, vs, os;
+  const int32_t* position;
+  const double* freq;
+  const void *qn, *kn;
+  double eps, factor;
+  uint32_t type, hd, nh, half;  // half: rotated pairs of a head
+  uint32_t kv_heads, q_heads;   // heads that a workgroup takes: of the cache, or of the queries
+  uint32_t kv_chunks, chunks;   // workgroups of a run for the cache's heads, and for all
+  bool interleaved, clear;
+};
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Over the 16 lanes of a DPP row, as row_max and row_sum.
+__device__ __forceinline__ double row_max64(double v) {
+  v = fmax(v, dpp64<0x128>(v));
+  v = fmax(v, dpp64<0x124>(v));
+  v = fmax(v, dpp64<0x122>(v));
+  return fmax(v, dpp64<0x121>(v));
+}
+__device__ __forceinline__ double row_sum64(double v) {
+  v += dpp64<0x128>(v);
+  v += dpp64<0x124>(v);
+  v += dpp64<0x122>(v);
+  return v + dpp64<0x121>(v);
+}
+
+// (cos, sin) of position times frequency, in 64 bits: as turns, of which the
+// whole ones go, then the quarters; what is left is within an eighth of a turn,
+// where the series to x^14 and x^15 are off by less than 2^-44. The turns are
+// products in two parts each, so that no position is too far.
+__device__ __forceinline__ double2 turn(int pos, double freq) {
+  constexpr double PER = 0.15915494309189533577, LEFT = -9.839338337591251e-18;  // 1 / (2 pi) in two parts
+  const double p = (double)pos, f = freq * PER, fl = fma(freq, PER, -f) + freq * LEFT;
+  const double h = p * f;
+  double t = (h - rint(h)) + (fma(p, f, -h) + p * fl);
+  t -= rint(t);
+  const double quarter = rint(4.0 * t), x = (t - 0.25 * quarter) * 6.28318530717958647693, x2 = x * x;
+  double s = 1.0 / 6227020800.0, c = -1.0 / 87178291200.0;
+  s = fma(s, x2, -1.0 / 39916800.0);
+  s = fma(s, x2, 1.0 / 362880.0);
+  s = fma(s, x2, -1.0 / 5040.0);
+  s = fma(s, x2, 1.0 / 120.0);
+  s = fma(s, x2, -1.0 / 6.0);
+  s = fma(s * x2, x, x);
+  c = fma(c, x2, 1.0 / 479001600.0);
+  c = fma(c, x2, -1.0 / 3628800.0);
+  c = fma(c, x2, 1.0 / 40320.0);
+  c = fma(c, x2, -1.0 / 720.0);
+  c = fma(c, x2, 1.0 / 24.0);
+  c = fma(c, x2, -0.5);
+  c = fma(c, x2, 1.0);
+  const int n = (int)quarter & 3;
+  const double a = n & 1 ? s : c, b = n & 1 ? c : s;
+  return double2{n == 1 || n == 2 ? -a : a, n >= 2 ? -b : b};
+}
+
+// A lane's 8 values from d = 8 n16 on (and the 8 from 128 + d on, where the head
+// has more than 128): normed, rotated. cs: the row's (cos, sin) of each pair.
+// VEC: 8 values are aligned, and so are the 8 they are paired with.
+template <bool VEC>
+__device__ __forceinline__ void turned(const AppendArgs& a, const void* p, int64_t at, const void* norm, const double2* cs,
+                                       uint32_t n16, double (*y)[8]) {
+  const uint32_t hd = a.hd, rotated = 2 * a.half;
+  float x[2][8], xp[2][8];  // the values, and the halves' other ones
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h) {
+    if (h && hd <= 128) break;
+    const uint32_t d = 128 * h + 8 * n16;
+    load8(p, at, d, hd, a.type, VEC, x[h]);
+    if (a.interleaved) continue;
+    if (VEC) {
+      if (d < rotated) load8(p, at, d < a.half ? d + a.half : d - a.half, hd, a.type, true, xp[h]);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) {
+        const uint32_t i = d + e;
+        xp[h][e] = i < rotated ? load_value(p, at + (i < a.half ? i + a.half : i - a.half), a.type) : 0.0f;
+      }
+    }
+  }
+  double inv = 1.0;
+  if (norm) {
+    double ss = 0.0;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h)
+      if (h == 0 || hd > 128)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fma((double)x[h][e], (double)x[h][e], ss);
+    inv = 1.0 / sqrt(row_sum64(ss) / (double)hd + a.eps);
+  }
+#pragma unroll
+  for (uint32_t h = 0; h < 2; ++h) {
+    if (h && hd <= 128) break;
+    const uint32_t d = 128 * h + 8 * n16;
+    double z[8];
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+      z[e] = (double)x[h][e];
+      if (norm && d + e < hd) z[e] *= (double)load_value(norm, d + e, a.type) * inv;
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+      const uint32_t i = d + e;
+      y[h][e] = z[e];
+      if (i >= rotated) continue;
+      const bool second = a.interleaved ? e % 2 : i >= a.half;
+      const uint32_t pair = a.interleaved ? i / 2 : second ? i - a.half : i;
+      double o = a.interleaved ? z[e ^ 1] : (double)xp[h][e];
+      if (norm && !a.interleaved) o *= (double)load_value(norm, second ? i - a.half : i + a.half, a.type) * inv;
+      const double2 c = cs[pair];
+      y[h][e] = fma(z[e], c.x, second ? o * c.y : -(o * c.y));
+    }
+  }
+}
+
+// A workgroup takes the rows of 16 places of a page (as k_kv_write's, whose
+// places they are) and some heads: of the cache's keys and values, or of the
+// queries. The rows' angles are formed once, 64 bits, in LDS; then 16 lanes take
+// a row's head. Keys, scales and codes are those of the formula in 64 bits, as
+// everywhere here.
+template <bool VEC>
+__global__ __launch_bounds__(256) void k_append(AppendArgs a) {
+  extern __shared__ __align__(16) uint8_t lds[];  // [rows][half] angles, then [heads][rows][KV_ROW] value codes
+  const uint32_t per = kv_runs(a.r.most_rows), most = min(a.r.most_rows, (uint32_t)KV_RUN);
+  const uint32_t chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks % per, seq = blockIdx.x / a.chunks / per;
+  const uint32_t n16 = threadIdx.x % 16, quad = threadIdx.x / 16, quads = blockDim.x / 16, hd = a.hd;
+  if (seq == a.r.sequences) {  // zeros for the rows of no sequence
+    const int64_t lo = span_of(a.r.row_start, a.r.kv_len, 0, a.r.rows).start;
+    const int64_t hi = max(lo, min((int64_t)a.r.row_start[seq], (int64_t)a.r.rows));
+    const int64_t n = a.nh * hd;
+    for (int64_t i = b * a.chunks + chunk; i < lo + ((int64_t)a.r.rows - hi); i += per * a.chunks) {
+      const int64_t row = i < lo ? i : hi + (i - lo);
+      for (int64_t d = threadIdx.x; d < n; d += blockDim.x) store_value(a.out, row * a.os + d, a.type, 0.0f);
+    }
+    return;
+  }
+  const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
+  auto down = [](int64_t t, int n) { return t >= 0 ? t / n : -((-t + n - 1) / n); };
+  const int64_t p0 = sp.pos(0), run = down(p0, KV_RUN) + b;
+  const int64_t t0 = max(p0, run * KV_RUN), t1 = min((int64_t)sp.len, (run + 1) * KV_RUN);
+  if (t0 >= t1) return;
+  const uint32_t n = min((uint32_t)(t1 - t0), most);  // rows
+  const int64_t row0 = sp.start + (t0 - p0);
+  double2* cs = reinterpret_cast<double2*>(lds);
+  int8_t* tile = reinterpret_cast<int8_t*>(cs + most * a.half);
+  for (uint32_t i = threadIdx.x; i < n * a.half; i += blockDim.x) {
+    const uint32_t j = i / a.half;
+    double2 c = turn(a.position ? a.position[row0 + j] : (int)(t0 + j), a.freq[i - j * a.half]);
+    cs[i] = double2{c.x * a.factor, c.y * a.factor};
+  }
+  __syncthreads();
+
+  if (chunk >= a.kv_chunks) {
+    const uint32_t h0 = (chunk - a.kv_chunks) * a.q_heads, heads = min(a.q_heads, a.nh - h0);
+    for (uint32_t i = quad; i < heads * n; i += quads) {
+      const uint32_t j = i / heads, h = h0 + i % heads;
+      double y[2][8];
+      turned<VEC>(a, a.q, (row0 + j) * a.qs + (int64_t)h * hd, a.qn, cs + j * a.half, n16, y);
+#pragma unroll
+      for (uint32_t g = 0; g < 2; ++g) {
+        if (g && hd <= 128) break;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (float)y[g][e];
+        store8(a.out, (row0 + j) * a.os + (int64_t)h * hd, 128 * g + 8 * n16, hd, a.type, VEC, o);
+      }
+    }
+    return;
+  }
+
+  // the cache's heads: keys and values that have a place and a page
+  const int64_t block = down(run, PAGE / KV_RUN);
+  const int32_t* table;
+  uint32_t width;
+  const SeqPages pool = pool_of(a.p, seq, table, width);
+  const int page = page_of(table, width, pool.pages, block);
+  if (page < 0) return;  // (places before 0 among them)
+  const uint32_t g0 = chunk * a.kv_heads, heads = min(a.kv_heads, a.p.heads - g0);
+  const int a0 = (int)(t0 - block * PAGE);  // the first row's place in its page
+  for (uint32_t i = quad; i < 2 * heads * n; i += quads) {
+    const bool value = i >= heads * n;
+    const uint32_t it = value ? i - heads * n : i, j = it / heads, gl = it % heads, g = g0 + gl;
+    const size_t hp = (size_t)page * a.p.heads + g;
+    double y[2][8];
+    if (value) {
+      float x[2][8];
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        if (h && hd <= 128) break;
+        load8(a.v, (row0 + j) * a.vs + (int64_t)g * hd, 128 * h + 8 * n16, hd, a.type, VEC, x[h]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[h][e] = (double)x[h][e];
+      }
+    } else {
+      turned<VEC>(a, a.k, (row0 + j) * a.ks + (int64_t)g * hd, a.kn, cs + j * a.half, n16, y);
+    }
+    double top = 0.0, bad = 0.0;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h)
+      if (h == 0 || hd > 128)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          top = fmax(top, fabs(y[h][e]));
+          bad = fma(y[h][e], 0.0, bad);
+        }
+    const float scale = scale_of(row_max64(top), isnan(row_sum64(bad)));
+    const Coder code(scale);
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t d = 128 * h + 8 * n16;
+      if (d >= hd) continue;
+      uint64_t c = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c |= (uint64_t)(uint8_t)code(y[h][e]) << (8 * e);
+      // a page's row is a multiple of 64 codes: those behind hd are zeros
+      int8_t* to = value ? tile + (gl * most + j) * KV_ROW + d : pool.keys + (hp * PAGE + a0 + j) * a.p.dp + d;
+      *reinterpret_cast<uint64_t*>(to) = c;
+    }
+    if (n16 == 0) (value ? pool.value_scale : pool.key_scale)[hp * PAGE + a0 + j] = scale;
+  }
+  __syncthreads();
+  // value codes into their transposed pages
+  int8_t* vc = pool.values + ((size_t)page * a.p.heads + g0) * PAGE * a.p.dp;
+  if (n < KV_RUN) {  // some of the run: byte by byte
+    for (uint32_t i = threadIdx.x; i < heads * n * hd; i += blockDim.x) {
+      const uint32_t d = i % hd, hj = i / hd, j = hj % n, gl = hj / n;
+      vc[((size_t)gl * a.p.dp + d) * PAGE + a0 + j] = tile[(gl * most + j) * KV_ROW + d];
+    }
+    return;
+  }
+  const uint32_t quarters = (hd + 3) / 4;
+  for (uint32_t i = threadIdx.x; i < heads * quarters; i += blockDim.x) {  // four channels a thread
+    const uint32_t gl = i / quarters, d = 4 * (i % quarters);
+    uint32_t w[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t in[4], out[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in[e] = *reinterpret_cast<const uint32_t*>(tile + (gl * most + 4 * u + e) * KV_ROW + d);
+      transpose4(in, out);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[c][u] = out[c];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (d + c < hd)
+        *reinterpret_cast<v4i*>(vc + ((size_t)gl * a.p.dp + d + c) * PAGE + a0) =
+            v4i{(int)w[c][0], (int)w[c][1], (int)w[c][2], (int)w[c][3]};
+  }
+}
+
+// ------------------------------------------------------------- keep
+
+struct KeepArgs {
+  Pages p;
+  Rows r;
+  const int32_t *keep, *kept;
+  int32_t* kv_len_out;
+  uint32_t hd;
+};
+
+// One workgroup for a sequence and head: its kept rows' codes and scales all
+// come into LDS, then go to their new places, so that the order of rows and
+// places that are both does not matter.
+__global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
+  const uint32_t g = blockIdx.x % a.p.heads, seq = blockIdx.x / a.p.heads;
+  const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
+  const int n = min(max(a.kept[seq], 0), sp.n);  // rows that stay
+  if (g == 0 && threadIdx.x == 0) a.kv_len_out[seq] = (int32_t)max(sp.pos(n), (int64_t)INT32_MIN);
+  const int move = min(n, (int)a.r.most_rows);
+  __shared__ __align__(16) int8_t keys[MAX_TREE * 256], values[MAX_TREE * 256];
+  __shared__ float scales[2][MAX_TREE];
+  __shared__ int64_t from[MAX_TREE], to[MAX_TREE];  // places: page * 64 + position, or -1
+  if (move <= 0) return;
+  const int32_t* table;
+  uint32_t width;
+  const SeqPages pool = pool_of(a.p, seq, table, width);
+  auto place = [&](int64_t pos) -> int64_t {
+    const int page = pos < 0 ? -1 : page_of(table, width, pool.pages, pos / PAGE);
+    return page < 0 ? -1 : (int64_t)page * PAGE + pos % PAGE;
+  };
+  for (int t = threadIdx.x; t < move; t += blockDim.x) {
+    const int j = a.keep[sp.start + t];
+    const int64_t f = j >= 0 && j < sp.n && j != t ? place(sp.pos(j)) : -1;
+    from[t] = f;
+    to[t] = f < 0 ? -1 : place(sp.pos(t));
+  }
+  __syncthreads();
+  const uint32_t dp = a.p.dp;
+  auto head = [&](int64_t at) { return (size_t)(at / PAGE) * a.p.heads + g; };  // of a place
+  // keys by 16 bytes, values by the byte: rows fastest, so that lanes share a line
+  for (uint32_t i = threadIdx.x; i < move * dp / 16; i += blockDim.x) {
+    const uint32_t t = i / (dp / 16), d = i % (dp / 16) * 16;
+    if (to[t] >= 0)
+      *reinterpret_cast<v4i*>(keys + t * 256 + d) =
+          *reinterpret_cast<const v4i*>(pool.keys + (head(from[t]) * PAGE + from[t] % PAGE) * dp + d);
+  }
+  for (uint32_t i = threadIdx.x; i < move * a.hd; i += blockDim.x) {
+    const uint32_t t = i % move, d = i / move;
+    if (to[t] >= 0) values[t * 256 + d] = pool.values[(head(from[t]) * dp + d) * PAGE + from[t] % PAGE];
+  }
+  for (int t = threadIdx.x; t < move; t += blockDim.x)
+    if (to[t] >= 0) {
+      scales[0][t] = pool.key_scale[head(from[t]) * PAGE + from[t] % PAGE];
+      scales[1][t] = pool.value_scale[head(from[t]) * PAGE + from[t] % PAGE];
+    }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < move * dp / 16; i += blockDim.x) {
+    const uint32_t t = i / (dp / 16), d = i % (dp / 16) * 16;
+    if (to[t] >= 0)
+      *reinterpret_cast<v4i*>(pool.keys + (head(to[t]) * PAGE + to[t] % PAGE) * dp + d) =
+          *reinterpret_cast<const v4i*>(keys + t * 256 + d);
+  }
+  for (uint32_t i = threadIdx.x; i < move * a.hd; i += blockDim.x) {
+    const uint32_t t = i % move, d = i / move;
+    if (to[t] >= 0) pool.values[(head(to[t]) * dp + d) * PAGE + to[t] % PAGE] = values[t * 256 + d];
+  }
+  for (int t = threadIdx.x; t < move; t += blockDim.x)
+    if (to[t] >= 0) {
+      pool.key_scale[head(to[t]) * PAGE + to[t] % PAGE] = scales[0][t];
+      pool.value_scale[head(to[t]) * PAGE + to[t] % PAGE] = scales[1][t];
+    }
+}
+
+// ------------------------------------------------------------- log probabilities
+
+constexpr int SCORE_THREADS = 1024, SCORE_EACH = 16, SCORE_CHUNK = SCORE_THREADS * SCORE_EACH;  // logits of a workgroup
+constexpr int SCORE_FEW = 512;  // candidates that are ranked against each other
+
+// What a workgroup leaves of its chunk of a row, joined in the order of chunks.
+struct ScorePart {
+  float top, sum, moment;  // maximum m; sum of e = exp(scale (x - m)); sum of e (x - m)
+  uint32_t above;          // logits over the target's
+};
+
+struct ScoreArgs {
+  const void* x;
+  int64_t xs;
+  const int32_t* target;
+  uint32_t rows, n, top, chunks;
+  float scale;
+  float *log_p, *entropy, *top_log_p;
+  int32_t *rank, *top_index;
+  ScorePart* part;   // [rows][chunks]
+  uint64_t* best;    // [rows][chunks][top], the largest first; 0: none
+};
+
+// A whole number that orders logits by value, then by the lower column. -0 is
+// 0; a NaN comes last. No logit's is 0.
+__device__ __forceinline__ uint64_t score_key(float v, uint32_t column) {
+  v = isnan(v) ? -INFINITY : v + 0.0f;
+  const uint32_t b = __builtin_bit_cast(uint32_t, v), o = b ^ (uint32_t)((int32_t)b >> 31 | (int32_t)0x80000000);
+  return (uint64_t)o << 32 | (0xffffffffu - column);
+}
+__device__ __forceinline__ uint32_t column_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// The row's outputs from its joined statistics (every lane has them) and its
+// best (lane t < top: the t-th). In 64 bits: logarithms next to zero.
+__device__ __forceinline__ void score_store(const ScoreArgs& a, uint32_t row, uint32_t t, float top, double sum, double moment,
+                                            uint32_t above, float xt, bool has, uint64_t key) {
+  const float nan = __builtin_nanf("");
+  const bool none = !(sum >= 1.0);  // a NaN, an infinity, or nothing over -inf: no distribution
+  const double log_sum = log(sum);
+  if (t == 0) {
+    a.log_p[row] = none || !has ? nan : (float)((double)a.scale * ((double)xt - (double)top) - log_sum);
+    a.entropy[row] = none ? nan : (float)fmax(0.0, log_sum - (double)a.scale * moment / sum);
+    a.rank[row] = none || !has ? -1 : (int32_t)above;
+  }
+  if (t < a.top) {
+    a.top_log_p[(size_t)row * a.top + t] = none ? nan : (float)((double)a.scale * ((double)value_of(key) - (double)top) - log_sum);
+    a.top_index[(size_t)row * a.top + t] = none ? -1 : (int32_t)column_of(key);
+  }
+}
+
+// One chunk of a row: in registers, 16 logits a thread, read once. Its maximum,
+// then the sums relative to it. The best: a bound that at least `top` logits
+// reach is the top-th of the maxima of each 16 lanes; the few that reach it are
+// ranked against each other.
+template <class T, bool VEC>
+__global__ __launch_bounds__(SCORE_THREADS) void k_score(ScoreArgs a) {
+  constexpr int V = 16 / sizeof(T), NV = SCORE_EACH / V;
+  typedef T vt __attribute__((ext_vector_type(V)));
+  const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
+  const uint32_t lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, c0 = chunk * SCORE_CHUNK;
+  const T* p = static_cast<const T*>(a.x) + (int64_t)row * a.xs;
+  const int32_t target = a.target ? a.target[row] : -1;
+  const bool has = target >= 0 && (uint32_t)target < a.n;
+  const float xt = has ? (float)p[target] : INFINITY;
+  __shared__ float s_max[SCORE_THREADS / 16], s_bound;
+  __shared__ ScorePart s_part[SCORE_THREADS / WAVE];
+  __shared__ uint64_t s_few[SCORE_FEW], s_best[SCORE_THREADS / WAVE];
+  __shared__ uint32_t s_count;
+  if (threadIdx.x == 0) s_count = 0;
+
+  auto column = [&](int i) { return c0 + ((i / V) * SCORE_THREADS + threadIdx.x) * V + i % V; };
+  float x[SCORE_EACH];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const uint32_t c = column(v * V);
+    if (VEC && c + V <= a.n) {
+      const vt w = *reinterpret_cast<const vt*>(p + c);
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[v * V + e] = (float)w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[v * V + e] = c + e < a.n ? (float)p[c + e] : -INFINITY;
+    }
+  }
+  float mine = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SCORE_EACH; ++i) mine = fmaxf(mine, x[i]);
+  const float group = row_max(mine);
+  if (lane % 16 == 0) s_max[threadIdx.x / 16] = group;
+  __syncthreads();
+  static_assert(SCORE_THREADS / 16 == WAVE, "a group's maximum for each lane");
+  const float maxima = s_max[lane];
+  const float m = wave_max(maxima), m0 = m == -INFINITY ? 0.0f : m;
+  if (wave == 0 && a.top) {  // the top-th of the groups' maxima
+    uint32_t before = 0;
+    for (int i = 0; i < WAVE; ++i) {
+      const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, maxima), i));
+      before += o > maxima || (o == maxima && i < (int)lane);
+    }
+    if (before == a.top - 1) s_bound = maxima;
+  }
+  const float unit = a.scale * 1.44269504088896340736f;
+  float sum = 0.0f, moment = 0.0f;
+  uint32_t above = 0;
+#pragma unroll
+  for (int i = 0; i < SCORE_EACH; ++i) {
+    const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
+    sum += e;
+    moment = fmaf(e == 0.0f ? 0.0f : d, e, moment);
+    above += x[i] > xt;
+  }
+  sum = wave_add(sum);
+  moment = wave_add(moment);
+  above = wave_add(above);
+  if (lane == 0) s_part[wave] = ScorePart{m, sum, moment, above};
+  __syncthreads();
+  if (a.top && mine >= s_bound) {
+#pragma unroll
+    for (int i = 0; i < SCORE_EACH; ++i)
+      if (x[i] >= s_bound && column(i) < a.n) {
+        const uint32_t at = atomicAdd(&s_count, 1u);
+        if (at < SCORE_FEW) s_few[at] = score_key(x[i], column(i));
+      }
+  }
+  __syncthreads();
+  const uint32_t count = s_count;
+  ScorePart r = s_part[0];
+  for (int w = 1; w < SCORE_THREADS / WAVE; ++w) {
+    r.sum += s_part[w].sum;
+    r.moment += s_part[w].moment;
+    r.above += s_part[w].above;
+  }
+  const uint32_t out = row * a.chunks + chunk;
+  uint64_t* best = a.best + (size_t)out * a.top;
+  if (threadIdx.x == 0) a.part[out] = r;
+  const uint32_t most = min(a.top, min(a.n - c0, (uint32_t)SCORE_CHUNK));
+  if (threadIdx.x >= most && threadIdx.x < a.top) best[threadIdx.x] = 0;
+  if (count <= SCORE_FEW && count >= most) {
+    if (threadIdx.x < count) {
+      const uint64_t k = s_few[threadIdx.x];
+      uint32_t before = 0;
+      for (uint32_t i = 0; i < count; ++i) before += s_few[i] > k;
+      if (before < most) best[before] = k;
+    }
+    return;
+  }
+  // many equal ones, or ones that are no numbers: the largest below the last, over and over
+  uint64_t last = ~0ull;
+  for (uint32_t t = 0; t < most; ++t) {
+    uint64_t k = 0;
+#pragma unroll
+    for (int i = 0; i < SCORE_EACH; ++i) {
+      const uint64_t o = column(i) < a.n ? score_key(x[i], column(i)) : 0;
+      k = o < last && o > k ? o : k;
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t other = __shfl_xor((unsigned long long)k, o);
+      k = other > k ? other : k;
+    }
+    if (lane == 0) s_best[wave] = k;
+    __syncthreads();
+    last = s_best[0];
+    for (int w = 1; w < SCORE_THREADS / WAVE; ++w) last = s_best[w] > last ? s_best[w] : last;
+    if (threadIdx.x == 0) best[t] = last;
+    __syncthreads();
+  }
+}
+
+// A row's chunks joined in order, its best of theirs.
+__global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) {
+  __shared__ uint64_t s_key[MAX_SCORE_CHUNKS * MAX_TOP], s_best[MAX_TOP];
+  const uint32_t row = blockIdx.x, keys = a.chunks * a.top;
+  const ScorePart* part = a.part + (size_t)row * a.chunks;
+  for (uint32_t i = threadIdx.x; i < keys; i += 256) s_key[i] = a.best[(size_t)row * keys + i];
+  const int32_t target = a.target ? a.target[row] : -1;
+  const bool has = target >= 0 && (uint32_t)target < a.n;
+  const float xt = has ? load_value(a.x, (int64_t)row * a.xs + target, type) : 0.0f;
+  float top = -INFINITY;
+  for (uint32_t c = 0; c < a.chunks; ++c) top = fmaxf(top, part[c].top);
+  double sum = 0.0, moment = 0.0;
+  uint32_t above = 0;
+  for (uint32_t c = 0; c < a.chunks; ++c) {
+    const ScorePart s = part[c];
+    above += s.above;
+    if (s.top == -INFINITY && s.sum == 0.0f) continue;  // nothing over -inf
+    const double d = (double)s.top - (double)top, e = exp((double)a.scale * d);
+    sum = fma(e, (double)s.sum, sum);
+    moment = fma(e, e == 0.0 ? 0.0 : fma(d, (double)s.sum, (double)s.moment), moment);
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < keys; i += 256) {
+    const uint64_t k = s_key[i];
+    uint32_t before = 0;
+    for (uint32_t j = 0; j < keys; ++j) before += s_key[j] > k;
+    if (k && before < a.top) s_best[before] = k;
+  }
+  __syncthreads();
+  if (threadIdx.x < WAVE)
+    score_store(a, row, threadIdx.x, top, sum, moment, above, xt, has, threadIdx.x < a.top ? s_best[threadIdx.x] : 1);
+}
+
+template <class T>
+int score_launch(const ScoreArgs& a, bool vec, hipStream_t s) {
+  return launch(vec ? k_score<T, true> : k_score<T, false>, a.rows * a.chunks, SCORE_THREADS, 0, s, a);
+}
+
+uint32_t score_chunks(uint32_t n) { return (n + SCORE_CHUNK - 1) / SCORE_CHUNK; }
+
+}  // namespace
+
+}  // namespace q8
+
+// ------------------------------------------------------------- C entry points
+
+using namespace q8;
+
+extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
+                                      const defer_gpu_q8_rotary* rotary, const void* q, int64_t q_stride, uint32_t q_heads,
+                                      const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* out,
+                                      int64_t out_stride, uint32_t clear, void* stream) {
+  Pages p;
+  Rows r;
+  int rc = check_pages(pages, rows, &p, &r);
+  if (!rc) rc = check_heads(pages, q_heads, 0);
+  if (rc) return rc;
+  const uint32_t hd = pages->head_dim, nkv = p.heads * hd, nq = q_heads * hd;
+  rc = check_rows_values(type, q, q_stride, r.rows, nq, "q");
+  if (!rc) rc = check_rows_values(type, k, k_stride, r.rows, nkv, "k");
+  if (!rc) rc = check_rows_values(type, v, v_stride, r.rows, nkv, "v");
+  if (!rc) rc = check_rows_values(type, out, out_stride, r.rows, nq, "out");
+  if (rc) return rc;
+  Q8_REQUIRE(rotary, "rotary is null");
+  Q8_REQUIRE(rotary->rotated <= hd && rotary->rotated % 2 == 0, "%u values of %u rotated", rotary->rotated, hd);
+  Q8_REQUIRE(rotary->rotated == 0 || (rotary->freq && aligned_to(rotary->freq, 8)), "freq is null or not aligned to its type");
+  Q8_REQUIRE(aligned_to(rotary->position, 4), "position is not aligned to its type");
+  Q8_REQUIRE(aligned_to(rotary->q_norm, value_size(type)) && aligned_to(rotary->k_norm, value_size(type)),
+             "a norm's weight is not aligned to its type");
+  Q8_REQUIRE(rotary->eps >= 0.0f && rotary->eps < INFINITY, "eps %g", (double)rotary->eps);
+  Q8_REQUIRE(fabsf(rotary->factor) < INFINITY, "factor %g", (double)rotary->factor);
+  const int64_t vs = (int64_t)value_size(type), row = nq * vs;
+  Q8_REQUIRE(!overlap(out, out_stride * vs, r.rows, q, q_stride * vs, r.rows, row), "out overlaps q");
+  Q8_REQUIRE(!overlap(out, out_stride * vs, r.rows, row, k, k_stride * vs, r.rows, nkv * vs), "out overlaps k");
+  Q8_REQUIRE(!overlap(out, out_stride * vs, r.rows, row, v, v_stride * vs, r.rows, nkv * vs), "out overlaps v");
+  if (!r.rows) return DEFER_GPU_OK;
+  const hipStream_t s = (hipStream_t)stream;
+  if (!r.sequences || !r.most_rows)
+    return clear ? launch(k_zero_rows, r.rows, 256, 0, s, out, out_stride, nq, type) : DEFER_GPU_OK;
+  AppendArgs a{};
+  a.p = p;
+  a.r = r;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.qs = q_stride;
+  a.ks = k_stride;
+  a.vs = v_stride;
+  a.os = out_stride;
+  a.position = rotary->position;
+  a.freq = rotary->freq;
+  a.qn = rotary->q_norm;
+  a.kn = rotary->k_norm;
+  a.eps = (double)rotary->eps;
+  a.factor = (double)rotary->factor;
+  a.type = type;
+  a.hd = hd;
+  a.nh = q_heads;
+  a.half = rotary->rotated / 2;
+  a.interleaved = rotary->interleaved != 0;
+  a.clear = clear && r.row_start;
+  // Heads of a workgroup: 16 of its lanes take a row's head, four rounds of them
+  // where a run is full.
+  const uint32_t most = std::min(r.most_rows, (uint32_t)KV_RUN), items = most >= 8 ? 64 : 16;
+  a.q_heads = std::min(std::max(1u, items / most), q_heads);
+  a.kv_heads = std::min(std::max(1u, items / 2 / most), p.heads);
+  a.kv_chunks = (p.heads + a.kv_heads - 1) / a.kv_heads;
+  a.chunks = a.kv_chunks + (q_heads + a.q_heads - 1) / a.q_heads;
+  const uint64_t blocks = ((uint64_t)r.sequences + a.clear) * kv_runs(r.most_rows) * a.chunks;
+  Q8_REQUIRE(blocks <= MAX_THREADS / 256, "too many rows for one call");
+  const bool vec = hd % 8 == 0 && (a.interleaved || a.half % 8 == 0) &&
+                   ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)(q_stride * vs) |
+                    (uintptr_t)(k_stride * vs) | (uintptr_t)(v_stride * vs) | (uintptr_t)(out_stride * vs)) % 16 == 0;
+  const size_t lds = (size_t)most * a.half * sizeof(double2) + (size_t)a.kv_heads * most * KV_ROW;
+  return launch(vec ? k_append<true> : k_append<false>, (uint32_t)blocks, 256, lds, s, a);
+}
+
+extern "C" int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, const int32_t* keep,
+                                    const int32_t* kept, int32_t* kv_len_out, void* stream) {
+  Pages p;
+  Rows r;
+  const int rc = check_pages(pages, rows, &p, &r);
+  if (rc) return rc;
+  Q8_REQUIRE(r.most_rows <= MAX_TREE, "%u rows of a sequence: at most %u", r.most_rows, MAX_TREE);
+  if (!r.sequences) return DEFER_GPU_OK;
+  Q8_REQUIRE(r.kv_len && kept && kv_len_out, "null argument");
+  Q8_REQUIRE(r.rows == 0 || keep, "keep is null");
+  Q8_REQUIRE(r.row_start || r.rows == r.sequences, "%u rows of %u sequences without row_start", r.rows, r.sequences);
+  Q8_REQUIRE(aligned_to(keep, 4) && aligned_to(kept, 4) && aligned_to(kv_len_out, 4), "an array is not aligned to its type");
+  const int64_t n = (int64_t)r.sequences * 4;
+  auto apart = [&](const void* in, int64_t bytes) {
+    return in == nullptr || (const char*)kv_len_out + n <= (const char*)in || (const char*)in + bytes <= (const char*)kv_len_out;
+  };
+  Q8_REQUIRE(apart(r.kv_len, n) && apart(kept, n) && apart(r.row_start, n + 4) && apart(keep, (int64_t)r.rows * 4),
+             "kv_len_out overlaps an input");
+  const uint64_t blocks = (uint64_t)r.sequences * p.heads;
+  Q8_REQUIRE(blocks <= MAX_THREADS / 256, "too many sequences for one call");
+  const KeepArgs a{p, r, keep, kept, kv_len_out, pages->head_dim};
+  return launch(k_keep, (uint32_t)blocks, 256, 0, (hipStream_t)stream, a);
+}
+
+extern "C" size_t defer_gpu_q8_log_probs_workspace(uint32_t rows, uint32_t n, uint32_t top) {
+  if (rows > MAX_THREADS / SCORE_THREADS || n > MAX_SCORE || top > MAX_TOP) return 0;
+  return (size_t)rows * score_chunks(n) * (sizeof(ScorePart) + top * sizeof(uint64_t));
+}
+
+extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_stride, uint32_t rows, uint32_t n,
+                                      const int32_t* target, float scale, uint32_t top, float* log_p, float* entropy,
+                                      int32_t* rank, int32_t* top_index, float* top_log_p, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  const int rc = check_rows_values(type, x, x_stride, rows, n, "logits");
+  if (rc) return rc;
+  Q8_REQUIRE(n <= MAX_SCORE, "%u logits: at most %u", n, MAX_SCORE);
+  Q8_REQUIRE(top <= MAX_TOP && top <= n, "the %u best of %u: at most %u", top, n, MAX_TOP);
+  Q8_REQUIRE(scale > 0.0f && scale <= 1e30f, "scale %g", (double)scale);
+  Q8_REQUIRE(rows == 0 || (log_p && entropy && rank && (top == 0 || (top_index && top_log_p))), "null output");
+  Q8_REQUIRE(aligned_to(target, 4) && aligned_to(log_p, 4) && aligned_to(entropy, 4) && aligned_to(rank, 4) &&
+                 aligned_to(top_index, 4) && aligned_to(top_log_p, 4),
+             "an array is not aligned to its type");
+  Q8_REQUIRE((uint64_t)rows * score_chunks(n) <= MAX_THREADS / SCORE_THREADS, "too many rows for one call");
+  if (!rows) return DEFER_GPU_OK;
+  const size_t need = defer_gpu_q8_log_probs_workspace(rows, n, top);
+  Q8_REQUIRE(workspace && workspace_bytes >= need, "log_probs needs a workspace of %zu bytes, got %zu", need,
+             workspace ? workspace_bytes : (size_t)0);
+  Q8_REQUIRE(aligned16(workspace), "workspace is not 16-byte aligned");
+  ScoreArgs a{x, x_stride, target, rows, n, top, score_chunks(n), scale, log_p, entropy, top_log_p, rank, top_index,
+              static_cast<ScorePart*>(workspace), nullptr};
+  a.best = reinterpret_cast<uint64_t*>(a.part + (size_t)rows * a.chunks);
+  const bool vec = ((uintptr_t)x | (uintptr_t)(x_stride * (int64_t)value_size(type))) % 16 == 0;
+  const hipStream_t s = (hipStream_t)stream;
+  const int e = type == DEFER_GPU_F32    ? score_launch<float>(a, vec, s)
+                : type == DEFER_GPU_BF16 ? score_launch<__bf16>(a, vec, s)
+                                         : score_launch<_Float16>(a, vec, s);
+  return e ? e : launch(k_score_join, rows, 256, 0, s, a, type);
+}

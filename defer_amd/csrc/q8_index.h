@@ -18,6 +18,10 @@ constexpr int UNIT_GROWS = 8192;       // ... which grows by as much every so ma
 constexpr int MAX_UNITS = UNIT_GROWS / UNIT;  // so a row has at most so many units
 constexpr uint32_t MAX_HEAD_DIM = 256;
 constexpr uint32_t MAX_K = 131072;     // sums of fewer code products than this fit 32 bits
+constexpr uint32_t MAX_TREE = 64;      // drafted rows of a sequence: a wave's lanes
+constexpr uint32_t MAX_SCORE = 1u << 20;   // logits of a row
+constexpr uint32_t MAX_SCORE_CHUNKS = 64;  // ... in workgroups' chunks
+constexpr uint32_t MAX_TOP = 32;           // alternatives of a row
 
 // The head size as a page holds it.
 Q8_HD uint32_t padded(uint32_t head_dim) { return (head_dim + 63) / 64 * 64; }
@@ -61,30 +65,34 @@ Q8_HD int most_units(int64_t len) {
 }
 
 // Whether two sets of rows share memory other than row by row, each row the
-// same in both: rows of `row` bytes from a and b on, as and bs bytes apart (at
-// least `row`; any number where there is one row).
-inline bool overlap(const void* a, int64_t as, uint32_t a_rows, const void* b, int64_t bs, uint32_t b_rows, int64_t row) {
+// same in both: rows of ar and br bytes from a and b on, as and bs bytes apart
+// (at least their length; any number where there is one row).
+inline bool overlap(const void* a, int64_t as, uint32_t a_rows, int64_t ar, const void* b, int64_t bs, uint32_t b_rows, int64_t br) {
   const int64_t x = (int64_t)(uintptr_t)a, y = (int64_t)(uintptr_t)b;
   const int64_t na = a_rows, nb = b_rows;
   if (!na || !nb) return false;
-  if (na == 1) as = row;
-  if (nb == 1) bs = row;
-  if (x == y && na == nb && as == bs) return false;
-  if (x + (na - 1) * as + row <= y || y + (nb - 1) * bs + row <= x) return false;
+  if (na == 1) as = ar;
+  if (nb == 1) bs = br;
+  if (x == y && na == nb && as == bs && ar == br) return false;
+  if (x + (na - 1) * as + ar <= y || y + (nb - 1) * bs + br <= x) return false;
   if (as == bs) {  // columns of one matrix: the later one's first row lies between two of the other's
     const int64_t d = x < y ? y - x : x - y, n = x < y ? na : nb, k = d / as, left = d % as;
-    return (k < n && left < row) || (k + 1 < n && as - left < row);
+    const int64_t first = x < y ? ar : br, later = x < y ? br : ar;
+    return (k < n && left < first) || (k + 1 < n && as - left < later);
   }
   for (int64_t i = 0, j = 0; i < na && j < nb;) {
     const int64_t p = x + i * as, q = y + j * bs;
-    if (p + row <= q)
+    if (p + ar <= q)
       ++i;
-    else if (q + row <= p)
+    else if (q + br <= p)
       ++j;
     else
       return true;
   }
   return false;
+}
+inline bool overlap(const void* a, int64_t as, uint32_t a_rows, const void* b, int64_t bs, uint32_t b_rows, int64_t row) {
+  return overlap(a, as, a_rows, row, b, bs, b_rows, row);
 }
 
 }  // namespace q8

@@ -40,6 +40,11 @@ struct {
   decltype(&defer_gpu_q8_kv_read) kv_read;
   decltype(&defer_gpu_q8_attention_workspace) attention_workspace;
   decltype(&defer_gpu_q8_attention) attention;
+  decltype(&defer_gpu_q8_tree_attention) tree_attention;
+  decltype(&defer_gpu_q8_kv_append) kv_append;
+  decltype(&defer_gpu_q8_kv_keep) kv_keep;
+  decltype(&defer_gpu_q8_log_probs_workspace) log_probs_workspace;
+  decltype(&defer_gpu_q8_log_probs) log_probs;
   PyObject* stream_of;  // device -> raw current stream
   PyObject* check;      // raises for a code that is not OK
   PyObject* out_of_memory;
@@ -112,8 +117,9 @@ int64_t row_stride(const Tensor& t, const char* what, at::Device dev, ScalarType
 
 // Rows that a call writes lie apart from those it reads, or are the same rows.
 void apart(const Tensor& out, int64_t os, const Tensor& in, int64_t is, const char* what) {
-  const int64_t rows = out.size(0), v = out.element_size(), n = rows ? out.numel() / rows * v : 0;
-  if (rows <= 0xffffffffll && q8::overlap(out.data_ptr(), os * v, (uint32_t)rows, in.data_ptr(), is * v, (uint32_t)rows, n))
+  const int64_t rows = out.size(0), v = out.element_size();
+  const int64_t n = rows ? out.numel() / rows * v : 0, m = rows ? in.numel() / rows * v : 0;
+  if (rows <= 0xffffffffll && q8::overlap(out.data_ptr(), os * v, (uint32_t)rows, n, in.data_ptr(), is * v, (uint32_t)rows, m))
     throw Refused(std::string("out overlaps ") + what);
 }
 
@@ -217,6 +223,13 @@ struct Cache {
     r.kv_len = take<int32_t>(kv_len, "kv_len", dev, ScalarType::Int, {(int64_t)r.sequences});
     r.rows = u32(n, "rows");
     r.most_rows = (uint32_t)most;
+  }
+  // ... of which a sequence has at most 64: without most_rows, no more of them
+  void drafted(PyObject* kv_len, PyObject* row_start, int64_t n, PyObject* most_rows, at::Device dev) {
+    rows(kv_len, row_start, n, most_rows, dev);
+    if (most_rows == Py_None) r.most_rows = std::min(r.most_rows, q8::MAX_TREE);
+    if (r.most_rows > q8::MAX_TREE)
+      throw Refused("most_rows " + std::to_string(r.most_rows) + ": at most " + std::to_string(q8::MAX_TREE) + " drafted rows of a sequence");
   }
 };
 
@@ -325,7 +338,8 @@ PyObject* kv_read(PyObject* const* a) {  // pages, kv_len, row_start, rows, head
   return tuple(k, v);
 }
 
-PyObject* attention(PyObject* const* a) {  // q, pages, kv_len, row_start, most_rows, most_len, scale, hidden, out
+// Both attentions: q, pages, kv_len, row_start, most_rows, most_len, scale, hidden, out; of a tree: parent.
+PyObject* attend(PyObject* const* a, PyObject* parent) {
   const Tensor& q = on_gpu(a[0], "q");
   const ScalarType type = q.scalar_type();
   const uint32_t ty = value_type(type, "q");
@@ -335,7 +349,9 @@ PyObject* attention(PyObject* const* a) {  // q, pages, kv_len, row_start, most_
   const uint32_t heads = u32(q.size(1), "heads");
   Cache c(a[1], hd, dev);
   const int64_t qs = row_stride(q, "q", dev, type, q.sizes());
-  c.rows(a[2], a[3], rows, a[4], dev);
+  if (parent) c.drafted(a[2], a[3], rows, a[4], dev);
+  else c.rows(a[2], a[3], rows, a[4], dev);
+  const int32_t* const up = parent ? take<int32_t>(parent, "parent", dev, ScalarType::Int, {rows}) : nullptr;
   const int64_t most_len = a[5] != Py_None ? integer(a[5]) : std::min<int64_t>(PAGE * c.p.table_width, 0x7fffffff);
   if (!(most_len >= 0 && most_len <= 0x7fffffff)) throw Refused("most_len " + std::to_string(most_len));
   const float scale = a[6] != Py_None ? real(a[6]) : (float)std::pow((double)hd, -0.5);
@@ -363,14 +379,112 @@ PyObject* attention(PyObject* const* a) {  // q, pages, kv_len, row_start, most_
   const size_t need_bytes = lib.attention_workspace(&c.p, &c.r, heads, (uint32_t)most_len);
   Tensor work;
   if (need_bytes) work = fresh({(int64_t)need_bytes}, ScalarType::Byte, dev);
+  void* const w = need_bytes ? work.data_ptr() : nullptr;
   call(dev, [&](void* s) {
-    return lib.attention(&c.p, &c.r, ty, q.data_ptr(), qs, heads, (uint32_t)most_len, scale, hidden, hs, hn, out.data_ptr(),
-                         os, clear, need_bytes ? work.data_ptr() : nullptr, need_bytes, s);
+    return parent ? lib.tree_attention(&c.p, &c.r, ty, q.data_ptr(), qs, heads, up, (uint32_t)most_len, scale, hidden, hs, hn,
+                                       out.data_ptr(), os, clear, w, need_bytes, s)
+                  : lib.attention(&c.p, &c.r, ty, q.data_ptr(), qs, heads, (uint32_t)most_len, scale, hidden, hs, hn,
+                                  out.data_ptr(), os, clear, w, need_bytes, s);
   });
   if (clear) return THPVariable_Wrap(out);
   written(out);
   Py_INCREF(a[8]);
   return a[8];
+}
+PyObject* attention(PyObject* const* a) { return attend(a, nullptr); }
+PyObject* tree_attention(PyObject* const* a) { return attend(a + 1, a[0]); }
+
+// pages, q, k, v, kv_len, row_start, most_rows, freq, interleaved, factor, position, q_norm, k_norm, eps, out
+PyObject* kv_append(PyObject* const* a) {
+  const Tensor &q = on_gpu(a[1], "q"), &k = tensor(a[2], "k"), &v = tensor(a[3], "v");
+  const ScalarType type = q.scalar_type();
+  const uint32_t ty = value_type(type, "q");
+  need(q.dim() == 3, "q: need [rows, heads, head_dim]");
+  const auto dev = q.device();
+  const int64_t rows = q.size(0), hd = q.size(2), n = q.size(1) * hd;
+  const uint32_t heads = u32(q.size(1), "heads");
+  Cache c(a[0], hd, dev);
+  const int64_t qs = row_stride(q, "q", dev, type, q.sizes());
+  const int64_t ks = row_stride(k, "k", dev, type, {rows, (int64_t)c.p.heads, hd});
+  const int64_t vs = row_stride(v, "v", dev, type, {rows, (int64_t)c.p.heads, hd});
+  c.rows(a[4], a[5], rows, a[6], dev);
+  defer_gpu_q8_rotary t;
+  const Tensor& freq = tensor(a[7], "freq");
+  need(freq.dim() == 1 && 2 * freq.size(0) <= hd, "freq: need [rotated / 2], at most half a head");
+  t.freq = take<double>(a[7], "freq", dev, ScalarType::Double, freq.sizes());
+  t.rotated = (uint32_t)(2 * freq.size(0));
+  const int interleaved = PyObject_IsTrue(a[8]);
+  if (interleaved < 0) throw PythonError();
+  t.interleaved = (uint32_t)interleaved;
+  t.factor = real(a[9]);
+  t.position = a[10] != Py_None ? take<int32_t>(a[10], "position", dev, ScalarType::Int, {rows}) : nullptr;
+  t.q_norm = a[11] != Py_None ? take<void>(a[11], "q_norm", dev, type, {hd}) : nullptr;
+  t.k_norm = a[12] != Py_None ? take<void>(a[12], "k_norm", dev, type, {hd}) : nullptr;
+  t.eps = real(a[13]);
+  const bool clear = a[14] == Py_None;
+  Tensor out;
+  int64_t os = n;
+  if (clear) {
+    out = fresh(q.sizes(), type, dev);
+  } else {
+    out = tensor(a[14], "out");
+    os = row_stride(out, "out", dev, type, q.sizes());
+    apart(out, os, q, qs, "q");
+    apart(out, os, k, ks, "k");
+    apart(out, os, v, vs, "v");
+  }
+  call(dev, [&](void* s) {
+    return lib.kv_append(&c.p, &c.r, ty, &t, q.data_ptr(), qs, heads, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
+                         clear, s);
+  });
+  for (Py_ssize_t i = 0; i < 4; ++i) written(THPVariable_Unpack(PyTuple_GET_ITEM(a[0], i)));
+  if (clear) return THPVariable_Wrap(out);
+  written(out);
+  Py_INCREF(a[14]);
+  return a[14];
+}
+
+PyObject* kv_keep(PyObject* const* a) {  // pages, kv_len, row_start, keep, kept, most_rows
+  const auto dev = on_gpu(a[1], "kv_len").device();
+  need(PyTuple_Check(a[0]) && PyTuple_GET_SIZE(a[0]) == 5, "pages: need Pages");
+  const Tensor& keys = tensor(PyTuple_GET_ITEM(a[0], 0), "keys");
+  need(keys.dim() == 4, "keys: need [pages, heads, 64, D]");
+  Cache c(a[0], keys.size(3), dev);  // whole rows of codes move
+  const Tensor& keep = tensor(a[3], "keep");
+  need(keep.dim() == 1, "keep: need [rows]");
+  c.drafted(a[1], a[2], keep.size(0), a[5], dev);
+  const int32_t* const which = take<int32_t>(a[3], "keep", dev, ScalarType::Int, keep.sizes());
+  const int32_t* const kept = take<int32_t>(a[4], "kept", dev, ScalarType::Int, {(int64_t)c.r.sequences});
+  const Tensor out = fresh({(int64_t)c.r.sequences}, ScalarType::Int, dev);
+  call(dev, [&](void* s) { return lib.kv_keep(&c.p, &c.r, which, kept, out.data_ptr<int32_t>(), s); });
+  for (Py_ssize_t i = 0; i < 4; ++i) written(THPVariable_Unpack(PyTuple_GET_ITEM(a[0], i)));
+  return THPVariable_Wrap(out);
+}
+
+PyObject* log_probs(PyObject* const* a) {  // logits, target, top, scale
+  const Tensor& x = on_gpu(a[0], "logits");
+  const uint32_t ty = value_type(x.scalar_type(), "logits");
+  need(x.dim() == 2 && x.size(1) > 0, "logits: need [rows, n]");
+  const auto dev = x.device();
+  const int64_t rows = x.size(0), xs = row_stride(x, "logits", dev, x.scalar_type(), x.sizes()), top = integer(a[2]);
+  if (!(top >= 0 && top <= std::min<int64_t>(x.size(1), q8::MAX_TOP)))
+    throw Refused("top " + std::to_string(top) + " of " + std::to_string(x.size(1)) + ": at most " + std::to_string(q8::MAX_TOP));
+  const int32_t* const target = a[1] != Py_None ? take<int32_t>(a[1], "target", dev, ScalarType::Int, {rows}) : nullptr;
+  const float scale = real(a[3]);
+  const uint32_t r32 = u32(rows, "rows"), n32 = u32(x.size(1), "n"), t32 = (uint32_t)top;
+  const Tensor log_p = fresh({rows}, ScalarType::Float, dev), entropy = fresh({rows}, ScalarType::Float, dev);
+  const Tensor rank = fresh({rows}, ScalarType::Int, dev), index = fresh({rows, top}, ScalarType::Int, dev);
+  const Tensor top_log_p = fresh({rows, top}, ScalarType::Float, dev);
+  const size_t need_bytes = lib.log_probs_workspace(r32, n32, t32);
+  Tensor work;
+  if (need_bytes) work = fresh({(int64_t)need_bytes}, ScalarType::Byte, dev);
+  call(dev, [&](void* s) {
+    return lib.log_probs(ty, x.data_ptr(), xs, r32, n32, target, scale, t32, log_p.data_ptr<float>(), entropy.data_ptr<float>(),
+                         rank.data_ptr<int32_t>(), index.data_ptr<int32_t>(), top_log_p.data_ptr<float>(),
+                         need_bytes ? work.data_ptr() : nullptr, need_bytes, s);
+  });
+  return Py_BuildValue("(NNNNN)", THPVariable_Wrap(log_p), THPVariable_Wrap(entropy), THPVariable_Wrap(rank),
+                       THPVariable_Wrap(index), THPVariable_Wrap(top_log_p));
 }
 
 // A call from Python: the argument count, and no C++ exception gets out.
@@ -410,7 +524,10 @@ PyObject* bind(PyObject*, PyObject* args) {
   if (!(take("defer_gpu_q8_quantize", lib.quantize) && take("defer_gpu_q8_rms_norm", lib.rms_norm) &&
         take("defer_gpu_q8_linear", lib.linear) && take("defer_gpu_q8_kv_write", lib.kv_write) &&
         take("defer_gpu_q8_kv_read", lib.kv_read) &&
-        take("defer_gpu_q8_attention_workspace", lib.attention_workspace)))
+        take("defer_gpu_q8_attention_workspace", lib.attention_workspace) &&
+        take("defer_gpu_q8_tree_attention", lib.tree_attention) && take("defer_gpu_q8_kv_append", lib.kv_append) &&
+        take("defer_gpu_q8_kv_keep", lib.kv_keep) && take("defer_gpu_q8_log_probs_workspace", lib.log_probs_workspace) &&
+        take("defer_gpu_q8_log_probs", lib.log_probs)))
     return nullptr;
   Py_INCREF(stream_of);
   Py_INCREF(check);
@@ -428,7 +545,9 @@ PyMethodDef method(const char* name) {
 }
 PyMethodDef methods[] = {method<quantize, 1>("quantize"), method<rms_norm, 5>("rms_norm"), method<linear, 5>("linear"),
                          method<kv_write, 6>("kv_write"), method<kv_read, 7>("kv_read"),
-                         method<attention, 9>("attention"), {"bind", bind, METH_VARARGS, nullptr},
+                         method<attention, 9>("attention"), method<tree_attention, 10>("tree_attention"),
+                         method<kv_append, 15>("kv_append"), method<kv_keep, 6>("kv_keep"),
+                         method<log_probs, 4>("log_probs"), {"bind", bind, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_q8_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

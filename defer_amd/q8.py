@@ -2,7 +2,10 @@
 
 What a decoder layer needs to run on 8-bit weights, activations and cache: rows
 to codes, the norm that leaves codes, the product of codes, the cache in codes
-and the attention over it. A row of n values is held as n int8 codes and one
+and the attention over it; and what a program needs next to these that drafts a tree
+of tokens and verifies it in one step: rows appended with their rotary positions,
+the tree's attention, log probabilities of given tokens, the accepted path moved
+together. A row of n values is held as n int8 codes and one
 float32 scale (max / 127); the header says what is rounded where.
 
 Every call is queued on torch's current stream of its tensors' device, returns
@@ -15,6 +18,7 @@ where gradients are on, as is any call under torch.jit.trace.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -54,6 +58,43 @@ def padded(head_dim: int) -> int:
     return -(-head_dim // PAGE) * PAGE
 
 
+class Rotary(NamedTuple):
+    """How positions turn heads: of each, the first 2 len(freq) values form pairs
+    (i, i + len(freq)), or (2 i, 2 i + 1) if ``interleaved``; pair i is turned by position *
+    freq[i] and multiplied by ``factor``. ``freq`` is float64: radians a position."""
+
+    freq: torch.Tensor
+    interleaved: bool = False
+    factor: float = 1.0
+
+
+def rotary(rotated: int, theta: float = 10000.0, scale: float = 1.0, original_len: Optional[int] = None, low: float = 1.0,
+           high: float = 4.0, interleaved: bool = False, factor: float = 1.0, device="cuda") -> Rotary:
+    """The frequencies theta^(-2 i / rotated) of a head's first ``rotated`` values. ``scale``: contexts that
+    many times longer than the model's own, by frequencies so many times lower; with ``original_len`` (the
+    model's own) only of pairs that make fewer than ``high`` turns in it, and by less the more of them above ``low``."""
+    if rotated < 0 or rotated % 2:
+        raise ValueError(f"rotated {rotated}: need an even number")
+    if not (theta > 0 and scale > 0 and (original_len is None or (original_len > 0 and low < high))):
+        raise ValueError(f"theta {theta}, scale {scale}, original_len {original_len}, low {low}, high {high}")
+    f = float(theta) ** (-torch.arange(0, rotated, 2, dtype=torch.float64) / max(rotated, 1))
+    if scale != 1.0:
+        keep = torch.zeros_like(f) if original_len is None else ((original_len * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = keep * f + (1 - keep) * f / scale
+    return Rotary(f.to(device), interleaved, factor)
+
+
+class LogProbs(NamedTuple):
+    """Of each row: the target's ``log_p``, the ``entropy``, the target's ``rank`` (how many logits are larger), the
+    likeliest ``top_index`` and their ``top_log_p``."""
+
+    log_p: torch.Tensor
+    entropy: torch.Tensor
+    rank: torch.Tensor
+    top_index: torch.Tensor
+    top_log_p: torch.Tensor
+
+
 class _CPages(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("keys", "values", "key_scale", "value_scale", "table")] + \
                [(n, ctypes.c_uint32) for n in ("pages", "heads", "head_dim", "table_width")]
@@ -62,6 +103,11 @@ class _CPages(ctypes.Structure):
 class _CRows(ctypes.Structure):
     _fields_ = [("row_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p)] + \
                [(n, ctypes.c_uint32) for n in ("sequences", "rows", "most_rows")]
+
+
+class _CRotary(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("freq", "position", "q_norm", "k_norm")] + \
+               [("eps", ctypes.c_float), ("factor", ctypes.c_float), ("rotated", ctypes.c_uint32), ("interleaved", ctypes.c_uint32)]
 
 
 _L = None
@@ -82,7 +128,14 @@ def _lib():
                 ("kv_read", [pages, rows, u32, vp, vp, vp], ctypes.c_int),
                 ("attention_workspace", [pages, rows, u32, u32], sz),
                 ("attention", [pages, rows, u32, vp, i64, u32, u32, f32, vp, i64, u32, vp, i64, u32, vp, sz, vp],
-                 ctypes.c_int)):
+                 ctypes.c_int),
+                ("tree_attention", [pages, rows, u32, vp, i64, u32, vp, u32, f32, vp, i64, u32, vp, i64, u32, vp, sz, vp],
+                 ctypes.c_int),
+                ("kv_append", [pages, rows, u32, ctypes.POINTER(_CRotary), vp, i64, u32, vp, i64, vp, i64, vp, i64, u32, vp],
+                 ctypes.c_int),
+                ("kv_keep", [pages, rows, vp, vp, vp, vp], ctypes.c_int),
+                ("log_probs_workspace", [u32, u32, u32], sz),
+                ("log_probs", [u32, vp, i64, u32, u32, vp, f32, u32, vp, vp, vp, vp, vp, vp, sz, vp], ctypes.c_int)):
             f = getattr(L, "defer_gpu_q8_" + name)
             f.argtypes, f.restype = args, res
         _L = L
@@ -154,3 +207,42 @@ def attention(q: torch.Tensor, pages: Pages, kv_len: torch.Tensor, row_start: Op
     no sequence are left as ``out`` has them (without ``out``: zeros). ``out`` may
     be q itself, or rows apart from it."""
     return _native().attention(q, pages, kv_len, row_start, most_rows, most_len, scale, hidden, out)
+
+
+def kv_append(pages: Pages, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_len: torch.Tensor, rotary: Rotary,
+              row_start: Optional[torch.Tensor] = None, most_rows: Optional[int] = None,
+              position: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None,
+              k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Turns q [rows, heads, head_dim] and k [rows, cache heads, head_dim] by their rows' positions, quantises k and v
+    into the pages as kv_write does, and returns q (into ``out``, which may be q itself, or rows apart from q, k and v;
+    rows of no sequence as attention has them). ``position`` [rows] int32: without, where rows lie in the cache.
+    ``q_norm``, ``k_norm`` [head_dim]: first divides each head by sqrt(mean(x^2) + eps) and multiplies by it."""
+    freq, interleaved, factor = rotary
+    return _native().kv_append(pages, q, k, v, kv_len, row_start, most_rows, freq, interleaved, factor, position, q_norm,
+                               k_norm, eps, out)
+
+
+def tree_attention(q: torch.Tensor, pages: Pages, parent: torch.Tensor, kv_len: torch.Tensor,
+                   row_start: Optional[torch.Tensor] = None, most_rows: Optional[int] = None, most_len: Optional[int] = None,
+                   scale: Optional[float] = None, hidden: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """attention of rows that are nodes of a tree, at most 64 a sequence: ``parent`` [rows] int32 is the number of a row's
+    parent among its sequence's rows, a lower one than its own, or -1: it follows the history. A row sees the history,
+    the rows above it and itself, with the bits of attention over a cache that holds this path alone. kv_len counts all
+    of a sequence's rows; ``hidden`` goes by places, as written."""
+    return _native().tree_attention(parent, q, pages, kv_len, row_start, most_rows, most_len, scale, hidden, out)
+
+
+def kv_keep(pages: Pages, kv_len: torch.Tensor, row_start: Optional[torch.Tensor], keep: torch.Tensor, kept: torch.Tensor,
+            most_rows: Optional[int] = None) -> torch.Tensor:
+    """Moves drafted rows (at most 64 a sequence) together: the keep[row_start[i] + t]-th row of sequence i to the place
+    of its t-th, for t < kept[i], and returns the lengths that the sequences then have (int32): the rest is as if it
+    had never been written. ``keep`` [rows] and ``kept`` [sequences] int32."""
+    return _native().kv_keep(pages, kv_len, row_start, keep, kept, most_rows)
+
+
+def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0) -> LogProbs:
+    """Log probabilities under softmax(scale * logits) [rows, n] of ``target`` [rows] int32, and of the ``top`` <= 32
+    likeliest (the lower index first among equals). A target outside [0, n) has NaN and rank -1; a row with a NaN or
+    +inf, or nothing over -inf, NaN and -1 throughout."""
+    return LogProbs(*_native().log_probs(logits, target, top, scale))

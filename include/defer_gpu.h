@@ -364,6 +364,75 @@ int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_r
                            uint32_t hidden_len, void* out, int64_t out_stride, uint32_t clear,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------- drafted tokens
+ *
+ * What a program that drafts tokens and verifies them in one call needs next to
+ * the 8-bit operators, whose rules hold here too: rows appended with their
+ * rotary positions, the attention of a tree of drafts, log probabilities of given
+ * tokens, the accepted path moved together. */
+
+/* How rows are turned. Of each head the first `rotated` values (even) form pairs:
+ * (i, i + rotated / 2), or (2 i, 2 i + 1) where interleaved != 0. Pair i of a row at
+ * position p is turned by p * freq[i], in 64 bits, and multiplied by factor. A row's
+ * position is position[row], or its own in the cache where that is NULL. With a
+ * norm (nullable, [head_dim] of the values' type) a head is first divided by
+ * sqrt(mean(x^2) + eps) and multiplied by it. Nothing is rounded in between. */
+typedef struct defer_gpu_q8_rotary {
+  const double* freq;       /* [rotated / 2]: radians a position */
+  const int32_t* position;  /* [rows] or NULL */
+  const void *q_norm, *k_norm;
+  float eps, factor;
+  uint32_t rotated, interleaved;
+} defer_gpu_q8_rotary;
+
+/* out = q [rows, q_heads, head_dim] turned and rounded to its type; k, turned,
+ * and v [rows, heads, head_dim] quantised into the cache as defer_gpu_q8_kv_write
+ * does. out may be q itself; it shares no memory with k and v. Rows before position
+ * 0 have an out, too. clear != 0: out is zeros for rows of no sequence. */
+int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
+                           const defer_gpu_q8_rotary* rotary, const void* q, int64_t q_stride,
+                           uint32_t q_heads, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, void* out, int64_t out_stride, uint32_t clear,
+                           void* stream);
+
+/* Attention as defer_gpu_q8_attention's, of rows that are nodes of a tree, at most 64 a
+ * sequence: parent[r] [rows] is the number of row r's parent among its
+ * sequence's rows, a lower one than its own, or -1 (or any other): it follows the
+ * history, which is what the sequence has before these rows. A row sees the
+ * history, the rows above it and itself, at the positions that they would have
+ * in a cache with this path alone, and has the bits of attention over that. hidden
+ * goes by places, as written. A sequence of fewer positions than rows attends to
+ * nothing. Workspace as defer_gpu_q8_attention's. */
+int defer_gpu_q8_tree_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
+                                uint32_t type, const void* q, int64_t q_stride, uint32_t q_heads,
+                                const int32_t* parent, uint32_t most_len, float scale,
+                                const uint8_t* hidden, int64_t hidden_stride, uint32_t hidden_len,
+                                void* out, int64_t out_stride, uint32_t clear, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* Moves rows of each sequence together: of its n rows (at most 64) the keep[row_start[i] + t]-th,
+ * for t < kept[i], to the place of the t-th, as if the others had never been written.
+ * An entry outside [0, n) leaves its place as it is. kv_len_out[i] = kv_len[i] - n +
+ * min(kept[i], n), apart from all inputs. No two sequences of a call have a page
+ * of these rows in common. */
+int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
+                         const int32_t* keep, const int32_t* kept, int32_t* kv_len_out, void* stream);
+
+/* Of rows of n <= 1,048,576 logits x [rows, n], rows x_stride values apart, with p =
+ * softmax(scale * x): log_p[r] = log p[target[r]]; entropy[r] = -sum p log p;
+ * rank[r] = how many logits are larger than the target's; top_index and top_log_p
+ * [rows, top]: the top <= 32 largest, the lower index first among equals. A target
+ * outside [0, n) (or target NULL) has log_p NaN and rank -1. A logit of -inf has
+ * probability 0. A row with a NaN or +inf, or with nothing over -inf, has no
+ * distribution: NaN throughout, ranks and indexes -1. `workspace` (16-byte
+ * aligned) is scratch of the size that defer_gpu_q8_log_probs_workspace gives, one
+ * for each call that may overlap. */
+size_t defer_gpu_q8_log_probs_workspace(uint32_t rows, uint32_t n, uint32_t top);
+int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_stride, uint32_t rows, uint32_t n,
+                           const int32_t* target, float scale, uint32_t top, float* log_p,
+                           float* entropy, int32_t* rank, int32_t* top_index, float* top_log_p,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* Thread-local description of the last failing call. */
 const char* defer_gpu_last_error(void);
 
