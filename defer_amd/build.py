@@ -59,7 +59,7 @@ def build_gpu() -> str:
     out = os.path.join(PKG, "libdefer_gpu.so")
     arc = os.path.join(PKG, "libdefer_gpu.a")
     os.makedirs(BUILD, exist_ok=True)
-    srcs = [os.path.join(CSRC, f) for f in ("defer_gpu.hip", "q8.hip", "q8_draft.hip")] + sorted(
+    srcs = [os.path.join(CSRC, f) for f in ("defer_gpu.hip", "q8.hip", "q8_tree.hip", "q8_draft.hip")] + sorted(
         os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.startswith("kernels_") and f.endswith(".hip"))
     flags = [f for f in GPU_FLAGS if f != "-shared"]
     objs = [os.path.join(BUILD, os.path.basename(src).replace(".hip", ".o")) for src in srcs]

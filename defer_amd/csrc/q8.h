@@ -62,5 +62,9 @@ struct Attention {
 size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len);
 int attention(const Pages& p, const Rows& r, const Attention& a, void* workspace, size_t workspace_bytes,
               hipStream_t s);
+// ... of rows that are nodes of trees (a.parent).
+size_t tree_attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len);
+int tree_attention(const Pages& p, const Rows& r, const Attention& a, void* workspace, size_t workspace_bytes,
+                   hipStream_t s);
 
 }  // namespace q8

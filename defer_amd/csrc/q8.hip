@@ -4,7 +4,7 @@
 // Sums of code products are exact in 32-bit integers (v_mfma_i32_16x16x64_i8),
 // so they have no order; every other sum has one that depends on its own row
 // only. Nothing here keeps state, allocates or waits.
-#include "q8_common.h"
+#include "q8_attn.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -722,80 +722,8 @@ __global__ __launch_bounds__(256) void k_kv_read(KvArgs a) {
 
 // ------------------------------------------------------------- attention
 
-struct AttnArgs {
-  Pages p;
-  Rows r;
-  const void* q;
-  void* out;
-  int64_t qs, os;
-  uint32_t type, nh, group, hd, tiles, units;
-  uint32_t per_wave;  // units a wave takes (SPLIT)
-  bool q_vec;  // a head's 16 values are 16-byte loads
-  bool clear;  // zeros for the rows of no sequence
-  int64_t most_len;
-  float scale2;  // scale * log2(e)
-  const uint8_t* hidden;
-  int64_t hs;
-  uint32_t hidden_len;
-  float* part;  // [rows][nh][units][2 + dp]: maximum, sum, accumulators
-  const int32_t* parent;  // [rows] (TREE)
-};
-
-// Four signed base-256 digits of x, one a byte: x = sum of byte_i 256^i.
-__device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x00808080u) ^ 0x00808080u; }
-// ... and back, from sums of products of each digit with codes.
-__device__ __forceinline__ float undigit(v4i d) {
-  return fmaf((float)((d[3] << 8) + d[2]), 65536.0f, (float)((d[1] << 8) + d[0]));
-}
-__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// A running softmax: maximum (as an exponent of 2), sum, accumulators. The
-// next part (m, l, acc) joins it with the weights x and y.
-__device__ __forceinline__ void join_weights(float& M, float m, float* x, float* y) {
-  const float mn = fmaxf(M, m), m0 = mn == -INFINITY ? 0.0f : mn;
-  *x = exp2_of(M - m0);
-  *y = exp2_of(m - m0);
-  M = mn;
-}
-
-// A sequence's drafted rows as a tree, a row each lane: the rows that are its
-// own or above it. A parent that is no earlier row is none: the row hangs on the
-// history. Each step doubles how far up a row has looked.
-struct Tree {
-  uint64_t path;
-  __device__ __forceinline__ Tree(const int32_t* parent, const Span& sp) {
-    const int lane = threadIdx.x % WAVE;
-    int up = lane < sp.n ? parent[sp.start + lane] : -1;
-    up = up < lane ? up : -1;
-    path = 1ull << lane;
-    while (__any(up >= 0)) {
-      const int from = max(up, 0), above = __shfl(up, from);
-      const uint64_t more = __shfl((unsigned long long)path, from);
-      if (up >= 0) {
-        path |= more;
-        up = above;
-      }
-    }
-  }
-  // how many rows are above the lane's own
-  __device__ __forceinline__ int depth() const { return __popcll(path) - 1; }
-  // the position of row j, which is as far behind the history as the row is deep; -1: it has none
-  __device__ __forceinline__ int64_t pos(const Span& sp, uint32_t j) const {
-    const int64_t history = (int64_t)sp.len - sp.n, d = __shfl(depth(), (int)j);
-    return history < 0 || j >= MAX_TREE ? -1 : history + d;
-  }
-};
-struct NoTree {
-  __device__ __forceinline__ NoTree(const int32_t*, const Span&) {}
-  __device__ __forceinline__ int64_t pos(const Span& sp, uint32_t j) const { return sp.pos((int)j); }
-};
-
 enum AttnMode { DIRECT, SPLIT, GROUP };
 constexpr uint32_t SPLIT_WAVES = 4096;
-constexpr int P_ROW = 80;  // bytes of a digit row of 64 probabilities in LDS: rows of four heads on other banks
-constexpr int PATH_LDS = 3 * 4 * PAGE * 4;  // a tile's scores, value scales and marks by position (TREE)
-// Bytes of LDS of a wave's probabilities.
-constexpr size_t attn_lds(uint32_t R, bool tree) { return R * 16 * P_ROW * (tree ? 2 : 1) + (tree ? PATH_LDS : 0); }
 
 // What a wave does: the attention of R tiles of four (row, query head) pairs
 // of one sequence and cache head, over blocks of 64 positions.
@@ -845,22 +773,14 @@ constexpr size_t attn_lds(uint32_t R, bool tree) { return R * 16 * P_ROW * (tree
 // in L1). SPLIT: a few units for each wave, left in the workspace for
 // k_attn_join. GROUP: the units of a tile are the waves of one workgroup, which
 // joins them through LDS.
-//
-// TREE: rows are nodes of a tree. Each has the history and the path from there
-// down to itself, which it meets at the positions that the path would have alone:
-// blocks before the history's end are those of every row; in the others the
-// scores of the nodes' own places go through LDS to the path's positions, the
-// probabilities back from there. Sums over a block's positions of digits times
-// codes are exact, so the places' order changes nothing: the bits are those of
-// the path alone.
-template <int KC, int R, AttnMode MODE, bool TREE>
+template <int KC, int R, AttnMode MODE>
 __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 1 ? 3 : MODE != GROUP && (KC == 1 || (KC == 2 && R == 1)) ? 2 : 1) void k_attn(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
   constexpr bool AHEAD = R == 1 && KC <= 2 && MODE != GROUP;  // the next values wait in registers of their own
   extern __shared__ __align__(16) uint8_t lds[];  // [waves][R][16][P_ROW], GROUP: then [4 R][units][2 + DP] floats
   const uint32_t lane = threadIdx.x % WAVE, n16 = lane % 16, quad = lane / 16;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
-  uint8_t* pl = lds + wave * attn_lds(R, TREE);
+  uint8_t* pl = lds + wave * R * 16 * P_ROW;
 
   // which wave does what: (tile, unit) slowest, (sequence, cache head) fastest
   const uint32_t shs = a.r.sequences * a.p.heads;
@@ -879,7 +799,6 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
   }
   if (MODE == SPLIT ? tile >= a.tiles : item >= a.tiles) return;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
-  const typename std::conditional<TREE, Tree, NoTree>::type tree(a.parent, sp);
   const uint32_t pair0 = tile * 4 * R;
   if (sp.n <= 0 || pair0 >= (uint32_t)sp.n * a.group) return;
   const int32_t* table;
@@ -892,7 +811,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint32_t j = (pair0 + 4 * r + quad) / a.group;
-    const int64_t at = tree.pos(sp, j), t = j < (uint32_t)sp.n ? min(at, a.most_len - 1) : -1;  // (by all lanes)
+    const int64_t t = j < (uint32_t)sp.n ? min(sp.pos((int)j), a.most_len - 1) : -1;
     pos[r] = t < 0 ? -1 : (int)t;
     max_pos = max(max_pos, pos[r]);
     min_pos = min(min_pos, pos[r] < 0 ? 0x7fffffff : pos[r]);
@@ -930,67 +849,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
     const uint32_t pr = pair0 + 4 * r + n16 / 4, j = pr / a.group;
     const bool ok = j < (uint32_t)sp.n;
     const int64_t q0 = (int64_t)(sp.start + (ok ? j : 0)) * a.qs + (int64_t)(g * a.group + pr % a.group) * a.hd;
-    float x[KC][16], top = 0.0f, bad = 0.0f;
-#pragma unroll
-    for (int kk = 0; kk < KC; ++kk) {
-      const uint32_t d0 = kk * 64 + quad * 16;
-      if (a.q_vec) {
-        const int64_t at = q0 + (d0 < a.hd ? d0 : 0);
-        if (a.type == DEFER_GPU_F32) {
-          const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(a.q) + at);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[kk][e] = p[e / 4][e % 4];
-        } else {
-          typedef uint16_t v8h __attribute__((ext_vector_type(8)));
-          const v8h* p = reinterpret_cast<const v8h*>(static_cast<const uint16_t*>(a.q) + at);
-          const bool bf = a.type == DEFER_GPU_BF16;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint16_t h = p[e / 8][e % 8];
-            x[kk][e] = bf ? __builtin_bit_cast(float, (uint32_t)h << 16) : (float)__builtin_bit_cast(_Float16, h);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[kk][e] = ok && d0 < a.hd ? x[kk][e] : 0.0f;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[kk][e] = ok && d0 + e < a.hd ? load_value(a.q, q0 + d0 + e, a.type) : 0.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        top = fmaxf(top, fabsf(x[kk][e]));
-        bad = fmaf(x[kk][e], 0.0f, bad);
-      }
-    }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    bad += __shfl_xor(bad, 16);
-    bad += __shfl_xor(bad, 32);
-    const bool tiny = top > 0.0f && top < 0x1p-64f;
-    if (__builtin_expect(__any(tiny), 0)) {
-      const float lift = tiny ? 0x1p80f : 1.0f;
-      top *= lift;
-#pragma unroll
-      for (int kk = 0; kk < KC; ++kk)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[kk][e] *= lift;
-    }
-    int ex = 0;  // top < 2^ex
-    (void)frexpf(top, &ex);
-    ex = top > 0.0f ? ex : 0;
-    const float up = isnan(bad) ? 0.0f : a.scale2 < 0.0f ? -ldexpf(1.0f, 30 - ex) : ldexpf(1.0f, 30 - ex);
-    const int unit = (tiny ? ex - 80 : ex) - 30;  // of the digit sums
-    const float s = isnan(bad) ? __builtin_nanf("") : (ex > 64 ? -ldexpf(1.0f, unit) : ldexpf(1.0f, unit + 45)) * fabsf(a.scale2);
-    const uint32_t dg = n16 % 4, sel = dg | (4 + dg) << 8;
-#pragma unroll
-    for (int kk = 0; kk < KC; ++kk)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = digits(to_int(x[kk][4 * w + e] * up));
-        aq[r][kk][w] = (int)perm(perm(y[3], y[2], sel), perm(y[1], y[0], sel), 0x05040100u);
-      }
+    const float s = query_digits<KC>(a, q0, ok, aq[r]);
     sq[r] = __shfl(s, (int)quad * 4);
   }
 
@@ -1020,42 +879,6 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 #pragma unroll
       for (int t = 0; t < DT; ++t) A[r][t] = acc[r][t] = 0.0f;
     }
-
-    // A block's scores s of the positions that a lane sees, with their value scales,
-    // as the digits of their probabilities; xw and be: the weights of what came
-    // before and of this block. vbad: what makes the sum NaN (WHOLE).
-    auto weigh = [&](auto whole, int r, const float* s, const bool* see, const v4f& vs, float vbad, float* xw, float* be, uint32_t* y) {
-      constexpr bool WHOLE = decltype(whole)::value;
-      float w[4];
-      const float top = row_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-      const bool none = !WHOLE && top == -INFINITY;
-      const float m0 = none ? 0.0f : top * fabsf(sq[r]);
-      const bool sharp = fabsf(m0) > 0x1p26f;
-      const float before = sharp ? top : 0.0f, behind = sharp ? 0.0f : m0;
-      float lp = vbad;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float p = exp2_of(fmaf(s[j] - before, fabsf(sq[r]), -behind));
-        if (!WHOLE) {
-          p = see[j] ? p : 0.0f;
-          lp += see[j] ? fmaf(vs[j], 0.0f, p) : 0.0f;
-          w[j] = see[j] ? p * vs[j] : 0.0f;
-        } else {
-          lp += p;
-          w[j] = p * vs[j];
-        }
-      }
-      int ex = 0;
-      (void)frexpf(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))), &ex);
-      ex = max(ex, -96);
-      const float up = ldexpf(1.0f, 30 - ex);
-      float yw;
-      join_weights(m[r], none ? -INFINITY : m0, xw, &yw);
-      *be = yw * ldexpf(1.0f, ex - 30);
-      l[r] = fmaf(lp, yw, l[r] * *xw);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = digits(to_int(w[j] * up));
-    };
 
     // A block whose codes have been loaded: WHOLE if every row sees all of it.
     // next: the page to load meanwhile, or -1.
@@ -1097,7 +920,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
           s[j] = see[j] ? x : -INFINITY;
         }
         uint32_t y[4];
-        weigh(whole, r, s, see, vs, vbad, &xw[r], &be[r], y);
+        block_weights<WHOLE>(s, see, vs, vbad, fabsf(sq[r]), m[r], l[r], &xw[r], &be[r], y);
         uint32_t* pw = reinterpret_cast<uint32_t*>(pl + (16 * r + 4 * quad) * P_ROW) + n16;
         uint32_t by_digit[4];
         transpose4(y, by_digit);
@@ -1125,128 +948,6 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
       }
     };
 
-    // A block of a path's positions, behind the history's end or around it. The nodes
-    // on it are in this place's page or the next (a tree has no more than 64 rows).
-    const int history = (int)min((int64_t)sp.len - sp.n, (int64_t)0x7fffffff), first_path = TREE ? history / PAGE : 0x7fffffff;
-    auto path_block = [&](int b, int page, int page_behind, int next) {
-      if constexpr (TREE) {
-        float x[2][R][4];
-        int at[2][4];  // the position within the block of a place's node
-        uint32_t seen[2][R];
-        v4f vsp[2];
-        const int depth = tree.depth();
-#pragma unroll
-        for (int pb = 0; pb < 2; ++pb) {
-          if (pb) {
-            if (page_behind >= 0) load_k(page_behind);
-          }
-          vsp[pb] = vsn;
-          const v4f kp = ksn;
-          const bool there = (pb ? page_behind : page) >= 0;
-          bool on[4];
-          int node[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int t = (b + pb) * PAGE + 4 * n16 + j;
-            node[j] = t - history;
-            const int d = __shfl(depth, node[j] & (WAVE - 1));
-            at[pb][j] = (node[j] < 0 ? t : history + d) - b * PAGE;
-            on[j] = there && node[j] < min(sp.n, (int)MAX_TREE) && at[pb][j] >= 0 && at[pb][j] < PAGE;
-            if (hid && on[j]) on[j] = !((uint32_t)t < a.hidden_len && hid[t] != 0);
-          }
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float unit = sq[r] < 0.0f ? 1.0f : 0x1p-45f;
-            const uint64_t path = __shfl((unsigned long long)tree.path, (int)((pair0 + 4 * r + quad) / a.group) & (WAVE - 1));
-            seen[pb][r] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              v4i d = {0, 0, 0, 0};
-              if (there) {
-#pragma unroll
-                for (int kk = 0; kk < KC; ++kk) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(aq[r][kk], k[j][kk], d, 0, 0, 0);
-              }
-              x[pb][r][j] = undigit(d) * unit * kp[j];
-              const bool see = on[j] && b * PAGE + at[pb][j] <= ps[r] && (node[j] < 0 || (path >> (node[j] & (WAVE - 1)) & 1));
-              seen[pb][r] |= (uint32_t)see << j;
-            }
-          }
-        }
-        float* const sl = reinterpret_cast<float*>(pl + 2 * R * 16 * P_ROW) + quad * PAGE;  // this quad's pair
-        float* const vl = sl + 4 * PAGE;
-        uint32_t* const ml = reinterpret_cast<uint32_t*>(vl + 4 * PAGE);
-        float xw[R], be[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          *reinterpret_cast<v4i*>(ml + 4 * n16) = v4i{0, 0, 0, 0};
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int pb = 0; pb < 2; ++pb)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (seen[pb][r] >> j & 1) {
-                sl[at[pb][j]] = x[pb][r][j];
-                vl[at[pb][j]] = vsp[pb][j];
-                ml[at[pb][j]] = 1;
-              }
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-          const v4f sv = *reinterpret_cast<const v4f*>(sl + 4 * n16), vv = *reinterpret_cast<const v4f*>(vl + 4 * n16);
-          const v4i mv = *reinterpret_cast<const v4i*>(ml + 4 * n16);
-          float s[4];
-          bool see[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            see[j] = mv[j] != 0;
-            s[j] = see[j] ? sv[j] : -INFINITY;
-          }
-          uint32_t y[4];
-          weigh(std::false_type(), r, s, see, vv, 0.0f, &xw[r], &be[r], y);
-          *reinterpret_cast<v4i*>(ml + 4 * n16) = v4i{(int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int pb = 0; pb < 2; ++pb) {
-            uint32_t p[4], by_digit[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = seen[pb][r] >> j & 1 ? ml[at[pb][j]] : 0;
-            transpose4(p, by_digit);
-            uint32_t* pw = reinterpret_cast<uint32_t*>(pl + (16 * (2 * r + pb) + 4 * quad) * P_ROW) + n16;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pw[i * P_ROW / 4] = by_digit[i];
-          }
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
-        }
-        v4i pa[R][2];
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int pb = 0; pb < 2; ++pb)
-            pa[r][pb] = *reinterpret_cast<const v4i*>(pl + (16 * (2 * r + pb) + n16) * P_ROW + quad * 16);
-        const int8_t* const vb = v0 + (size_t)max(page_behind, 0) * a.p.heads * PAGE * DP;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-          v4i vt = {0, 0, 0, 0};
-          if (page_behind >= 0) vt = *reinterpret_cast<const v4i*>(vb + 16 * t * PAGE);
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            v4i o = {0, 0, 0, 0};
-            if (page >= 0) o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[r][0], v[t], o, 0, 0, 0);
-            if (page_behind >= 0) o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[r][1], vt, o, 0, 0, 0);
-            acc[r][t] = fmaf(undigit(o), be[r], acc[r][t] * xw[r]);
-          }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (next >= 0) {
-          load_k(next);
-          load_v(next, v);
-        }
-      }
-    };
-
     const int bpu = ul / PAGE, blocks = pmax < 0 ? 0 : pmax / PAGE + 1;
     const int du = MODE == GROUP ? (int)waves : 1;
     int u = MODE == SPLIT ? (int)(item % chunks * a.per_wave) : MODE == GROUP ? (int)wave : 0;
@@ -1271,10 +972,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
       const bool unit_ends = b + 1 == blocks || (b + 1) % bpu == 0;
       const int bn = unit_ends ? (u + du) * bpu : b + 1;
       const int next = bn < blocks && (!unit_ends || u + du < u_end) ? page_at(bn) : -1;
-      if (TREE && b >= first_path) {
-        const int last = (history + min(sp.n, (int)MAX_TREE) - 1) / PAGE;  // the last place's page
-        path_block(b, page, b < last ? page_at(b + 1) : -1, next);
-      } else if (page >= 0) {
+      if (page >= 0) {
         if (!hid && b * PAGE + PAGE - 1 <= pmin)
           block(std::true_type(), b, next);
         else
@@ -1296,7 +994,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
           } else if (ps[r] >= 0 && u < unit_count(ps[r])) {
             const uint32_t pr = pair0 + 4 * r + quad;
             float* o = MODE == SPLIT ? a.part + (((size_t)(sp.start + pr / a.group) * a.nh + g * a.group + pr % a.group) * a.units + u) * (2 + DP)
-                                     : reinterpret_cast<float*>(lds + waves * attn_lds(R, TREE)) +
+                                     : reinterpret_cast<float*>(lds + waves * R * 16 * P_ROW) +
                                            ((4 * r + quad) * a.units + u) * (2 + DP);
             if (n16 == 0) {
               o[0] = m[r];
@@ -1333,11 +1031,11 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
   }
   if (MODE == GROUP) {
     __syncthreads();
-    const float* parts = reinterpret_cast<const float*>(lds + waves * attn_lds(R, TREE));
+    const float* parts = reinterpret_cast<const float*>(lds + waves * R * 16 * P_ROW);
     for (uint32_t i = threadIdx.x; i < 4u * R * DP; i += blockDim.x) {
-      const uint32_t pr = pair0 + i / DP, j = pr / a.group, d = i % DP;  // (pr: the same in all lanes)
+      const uint32_t pr = pair0 + i / DP, j = pr / a.group, d = i % DP;
       if (j >= (uint32_t)sp.n) continue;
-      const int n = unit_count(min(tree.pos(sp, j), a.most_len - 1));
+      const int n = unit_count(min(sp.pos((int)j), a.most_len - 1));
       const float* p = parts + i / DP * a.units * (2 + DP);
       float M = -INFINITY, L = 0.0f, A = 0.0f;
       for (int u = 0; u < n; ++u, p += 2 + DP) {
@@ -1358,13 +1056,11 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256, MODE == DIRECT && KC == 
 // sum, the accumulators of 32 units are on their way at a time. Three dependent
 // reads of what other XCDs wrote: 10 us for 11 x 32 heads of 47 units (8.6 MB);
 // 64 units at a time changed nothing.
-template <bool TREE>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   const uint32_t h = blockIdx.x % a.nh, j = blockIdx.x / a.nh % a.r.most_rows, seq = blockIdx.x / a.nh / a.r.most_rows;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
   if (j >= (uint32_t)sp.n) return;
-  const typename std::conditional<TREE, Tree, NoTree>::type tree(a.parent, sp);
-  const int64_t pos = min(tree.pos(sp, j), a.most_len - 1);
+  const int64_t pos = min(sp.pos((int)j), a.most_len - 1);
   const uint32_t row = sp.start + j, d = threadIdx.x, dp = a.p.dp, lane = threadIdx.x % WAVE;
   const float* p = a.part + ((size_t)row * a.nh + h) * a.units * (2 + dp);
   const int n = unit_count(pos);
@@ -1418,16 +1114,16 @@ int rows_launch(uint32_t type, const NormArgs& a, uint32_t rows, hipStream_t s) 
   return rows_launch_as<_Float16, NORM>(a, rows, s);
 }
 
-template <int R, AttnMode MODE, bool TREE>
+template <int R, AttnMode MODE>
 int attn_launch(const AttnArgs& a, uint32_t blocks, uint32_t threads, size_t lds, hipStream_t s) {
   const uint32_t kc = a.p.dp / 64;
   if constexpr (R <= 2)
-    if (kc == 1) return launch(k_attn<1, R, MODE, TREE>, blocks, threads, lds, s, a);
-  if (kc == 2) return launch(k_attn<2, R, MODE, TREE>, blocks, threads, lds, s, a);
+    if (kc == 1) return launch(k_attn<1, R, MODE>, blocks, threads, lds, s, a);
+  if (kc == 2) return launch(k_attn<2, R, MODE>, blocks, threads, lds, s, a);
   if constexpr (MODE != GROUP && R <= 2)
-    if (kc == 3) return launch(k_attn<3, R, MODE, TREE>, blocks, threads, lds, s, a);
+    if (kc == 3) return launch(k_attn<3, R, MODE>, blocks, threads, lds, s, a);
   if constexpr (MODE != GROUP && R == 1)
-    if (kc == 4) return launch(k_attn<4, R, MODE, TREE>, blocks, threads, lds, s, a);
+    if (kc == 4) return launch(k_attn<4, R, MODE>, blocks, threads, lds, s, a);
   return defer_gpu_fail_(DEFER_GPU_E_INVALID, "no attention kernel for head_dim %u", a.hd);
 }
 
@@ -1442,7 +1138,7 @@ struct Plan {
   uint32_t R, tiles, units, per_wave, waves;  // tiles of 4 R pairs; units of a row at most, of a wave; waves of a workgroup
   size_t lds, workspace;
 };
-Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint32_t most_len, bool tree) {
+Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint32_t most_len) {
   const uint32_t pairs = (uint32_t)pairs_of(r, heads, kv_heads);
   Plan p;
   // Tiles share the codes a wave has loaded, so the more the better, as far as
@@ -1478,7 +1174,7 @@ Plan plan_of(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t dp, uint
   } else {
     p.mode = DIRECT;
   }
-  p.lds = p.waves * attn_lds(p.R, tree) + (p.mode == GROUP ? 4 * (size_t)p.R * p.units * (2 + dp) * sizeof(float) : 0);
+  p.lds = p.waves * p.R * 16 * P_ROW + (p.mode == GROUP ? 4 * (size_t)p.R * p.units * (2 + dp) * sizeof(float) : 0);
   return p;
 }
 
@@ -1590,22 +1286,11 @@ int kv_read(const Pages& p, const Rows& r, uint32_t type, void* k, void* v, uint
   return launch(k_kv_read, kv_grid(p, and_one), r.most_rows <= 8 ? 64 : 256, 0, s, a);
 }
 
-template <bool TREE>
-static int attn_dispatch(const AttnArgs& a, const Plan& pl, uint32_t nb, uint32_t nt, hipStream_t s) {
-  if (pl.mode == SPLIT) {
-    const int rc = pl.R == 1 ? attn_launch<1, SPLIT, TREE>(a, nb, nt, pl.lds, s) : attn_launch<2, SPLIT, TREE>(a, nb, nt, pl.lds, s);
-    return rc ? rc : launch(k_attn_join<TREE>, a.r.sequences * a.r.most_rows * a.nh, a.p.dp, 0, s, a);
-  }
-  if (pl.mode == GROUP)
-    return pl.R == 1 ? attn_launch<1, GROUP, TREE>(a, nb, nt, pl.lds, s) : attn_launch<2, GROUP, TREE>(a, nb, nt, pl.lds, s);
-  if (pl.R == 1) return attn_launch<1, DIRECT, TREE>(a, nb, nt, pl.lds, s);
-  return pl.R == 2 ? attn_launch<2, DIRECT, TREE>(a, nb, nt, pl.lds, s) : attn_launch<4, DIRECT, TREE>(a, nb, nt, pl.lds, s);
-}
-
 size_t attention_workspace(const Rows& r, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t most_len) {
   if (!r.rows || !r.sequences || !r.most_rows || pairs_of(r, heads, kv_heads) > MOST_PAIRS) return 0;
   const uint32_t dp = padded(head_dim);
-  return plan_of(r, heads, kv_heads, dp, most_len, false).workspace;
+  const Plan pl = plan_of(r, heads, kv_heads, dp, most_len);
+  return pl.workspace;
 }
 
 int attention(const Pages& p, const Rows& r, const Attention& in, void* workspace, size_t workspace_bytes,
@@ -1616,41 +1301,28 @@ int attention(const Pages& p, const Rows& r, const Attention& in, void* workspac
   }
   if (pairs_of(r, in.heads, p.heads) > MOST_PAIRS)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
-  const Plan pl = plan_of(r, in.heads, p.heads, p.dp, in.most_len, in.parent != nullptr);
+  const Plan pl = plan_of(r, in.heads, p.heads, p.dp, in.most_len);
   const size_t need = attention_workspace(r, in.heads, p.heads, in.head_dim, in.most_len);
   if (need && (!workspace || workspace_bytes < need))
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "attention needs a workspace of %zu bytes, got %zu", need,
                            workspace ? workspace_bytes : (size_t)0);
-  AttnArgs a{};
-  a.p = p;
-  a.r = r;
-  a.q = in.q;
-  a.out = in.out;
-  a.qs = in.q_stride;
-  a.os = in.out_stride;
-  a.type = in.type;
-  a.nh = in.heads;
-  a.group = in.heads / p.heads;
-  a.hd = in.head_dim;
+  AttnArgs a = attn_args(p, r, in, workspace);
   a.tiles = pl.tiles;
   a.units = pl.units;
   a.per_wave = pl.per_wave;
-  a.most_len = in.most_len;
-  a.scale2 = in.scale * 1.44269504088896340736f;
-  a.hidden = in.hidden;
-  a.hs = in.hidden_stride;
-  a.hidden_len = in.hidden_len;
-  a.part = static_cast<float*>(workspace);
-  a.parent = in.parent;
-  a.clear = in.clear && r.row_start;
-  const size_t vs = in.type == DEFER_GPU_F32 ? 4 : 2;
-  a.q_vec = in.head_dim % 16 == 0 && ((uintptr_t)in.q | (uintptr_t)(in.q_stride * (int64_t)vs)) % 16 == 0;
   const uint64_t items = (uint64_t)pl.tiles * (pl.mode == SPLIT ? (pl.units + pl.per_wave - 1) / pl.per_wave : 1);
   const uint64_t blocks = (pl.mode == GROUP ? items : (items + 3) / 4) * r.sequences * p.heads;
   if (blocks * pl.waves * WAVE > MAX_THREADS)
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
   const uint32_t nb = (uint32_t)blocks, nt = pl.waves * WAVE;
-  return in.parent ? attn_dispatch<true>(a, pl, nb, nt, s) : attn_dispatch<false>(a, pl, nb, nt, s);
+  if (pl.mode == SPLIT) {
+    const int rc = pl.R == 1 ? attn_launch<1, SPLIT>(a, nb, nt, pl.lds, s) : attn_launch<2, SPLIT>(a, nb, nt, pl.lds, s);
+    return rc ? rc : launch(k_attn_join, r.sequences * r.most_rows * in.heads, p.dp, 0, s, a);
+  }
+  if (pl.mode == GROUP)
+    return pl.R == 1 ? attn_launch<1, GROUP>(a, nb, nt, pl.lds, s) : attn_launch<2, GROUP>(a, nb, nt, pl.lds, s);
+  if (pl.R == 1) return attn_launch<1, DIRECT>(a, nb, nt, pl.lds, s);
+  return pl.R == 2 ? attn_launch<2, DIRECT>(a, nb, nt, pl.lds, s) : attn_launch<4, DIRECT>(a, nb, nt, pl.lds, s);
 }
 
 }  // namespace q8
@@ -1738,6 +1410,13 @@ extern "C" size_t defer_gpu_q8_attention_workspace(const defer_gpu_q8_pages* pag
   return attention_workspace(r, q_heads, pages->heads, pages->head_dim, most_len);
 }
 
+extern "C" size_t defer_gpu_q8_tree_attention_workspace(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
+                                                        uint32_t q_heads, uint32_t most_len) {
+  if (!pages || !rows || !pages->heads || !q_heads || pages->head_dim > MAX_HEAD_DIM) return 0;
+  const Rows r{rows->row_start, rows->kv_len, rows->sequences, rows->rows, rows->most_rows};
+  return tree_attention_workspace(r, q_heads, pages->heads, pages->head_dim, most_len);
+}
+
 static int attend(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type, const void* q,
                   int64_t q_stride, uint32_t q_heads, const int32_t* parent, uint32_t most_len, float scale,
                   const uint8_t* hidden, int64_t hidden_stride, uint32_t hidden_len, void* out, int64_t out_stride,
@@ -1758,7 +1437,7 @@ static int attend(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows
   Q8_REQUIRE(aligned16(workspace), "workspace is not 16-byte aligned");
   Attention a{type, q, q_stride, out, out_stride, q_heads, pages->head_dim, scale, most_len, hidden, hidden_stride,
               hidden_len, clear != 0, parent};
-  return attention(p, r, a, workspace, workspace_bytes, (hipStream_t)stream);
+  return (parent ? tree_attention : attention)(p, r, a, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 extern "C" int defer_gpu_q8_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,

@@ -196,10 +196,7 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs a) {
 
   // the cache's heads: keys and values that have a place and a page
   const int64_t block = down(run, PAGE / KV_RUN);
-  const int32_t* table;
-  uint32_t width;
-  const SeqPages pool = pool_of(a.p, seq, table, width);
-  const int page = page_of(table, width, pool.pages, block);
+  const int page = page_of(a.p.table + (size_t)seq * a.p.width, a.p.width, a.p.pages, block);
   if (page < 0) return;  // (places before 0 among them)
   const uint32_t g0 = chunk * a.kv_heads, heads = min(a.kv_heads, a.p.heads - g0);
   const int a0 = (int)(t0 - block * PAGE);  // the first row's place in its page
@@ -239,14 +236,14 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) c |= (uint64_t)(uint8_t)code(y[h][e]) << (8 * e);
       // a page's row is a multiple of 64 codes: those behind hd are zeros
-      int8_t* to = value ? tile + (gl * most + j) * KV_ROW + d : pool.keys + (hp * PAGE + a0 + j) * a.p.dp + d;
+      int8_t* to = value ? tile + (gl * most + j) * KV_ROW + d : a.p.keys + (hp * PAGE + a0 + j) * a.p.dp + d;
       *reinterpret_cast<uint64_t*>(to) = c;
     }
-    if (n16 == 0) (value ? pool.value_scale : pool.key_scale)[hp * PAGE + a0 + j] = scale;
+    if (n16 == 0) (value ? a.p.value_scale : a.p.key_scale)[hp * PAGE + a0 + j] = scale;
   }
   __syncthreads();
   // value codes into their transposed pages
-  int8_t* vc = pool.values + ((size_t)page * a.p.heads + g0) * PAGE * a.p.dp;
+  int8_t* vc = a.p.values + ((size_t)page * a.p.heads + g0) * PAGE * a.p.dp;
   if (n < KV_RUN) {  // some of the run: byte by byte
     for (uint32_t i = threadIdx.x; i < heads * n * hd; i += blockDim.x) {
       const uint32_t d = i % hd, hj = i / hd, j = hj % n, gl = hj / n;
@@ -298,11 +295,8 @@ __global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
   __shared__ float scales[2][MAX_TREE];
   __shared__ int64_t from[MAX_TREE], to[MAX_TREE];  // places: page * 64 + position, or -1
   if (move <= 0) return;
-  const int32_t* table;
-  uint32_t width;
-  const SeqPages pool = pool_of(a.p, seq, table, width);
   auto place = [&](int64_t pos) -> int64_t {
-    const int page = pos < 0 ? -1 : page_of(table, width, pool.pages, pos / PAGE);
+    const int page = pos < 0 ? -1 : page_of(a.p.table + (size_t)seq * a.p.width, a.p.width, a.p.pages, pos / PAGE);
     return page < 0 ? -1 : (int64_t)page * PAGE + pos % PAGE;
   };
   for (int t = threadIdx.x; t < move; t += blockDim.x) {
@@ -319,32 +313,32 @@ __global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
     const uint32_t t = i / (dp / 16), d = i % (dp / 16) * 16;
     if (to[t] >= 0)
       *reinterpret_cast<v4i*>(keys + t * 256 + d) =
-          *reinterpret_cast<const v4i*>(pool.keys + (head(from[t]) * PAGE + from[t] % PAGE) * dp + d);
+          *reinterpret_cast<const v4i*>(a.p.keys + (head(from[t]) * PAGE + from[t] % PAGE) * dp + d);
   }
   for (uint32_t i = threadIdx.x; i < move * a.hd; i += blockDim.x) {
     const uint32_t t = i % move, d = i / move;
-    if (to[t] >= 0) values[t * 256 + d] = pool.values[(head(from[t]) * dp + d) * PAGE + from[t] % PAGE];
+    if (to[t] >= 0) values[t * 256 + d] = a.p.values[(head(from[t]) * dp + d) * PAGE + from[t] % PAGE];
   }
   for (int t = threadIdx.x; t < move; t += blockDim.x)
     if (to[t] >= 0) {
-      scales[0][t] = pool.key_scale[head(from[t]) * PAGE + from[t] % PAGE];
-      scales[1][t] = pool.value_scale[head(from[t]) * PAGE + from[t] % PAGE];
+      scales[0][t] = a.p.key_scale[head(from[t]) * PAGE + from[t] % PAGE];
+      scales[1][t] = a.p.value_scale[head(from[t]) * PAGE + from[t] % PAGE];
     }
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < move * dp / 16; i += blockDim.x) {
     const uint32_t t = i / (dp / 16), d = i % (dp / 16) * 16;
     if (to[t] >= 0)
-      *reinterpret_cast<v4i*>(pool.keys + (head(to[t]) * PAGE + to[t] % PAGE) * dp + d) =
+      *reinterpret_cast<v4i*>(a.p.keys + (head(to[t]) * PAGE + to[t] % PAGE) * dp + d) =
           *reinterpret_cast<const v4i*>(keys + t * 256 + d);
   }
   for (uint32_t i = threadIdx.x; i < move * a.hd; i += blockDim.x) {
     const uint32_t t = i % move, d = i / move;
-    if (to[t] >= 0) pool.values[(head(to[t]) * dp + d) * PAGE + to[t] % PAGE] = values[t * 256 + d];
+    if (to[t] >= 0) a.p.values[(head(to[t]) * dp + d) * PAGE + to[t] % PAGE] = values[t * 256 + d];
   }
   for (int t = threadIdx.x; t < move; t += blockDim.x)
     if (to[t] >= 0) {
-      pool.key_scale[head(to[t]) * PAGE + to[t] % PAGE] = scales[0][t];
-      pool.value_scale[head(to[t]) * PAGE + to[t] % PAGE] = scales[1][t];
+      a.p.key_scale[head(to[t]) * PAGE + to[t] % PAGE] = scales[0][t];
+      a.p.value_scale[head(to[t]) * PAGE + to[t] % PAGE] = scales[1][t];
     }
 }
 

@@ -40,6 +40,7 @@ struct {
   decltype(&defer_gpu_q8_kv_read) kv_read;
   decltype(&defer_gpu_q8_attention_workspace) attention_workspace;
   decltype(&defer_gpu_q8_attention) attention;
+  decltype(&defer_gpu_q8_tree_attention_workspace) tree_attention_workspace;
   decltype(&defer_gpu_q8_tree_attention) tree_attention;
   decltype(&defer_gpu_q8_kv_append) kv_append;
   decltype(&defer_gpu_q8_kv_keep) kv_keep;
@@ -376,7 +377,7 @@ PyObject* attend(PyObject* const* a, PyObject* parent) {
     os = row_stride(out, "out", dev, type, q.sizes());
     apart(out, os, q, qs, "q");
   }
-  const size_t need_bytes = lib.attention_workspace(&c.p, &c.r, heads, (uint32_t)most_len);
+  const size_t need_bytes = (parent ? lib.tree_attention_workspace : lib.attention_workspace)(&c.p, &c.r, heads, (uint32_t)most_len);
   Tensor work;
   if (need_bytes) work = fresh({(int64_t)need_bytes}, ScalarType::Byte, dev);
   void* const w = need_bytes ? work.data_ptr() : nullptr;
@@ -525,6 +526,7 @@ PyObject* bind(PyObject*, PyObject* args) {
         take("defer_gpu_q8_linear", lib.linear) && take("defer_gpu_q8_kv_write", lib.kv_write) &&
         take("defer_gpu_q8_kv_read", lib.kv_read) &&
         take("defer_gpu_q8_attention_workspace", lib.attention_workspace) &&
+        take("defer_gpu_q8_tree_attention_workspace", lib.tree_attention_workspace) &&
         take("defer_gpu_q8_tree_attention", lib.tree_attention) && take("defer_gpu_q8_kv_append", lib.kv_append) &&
         take("defer_gpu_q8_kv_keep", lib.kv_keep) && take("defer_gpu_q8_log_probs_workspace", lib.log_probs_workspace) &&
         take("defer_gpu_q8_log_probs", lib.log_probs)))

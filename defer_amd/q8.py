@@ -129,6 +129,7 @@ def _lib():
                 ("attention_workspace", [pages, rows, u32, u32], sz),
                 ("attention", [pages, rows, u32, vp, i64, u32, u32, f32, vp, i64, u32, vp, i64, u32, vp, sz, vp],
                  ctypes.c_int),
+                ("tree_attention_workspace", [pages, rows, u32, u32], sz),
                 ("tree_attention", [pages, rows, u32, vp, i64, u32, vp, u32, f32, vp, i64, u32, vp, i64, u32, vp, sz, vp],
                  ctypes.c_int),
                 ("kv_append", [pages, rows, u32, ctypes.POINTER(_CRotary), vp, i64, u32, vp, i64, vp, i64, vp, i64, u32, vp],

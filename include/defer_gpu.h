@@ -402,7 +402,9 @@ int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const defer_gpu_q8_r
  * history, the rows above it and itself, at the positions that they would have
  * in a cache with this path alone, and has the bits of attention over that. hidden
  * goes by places, as written. A sequence of fewer positions than rows attends to
- * nothing. Workspace as defer_gpu_q8_attention's. */
+ * nothing. */
+size_t defer_gpu_q8_tree_attention_workspace(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
+                                             uint32_t q_heads, uint32_t most_len);
 int defer_gpu_q8_tree_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
                                 uint32_t type, const void* q, int64_t q_stride, uint32_t q_heads,
                                 const int32_t* parent, uint32_t most_len, float scale,

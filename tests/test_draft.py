@@ -83,7 +83,7 @@ def test_tree_attention_refuses():
                    (10, P + 4), (11, 255), (13, P + 8)):
         refused("tree_attention", p, r, *[bad if j == i else a for j, a in enumerate(TREE)])
     assert "at most 64" in refused("tree_attention", p, _rows(rows=100, most_rows=65), *TREE)
-    need = call("attention_workspace", p, _rows(), 4, 10000)
+    need = call("tree_attention_workspace", p, _rows(), 4, 10000)
     assert need > 0
     long = [10000 if j == 5 else a for j, a in enumerate(TREE)]
     assert "workspace" in refused("tree_attention", p, r, *[need - 1 if j == 14 else a for j, a in enumerate(long)])
