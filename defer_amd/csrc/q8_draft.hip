@@ -5,6 +5,8 @@
 // the one whose bits it has.)
 #include "q8_common.h"
 
+#include <float.h>
+
 #include <algorithm>
 
 namespace q8 {
@@ -344,12 +346,15 @@ __global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
 
 // ------------------------------------------------------------- log probabilities
 
-constexpr int SCORE_THREADS = 1024, SCORE_EACH = 16, SCORE_CHUNK = SCORE_THREADS * SCORE_EACH;  // logits of a workgroup
-constexpr int SCORE_FEW = 512;  // candidates that are ranked against each other
+constexpr int SCORE_THREADS = 512, SCORE_EACH = 16, SCORE_CHUNK = SCORE_THREADS * SCORE_EACH;  // logits of a workgroup
+constexpr int SCORE_WAVES = SCORE_THREADS / WAVE;
+constexpr int SCORE_GROUP = SCORE_THREADS / WAVE;  // threads whose logits have a maximum together: 64 maxima a chunk
+constexpr uint32_t SCORE_FEW = 2048;               // candidates for the best that a row may have in LDS
+constexpr uint32_t SCORE_LIST = 1024;              // ... and groups that they come from
 
 // What a workgroup leaves of its chunk of a row, joined in the order of chunks.
 struct ScorePart {
-  float top, sum, moment;  // maximum m; sum of e = exp(scale (x - m)); sum of e (x - m)
+  float top, sum, moment;  // maximum m; sum of e = exp(scale (x - m)), and of e (x - m)
   uint32_t above;          // logits over the target's
 };
 
@@ -362,7 +367,7 @@ struct ScoreArgs {
   float *log_p, *entropy, *top_log_p;
   int32_t *rank, *top_index;
   ScorePart* part;   // [rows][chunks]
-  uint64_t* best;    // [rows][chunks][top], the largest first; 0: none
+  float* maxima;     // [rows][chunks][64], for the best
 };
 
 // A whole number that orders logits by value, then by the lower column. -0 is
@@ -378,173 +383,346 @@ __device__ __forceinline__ float value_of(uint64_t key) {
   return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-// The row's outputs from its joined statistics (every lane has them) and its
-// best (lane t < top: the t-th). In 64 bits: logarithms next to zero.
-__device__ __forceinline__ void score_store(const ScoreArgs& a, uint32_t row, uint32_t t, float top, double sum, double moment,
-                                            uint32_t above, float xt, bool has, uint64_t key) {
-  const float nan = __builtin_nanf("");
-  const bool none = !(sum >= 1.0);  // a NaN, an infinity, or nothing over -inf: no distribution
-  const double log_sum = log(sum);
-  if (t == 0) {
-    a.log_p[row] = none || !has ? nan : (float)((double)a.scale * ((double)xt - (double)top) - log_sum);
-    a.entropy[row] = none ? nan : (float)fmax(0.0, log_sum - (double)a.scale * moment / sum);
-    a.rank[row] = none || !has ? -1 : (int32_t)above;
+// A bound that `top` of the wave's numbers reach and at most `slack` more, unless they are equal;
+// 0 if fewer are over 0. Steps down from the largest, then halves.
+__device__ __forceinline__ uint32_t score_bound(uint32_t o, uint32_t top, uint32_t slack) {
+  uint32_t most = o;
+  for (int s = 32; s > 0; s >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, s));
+  most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
+  uint32_t lo = 0, hi = most + 1, step = 1u << 20;  // `top` reach lo (or it is 0), fewer reach hi
+  while (hi - lo > 1) {
+    const uint32_t t = lo ? lo + (hi - lo) / 2 : most > step ? most - step : 1;
+    const uint32_t n = (uint32_t)__popcll(__ballot(o >= t));
+    if (n >= top) {
+      lo = t;
+      if (n <= top + slack) break;
+    } else {
+      hi = t;
+      step = step >= 1u << 30 ? 0xffffffffu : step * 4;
+    }
   }
-  if (t < a.top) {
-    a.top_log_p[(size_t)row * a.top + t] = none ? nan : (float)((double)a.scale * ((double)value_of(key) - (double)top) - log_sum);
-    a.top_index[(size_t)row * a.top + t] = none ? -1 : (int32_t)column_of(key);
+  return lo;
+}
+
+// The `top` largest of `count` different keys in LDS, in their order, by one wave, which
+// gathers those over a bound at their front and ranks them; two of them a lane are enough
+// but for rows of many equal logits.
+template <class F>
+__device__ __forceinline__ void score_pick(uint64_t* keys, uint32_t count, uint32_t top, F store) {
+  const uint32_t lane = threadIdx.x % WAVE;
+  auto meet = [] {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  if (count > WAVE) {
+    uint32_t o = 0;
+    for (uint32_t i = lane; i < count; i += WAVE) o = max(o, (uint32_t)(keys[i] >> 32));
+    const uint32_t bound = score_bound(o, top, top / 4);
+    uint32_t n = 0;
+    for (uint32_t i = lane; i < (count + WAVE - 1) / WAVE * WAVE; i += WAVE) {
+      const uint64_t k = i < count ? keys[i] : 0;
+      const bool is = k && (uint32_t)(k >> 32) >= bound;
+      const uint64_t mask = __ballot(is);
+      meet();
+      if (is) keys[n + (uint32_t)__popcll(mask & ((1ull << lane) - 1))] = k;
+      n += (uint32_t)__popcll(mask);
+    }
+    count = n;
+    meet();
+  }
+  if (count <= 2 * WAVE) {
+    const uint64_t k0 = lane < count ? keys[lane] : 0, k1 = lane + WAVE < count ? keys[lane + WAVE] : 0;
+    uint32_t b0 = 0, b1 = 0;
+    auto against = [&](uint64_t k, int n) {
+      for (int i = 0; i < n; ++i) {
+        const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(k >> 32), i) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, i);
+        b0 += o > k0;
+        b1 += o > k1;
+      }
+    };
+    against(k0, (int)min(count, (uint32_t)WAVE));
+    if (count > WAVE) against(k1, (int)(count - WAVE));
+    if (lane < count && b0 < top) store(b0, k0);
+    if (lane + WAVE < count && b1 < top) store(b1, k1);
+    return;
+  }
+  for (uint32_t i = lane; i < count; i += WAVE) {
+    const uint64_t k = keys[i];
+    uint32_t before = 0;
+    for (uint32_t j = 0; j < count; ++j) before += keys[j] > k;
+    if (before < top) store(before, k);
   }
 }
 
-// One chunk of a row: in registers, 16 logits a thread, read once. Its maximum,
-// then the sums relative to it. The best: a bound that at least `top` logits
-// reach is the top-th of the maxima of each 16 lanes; the few that reach it are
-// ranked against each other.
+// Over N neighbouring lanes: in each of them.
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
+  v = fmaxf(v, dpp<0xb1>(v));                 // quad_perm 1 0 3 2
+  v = fmaxf(v, dpp<0x4e>(v));                 // quad_perm 2 3 0 1
+  if (N >= 8) v = fmaxf(v, dpp<0x141>(v));    // row_half_mirror
+  if (N >= 16) v = fmaxf(v, dpp<0x140>(v));   // row_mirror
+  return v;
+}
+
+// Over the wave: 16 lanes, then the rows.
+__device__ __forceinline__ float wave_sum(float v) {
+  v = row_sum(v);
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// One chunk of a row: in registers, 16 logits a thread, read once; each wave's
+// sums are relative to its own maximum, the first wave joins them. For the best, the
+// maxima of 64 groups of threads are left: k_score_join reads the few groups again
+// that can hold one.
 template <class T, bool VEC>
-__global__ __launch_bounds__(SCORE_THREADS) void k_score(ScoreArgs a) {
+__global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
   constexpr int V = 16 / sizeof(T), NV = SCORE_EACH / V;
   typedef T vt __attribute__((ext_vector_type(V)));
   const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
-  const uint32_t lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, c0 = chunk * SCORE_CHUNK;
+  const uint32_t lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), c0 = chunk * SCORE_CHUNK;
   const T* p = static_cast<const T*>(a.x) + (int64_t)row * a.xs;
+  __shared__ ScorePart s_part[SCORE_WAVES];
   const int32_t target = a.target ? a.target[row] : -1;
-  const bool has = target >= 0 && (uint32_t)target < a.n;
-  const float xt = has ? (float)p[target] : INFINITY;
-  __shared__ float s_max[SCORE_THREADS / 16], s_bound;
-  __shared__ ScorePart s_part[SCORE_THREADS / WAVE];
-  __shared__ uint64_t s_few[SCORE_FEW], s_best[SCORE_THREADS / WAVE];
-  __shared__ uint32_t s_count;
-  if (threadIdx.x == 0) s_count = 0;
+  const uint32_t out = row * a.chunks + chunk;
 
   auto column = [&](int i) { return c0 + ((i / V) * SCORE_THREADS + threadIdx.x) * V + i % V; };
   float x[SCORE_EACH];
+  if (VEC && c0 + SCORE_CHUNK <= a.n) {
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const uint32_t c = column(v * V);
-    if (VEC && c + V <= a.n) {
-      const vt w = *reinterpret_cast<const vt*>(p + c);
+    for (int v = 0; v < NV; ++v) {
+      const vt w = *reinterpret_cast<const vt*>(p + column(v * V));
 #pragma unroll
       for (int e = 0; e < V; ++e) x[v * V + e] = (float)w[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[v * V + e] = c + e < a.n ? (float)p[c + e] : -INFINITY;
     }
-  }
-  float mine = -INFINITY;
+  } else {
 #pragma unroll
-  for (int i = 0; i < SCORE_EACH; ++i) mine = fmaxf(mine, x[i]);
-  const float group = row_max(mine);
-  if (lane % 16 == 0) s_max[threadIdx.x / 16] = group;
-  __syncthreads();
-  static_assert(SCORE_THREADS / 16 == WAVE, "a group's maximum for each lane");
-  const float maxima = s_max[lane];
-  const float m = wave_max(maxima), m0 = m == -INFINITY ? 0.0f : m;
-  if (wave == 0 && a.top) {  // the top-th of the groups' maxima
-    uint32_t before = 0;
-    for (int i = 0; i < WAVE; ++i) {
-      const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, maxima), i));
-      before += o > maxima || (o == maxima && i < (int)lane);
-    }
-    if (before == a.top - 1) s_bound = maxima;
-  }
-  const float unit = a.scale * 1.44269504088896340736f;
-  float sum = 0.0f, moment = 0.0f;
-  uint32_t above = 0;
+    for (int v = 0; v < NV; ++v) {
+      const uint32_t c = column(v * V);
+      if (VEC && c + V <= a.n) {
+        const vt w = *reinterpret_cast<const vt*>(p + c);
 #pragma unroll
-  for (int i = 0; i < SCORE_EACH; ++i) {
-    const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
-    sum += e;
-    moment = fmaf(e == 0.0f ? 0.0f : d, e, moment);
-    above += x[i] > xt;
-  }
-  sum = wave_add(sum);
-  moment = wave_add(moment);
-  above = wave_add(above);
-  if (lane == 0) s_part[wave] = ScorePart{m, sum, moment, above};
-  __syncthreads();
-  if (a.top && mine >= s_bound) {
+        for (int e = 0; e < V; ++e) x[v * V + e] = (float)w[e];
+      } else {
 #pragma unroll
-    for (int i = 0; i < SCORE_EACH; ++i)
-      if (x[i] >= s_bound && column(i) < a.n) {
-        const uint32_t at = atomicAdd(&s_count, 1u);
-        if (at < SCORE_FEW) s_few[at] = score_key(x[i], column(i));
+        for (int e = 0; e < V; ++e) x[v * V + e] = c + e < a.n ? (float)p[c + e] : -INFINITY;
       }
-  }
-  __syncthreads();
-  const uint32_t count = s_count;
-  ScorePart r = s_part[0];
-  for (int w = 1; w < SCORE_THREADS / WAVE; ++w) {
-    r.sum += s_part[w].sum;
-    r.moment += s_part[w].moment;
-    r.above += s_part[w].above;
-  }
-  const uint32_t out = row * a.chunks + chunk;
-  uint64_t* best = a.best + (size_t)out * a.top;
-  if (threadIdx.x == 0) a.part[out] = r;
-  const uint32_t most = min(a.top, min(a.n - c0, (uint32_t)SCORE_CHUNK));
-  if (threadIdx.x >= most && threadIdx.x < a.top) best[threadIdx.x] = 0;
-  if (count <= SCORE_FEW && count >= most) {
-    if (threadIdx.x < count) {
-      const uint64_t k = s_few[threadIdx.x];
-      uint32_t before = 0;
-      for (uint32_t i = 0; i < count; ++i) before += s_few[i] > k;
-      if (before < most) best[before] = k;
     }
-    return;
   }
-  // many equal ones, or ones that are no numbers: the largest below the last, over and over
-  uint64_t last = ~0ull;
-  for (uint32_t t = 0; t < most; ++t) {
-    uint64_t k = 0;
+  const float xt = target >= 0 && (uint32_t)target < a.n ? (float)p[target] : INFINITY;
+  float mine = x[0], least = x[0];
+#pragma unroll
+  for (int i = 1; i < SCORE_EACH; ++i) {
+    mine = fmaxf(mine, x[i]);
+    least = fminf(least, x[i]);
+  }
+  const float group = lanes_max<SCORE_GROUP>(mine);
+  if (a.top && lane % SCORE_GROUP == 0) a.maxima[(size_t)out * WAVE + threadIdx.x / SCORE_GROUP] = group;
+  float m = lanes_max<16>(group);
+  m = fmaxf(m, __shfl_xor(m, 16));
+  m = fmaxf(m, __shfl_xor(m, 32));
+  const float m0 = m == -INFINITY ? 0.0f : m, unit = a.scale * 1.44269504088896340736f;
+  float sum = 0.0f, moment = 0.0f;
+  if (__builtin_expect(!__any(least == -INFINITY), 1)) {
 #pragma unroll
     for (int i = 0; i < SCORE_EACH; ++i) {
-      const uint64_t o = column(i) < a.n ? score_key(x[i], column(i)) : 0;
-      k = o < last && o > k ? o : k;
+      const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
+      sum += e;
+      moment = fmaf(d, e, moment);
     }
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)k, o);
-      k = other > k ? other : k;
+  } else {
+#pragma unroll
+    for (int i = 0; i < SCORE_EACH; ++i) {
+      const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
+      sum += e;
+      moment = fmaf(fmaxf(d, -FLT_MAX), e, moment);  // -inf has 0 of the sum
     }
-    if (lane == 0) s_best[wave] = k;
-    __syncthreads();
-    last = s_best[0];
-    for (int w = 1; w < SCORE_THREADS / WAVE; ++w) last = s_best[w] > last ? s_best[w] : last;
-    if (threadIdx.x == 0) best[t] = last;
-    __syncthreads();
+  }
+  uint32_t above = 0;
+  if (m > xt) {  // (the same in all lanes)
+#pragma unroll
+    for (int i = 0; i < SCORE_EACH; ++i) above += (uint32_t)__popcll(__ballot(x[i] > xt));
+  }
+  sum = wave_sum(sum);
+  moment = wave_sum(moment);
+  if (lane == 0) s_part[wave] = ScorePart{m, sum, moment, above};
+  __syncthreads();
+  if (wave == 0) {
+    static_assert(SCORE_WAVES <= 16, "a wave's part for each of 16 lanes");
+    const ScorePart s = lane < SCORE_WAVES ? s_part[lane] : ScorePart{-INFINITY, 0.0f, 0.0f, 0};
+    const float mm = lanes_max<16>(s.top), d = s.top - (mm == -INFINITY ? 0.0f : mm), e = __builtin_amdgcn_exp2f(d * unit);
+    const float sums = row_sum(s.sum * e), moments = row_sum(fmaf(fmaxf(d, -FLT_MAX), s.sum, s.moment) * e);
+    uint32_t higher = s.above;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) higher += __shfl_xor(higher, o);
+    if (lane == 0) a.part[out] = ScorePart{mm, sums, moments, higher};
   }
 }
 
-// A row's chunks joined in order, its best of theirs.
+// A row's chunks joined in order, in 64 bits, by the last wave; its best by the others:
+// from the groups of logits whose maximum reaches a bound that `top` groups' maxima reach (the
+// top-th of 64 maxima of groups), read again. Where more than LDS takes reach it, because
+// many are equal to it: those over it, and of the equal ones the first in the row.
+// Where those over it are too many still, one after the other.
 __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) {
-  __shared__ uint64_t s_key[MAX_SCORE_CHUNKS * MAX_TOP], s_best[MAX_TOP];
-  const uint32_t row = blockIdx.x, keys = a.chunks * a.top;
-  const ScorePart* part = a.part + (size_t)row * a.chunks;
-  for (uint32_t i = threadIdx.x; i < keys; i += 256) s_key[i] = a.best[(size_t)row * keys + i];
-  const int32_t target = a.target ? a.target[row] : -1;
-  const bool has = target >= 0 && (uint32_t)target < a.n;
-  const float xt = has ? load_value(a.x, (int64_t)row * a.xs + target, type) : 0.0f;
-  float top = -INFINITY;
-  for (uint32_t c = 0; c < a.chunks; ++c) top = fmaxf(top, part[c].top);
-  double sum = 0.0, moment = 0.0;
-  uint32_t above = 0;
-  for (uint32_t c = 0; c < a.chunks; ++c) {
-    const ScorePart s = part[c];
-    above += s.above;
-    if (s.top == -INFINITY && s.sum == 0.0f) continue;  // nothing over -inf
-    const double d = (double)s.top - (double)top, e = exp((double)a.scale * d);
-    sum = fma(e, (double)s.sum, sum);
-    moment = fma(e, e == 0.0 ? 0.0 : fma(d, (double)s.sum, (double)s.moment), moment);
+  constexpr uint32_t HELD = 4;  // groups' maxima that a thread keeps
+  __shared__ uint64_t s_key[SCORE_FEW], s_wave[4];
+  __shared__ uint32_t s_max[4][WAVE];
+  __shared__ uint16_t s_list[SCORE_LIST];
+  __shared__ uint32_t s_count, s_groups;
+  __shared__ double s_sum;
+  __shared__ float s_top;
+  static_assert(MAX_SCORE / SCORE_CHUNK * WAVE <= 0x10000 && MAX_TOP <= WAVE, "a group's number in 16 bits");
+  const uint32_t row = blockIdx.x, lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int64_t x0 = (int64_t)row * a.xs;
+  const uint32_t groups = a.chunks * WAVE;
+  const float* maxima = a.maxima + (size_t)row * groups;
+  auto ordered = [](float v) { return (uint32_t)(score_key(v, 0) >> 32); };
+  auto group_max = [&](uint32_t i) { return i < groups ? ordered(maxima[i]) : 0u; };
+  uint32_t held[HELD], most = 0;
+  if (a.top) {
+#pragma unroll
+    for (uint32_t h = 0; h < HELD; ++h) held[h] = group_max(threadIdx.x + 256 * h);
+#pragma unroll
+    for (uint32_t h = 0; h < HELD; ++h) most = max(most, held[h]);
+    for (uint32_t i = threadIdx.x + 256 * HELD; i < groups; i += 256) most = max(most, group_max(i));
+    s_max[wave][lane] = most;
+    if (threadIdx.x == 0) s_count = s_groups = 0;
   }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < keys; i += 256) {
-    const uint64_t k = s_key[i];
-    uint32_t before = 0;
-    for (uint32_t j = 0; j < keys; ++j) before += s_key[j] > k;
-    if (k && before < a.top) s_best[before] = k;
+
+  if (wave == 3) {  // what the whole row's sums say
+    const int32_t target = a.target ? a.target[row] : -1;
+    const ScorePart* part = a.part + (size_t)row * a.chunks;
+    float top = -INFINITY;
+    double sum = 0.0, moment = 0.0;
+    uint32_t above = 0;
+    for (uint32_t c = lane; c < a.chunks; c += WAVE) top = fmaxf(top, part[c].top);
+    top = wave_max(top);
+    for (uint32_t c0 = 0; c0 < a.chunks; c0 += WAVE) {
+      const ScorePart s = c0 + lane < a.chunks ? part[c0 + lane] : ScorePart{-INFINITY, 0.0f, 0.0f, 0};
+      above += wave_add(s.above);
+      const bool none = s.top == -INFINITY && s.sum == 0.0f;  // nothing over -inf: nothing of the sum
+      const double d = none ? 0.0 : (double)s.top - (double)top, e = none ? 0.0 : exp((double)a.scale * d);
+      const double mine = e * (double)s.sum, moments = e == 0.0 ? 0.0 : e * fma(d, (double)s.sum, (double)s.moment);
+      for (int c = 0; c < (int)min(a.chunks - c0, (uint32_t)WAVE); ++c) {
+        sum += __shfl(mine, c);
+        moment += __shfl(moments, c);
+      }
+    }
+    if (lane == 0) {
+      const float nan = __builtin_nanf("");
+      const bool none = !(sum >= 1.0);  // a NaN, an infinity, or nothing over -inf: no distribution
+      const bool has = target >= 0 && (uint32_t)target < a.n && !none;
+      const double scale = (double)a.scale, log_sum = none ? (double)nan : log(sum);
+      a.log_p[row] = has ? (float)(scale * ((double)load_value(a.x, x0 + target, type) - (double)top) - log_sum) : nan;
+      a.entropy[row] = (float)(log_sum - scale * moment / sum);
+      a.rank[row] = has ? (int32_t)above : -1;
+      s_sum = log_sum;
+      s_top = top;
+    }
   }
+  if (!a.top) return;
   __syncthreads();
-  if (threadIdx.x < WAVE)
-    score_store(a, row, threadIdx.x, top, sum, moment, above, xt, has, threadIdx.x < a.top ? s_best[threadIdx.x] : 1);
+  const uint32_t o = max(max(s_max[0][lane], s_max[1][lane]), max(s_max[2][lane], s_max[3][lane]));
+  // columns of a group: of each 16-byte vector of a thread's, a run
+  const uint32_t vector = type == DEFER_GPU_F32 ? 4 : 8, run = SCORE_GROUP * vector;
+  auto column = [&](uint32_t group, uint32_t e) {
+    return group / WAVE * SCORE_CHUNK + e / run * (SCORE_THREADS * vector) + group % WAVE * run + e % run;
+  };
+  // Keys of the logits that reach `from` (counts are 0); returns how many there are.
+  auto gather = [&](uint32_t from) {
+    auto list = [&](uint32_t i, uint32_t m) {
+      if (i < groups && m >= from) {
+        const uint32_t at = atomicAdd(&s_groups, 1u);
+        if (at < SCORE_LIST) s_list[at] = (uint16_t)i;
+      }
+    };
+#pragma unroll
+    for (uint32_t h = 0; h < HELD; ++h) list(threadIdx.x + 256 * h, held[h]);
+    for (uint32_t i = threadIdx.x + 256 * HELD; i < groups; i += 256) list(i, group_max(i));
+    __syncthreads();
+    const uint32_t n = s_groups;
+    if (n > SCORE_LIST) return SCORE_FEW + 1;
+    for (uint32_t i = threadIdx.x / 16; i < n; i += 16) {  // 16 lanes a group
+      const uint32_t group = s_list[i];
+      constexpr uint32_t EACH = SCORE_GROUP * SCORE_EACH / 16;
+      float v[EACH];
+#pragma unroll
+      for (uint32_t s = 0; s < EACH; ++s) {
+        const uint32_t c = column(group, 16 * s + lane % 16);
+        v[s] = c < a.n ? load_value(a.x, x0 + c, type) : -INFINITY;
+      }
+#pragma unroll
+      for (uint32_t s = 0; s < EACH; ++s) {
+        const uint32_t c = column(group, 16 * s + lane % 16);
+        if (c < a.n && ordered(v[s]) >= from) {
+          const uint32_t at = atomicAdd(&s_count, 1u);
+          if (at < SCORE_FEW) s_key[at] = score_key(v[s], c);
+        }
+      }
+    }
+    __syncthreads();
+    return s_count;
+  };
+  uint32_t bound = score_bound(o, a.top, a.top / 4), count = gather(bound);
+  const double log_sum = s_sum;
+  const bool none = isnan(log_sum);
+  if (count > SCORE_FEW && !none) {
+    bound = score_bound(o, a.top, 0);  // a maximum's own number
+    __syncthreads();
+    if (threadIdx.x == 0) s_count = s_groups = 0;
+    __syncthreads();
+    count = gather(bound + 1);
+    if (count < a.top) {  // ... and the first of the equal ones
+      const float equal = value_of((uint64_t)bound << 32);
+      if (wave == 0)
+        for (uint32_t c0 = 0; c0 < a.n && count < a.top; c0 += WAVE) {
+          const uint32_t c = c0 + lane;
+          const float v = c < a.n ? load_value(a.x, x0 + c, type) : 0.0f;
+          const bool is = c < a.n && v == equal;
+          const uint64_t mask = __ballot(is);
+          const uint32_t at = count + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
+          if (is && at < a.top) s_key[at] = score_key(v, c);
+          count += (uint32_t)__popcll(mask);
+        }
+      count = a.top;
+    } else if (count > SCORE_FEW) {  // one after the other
+      uint64_t last = ~0ull;
+      for (uint32_t t = 0; t < a.top; ++t) {
+        uint64_t k = 0;
+        for (uint32_t c = threadIdx.x; c < a.n; c += 256) {
+          const uint64_t key = score_key(load_value(a.x, x0 + c, type), c);
+          k = key < last && key > k ? key : k;
+        }
+        for (int s = 32; s > 0; s >>= 1) {
+          const uint64_t other = __shfl_xor((unsigned long long)k, s);
+          k = other > k ? other : k;
+        }
+        __syncthreads();
+        if (lane == 0) s_wave[wave] = k;
+        __syncthreads();
+        last = s_wave[0];
+        for (int w = 1; w < 4; ++w) last = s_wave[w] > last ? s_wave[w] : last;
+        if (threadIdx.x == 0) s_key[t] = last;
+      }
+      count = a.top;
+    }
+  }
+  if (wave) return;
+  const size_t out = (size_t)row * a.top;
+  if (none) {
+    if (lane < a.top) {
+      a.top_index[out + lane] = -1;
+      a.top_log_p[out + lane] = __builtin_nanf("");
+    }
+    return;
+  }
+  const double scale = (double)a.scale, top = (double)s_top;
+  score_pick(s_key, count, a.top, [&](uint32_t t, uint64_t k) {
+    a.top_index[out + t] = (int32_t)column_of(k);
+    a.top_log_p[out + t] = (float)(scale * ((double)value_of(k) - top) - log_sum);
+  });
 }
 
 template <class T>
@@ -658,7 +836,7 @@ extern "C" int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer
 
 extern "C" size_t defer_gpu_q8_log_probs_workspace(uint32_t rows, uint32_t n, uint32_t top) {
   if (rows > MAX_THREADS / SCORE_THREADS || n > MAX_SCORE || top > MAX_TOP) return 0;
-  return (size_t)rows * score_chunks(n) * (sizeof(ScorePart) + top * sizeof(uint64_t));
+  return (size_t)rows * score_chunks(n) * (sizeof(ScorePart) + (top ? WAVE * sizeof(float) : 0));
 }
 
 extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_stride, uint32_t rows, uint32_t n,
@@ -682,7 +860,7 @@ extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_st
   Q8_REQUIRE(aligned16(workspace), "workspace is not 16-byte aligned");
   ScoreArgs a{x, x_stride, target, rows, n, top, score_chunks(n), scale, log_p, entropy, top_log_p, rank, top_index,
               static_cast<ScorePart*>(workspace), nullptr};
-  a.best = reinterpret_cast<uint64_t*>(a.part + (size_t)rows * a.chunks);
+  a.maxima = reinterpret_cast<float*>(a.part + (size_t)rows * a.chunks);
   const bool vec = ((uintptr_t)x | (uintptr_t)(x_stride * (int64_t)value_size(type))) % 16 == 0;
   const hipStream_t s = (hipStream_t)stream;
   const int e = type == DEFER_GPU_F32    ? score_launch<float>(a, vec, s)

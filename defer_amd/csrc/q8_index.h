@@ -20,7 +20,6 @@ constexpr uint32_t MAX_HEAD_DIM = 256;
 constexpr uint32_t MAX_K = 131072;     // sums of fewer code products than this fit 32 bits
 constexpr uint32_t MAX_TREE = 64;      // drafted rows of a sequence: a wave's lanes
 constexpr uint32_t MAX_SCORE = 1u << 20;   // logits of a row
-constexpr uint32_t MAX_SCORE_CHUNKS = 64;  // ... in workgroups' chunks
 constexpr uint32_t MAX_TOP = 32;           // alternatives of a row
 
 // The head size as a page holds it.
