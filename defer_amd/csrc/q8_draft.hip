@@ -25,8 +25,8 @@ struct AppendArgs {
   const double* freq;
   const void *qn, *kn;
   double eps, factor;
-  uint32_t type, hd, nh, half;  // half: rotated pairs of a head
-  uint32_t kv_heads, q_heads;   // heads that a workgroup takes: of the cache, or of the queries
+  uint32_t hd, nh, half;        // half: rotated pairs of a head
+  uint32_t kv_shift, q_shift;   // a workgroup takes so many heads, as a power of 2: of the cache, or of the queries
   uint32_t kv_chunks, chunks;   // workgroups of a run for the cache's heads, and for all
   bool interleaved, clear;
 };
@@ -38,12 +38,20 @@ __device__ __forceinline__ double dpp64(double v) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// Over the 16 lanes of a DPP row, as row_max and row_sum.
+// (Written out: the compiler quiets both operands first. Another lane reads a register two wait
+// states after it was written.)
+__device__ __forceinline__ double max_abs(double v, double x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("v_max_f64 %0, %0, |%1|\n\ts_nop 1" : "+v"(v) : "v"(x));
+#endif
+  return v;
+}
+// Over the 16 lanes of a DPP row, as row_max and row_sum; the maximum of numbers that are not negative.
 __device__ __forceinline__ double row_max64(double v) {
-  v = fmax(v, dpp64<0x128>(v));
-  v = fmax(v, dpp64<0x124>(v));
-  v = fmax(v, dpp64<0x122>(v));
-  return fmax(v, dpp64<0x121>(v));
+  v = max_abs(v, dpp64<0x128>(v));
+  v = max_abs(v, dpp64<0x124>(v));
+  v = max_abs(v, dpp64<0x122>(v));
+  return max_abs(v, dpp64<0x121>(v));
 }
 __device__ __forceinline__ double row_sum64(double v) {
   v += dpp64<0x128>(v);
@@ -82,83 +90,85 @@ __device__ __forceinline__ double2 turn(int pos, double freq) {
   return double2{n == 1 || n == 2 ? -a : a, n >= 2 ? -b : b};
 }
 
-// A lane's 8 values from d = 8 n16 on (and the 8 from 128 + d on, where the head
-// has more than 128): normed, rotated. cs: the row's (cos, sin) of each pair.
-// VEC: 8 values are aligned, and so are the 8 they are paired with.
-template <bool VEC>
-__device__ __forceinline__ void turned(const AppendArgs& a, const void* p, int64_t at, const void* norm, const double2* cs,
-                                       uint32_t n16, double (*y)[8]) {
-  const uint32_t hd = a.hd, rotated = 2 * a.half;
-  float x[2][8], xp[2][8];  // the values, and the halves' other ones
+// 8 values of a head.
+template <class T>
+struct Eight {
+  typedef T type __attribute__((ext_vector_type(8), aligned(16)));
+};
+
+// Where pair `i` of a row's (cos, sin) lies in LDS: lanes that take 8 values each (and so 8 or,
+// side by side, 4 pairs) read neighbouring ones.
+struct Angles {
+  uint32_t step, line;  // pairs of a lane, and places of each of them
+  __device__ __forceinline__ Angles(uint32_t half, bool interleaved) : step(interleaved ? 4 : 8), line((half + step - 1) / step) {}
+  __device__ __forceinline__ uint32_t at(uint32_t i) const { return i % step * line + i / step; }
+};
+// ... of a row.
+Q8_HD uint32_t angles_of(uint32_t half, bool interleaved) {
+  const uint32_t step = interleaved ? 4 : 8;
+  return (half + step - 1) / step * step;
+}
+
+// The codes of a lane's values at a scale. A quotient in f32 is off by less than
+// 2^-15 (three roundings of up to 127), so only where one of the wave's lies that near a half
+// does it take 64 bits to say on which side.
+template <uint32_t W>
+struct Codes {
+  uint64_t c[W];
+  __device__ __forceinline__ Codes(const double (*y)[8], float scale) {
+    const float r = scale > 0.0f ? 1.0f / scale : 0.0f;  // (zeros, and rows with what is no number: codes 0)
+    float off = 0.0f;
+    int q[W][8];
 #pragma unroll
-  for (uint32_t h = 0; h < 2; ++h) {
-    if (h && hd <= 128) break;
-    const uint32_t d = 128 * h + 8 * n16;
-    load8(p, at, d, hd, a.type, VEC, x[h]);
-    if (a.interleaved) continue;
-    if (VEC) {
-      if (d < rotated) load8(p, at, d < a.half ? d + a.half : d - a.half, hd, a.type, true, xp[h]);
-    } else {
+    for (uint32_t w = 0; w < W; ++w)
 #pragma unroll
       for (uint32_t e = 0; e < 8; ++e) {
-        const uint32_t i = d + e;
-        xp[h][e] = i < rotated ? load_value(p, at + (i < a.half ? i + a.half : i - a.half), a.type) : 0.0f;
+        const float x = r > 0.0f ? (float)y[w][e] * r : 0.0f, n = rintf(x);
+        off = fmaxf(off, fabsf(x - n));
+        q[w][e] = (int)n;
       }
-    }
-  }
-  double inv = 1.0;
-  if (norm) {
-    double ss = 0.0;
+    if (__any(!(off < 0.5f - 0x1p-14f) || scale > 0x1p118f)) {  // (values that f32 may not hold)
+      const Coder code(scale);
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h)
-      if (h == 0 || hd > 128)
+      for (uint32_t w = 0; w < W; ++w)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fma((double)x[h][e], (double)x[h][e], ss);
-    inv = 1.0 / sqrt(row_sum64(ss) / (double)hd + a.eps);
-  }
-#pragma unroll
-  for (uint32_t h = 0; h < 2; ++h) {
-    if (h && hd <= 128) break;
-    const uint32_t d = 128 * h + 8 * n16;
-    double z[8];
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) {
-      z[e] = (double)x[h][e];
-      if (norm && d + e < hd) z[e] *= (double)load_value(norm, d + e, a.type) * inv;
+        for (uint32_t e = 0; e < 8; ++e) q[w][e] = code(y[w][e]);
     }
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) {
-      const uint32_t i = d + e;
-      y[h][e] = z[e];
-      if (i >= rotated) continue;
-      const bool second = a.interleaved ? e % 2 : i >= a.half;
-      const uint32_t pair = a.interleaved ? i / 2 : second ? i - a.half : i;
-      double o = a.interleaved ? z[e ^ 1] : (double)xp[h][e];
-      if (norm && !a.interleaved) o *= (double)load_value(norm, second ? i - a.half : i + a.half, a.type) * inv;
-      const double2 c = cs[pair];
-      y[h][e] = fma(z[e], c.x, second ? o * c.y : -(o * c.y));
+    for (uint32_t w = 0; w < W; ++w) {
+      uint32_t h[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        h[i] = perm(perm((uint32_t)q[w][4 * i + 3], (uint32_t)q[w][4 * i + 2], 0x0c0c0400u),
+                    perm((uint32_t)q[w][4 * i + 1], (uint32_t)q[w][4 * i], 0x0c0c0400u), 0x05040100u);
+      c[w] = (uint64_t)h[1] << 32 | h[0];
     }
   }
-}
+};
 
 // A workgroup takes the rows of 16 places of a page (as k_kv_write's, whose
 // places they are) and some heads: of the cache's keys and values, or of the
 // queries. The rows' angles are formed once, 64 bits, in LDS; then 16 lanes take
-// a row's head. Keys, scales and codes are those of the formula in 64 bits, as
-// everywhere here.
-template <bool VEC>
+// a row's head, 8 values each (WIDE: and the 8 from 128 on), the next one's already on its
+// way. Keys, scales and codes are those of the formula in 64 bits, as everywhere here.
+// VEC: 8 values are aligned, and so are the 8 they are paired with.
+template <class T, bool VEC, bool WIDE>
 __global__ __launch_bounds__(256) void k_append(AppendArgs a) {
-  extern __shared__ __align__(16) uint8_t lds[];  // [rows][half] angles, then [heads][rows][KV_ROW] value codes
+  typedef typename Eight<T>::type t8;
+  constexpr uint32_t W = WIDE ? 2 : 1;
+  extern __shared__ __align__(16) uint8_t lds[];  // the rows' angles, then [heads][rows][KV_ROW] value codes
   const uint32_t per = kv_runs(a.r.most_rows), most = min(a.r.most_rows, (uint32_t)KV_RUN);
   const uint32_t chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks % per, seq = blockIdx.x / a.chunks / per;
-  const uint32_t n16 = threadIdx.x % 16, quad = threadIdx.x / 16, quads = blockDim.x / 16, hd = a.hd;
+  const uint32_t n16 = threadIdx.x % 16, quad = threadIdx.x / 16, hd = a.hd, rotated = 2 * a.half;
+  constexpr uint32_t quads = 16;
+  T* const out = static_cast<T*>(a.out);
   if (seq == a.r.sequences) {  // zeros for the rows of no sequence
     const int64_t lo = span_of(a.r.row_start, a.r.kv_len, 0, a.r.rows).start;
     const int64_t hi = max(lo, min((int64_t)a.r.row_start[seq], (int64_t)a.r.rows));
     const int64_t n = a.nh * hd;
     for (int64_t i = b * a.chunks + chunk; i < lo + ((int64_t)a.r.rows - hi); i += per * a.chunks) {
       const int64_t row = i < lo ? i : hi + (i - lo);
-      for (int64_t d = threadIdx.x; d < n; d += blockDim.x) store_value(a.out, row * a.os + d, a.type, 0.0f);
+      for (int64_t d = threadIdx.x; d < n; d += blockDim.x) out[row * a.os + d] = (T)0.0f;
     }
     return;
   }
@@ -169,109 +179,207 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs a) {
   if (t0 >= t1) return;
   const uint32_t n = min((uint32_t)(t1 - t0), most);  // rows
   const int64_t row0 = sp.start + (t0 - p0);
-  double2* cs = reinterpret_cast<double2*>(lds);
-  int8_t* tile = reinterpret_cast<int8_t*>(cs + most * a.half);
-  for (uint32_t i = threadIdx.x; i < n * a.half; i += blockDim.x) {
-    const uint32_t j = i / a.half;
-    double2 c = turn(a.position ? a.position[row0 + j] : (int)(t0 + j), a.freq[i - j * a.half]);
-    cs[i] = double2{c.x * a.factor, c.y * a.factor};
+  const bool queries = chunk >= a.kv_chunks;
+  const uint32_t shift = queries ? a.q_shift : a.kv_shift, h0 = (queries ? chunk - a.kv_chunks : chunk) << shift;
+  const uint32_t heads = min(1u << shift, (queries ? a.nh : a.p.heads) - h0);
+  // keys and values that have a place and a page (places before 0 have none)
+  const int64_t block = down(run, PAGE / KV_RUN);
+  int page = 0;
+  if (!queries) {
+    page = page_of(a.p.table + (size_t)seq * a.p.width, a.p.width, a.p.pages, block);
+    if (page < 0) return;
+  }
+  const uint32_t turning = n << shift, items = queries ? turning : 2 * turning;  // keys, then values; of 2^shift heads
+
+  auto load = [&](const T* p, uint32_t d) {
+    t8 v;
+    if (VEC && d < hd) {
+      v = *reinterpret_cast<const t8*>(p + d);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) v[e] = d + e < hd ? p[d + e] : (T)0.0f;
+    }
+    return v;
+  };
+  // the values that a half layout pairs with the 8 from d on
+  auto load_pairs = [&](const T* p, uint32_t d) {
+    t8 v;
+    if (VEC && d < rotated) {
+      v = *reinterpret_cast<const t8*>(p + (d < a.half ? d + a.half : d - a.half));
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) v[e] = d + e < rotated ? p[d + e < a.half ? d + e + a.half : d + e - a.half] : (T)0.0f;
+    }
+    return v;
+  };
+  t8 x[W], xp[W];
+  auto fetch = [&](uint32_t i) {
+    const uint32_t it = i < turning ? i : i - turning, j = it >> shift, hl = it & ((1u << shift) - 1);
+    const T* p = queries       ? static_cast<const T*>(a.q) + (row0 + j) * a.qs
+                 : i < turning ? static_cast<const T*>(a.k) + (row0 + j) * a.ks
+                               : static_cast<const T*>(a.v) + (row0 + j) * a.vs;
+    p += (int64_t)(h0 + min(hl, heads - 1)) * hd;  // (none: another's, not used)
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+      x[w] = load(p, 128 * w + 8 * n16);
+      if (!a.interleaved && i < turning) xp[w] = load_pairs(p, 128 * w + 8 * n16);
+    }
+  };
+  if (quad < items) fetch(quad);
+  const T* const norm = static_cast<const T*>(queries ? a.qn : a.kn);
+  t8 weight[W], weight_p[W];
+  if (norm) {
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+      weight[w] = load(norm, 128 * w + 8 * n16);
+      if (!a.interleaved) weight_p[w] = load_pairs(norm, 128 * w + 8 * n16);
+    }
+  }
+
+  const uint32_t of_row = angles_of(a.half, a.interleaved);
+  const Angles angles(a.half, a.interleaved);
+  double2* const cs = reinterpret_cast<double2*>(lds);
+  int8_t* const tile = reinterpret_cast<int8_t*>(cs + most * of_row);
+  for (uint32_t i = threadIdx.x; i < n * a.half; i += 256) {
+    const uint32_t j = i / a.half, pair = i - j * a.half;
+    const double2 c = turn(a.position ? a.position[row0 + j] : (int)(t0 + j), a.freq[pair]);
+    cs[j * of_row + angles.at(pair)] = double2{c.x * a.factor, c.y * a.factor};
   }
   __syncthreads();
 
-  if (chunk >= a.kv_chunks) {
-    const uint32_t h0 = (chunk - a.kv_chunks) * a.q_heads, heads = min(a.q_heads, a.nh - h0);
-    for (uint32_t i = quad; i < heads * n; i += quads) {
-      const uint32_t j = i / heads, h = h0 + i % heads;
-      double y[2][8];
-      turned<VEC>(a, a.q, (row0 + j) * a.qs + (int64_t)h * hd, a.qn, cs + j * a.half, n16, y);
+  const int a0 = (int)(t0 - block * PAGE);  // the first row's place in its page
+  for (uint32_t i = quad; i < items; i += quads) {
+    const bool value = i >= turning;
+    const uint32_t it = value ? i - turning : i, j = it >> shift, hl = it & ((1u << shift) - 1), h = h0 + hl;
+    double y[W][8];
 #pragma unroll
-      for (uint32_t g = 0; g < 2; ++g) {
-        if (g && hd <= 128) break;
-        float o[8];
+    for (uint32_t w = 0; w < W; ++w)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = (float)y[g][e];
-        store8(a.out, (row0 + j) * a.os + (int64_t)h * hd, 128 * g + 8 * n16, hd, a.type, VEC, o);
+      for (uint32_t e = 0; e < 8; ++e) y[w][e] = (double)(float)x[w][e];
+    if (!value) {
+      double inv = 1.0;
+      if (norm) {
+        double ss = 0.0;
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w)
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) ss = fma(y[w][e], y[w][e], ss);
+        inv = 1.0 / sqrt(row_sum64(ss) / (double)hd + a.eps);
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w)
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) y[w][e] *= (double)(float)weight[w][e] * inv;
+      }
+      const double2* const row = cs + j * of_row;
+#pragma unroll
+      for (uint32_t w = 0; w < W; ++w) {
+        const uint32_t d = 128 * w + 8 * n16;
+        if (VEC ? d >= rotated : false) continue;
+        if (a.interleaved) {
+#pragma unroll
+          for (uint32_t e = 0; e < 8; e += 2) {
+            if (!VEC && d + e >= rotated) continue;
+            const double2 c = row[e / 2 * angles.line + d / 8];
+            const double p = y[w][e], q = y[w][e + 1];
+            y[w][e] = fma(p, c.x, -(q * c.y));
+            y[w][e + 1] = fma(q, c.x, p * c.y);
+          }
+        } else {
+          const bool all_second = d >= a.half;  // (VEC: all of them or none)
+          const double2* const from = row + (all_second ? d - a.half : d) / 8;
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) {
+            const uint32_t k = d + e;
+            if (!VEC && k >= rotated) continue;
+            const bool second = VEC ? all_second : k >= a.half;
+            const double2 c = VEC ? from[e * angles.line] : row[angles.at(second ? k - a.half : k)];
+            const float of = (float)xp[w][e];
+            double o = (double)(second ? of : -of);
+            if (norm) o *= (double)(float)weight_p[w][e] * inv;
+            y[w][e] = fma(o, c.y, y[w][e] * c.x);
+          }
+        }
       }
     }
-    return;
-  }
-
-  // the cache's heads: keys and values that have a place and a page
-  const int64_t block = down(run, PAGE / KV_RUN);
-  const int page = page_of(a.p.table + (size_t)seq * a.p.width, a.p.width, a.p.pages, block);
-  if (page < 0) return;  // (places before 0 among them)
-  const uint32_t g0 = chunk * a.kv_heads, heads = min(a.kv_heads, a.p.heads - g0);
-  const int a0 = (int)(t0 - block * PAGE);  // the first row's place in its page
-  for (uint32_t i = quad; i < 2 * heads * n; i += quads) {
-    const bool value = i >= heads * n;
-    const uint32_t it = value ? i - heads * n : i, j = it / heads, gl = it % heads, g = g0 + gl;
-    const size_t hp = (size_t)page * a.p.heads + g;
-    double y[2][8];
-    if (value) {
-      float x[2][8];
+    if (i + quads < items) fetch(i + quads);
+    if (hl >= heads) continue;
+    if (queries) {
+      T* const to = out + (row0 + j) * a.os + (int64_t)h * hd;
 #pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-        if (h && hd <= 128) break;
-        load8(a.v, (row0 + j) * a.vs + (int64_t)g * hd, 128 * h + 8 * n16, hd, a.type, VEC, x[h]);
+      for (uint32_t w = 0; w < W; ++w) {
+        const uint32_t d = 128 * w + 8 * n16;
+        t8 v;  // (through f32: at most half a step of it more than rounded at once)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[h][e] = (double)x[h][e];
+        for (uint32_t e = 0; e < 8; ++e) v[e] = (T)(float)y[w][e];
+        if (VEC && d < hd) {
+          *reinterpret_cast<t8*>(to + d) = v;
+        } else {
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e)
+            if (d + e < hd) to[d + e] = v[e];
+        }
       }
-    } else {
-      turned<VEC>(a, a.k, (row0 + j) * a.ks + (int64_t)g * hd, a.kn, cs + j * a.half, n16, y);
+      continue;
     }
     double top = 0.0, bad = 0.0;
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h)
-      if (h == 0 || hd > 128)
+    for (uint32_t w = 0; w < W; ++w)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          top = fmax(top, fabs(y[h][e]));
-          bad = fma(y[h][e], 0.0, bad);
-        }
+      for (uint32_t e = 0; e < 8; ++e) {
+        top = max_abs(top, y[w][e]);
+        bad = fma(y[w][e], 0.0, bad);
+      }
     const float scale = scale_of(row_max64(top), isnan(row_sum64(bad)));
-    const Coder code(scale);
+    const Codes<W> codes(y, scale);
+    const size_t hp = (size_t)page * a.p.heads + h;
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-      const uint32_t d = 128 * h + 8 * n16;
+    for (uint32_t w = 0; w < W; ++w) {
+      const uint32_t d = 128 * w + 8 * n16;
       if (d >= hd) continue;
-      uint64_t c = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) c |= (uint64_t)(uint8_t)code(y[h][e]) << (8 * e);
       // a page's row is a multiple of 64 codes: those behind hd are zeros
-      int8_t* to = value ? tile + (gl * most + j) * KV_ROW + d : a.p.keys + (hp * PAGE + a0 + j) * a.p.dp + d;
-      *reinterpret_cast<uint64_t*>(to) = c;
+      if (value)
+        *reinterpret_cast<uint64_t*>(tile + (hl * most + j) * KV_ROW + d) = codes.c[w];
+      else
+        *reinterpret_cast<uint64_t*>(a.p.keys + (hp * PAGE + a0 + j) * a.p.dp + d) = codes.c[w];
     }
     if (n16 == 0) (value ? a.p.value_scale : a.p.key_scale)[hp * PAGE + a0 + j] = scale;
   }
+  if (queries) return;
   __syncthreads();
   // value codes into their transposed pages
-  int8_t* vc = a.p.values + ((size_t)page * a.p.heads + g0) * PAGE * a.p.dp;
+  int8_t* const vc = a.p.values + ((size_t)page * a.p.heads + h0) * PAGE * a.p.dp;
   if (n < KV_RUN) {  // some of the run: byte by byte
-    for (uint32_t i = threadIdx.x; i < heads * n * hd; i += blockDim.x) {
-      const uint32_t d = i % hd, hj = i / hd, j = hj % n, gl = hj / n;
-      vc[((size_t)gl * a.p.dp + d) * PAGE + a0 + j] = tile[(gl * most + j) * KV_ROW + d];
+    for (uint32_t i = threadIdx.x; i < heads * n * hd; i += 256) {
+      const uint32_t d = i % hd, hj = i / hd, j = hj % n, hl = hj / n;
+      vc[((size_t)hl * a.p.dp + d) * PAGE + a0 + j] = tile[(hl * most + j) * KV_ROW + d];
     }
     return;
   }
   const uint32_t quarters = (hd + 3) / 4;
-  for (uint32_t i = threadIdx.x; i < heads * quarters; i += blockDim.x) {  // four channels a thread
-    const uint32_t gl = i / quarters, d = 4 * (i % quarters);
+  for (uint32_t i = threadIdx.x; i < heads * quarters; i += 256) {  // four channels a thread
+    const uint32_t hl = i / quarters, d = 4 * (i % quarters);
     uint32_t w[4][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      uint32_t in[4], out[4];
+      uint32_t in[4], by[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) in[e] = *reinterpret_cast<const uint32_t*>(tile + (gl * most + 4 * u + e) * KV_ROW + d);
-      transpose4(in, out);
+      for (int e = 0; e < 4; ++e) in[e] = *reinterpret_cast<const uint32_t*>(tile + (hl * most + 4 * u + e) * KV_ROW + d);
+      transpose4(in, by);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) w[c][u] = out[c];
+      for (int c = 0; c < 4; ++c) w[c][u] = by[c];
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       if (d + c < hd)
-        *reinterpret_cast<v4i*>(vc + ((size_t)gl * a.p.dp + d + c) * PAGE + a0) =
+        *reinterpret_cast<v4i*>(vc + ((size_t)hl * a.p.dp + d + c) * PAGE + a0) =
             v4i{(int)w[c][0], (int)w[c][1], (int)w[c][2], (int)w[c][3]};
   }
+}
+
+template <class T>
+int append_launch(const AppendArgs& a, uint32_t blocks, size_t lds, bool vec, hipStream_t s) {
+  if (a.hd <= 128) return launch(vec ? k_append<T, true, false> : k_append<T, false, false>, blocks, 256, lds, s, a);
+  return launch(vec ? k_append<T, true, true> : k_append<T, false, true>, blocks, 256, lds, s, a);
 }
 
 // ------------------------------------------------------------- keep
@@ -788,26 +896,41 @@ extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const def
   a.kn = rotary->k_norm;
   a.eps = (double)rotary->eps;
   a.factor = (double)rotary->factor;
-  a.type = type;
   a.hd = hd;
   a.nh = q_heads;
   a.half = rotary->rotated / 2;
   a.interleaved = rotary->interleaved != 0;
   a.clear = clear && r.row_start;
-  // Heads of a workgroup: 16 of its lanes take a row's head, four rounds of them
-  // where a run is full.
-  const uint32_t most = std::min(r.most_rows, (uint32_t)KV_RUN), items = most >= 8 ? 64 : 16;
-  a.q_heads = std::min(std::max(1u, items / most), q_heads);
-  a.kv_heads = std::min(std::max(1u, items / 2 / most), p.heads);
-  a.kv_chunks = (p.heads + a.kv_heads - 1) / a.kv_heads;
-  a.chunks = a.kv_chunks + (q_heads + a.q_heads - 1) / a.q_heads;
-  const uint64_t blocks = ((uint64_t)r.sequences + a.clear) * kv_runs(r.most_rows) * a.chunks;
+  // Heads of a workgroup: 16 of its lanes take a row's head, so that a full run of queries takes
+  // it 4 rounds and one of the cache's heads 2 (keys, values); fewer rows take more heads, so
+  // that the lanes have work. Where those would be more workgroups than the chip holds at once
+  // (4 on a CU), each takes twice as many heads and forms the rows' angles for all of them:
+  // 2048 rows of 32 + 8 heads of 128 in 21 us rather than 25 (4 times as many: 23), but 11 x 33
+  // normed rows of 24 + 4 heads of 96, too few for that, in 11.2 rather than 8.8.
+  const uint32_t most = std::min(r.most_rows, (uint32_t)KV_RUN);
+  auto power = [&](uint32_t n, uint32_t heads) {  // the largest one up to n, no more than heads need
+    uint32_t s = 0;
+    while ((2u << s) <= n && (1u << s) < heads) ++s;
+    return s;
+  };
+  uint64_t blocks = 0;
+  for (uint32_t items = most >= 8 ? 64 : 16, twice = 0; twice < 2; ++twice, items *= 2) {
+    a.q_shift = power(items / most, q_heads);
+    a.kv_shift = power(items / 4 / most, p.heads);
+    a.kv_chunks = (p.heads + (1u << a.kv_shift) - 1) >> a.kv_shift;
+    a.chunks = a.kv_chunks + ((q_heads + (1u << a.q_shift) - 1) >> a.q_shift);
+    blocks = ((uint64_t)r.sequences + a.clear) * kv_runs(r.most_rows) * a.chunks;
+    if (blocks <= 1024) break;
+  }
   Q8_REQUIRE(blocks <= MAX_THREADS / 256, "too many rows for one call");
-  const bool vec = hd % 8 == 0 && (a.interleaved || a.half % 8 == 0) &&
-                   ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)(q_stride * vs) |
+  const bool vec = hd % 8 == 0 && (a.interleaved ? a.half % 4 == 0 : a.half % 8 == 0) &&
+                   ((uintptr_t)a.qn | (uintptr_t)a.kn | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)(q_stride * vs) |
                     (uintptr_t)(k_stride * vs) | (uintptr_t)(v_stride * vs) | (uintptr_t)(out_stride * vs)) % 16 == 0;
-  const size_t lds = (size_t)most * a.half * sizeof(double2) + (size_t)a.kv_heads * most * KV_ROW;
-  return launch(vec ? k_append<true> : k_append<false>, (uint32_t)blocks, 256, lds, s, a);
+  const size_t lds = (size_t)most * angles_of(a.half, a.interleaved) * sizeof(double2) + ((size_t)most * KV_ROW << a.kv_shift);
+  const uint32_t nb = (uint32_t)blocks;
+  return type == DEFER_GPU_F32    ? append_launch<float>(a, nb, lds, vec, s)
+         : type == DEFER_GPU_BF16 ? append_launch<__bf16>(a, nb, lds, vec, s)
+                                  : append_launch<_Float16>(a, nb, lds, vec, s);
 }
 
 extern "C" int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, const int32_t* keep,
