@@ -28,7 +28,7 @@ struct AppendArgs {
   uint32_t hd, nh, half;        // half: rotated pairs of a head
   uint32_t kv_shift, q_shift;   // a workgroup takes so many heads, as a power of 2: of the cache, or of the queries
   uint32_t kv_chunks, chunks;   // workgroups of a run for the cache's heads, and for all
-  bool interleaved, clear;
+  bool interleaved;
 };
 
 template <int CTRL>
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
   m = fmaxf(m, __shfl_xor(m, 32));
   const float m0 = m == -INFINITY ? 0.0f : m, unit = a.scale * 1.44269504088896340736f;
   float sum = 0.0f, moment = 0.0f;
-  if (__builtin_expect(!__any(least == -INFINITY), 1)) {
+  if (__builtin_expect(!__any(least - m0 == -INFINITY), 1)) {
 #pragma unroll
     for (int i = 0; i < SCORE_EACH; ++i) {
       const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
@@ -644,7 +644,7 @@ __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
     for (int i = 0; i < SCORE_EACH; ++i) {
       const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
       sum += e;
-      moment = fmaf(fmaxf(d, -FLT_MAX), e, moment);  // -inf has 0 of the sum
+      moment = fmaf(fmaxf(d, -FLT_MAX), e, moment);  // so far below (or -inf): 0 of the sum
     }
   }
   uint32_t above = 0;
@@ -660,7 +660,7 @@ __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
     static_assert(SCORE_WAVES <= 16, "a wave's part for each of 16 lanes");
     const ScorePart s = lane < SCORE_WAVES ? s_part[lane] : ScorePart{-INFINITY, 0.0f, 0.0f, 0};
     const float mm = lanes_max<16>(s.top), d = s.top - (mm == -INFINITY ? 0.0f : mm), e = __builtin_amdgcn_exp2f(d * unit);
-    const float sums = row_sum(s.sum * e), moments = row_sum(fmaf(fmaxf(d, -FLT_MAX), s.sum, s.moment) * e);
+    const float sums = row_sum(s.sum * e), moments = row_sum(e == 0.0f ? 0.0f : fmaf(d, s.sum, s.moment) * e);
     uint32_t higher = s.above;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) higher += __shfl_xor(higher, o);
@@ -900,7 +900,6 @@ extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const def
   a.nh = q_heads;
   a.half = rotary->rotated / 2;
   a.interleaved = rotary->interleaved != 0;
-  a.clear = clear && r.row_start;
   // Heads of a workgroup: 16 of its lanes take a row's head, so that a full run of queries takes
   // it 4 rounds and one of the cache's heads 2 (keys, values); fewer rows take more heads, so
   // that the lanes have work. Where those would be more workgroups than the chip holds at once
@@ -919,7 +918,7 @@ extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const def
     a.kv_shift = power(items / 4 / most, p.heads);
     a.kv_chunks = (p.heads + (1u << a.kv_shift) - 1) >> a.kv_shift;
     a.chunks = a.kv_chunks + ((q_heads + (1u << a.q_shift) - 1) >> a.q_shift);
-    blocks = ((uint64_t)r.sequences + a.clear) * kv_runs(r.most_rows) * a.chunks;
+    blocks = ((uint64_t)r.sequences + (clear && r.row_start)) * kv_runs(r.most_rows) * a.chunks;
     if (blocks <= 1024) break;
   }
   Q8_REQUIRE(blocks <= MAX_THREADS / 256, "too many rows for one call");
@@ -970,7 +969,7 @@ extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_st
   if (rc) return rc;
   Q8_REQUIRE(n <= MAX_SCORE, "%u logits: at most %u", n, MAX_SCORE);
   Q8_REQUIRE(top <= MAX_TOP && top <= n, "the %u best of %u: at most %u", top, n, MAX_TOP);
-  Q8_REQUIRE(scale > 0.0f && scale <= 1e30f, "scale %g", (double)scale);
+  Q8_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "scale %g", (double)scale);
   Q8_REQUIRE(rows == 0 || (log_p && entropy && rank && (top == 0 || (top_index && top_log_p))), "null output");
   Q8_REQUIRE(aligned_to(target, 4) && aligned_to(log_p, 4) && aligned_to(entropy, 4) && aligned_to(rank, 4) &&
                  aligned_to(top_index, 4) && aligned_to(top_log_p, 4),

@@ -595,7 +595,7 @@ int tree_attention(const Pages& p, const Rows& r, const Attention& in, void* wor
     return defer_gpu_fail_(DEFER_GPU_E_INVALID, "too many rows for one call");
   const uint32_t nb = (uint32_t)blocks;
   if (!pl.split) return pl.R == 1 ? tree_launch<1, false>(a, nb, pl.lds, s) : tree_launch<2, false>(a, nb, pl.lds, s);
-  const int rc = pl.R == 1 ? tree_launch<1, true>(a, nb, pl.lds, s) : tree_launch<2, true>(a, nb, pl.lds, s);
+  const int rc = tree_launch<1, true>(a, nb, pl.lds, s);  // (two tiles a wave are for many workgroups)
   return rc ? rc : launch(k_tree_join, r.sequences * r.most_rows * in.heads, p.dp, 0, s, a);
 }
 

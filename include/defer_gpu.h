@@ -421,7 +421,7 @@ int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer_gpu_q8_row
                          const int32_t* keep, const int32_t* kept, int32_t* kv_len_out, void* stream);
 
 /* Of rows of n <= 1,048,576 logits x [rows, n], rows x_stride values apart, with p =
- * softmax(scale * x): log_p[r] = log p[target[r]]; entropy[r] = -sum p log p;
+ * softmax(scale * x), 1e-30 <= scale <= 1e30: log_p[r] = log p[target[r]]; entropy[r] = -sum p log p;
  * rank[r] = how many logits are larger than the target's; top_index and top_log_p
  * [rows, top]: the top <= 32 largest, the lower index first among equals. A target
  * outside [0, n) (or target NULL) has log_p NaN and rank -1. A logit of -inf has

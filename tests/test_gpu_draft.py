@@ -222,6 +222,50 @@ def test_append_rows_of_no_sequence_bad_pages_and_odd_values():
     assert torch.isnan(out[0]).all() and torch.equal(out[1], torch.ones(nh, hd, device=DEV))
 
 
+@pytest.mark.parametrize("dtype,hd", [(torch.float32, 64), (torch.float32, 200), (torch.float32, 7), (torch.bfloat16, 128),
+                                      (torch.bfloat16, 256)])
+def test_append_codes_at_and_beside_halves_of_every_scale(dtype, hd):
+    """Without rotation the codes and scales are the cache write's, also of values half-way between codes, of their
+    neighbours, and where the scale is near either end of the type's range."""
+    powers = (-100, -94, -93, -60, -20, -1, 0, 1, 50, 110, 116, 117, 118, 119, 120)
+    g = torch.Generator().manual_seed(hd)
+    rows = []
+    for e in powers:
+        for near in (0, 1, -1):
+            codes = torch.randint(-127, 127, (hd,), generator=g).float() + 0.5
+            x = codes.to(dtype)
+            if near:
+                bits = torch.int32 if dtype == torch.float32 else torch.int16
+                x = (x.view(bits) + near).view(dtype)  # the next number, or the one before
+            x[0] = 127
+            rows.append((x.float() * 2.0 ** e).to(dtype))
+    x = torch.stack(rows)[:, None].to(DEV)
+    n = len(x)
+    a, b = make_cache([n], 1, hd, seed=1), make_cache([n], 1, hd, seed=1)
+    b.keys.copy_(a.keys)
+    b.values.copy_(a.values)
+    out = q8.kv_append(a, x, x, x, i32([n]), q8.rotary(0, device=DEV), starts([n]), n)
+    q8.kv_write(b, x, x, i32([n]), starts([n]), n)
+    assert torch.equal(out, x) and all(same(s, t) for s, t in zip(a, b))
+
+
+def test_append_of_many_runs_and_of_one_give_the_same_bits():
+    """Workgroups take more heads where there are many runs of rows: neither that nor a call's other rows show."""
+    nh, nkv, hd, n, seqs = 15, 5, 64, 47, 60
+    rot = q8.rotary(hd, 1e4, interleaved=True, device=DEV)
+    q, k, v = (rnd(seqs * n, h, hd, seed=i, dtype=torch.bfloat16).to(DEV) for i, h in enumerate((nh, nkv, nkv)))
+    lens = [n + 3 * i for i in range(seqs)]
+    pages, alone = make_cache(lens, nkv, hd, seed=1), make_cache(lens, nkv, hd, seed=1)
+    alone.keys.copy_(pages.keys)
+    alone.values.copy_(pages.values)
+    out = q8.kv_append(pages, q, k, v, i32(lens), rot, starts([n] * seqs), n)
+    for i in range(seqs):
+        one = alone._replace(table=alone.table[i:i + 1].contiguous())
+        r = slice(i * n, i * n + n)
+        assert torch.equal(q8.kv_append(one, q[r], k[r], v[r], i32(lens[i:i + 1]), rot, starts([n]), n), out[r])
+    assert all(same(a, b) for a, b in zip(pages, alone))
+
+
 # ------------------------------------------------------------------ trees
 
 def random_tree(n, seed, back=4):
@@ -338,6 +382,28 @@ def test_trees_split_over_workgroups_or_not(seqs):
         one = q8.attention(q[j:j + 1], own, i32([ctx + len(path)]))
         for i in (0, seqs // 2, seqs - 1):
             assert torch.equal(out[11 * i + j], one[0])
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(64, 8, 64), (64, 8, 40), (32, 8, 128), (48, 8, 72)])
+def test_trees_of_many_workgroups_and_of_few_give_the_same_bits(nh, nkv, hd):
+    """Where there are many, a wave takes two tiles of rows; the last ones of a sequence are not full."""
+    seqs, ctxs = 64 if nh == 64 else 128, (70, 0, 130, 57)
+    counts = [(17, 20, 1, 13, 20)[i % 5] for i in range(seqs)]
+    trees = [random_tree(c, i) for i, c in enumerate(counts)]
+    lens = [ctxs[i % 4] + c for i, c in enumerate(counts)]
+    pages = make_cache(lens, nkv, hd, seed=2)
+    fill(pages, lens, nkv, hd, seed=2)
+    q = rnd(sum(counts), nh, hd, seed=4).to(DEV)
+    h = (torch.rand(seqs, 140, generator=torch.Generator().manual_seed(3)) < 0.3).to(DEV)
+    for hidden in (None, h):
+        out = q8.tree_attention(q, pages, i32(sum(trees, [])), i32(lens), starts(counts), 20, max(lens), hidden=hidden)
+        at = 0
+        for i, c in enumerate(counts):
+            one = pages._replace(table=pages.table[i:i + 1].contiguous())
+            alone = q8.tree_attention(q[at:at + c], one, i32(trees[i]), i32(lens[i:i + 1]), starts([c]), c,
+                                      hidden=None if hidden is None else hidden[i:i + 1])
+            assert torch.equal(out[at:at + c], alone), i
+            at += c
 
 
 def test_trees_across_unit_lengths():
@@ -512,7 +578,8 @@ def check_scores(x, target, top, scale=1.0, x_gpu=None):
     assert [a.dtype for a in got] == [torch.float32] * 2 + [torch.int32] * 2 + [torch.float32]
     assert torch.equal(got.rank.cpu(), rank.int()) and torch.equal(got.top_index.cpu(), order.int())
     # A term e = exp(scale d), d = x - max: d, scale * log2(e) (twice), their product: half a step each, 4 u |scale d|
-    # of e; the exponential a step, 2 u. The sum: 16 terms a thread, 6 steps a wave, 16 waves: 37 u. So the sum's
+    # of e; the exponential a step, 2 u. The sum: 16 terms a thread, 6 steps a wave, then a factor of each wave
+    # (whose d is the rest of the terms' d) and 4 steps: under 37 u. So the sum's
     # logarithm is off by u (4 mean |scale d| + 39); chunks join in 64 bits. The moment's terms have
     # one product more and d itself, its sum as many roundings.
     u = 2.0 ** -24
@@ -562,6 +629,40 @@ def test_log_probs_of_equal_logits(n):
         got = check_scores(x, target, top)
         assert got.rank.tolist()[:2] == [0, 0] and got.rank.tolist()[3] == 2
         assert got.top_index[0].tolist() == list(range(top))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_log_probs_of_rows_whose_best_lie_together(dtype):
+    """More logits over any bound from groups' maxima than are held at once: in order, in blocks of columns, and equal."""
+    n = 49152
+    x = rnd(6, n, seed=5)
+    x[0] = torch.sort(x[0]).values
+    x[1] = torch.sort(x[1], descending=True).values
+    c = torch.arange(n)
+    for r, w in ((2, 32), (3, 64)):  # 31 of every 64 runs of 32, or 64, columns are far over the rest
+        x[r] = x[r] / 8 + torch.where(c // w % 64 < 31, 20.0, 0.0)
+    x[4] = torch.where(c // 32 % 64 < 31, torch.round(x[4]) + 8, x[4] - 20)
+    x[5] = torch.where(c % 3 == 0, 2.0, torch.where(c == 5, 3.0, -1.0))
+    for top in (1, 31, 32):
+        check_scores(x.to(dtype), torch.tensor([0, 1, 2, 3, 4, 5], dtype=torch.int32), top)
+
+
+def test_log_probs_of_logits_at_both_ends_of_the_range():
+    for n in (3 * 8192, 9000):
+        x = torch.full((4, n), -3e38)
+        x[0, 5] = 3e38
+        x[1, :n // 2] = 3e38
+        x[2] = rnd(n, seed=1) * 1e38
+        x[3, ::2], x[3, 1::2] = -math.inf, 1e38
+        assert (x[2] == math.inf).any()  # 3.4 standard deviations, and so no distribution
+        got = q8.log_probs(x[2:3].to(DEV), torch.tensor([3], dtype=torch.int32).to(DEV), 4)
+        assert torch.isnan(got.log_p[0]) and torch.isnan(got.entropy[0]) and got.rank[0] == -1 and (got.top_index[0] == -1).all()
+        x[2] = rnd(n, seed=1) * 5e37
+        got = check_scores(x, torch.tensor([5, 0, 3, 1], dtype=torch.int32), 4)
+        assert got.entropy[0] == 0 and abs(float(got.entropy[1]) - math.log(n // 2)) < 1e-5 and got.log_p[0] == 0
+        for scale in (1e-30, 1e30):
+            check_scores(rnd(3, n, seed=2), torch.tensor([1, 2, 3], dtype=torch.int32), 4, scale=scale)
+        check_scores(x[2:3] / 8, torch.tensor([1], dtype=torch.int32), 4, scale=1e-30)
 
 
 def test_log_probs_of_rows_without_a_distribution():
@@ -752,3 +853,86 @@ def test_a_verifying_step_in_a_graph_and_on_streams():
         want, want_pages = eager()
         assert all(same(a, b) for a, b in zip(got, want)) and all(same(a, b) for a, b in zip(pages, want_pages))
         assert i8(1, 1).numel() == 1 and torch.randn(100, device=DEV).sum().item() is not None  # the program's own work between
+
+
+def test_calls_without_row_start_and_defaults():
+    """One row of each sequence without row_start; most_rows and most_len as the call can know them."""
+    lens, nh, nkv, hd = [70, 1, 64, 200], 6, 2, 64
+    pages, other = make_cache(lens, nkv, hd), make_cache(lens, nkv, hd)
+    fill(pages, lens, nkv, hd)
+    fill(other, lens, nkv, hd)
+    q, k, v = (rnd(4, h, hd, seed=i).to(DEV) for i, h in enumerate((nh, nkv, nkv)))
+    rot = q8.rotary(hd, device=DEV)
+    a = q8.kv_append(pages, q, k, v, i32(lens), rot)
+    b = q8.kv_append(other, q, k, v, i32(lens), rot, starts([1] * 4))
+    assert torch.equal(a, b)
+    assert torch.equal(*(torch.cat([t.float().flatten() for t in q8.kv_read(p, i32(lens), starts(lens), sum(lens), hd)])
+                         for p in (pages, other)))
+    root = i32([-1] * 4)
+    want = q8.attention(a, pages, i32(lens))
+    assert torch.equal(q8.tree_attention(a, pages, root, i32(lens)), want)
+    assert torch.equal(q8.tree_attention(a, pages, root, i32(lens), starts([1] * 4)), want)
+    assert q8.kv_keep(pages, i32(lens), None, i32([0] * 4), i32([1, 1, 0, 1])).tolist() == [70, 1, 63, 200]
+    # 140 rows of three sequences, at most 64 each
+    counts = [64, 12, 64]
+    big = make_cache([64, 90, 300], nkv, hd)
+    fill(big, [64, 90, 300], nkv, hd)
+    q = rnd(140, nh, hd, seed=5).to(DEV)
+    tree = i32(sum((random_tree(n, n) for n in counts), []))
+    args = (q, big, tree, i32([64, 90, 300]), starts(counts))
+    assert torch.equal(q8.tree_attention(*args), q8.tree_attention(*args, 64, 300))
+    with pytest.raises(ValueError, match="at most 64"):
+        q8.tree_attention(*args, 65)
+    with pytest.raises(ValueError, match="at most 64"):
+        q8.kv_keep(big, i32([64, 90, 300]), starts(counts), tree, i32([0, 0, 0]), 65)
+
+
+def test_what_calls_write_has_a_new_version():
+    lens = [70]
+    pages = make_cache(lens, 2, 64)
+    fill(pages, lens, 2, 64)
+    q, k = rnd(4, 4, 64, seed=1).to(DEV), rnd(4, 2, 64, seed=2).to(DEV)
+    out, rot, before = torch.empty_like(q), q8.rotary(64, device=DEV), [t._version for t in pages]
+    q8.kv_append(pages, q, k, k, i32(lens), rot, starts([4]), out=out)
+    assert out._version == 1 and [t._version for t in pages] == [n + 1 for n in before[:4]] + before[4:]
+    q8.tree_attention(q, pages, i32([-1, 0, 0, 1]), i32(lens), starts([4]), out=out)
+    assert out._version == 2 and q._version == k._version == 0
+    q8.kv_keep(pages, i32(lens), starts([4]), i32([0, 2, 2, 2]), i32([2]))
+    assert [t._version for t in pages] == [n + 2 for n in before[:4]] + before[4:]
+
+
+def test_two_calls_at_once_have_workspaces_of_their_own():
+    """On two streams, each of them in turn, and in two graphs that are replayed together."""
+    nh, nkv, hd, lens, counts = 8, 2, 64, [1900, 800], [9, 20]
+    pages = make_cache(lens, nkv, hd)
+    fill(pages, lens, nkv, hd)
+    tree = i32(random_tree(9, 1) + random_tree(20, 2))
+    qs = [rnd(29, nh, hd, seed=i).to(DEV) for i in range(2)]
+    xs = [rnd(29, 50000, seed=i).to(DEV) for i in range(2)]
+    target, kv_len, start = i32(list(range(29))), i32(lens), starts(counts)
+
+    def work(i):
+        return (q8.tree_attention(qs[i], pages, tree, kv_len, start, 20, 1900),) + tuple(q8.log_probs(xs[i], target, 20))
+
+    want = [work(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        got = []
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got.append(work(i))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+    graphs, got = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            got.append(work(i))
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+        assert torch.randn(100, device=DEV).sum().item() is not None
