@@ -454,17 +454,22 @@ __global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
 
 // ------------------------------------------------------------- log probabilities
 
-constexpr int SCORE_THREADS = 512, SCORE_EACH = 16, SCORE_CHUNK = SCORE_THREADS * SCORE_EACH;  // logits of a workgroup
-constexpr int SCORE_WAVES = SCORE_THREADS / WAVE;
-constexpr int SCORE_GROUP = SCORE_THREADS / WAVE;  // threads whose logits have a maximum together: 64 maxima a chunk
+constexpr int SCORE_EACH = 16, SCORE_CHUNK = SCORE_EACH * WAVE;  // logits of a lane, and of a wave
+constexpr int SCORE_THREADS = 256, SCORE_WAVES = SCORE_THREADS / WAVE;
+constexpr int SCORE_GROUP = 8, SCORE_GROUPS = WAVE / SCORE_GROUP;  // lanes whose logits have a maximum together
 constexpr uint32_t SCORE_FEW = 2048;               // candidates for the best that a row may have in LDS
 constexpr uint32_t SCORE_LIST = 1024;              // ... and groups that they come from
 
-// What a workgroup leaves of its chunk of a row, joined in the order of chunks.
+// What a wave leaves of its chunk of a row.
 struct ScorePart {
-  float top, sum, moment;  // maximum m; sum of e = exp(scale (x - m)), and of e (x - m)
-  uint32_t above;          // logits over the target's
+  float top, sum, moment;  // maximum m; sum of e = 2^t, t = scale log2(e) (x - m) + r, and of e t
+  uint32_t above;          // logits over the target's; SCORE_FAR: r is 0
 };
+constexpr uint32_t SCORE_FAR = 1u << 31;
+// A logit's t is one fused product: fma(x, unit, -c), c = unit m rounded, which is r too large for
+// all of a wave's, r = fma(m, unit, -c) without a rounding: the sum is 2^r times too
+// large, the moment has r times it to lose.
+__device__ __forceinline__ float score_over(float m, float unit) { return fmaf(m, unit, -(m * unit)); }
 
 struct ScoreArgs {
   const void* x;
@@ -475,21 +480,24 @@ struct ScoreArgs {
   float *log_p, *entropy, *top_log_p;
   int32_t *rank, *top_index;
   ScorePart* part;   // [rows][chunks]
-  float* maxima;     // [rows][chunks][64], for the best
+  uint32_t* maxima;  // [rows][chunks][8], for the best: score_order's
 };
 
-// A whole number that orders logits by value, then by the lower column. -0 is
-// 0; a NaN comes last. No logit's is 0.
-__device__ __forceinline__ uint64_t score_key(float v, uint32_t column) {
-  v = isnan(v) ? -INFINITY : v + 0.0f;
-  const uint32_t b = __builtin_bit_cast(uint32_t, v), o = b ^ (uint32_t)((int32_t)b >> 31 | (int32_t)0x80000000);
-  return (uint64_t)o << 32 | (0xffffffffu - column);
+// A whole number that orders logits by value (-0 is 0), and back; no logit's is 0. (A
+// NaN's is anywhere: its row has no best.)
+__device__ __forceinline__ uint32_t score_order(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+  return b ^ (uint32_t)((int32_t)b >> 31 | (int32_t)0x80000000);
 }
-__device__ __forceinline__ uint32_t column_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
-__device__ __forceinline__ float value_of(uint64_t key) {
-  const uint32_t o = (uint32_t)(key >> 32);
+__device__ __forceinline__ float of_order(uint32_t o) {
   return __builtin_bit_cast(float, o ^ (o >> 31 ? 0x80000000u : 0xffffffffu));
 }
+// ... and one that orders equal ones by the lower column.
+__device__ __forceinline__ uint64_t score_key(float v, uint32_t column) {
+  return (uint64_t)score_order(v) << 32 | (0xffffffffu - column);
+}
+__device__ __forceinline__ uint32_t column_of(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+__device__ __forceinline__ float value_of(uint64_t key) { return of_order((uint32_t)(key >> 32)); }
 
 // A bound that `top` of the wave's numbers reach and at most `slack` more, unless they are equal;
 // 0 if fewer are over 0. Steps down from the largest, then halves.
@@ -563,109 +571,96 @@ __device__ __forceinline__ void score_pick(uint64_t* keys, uint32_t count, uint3
   }
 }
 
-// Over N neighbouring lanes: in each of them.
-template <int N>
-__device__ __forceinline__ float lanes_max(float v) {
-  v = fmaxf(v, dpp<0xb1>(v));                 // quad_perm 1 0 3 2
-  v = fmaxf(v, dpp<0x4e>(v));                 // quad_perm 2 3 0 1
-  if (N >= 8) v = fmaxf(v, dpp<0x141>(v));    // row_half_mirror
-  if (N >= 16) v = fmaxf(v, dpp<0x140>(v));   // row_mirror
-  return v;
+// Maxima and sums over lanes, a step an instruction: CTRL names the lanes that are read, ROWS the
+// rows of 16 that read them.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t max_step(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false));
 }
-
-// Over the wave: 16 lanes, then the rows.
-__device__ __forceinline__ float wave_sum(float v) {
-  v = row_sum(v);
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float add_step(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
 }
+// Over 8 neighbouring lanes: in each of them.
+__device__ __forceinline__ uint32_t max_of_8(uint32_t v) {
+  return max_step<0x141>(max_step<0x4e>(max_step<0xb1>(v)));  // quad_perm 1 0 3 2, 2 3 0 1, row_half_mirror
+}
+// Over the wave, of numbers that are the same in 8 neighbouring lanes: in all of it.
+__device__ __forceinline__ uint32_t max_of_wave(uint32_t v) {
+  v = max_step<0x143, 0xc>(max_step<0x142, 0xa>(max_step<0x140>(v)));  // row_mirror, row_bcast 15, 31
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, WAVE - 1);
+}
+// Over the wave: in its last lane.
+__device__ __forceinline__ float sum_of_wave(float v) { return add_step<0x143, 0xc>(add_step<0x142, 0xa>(row_sum(v))); }
 
-// One chunk of a row: in registers, 16 logits a thread, read once; each wave's
-// sums are relative to its own maximum, the first wave joins them. For the best, the
-// maxima of 64 groups of threads are left: k_score_join reads the few groups again
-// that can hold one.
+// A wave takes a chunk of a row, in registers, 16 logits a lane, read once; its sums are
+// relative to its own maximum m. For the best, the maxima of groups of lanes are left:
+// k_score_join reads the few groups again that can hold one. Where m is so far out that the
+// product that t comes from would be, or a logit is infinitely far below (t is -inf, the moment
+// NaN), x - m comes first.
 template <class T, bool VEC>
 __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
   constexpr int V = 16 / sizeof(T), NV = SCORE_EACH / V;
   typedef T vt __attribute__((ext_vector_type(V)));
-  const uint32_t chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
-  const uint32_t lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), c0 = chunk * SCORE_CHUNK;
-  const T* p = static_cast<const T*>(a.x) + (int64_t)row * a.xs;
-  __shared__ ScorePart s_part[SCORE_WAVES];
+  const uint32_t lane = threadIdx.x % WAVE, at = blockIdx.x * SCORE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  if (at >= a.rows * a.chunks) return;
+  const uint32_t row = at / a.chunks, c0 = (at - row * a.chunks) * SCORE_CHUNK;
+  const T* const p = static_cast<const T*>(a.x) + (int64_t)row * a.xs;
   const int32_t target = a.target ? a.target[row] : -1;
-  const uint32_t out = row * a.chunks + chunk;
-
-  auto column = [&](int i) { return c0 + ((i / V) * SCORE_THREADS + threadIdx.x) * V + i % V; };
-  float x[SCORE_EACH];
+  vt w[NV];
   if (VEC && c0 + SCORE_CHUNK <= a.n) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const vt w = *reinterpret_cast<const vt*>(p + column(v * V));
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[v * V + e] = (float)w[e];
-    }
+    for (int v = 0; v < NV; ++v) w[v] = *reinterpret_cast<const vt*>(p + c0 + (v * WAVE + lane) * V);
   } else {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const uint32_t c = column(v * V);
-      if (VEC && c + V <= a.n) {
-        const vt w = *reinterpret_cast<const vt*>(p + c);
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[v * V + e] = (float)w[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[v * V + e] = c + e < a.n ? (float)p[c + e] : -INFINITY;
-      }
+    for (int i = 0; i < SCORE_EACH; ++i) {
+      const uint32_t c = c0 + (i / V * WAVE + lane) * V + i % V;
+      w[i / V][i % V] = c < a.n ? p[c] : (T)-INFINITY;
     }
   }
-  const float xt = target >= 0 && (uint32_t)target < a.n ? (float)p[target] : INFINITY;
-  float mine = x[0], least = x[0];
+  T wt = (T)INFINITY;
+  if (target >= 0 && (uint32_t)target < a.n) wt = p[target];  // on its way with the others
+  __builtin_amdgcn_sched_barrier(0);
+  float x[SCORE_EACH];
 #pragma unroll
-  for (int i = 1; i < SCORE_EACH; ++i) {
-    mine = fmaxf(mine, x[i]);
-    least = fminf(least, x[i]);
-  }
-  const float group = lanes_max<SCORE_GROUP>(mine);
-  if (a.top && lane % SCORE_GROUP == 0) a.maxima[(size_t)out * WAVE + threadIdx.x / SCORE_GROUP] = group;
-  float m = lanes_max<16>(group);
-  m = fmaxf(m, __shfl_xor(m, 16));
-  m = fmaxf(m, __shfl_xor(m, 32));
-  const float m0 = m == -INFINITY ? 0.0f : m, unit = a.scale * 1.44269504088896340736f;
+  for (int i = 0; i < SCORE_EACH; ++i) x[i] = (float)w[i / V][i % V];
+  float mine = x[0];
+#pragma unroll
+  for (int i = 1; i < SCORE_EACH; ++i) mine = fmaxf(mine, x[i]);
+  const uint32_t group = max_of_8(score_order(mine));
+  if (a.top && lane % SCORE_GROUP == 0) a.maxima[(size_t)at * SCORE_GROUPS + lane / SCORE_GROUP] = group;
+  const float m = of_order(max_of_wave(group)), unit = a.scale * 1.44269504088896340736f, c = m * unit;
   float sum = 0.0f, moment = 0.0f;
-  if (__builtin_expect(!__any(least - m0 == -INFINITY), 1)) {
+  uint32_t above = 0;
+  bool far = !(fabsf(c) <= 0x1p20f);  // (or m is not finite)
+  if (!far) {
 #pragma unroll
     for (int i = 0; i < SCORE_EACH; ++i) {
-      const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
+      const float t = fmaf(x[i], unit, -c), e = __builtin_amdgcn_exp2f(t);
       sum += e;
-      moment = fmaf(d, e, moment);
+      moment = fmaf(t, e, moment);
     }
-  } else {
+    far = __any(!(moment > -FLT_MAX));
+  }
+  if (__builtin_expect(far, 0)) {
+    const float m0 = m == -INFINITY ? 0.0f : m;
+    sum = moment = 0.0f;
+    above = SCORE_FAR;
 #pragma unroll
     for (int i = 0; i < SCORE_EACH; ++i) {
-      const float d = x[i] - m0, e = __builtin_amdgcn_exp2f(d * unit);
+      const float t = (x[i] - m0) * unit, e = __builtin_amdgcn_exp2f(t);
       sum += e;
-      moment = fmaf(fmaxf(d, -FLT_MAX), e, moment);  // so far below (or -inf): 0 of the sum
+      moment = fmaf(fmaxf(t, -FLT_MAX), e, moment);  // so far below (or -inf): 0 of the sum
     }
   }
-  uint32_t above = 0;
+  const float xt = (float)wt;
   if (m > xt) {  // (the same in all lanes)
 #pragma unroll
     for (int i = 0; i < SCORE_EACH; ++i) above += (uint32_t)__popcll(__ballot(x[i] > xt));
   }
-  sum = wave_sum(sum);
-  moment = wave_sum(moment);
-  if (lane == 0) s_part[wave] = ScorePart{m, sum, moment, above};
-  __syncthreads();
-  if (wave == 0) {
-    static_assert(SCORE_WAVES <= 16, "a wave's part for each of 16 lanes");
-    const ScorePart s = lane < SCORE_WAVES ? s_part[lane] : ScorePart{-INFINITY, 0.0f, 0.0f, 0};
-    const float mm = lanes_max<16>(s.top), d = s.top - (mm == -INFINITY ? 0.0f : mm), e = __builtin_amdgcn_exp2f(d * unit);
-    const float sums = row_sum(s.sum * e), moments = row_sum(e == 0.0f ? 0.0f : fmaf(d, s.sum, s.moment) * e);
-    uint32_t higher = s.above;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) higher += __shfl_xor(higher, o);
-    if (lane == 0) a.part[out] = ScorePart{mm, sums, moments, higher};
-  }
+  sum = sum_of_wave(sum);
+  moment = sum_of_wave(moment);
+  if (lane == WAVE - 1) a.part[at] = ScorePart{m, sum, moment, above};
 }
 
 // A row's chunks joined in order, in 64 bits, by the last wave; its best by the others:
@@ -675,19 +670,19 @@ __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
 // Where those over it are too many still, one after the other.
 __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) {
   constexpr uint32_t HELD = 4;  // groups' maxima that a thread keeps
+  constexpr double LN2 = 0.69314718055994530942;
   __shared__ uint64_t s_key[SCORE_FEW], s_wave[4];
   __shared__ uint32_t s_max[4][WAVE];
   __shared__ uint16_t s_list[SCORE_LIST];
   __shared__ uint32_t s_count, s_groups;
   __shared__ double s_sum;
   __shared__ float s_top;
-  static_assert(MAX_SCORE / SCORE_CHUNK * WAVE <= 0x10000 && MAX_TOP <= WAVE, "a group's number in 16 bits");
+  static_assert(MAX_SCORE / SCORE_CHUNK * SCORE_GROUPS <= 0x10000 && MAX_TOP <= WAVE, "a group's number in 16 bits");
   const uint32_t row = blockIdx.x, lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int64_t x0 = (int64_t)row * a.xs;
-  const uint32_t groups = a.chunks * WAVE;
-  const float* maxima = a.maxima + (size_t)row * groups;
-  auto ordered = [](float v) { return (uint32_t)(score_key(v, 0) >> 32); };
-  auto group_max = [&](uint32_t i) { return i < groups ? ordered(maxima[i]) : 0u; };
+  const uint32_t groups = a.chunks * SCORE_GROUPS;
+  const uint32_t* maxima = a.maxima + (size_t)row * groups;
+  auto group_max = [&](uint32_t i) { return i < groups ? maxima[i] : 0u; };
   uint32_t held[HELD], most = 0;
   if (a.top) {
 #pragma unroll
@@ -702,21 +697,29 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
   if (wave == 3) {  // what the whole row's sums say
     const int32_t target = a.target ? a.target[row] : -1;
     const ScorePart* part = a.part + (size_t)row * a.chunks;
+    const float unit = a.scale * 1.44269504088896340736f;
     float top = -INFINITY;
     double sum = 0.0, moment = 0.0;
     uint32_t above = 0;
     for (uint32_t c = lane; c < a.chunks; c += WAVE) top = fmaxf(top, part[c].top);
     top = wave_max(top);
-    for (uint32_t c0 = 0; c0 < a.chunks; c0 += WAVE) {
-      const ScorePart s = c0 + lane < a.chunks ? part[c0 + lane] : ScorePart{-INFINITY, 0.0f, 0.0f, 0};
-      above += wave_add(s.above);
-      const bool none = s.top == -INFINITY && s.sum == 0.0f;  // nothing over -inf: nothing of the sum
-      const double d = none ? 0.0 : (double)s.top - (double)top, e = none ? 0.0 : exp((double)a.scale * d);
-      const double mine = e * (double)s.sum, moments = e == 0.0 ? 0.0 : e * fma(d, (double)s.sum, (double)s.moment);
-      for (int c = 0; c < (int)min(a.chunks - c0, (uint32_t)WAVE); ++c) {
-        sum += __shfl(mine, c);
-        moment += __shfl(moments, c);
-      }
+    for (uint32_t c = lane; c < a.chunks; c += WAVE) {
+      const ScorePart s = part[c];
+      if (s.top == -INFINITY && s.sum == 0.0f) continue;  // nothing over -inf: nothing of the sum
+      const float over = s.above & SCORE_FAR ? 0.0f : score_over(s.top, unit);
+      // what its sum is times: that of a wave of one logit is 1
+      const double own = (double)s.sum / (double)__builtin_amdgcn_exp2f(over);
+      const double left = ((double)s.moment - (double)(over * s.sum)) / (double)__builtin_amdgcn_exp2f(over);
+      const double t = (double)a.scale * ((double)s.top - (double)top), e = exp(t);
+      sum += e * own;
+      if (e > 0.0) moment += e * fma(t, own, LN2 * left);
+      above += s.above & ~SCORE_FAR;
+    }
+    above = wave_add(above);
+#pragma unroll
+    for (int o = 1; o < WAVE; o *= 2) {
+      sum += __shfl_xor(sum, o);
+      moment += __shfl_xor(moment, o);
     }
     if (lane == 0) {
       const float nan = __builtin_nanf("");
@@ -724,7 +727,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
       const bool has = target >= 0 && (uint32_t)target < a.n && !none;
       const double scale = (double)a.scale, log_sum = none ? (double)nan : log(sum);
       a.log_p[row] = has ? (float)(scale * ((double)load_value(a.x, x0 + target, type) - (double)top) - log_sum) : nan;
-      a.entropy[row] = (float)(log_sum - scale * moment / sum);
+      a.entropy[row] = (float)(log_sum - moment / sum);
       a.rank[row] = has ? (int32_t)above : -1;
       s_sum = log_sum;
       s_top = top;
@@ -736,7 +739,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
   // columns of a group: of each 16-byte vector of a thread's, a run
   const uint32_t vector = type == DEFER_GPU_F32 ? 4 : 8, run = SCORE_GROUP * vector;
   auto column = [&](uint32_t group, uint32_t e) {
-    return group / WAVE * SCORE_CHUNK + e / run * (SCORE_THREADS * vector) + group % WAVE * run + e % run;
+    return group / SCORE_GROUPS * SCORE_CHUNK + e / run * (WAVE * vector) + group % SCORE_GROUPS * run + e % run;
   };
   // Keys of the logits that reach `from` (counts are 0); returns how many there are.
   auto gather = [&](uint32_t from) {
@@ -764,7 +767,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
 #pragma unroll
       for (uint32_t s = 0; s < EACH; ++s) {
         const uint32_t c = column(group, 16 * s + lane % 16);
-        if (c < a.n && ordered(v[s]) >= from) {
+        if (c < a.n && score_order(v[s]) >= from) {
           const uint32_t at = atomicAdd(&s_count, 1u);
           if (at < SCORE_FEW) s_key[at] = score_key(v[s], c);
         }
@@ -835,7 +838,8 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
 
 template <class T>
 int score_launch(const ScoreArgs& a, bool vec, hipStream_t s) {
-  return launch(vec ? k_score<T, true> : k_score<T, false>, a.rows * a.chunks, SCORE_THREADS, 0, s, a);
+  const uint32_t blocks = (a.rows * a.chunks + SCORE_WAVES - 1) / SCORE_WAVES;
+  return launch(vec ? k_score<T, true> : k_score<T, false>, blocks, SCORE_THREADS, 0, s, a);
 }
 
 uint32_t score_chunks(uint32_t n) { return (n + SCORE_CHUNK - 1) / SCORE_CHUNK; }
@@ -957,8 +961,8 @@ extern "C" int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer
 }
 
 extern "C" size_t defer_gpu_q8_log_probs_workspace(uint32_t rows, uint32_t n, uint32_t top) {
-  if (rows > MAX_THREADS / SCORE_THREADS || n > MAX_SCORE || top > MAX_TOP) return 0;
-  return (size_t)rows * score_chunks(n) * (sizeof(ScorePart) + (top ? WAVE * sizeof(float) : 0));
+  if (rows > MAX_THREADS / WAVE || n > MAX_SCORE || top > MAX_TOP) return 0;
+  return (size_t)rows * score_chunks(n) * (sizeof(ScorePart) + (top ? SCORE_GROUPS * sizeof(uint32_t) : 0));
 }
 
 extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_stride, uint32_t rows, uint32_t n,
@@ -974,7 +978,7 @@ extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_st
   Q8_REQUIRE(aligned_to(target, 4) && aligned_to(log_p, 4) && aligned_to(entropy, 4) && aligned_to(rank, 4) &&
                  aligned_to(top_index, 4) && aligned_to(top_log_p, 4),
              "an array is not aligned to its type");
-  Q8_REQUIRE((uint64_t)rows * score_chunks(n) <= MAX_THREADS / SCORE_THREADS, "too many rows for one call");
+  Q8_REQUIRE((uint64_t)rows * score_chunks(n) <= MAX_THREADS / WAVE, "too many rows for one call");
   if (!rows) return DEFER_GPU_OK;
   const size_t need = defer_gpu_q8_log_probs_workspace(rows, n, top);
   Q8_REQUIRE(workspace && workspace_bytes >= need, "log_probs needs a workspace of %zu bytes, got %zu", need,
@@ -982,7 +986,7 @@ extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_st
   Q8_REQUIRE(aligned16(workspace), "workspace is not 16-byte aligned");
   ScoreArgs a{x, x_stride, target, rows, n, top, score_chunks(n), scale, log_p, entropy, top_log_p, rank, top_index,
               static_cast<ScorePart*>(workspace), nullptr};
-  a.maxima = reinterpret_cast<float*>(a.part + (size_t)rows * a.chunks);
+  a.maxima = reinterpret_cast<uint32_t*>(a.part + (size_t)rows * a.chunks);
   const bool vec = ((uintptr_t)x | (uintptr_t)(x_stride * (int64_t)value_size(type))) % 16 == 0;
   const hipStream_t s = (hipStream_t)stream;
   const int e = type == DEFER_GPU_F32    ? score_launch<float>(a, vec, s)
