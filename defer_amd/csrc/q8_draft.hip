@@ -1,8 +1,7 @@
 // q8_draft.hip -- what a program that drafts tokens and verifies them needs
 // around the attention: rows normed, rotated and appended to the cache in one
 // launch, the log probabilities of given tokens, and the accepted path moved
-// together in the cache. (The attention of a tree of drafts is in q8.hip, beside
-// the one whose bits it has.)
+// together in the cache. (The attention of a tree of drafts is in q8_tree.hip.)
 #include "q8_common.h"
 
 #include <float.h>
@@ -152,6 +151,16 @@ struct Codes {
 // a row's head, 8 values each (WIDE: and the 8 from 128 on), the next one's already on its
 // way. Keys, scales and codes are those of the formula in 64 bits, as everywhere here.
 // VEC: 8 values are aligned, and so are the 8 they are paired with.
+//
+// y = x w / sqrt(mean(x^2) + eps), or x; a pair (a, b) at an angle t becomes factor (a cos t - b
+// sin t, b cos t + a sin t). Every value is read once, but for the half layout's pairs, which lie
+// 8 lanes off and come from L1: cheaper than through LDS or the lanes.
+//
+// One row, 9 + 3 heads of 64, f32: 4.4 us, the chain of lengths, page, values and a launch. 64 such
+// rows of 32 + 8 heads 6.1. 2000 rows of 32 + 8 bf16 heads of 128, 45 MB: 21 us, 2.2 TB/s, where
+// a copy of the queries and a cache write alone take 7.9 + 9.1: bound by vector instructions, the
+// 64-bit rotation and codes (without rotation 17.5), at four waves a SIMD. Two items on their way
+// instead of one cost registers (27 us), angles formed anew by each lane 48.
 template <class T, bool VEC, bool WIDE>
 __global__ __launch_bounds__(256) void k_append(AppendArgs a) {
   typedef typename Eight<T>::type t8;
@@ -162,11 +171,12 @@ __global__ __launch_bounds__(256) void k_append(AppendArgs a) {
   const uint32_t n16 = threadIdx.x % 16, quad = threadIdx.x / 16, hd = a.hd, rotated = 2 * a.half;
   constexpr uint32_t quads = 16;
   T* const out = static_cast<T*>(a.out);
-  if (seq == a.r.sequences) {  // zeros for the rows of no sequence
+  if (seq >= a.r.sequences) {  // zeros for the rows of no sequence
     const int64_t lo = span_of(a.r.row_start, a.r.kv_len, 0, a.r.rows).start;
-    const int64_t hi = max(lo, min((int64_t)a.r.row_start[seq], (int64_t)a.r.rows));
+    const int64_t hi = max(lo, min((int64_t)a.r.row_start[a.r.sequences], (int64_t)a.r.rows));
+    const uint32_t first = a.r.sequences * per * a.chunks;
     const int64_t n = a.nh * hd;
-    for (int64_t i = b * a.chunks + chunk; i < lo + ((int64_t)a.r.rows - hi); i += per * a.chunks) {
+    for (int64_t i = blockIdx.x - first; i < lo + ((int64_t)a.r.rows - hi); i += gridDim.x - first) {
       const int64_t row = i < lo ? i : hi + (i - lo);
       for (int64_t d = threadIdx.x; d < n; d += blockDim.x) out[row * a.os + d] = (T)0.0f;
     }
@@ -394,7 +404,9 @@ struct KeepArgs {
 
 // One workgroup for a sequence and head: its kept rows' codes and scales all
 // come into LDS, then go to their new places, so that the order of rows and
-// places that are both does not matter.
+// places that are both does not matter. A chain of dependent reads (lengths, entry, page,
+// codes) bounds it: 4.0 us for one sequence of 3 heads of 64, 7.4 for 64 of 8 heads of 128, of
+// whose values each byte lies in a line of its own.
 __global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
   const uint32_t g = blockIdx.x % a.p.heads, seq = blockIdx.x / a.p.heads;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
@@ -598,6 +610,12 @@ __device__ __forceinline__ float sum_of_wave(float v) { return add_step<0x143, 0
 // k_score_join reads the few groups again that can hold one. Where m is so far out that the
 // product that t comes from would be, or a logit is infinitely far below (t is -inf, the moment
 // NaN), x - m comes first.
+//
+// 2047 rows of 128,256 bf16: 92 us, 5.7 TB/s, where a plain read takes 84; with the best's maxima
+// and targets 96; f32 178 of 169. Bound by memory and, nearly as much, by vector instructions (about 150 a
+// wave's 1,024 logits). Workgroups of 8 waves joined through LDS took 117 with more instructions
+// and 130 with fewer, waiting at their barrier; 32 logits a lane 94, and 30 more in the join, whose
+// groups are larger then; workgroups that stay and fetch the next chunk ahead 137.
 template <class T, bool VEC>
 __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
   constexpr int V = 16 / sizeof(T), NV = SCORE_EACH / V;
@@ -668,6 +686,10 @@ __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
 // top-th of 64 maxima of groups), read again. Where more than LDS takes reach it, because
 // many are equal to it: those over it, and of the equal ones the first in the row.
 // Where those over it are too many still, one after the other.
+//
+// 20 best of 2047 rows of 128,256: 21 us, of one row of 49,152: 5.8; without the best 4.7. Every
+// row's workgroup is on the chip at once: a chain of reads (maxima, then the groups') and of the
+// bound's and the ranking's serial steps.
 __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) {
   constexpr uint32_t HELD = 4;  // groups' maxima that a thread keeps
   constexpr double LN2 = 0.69314718055994530942;
@@ -908,7 +930,7 @@ extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const def
   // it 4 rounds and one of the cache's heads 2 (keys, values); fewer rows take more heads, so
   // that the lanes have work. Where those would be more workgroups than the chip holds at once
   // (4 on a CU), each takes twice as many heads and forms the rows' angles for all of them:
-  // 2048 rows of 32 + 8 heads of 128 in 21 us rather than 25 (4 times as many: 23), but 11 x 33
+  // 2000 rows of 32 + 8 heads of 128 in 21 us rather than 25 (4 times as many: 23), but 11 x 33
   // normed rows of 24 + 4 heads of 96, too few for that, in 11.2 rather than 8.8.
   const uint32_t most = std::min(r.most_rows, (uint32_t)KV_RUN);
   auto power = [&](uint32_t n, uint32_t heads) {  // the largest one up to n, no more than heads need
@@ -922,9 +944,10 @@ extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const def
     a.kv_shift = power(items / 4 / most, p.heads);
     a.kv_chunks = (p.heads + (1u << a.kv_shift) - 1) >> a.kv_shift;
     a.chunks = a.kv_chunks + ((q_heads + (1u << a.q_shift) - 1) >> a.q_shift);
-    blocks = ((uint64_t)r.sequences + (clear && r.row_start)) * kv_runs(r.most_rows) * a.chunks;
+    blocks = (uint64_t)r.sequences * kv_runs(r.most_rows) * a.chunks;
     if (blocks <= 1024) break;
   }
+  if (clear && r.row_start) blocks += std::min(blocks, (uint64_t)256);  // for the rows of no sequence
   Q8_REQUIRE(blocks <= MAX_THREADS / 256, "too many rows for one call");
   const bool vec = hd % 8 == 0 && (a.interleaved ? a.half % 4 == 0 : a.half % 8 == 0) &&
                    ((uintptr_t)a.qn | (uintptr_t)a.kn | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)(q_stride * vs) |

@@ -86,7 +86,15 @@ struct Stage {
 // positions of digits times codes are exact, so that the places' order changes
 // nothing.
 //
-// SPLIT: a workgroup takes per_wave units, left in the workspace for k_attn_join.
+// SPLIT: a workgroup takes per_wave units, left in the workspace for k_tree_join.
+//
+// 7 x 25 rows over 6000 positions, 32 heads on 8 of 128: 162 us, of which the digits' products are
+// 34 at the matrix cores' rate and the codes 15; bound by vector instructions (about 275 a
+// block and tile, scores' scaling, exponentials and digits) and by 392 workgroups on 256 CUs. 32 x
+// 12 rows over 384, 32 heads on 8 of 64: 26 us, three workgroups a CU that each go through seven
+// blocks. 7 rows at 203, 9 heads on 3 of 64: 8.1 to 9.7, a chain of reads and four blocks one after
+// the other. With each wave loading the codes of its own tile, as k_attn does, the first two took 541
+// and 59 us; three blocks in LDS instead of two gave nothing, for one workgroup less a CU.
 template <int KC, int R, bool SPLIT>
 __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
@@ -494,7 +502,8 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
 }
 
 // Joins a row's units in order, as k_attn_join: one workgroup of dp lanes per row of a
-// sequence and head. What a row leaves is read before it is known how many units it has.
+// sequence and head. What a row leaves is read before it is known how many units it has: the
+// chain of reads bounds it, 5 to 6 us (8 rows of 32 heads over 8000).
 __global__ __launch_bounds__(256) void k_tree_join(AttnArgs a) {
   const uint32_t h = blockIdx.x % a.nh, j = blockIdx.x / a.nh % a.r.most_rows, seq = blockIdx.x / a.nh / a.r.most_rows;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);

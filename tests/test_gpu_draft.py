@@ -577,11 +577,10 @@ def check_scores(x, target, top, scale=1.0, x_gpu=None):
     log_p, ent, rank, order, top_lp, mean, square = ref_scores(x, t, top, scale)
     assert [a.dtype for a in got] == [torch.float32] * 2 + [torch.int32] * 2 + [torch.float32]
     assert torch.equal(got.rank.cpu(), rank.int()) and torch.equal(got.top_index.cpu(), order.int())
-    # A term e = exp(scale d), d = x - max: d, scale * log2(e) (twice), their product: half a step each, 4 u |scale d|
-    # of e; the exponential a step, 2 u. The sum: 16 terms a thread, 6 steps a wave, then a factor of each wave
-    # (whose d is the rest of the terms' d) and 4 steps: under 37 u. So the sum's
-    # logarithm is off by u (4 mean |scale d| + 39); chunks join in 64 bits. The moment's terms have
-    # one product more and d itself, its sum as many roundings.
+    # A term e = exp(t), t = scale d, d = x - max: scale * log2(e) (twice) and the fused product, or d and a product:
+    # half a step each, 4 u |t| of e; the exponential a step, 2 u. The sum: 16 terms a lane, 6 steps a wave, the
+    # power it is taken back by: under 37 u. So the sum's logarithm is off by u (4 mean |t| + 39); waves join in
+    # 64 bits. The moment's terms have one product more and t itself, its sum as many roundings.
     u = 2.0 ** -24
     off = u * (4 * mean + 39)
     assert (got.entropy.cpu().double() - ent).abs().le(off * (1 + mean) + u * (4 * square + 42 * mean) + 1.01 * u * ent).all()
