@@ -91,12 +91,12 @@ struct Stage {
 // 7 x 25 rows over 6000 positions, 32 heads on 8 of 128: 162 us, of which the digits' products are
 // 34 at the matrix cores' rate and the codes 15; bound by vector instructions (about 275 a
 // block and tile, scores' scaling, exponentials and digits) and by 392 workgroups on 256 CUs. 32 x
-// 12 rows over 384, 32 heads on 8 of 64: 26 us, three workgroups a CU that each go through seven
-// blocks. 7 rows at 203, 9 heads on 3 of 64: 8.1 to 9.7, a chain of reads and four blocks one after
+// 12 rows over 384, 32 heads on 8 of 64, some places hidden: 23 us, three workgroups a CU that each go
+// through seven blocks (26 with each lane reading its four places' marks when it needs them). 7 rows at 203, 9 heads on 3 of 64: 8.1 to 9.7, a chain of reads and four blocks one after
 // the other. With each wave loading the codes of its own tile, as k_attn does, the first two took 541
 // and 59 us; three blocks in LDS instead of two gave nothing, for one workgroup less a CU.
 template <int KC, int R, bool SPLIT>
-__global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnArgs a) {
+__global__ __launch_bounds__(64 * TREE_WAVES, KC == 1 ? 3 : KC == 2 ? 2 : 1) void k_tree(AttnArgs a) {
   constexpr int DT = 4 * KC, DP = 64 * KC;
   typedef Stage<KC> St;
   extern __shared__ __align__(16) uint8_t lds[];  // two blocks' codes, then each wave's probabilities and path
@@ -246,15 +246,11 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
       __builtin_amdgcn_wave_barrier();
     };
 
-    // A block of the history. WHOLE: every row sees all of it.
-    auto block = [&](auto whole, int b, const uint8_t* codes) {
+    // A block of the history, its hidden places. WHOLE: every row sees all of it.
+    auto block = [&](auto whole, int b, uint64_t hide, const uint8_t* codes) {
       constexpr bool WHOLE = decltype(whole)::value;
       const int tb = b * PAGE + 4 * n16;
-      bool hide[4] = {false, false, false, false};
-      if (!WHOLE && hid) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) hide[j] = (uint32_t)(tb + j) < a.hidden_len && hid[tb + j] != 0;
-      }
+      const uint32_t hides = (uint32_t)(hide >> (4 * n16));
       const v4f ks = *reinterpret_cast<const v4f*>(codes + St::SCALES + 16 * n16);
       const v4f vs = *reinterpret_cast<const v4f*>(codes + St::SCALES + PAGE * 4 + 16 * n16);
       float vbad = 0.0f;
@@ -272,7 +268,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
         bool see[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          see[j] = WHOLE || (tb + j <= ps[r] && !hide[j]);
+          see[j] = WHOLE || (tb + j <= ps[r] && !(hides >> j & 1));
           s[j] = see[j] ? s[j] : -INFINITY;
         }
         uint32_t y[4], by_digit[4];
@@ -299,9 +295,9 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
     };
 
     // A block of a path's positions, around the history's end or behind it. The nodes
-    // on it are in this place's page or the next (a tree has no more than 64 rows).
-    // all: no place is hidden or without a page.
-    auto path_block = [&](int b, int page, int page_behind, bool all, const uint8_t* codes) {
+    // on it are in this place's page or the next (a tree has no more than 64 rows), whose
+    // hidden places are given. all: no place is hidden or without a page.
+    auto path_block = [&](int b, int page, int page_behind, uint64_t hide, uint64_t hide_behind, bool all, const uint8_t* codes) {
       float* const sl = reinterpret_cast<float*>(pl + R * 16 * P_ROW) + quad * PAGE;  // this quad's pair, of R
       constexpr int EACH = 4 * PAGE, VALUE = EACH, MARK = 2 * EACH, OF_R = 3 * EACH;
       uint32_t* const ml = reinterpret_cast<uint32_t*>(sl + MARK);
@@ -337,8 +333,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
         for (int j = 0; j < 4; ++j) {
           const int node = node0 + j, t = node + history, d = __shfl(depth, node & (WAVE - 1));
           const int to = (node < 0 ? t : history + d) - b * PAGE;
-          bool is = node < rows && to >= 0 && to < PAGE;
-          if (hid && is) is = !((uint32_t)t < a.hidden_len && hid[t] != 0);
+          const bool is = node < rows && to >= 0 && to < PAGE && !((pb ? hide_behind : hide) >> (4 * n16 + j) & 1);
           at[pb] |= (uint32_t)(to & (PAGE - 1)) << (8 * j);
           on |= (uint32_t)is << j;
         }
@@ -432,7 +427,13 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
     int u = u_first;
     const int blocks = SPLIT ? min(all_blocks, (u + (int)a.per_wave) * bpu) : all_blocks;
     const int last_place = (history + rows - 1) / PAGE;  // the last row's page
+    // whether a block's place is hidden, one a lane: on its way with the block before
+    auto hidden_at = [&](int b) -> uint32_t {
+      const int64_t t = (int64_t)b * PAGE + lane;
+      return hid && t < a.hidden_len ? hid[t] : 0;
+    };
     int b = u * bpu, page = b < blocks ? page_at(b) : -1;
+    uint32_t hidden = hidden_at(b);
     if (ul != ul_first) {
       meet();  // every wave is done with the codes of the rows before
       if (page >= 0) copy(page, 0);
@@ -441,16 +442,19 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
       meet();
       const int next = b + 1 < blocks ? page_at(b + 1) : -1;
       if (next >= 0) copy(next, buf ^ 1);
+      const uint32_t hidden_next = hidden_at(b + 1);
       const uint8_t* const codes = lds + buf * St::BYTES;
       if (b * PAGE <= pmax) {
+        const uint64_t hide = __ballot(hidden != 0);
         if (b >= first_path) {
           const int behind = b < last_place ? (b + 1 < blocks ? next : page_at(b + 1)) : -1;
-          path_block(b, page, behind, !hid && page >= 0 && (behind >= 0 || b >= last_place), codes);
+          const uint64_t hide_behind = b < last_place ? __ballot(hidden_next != 0) : 0;
+          path_block(b, page, behind, hide, hide_behind, !(hide | hide_behind) && page >= 0 && (behind >= 0 || b >= last_place), codes);
         } else if (page >= 0) {
-          if (!hid && b * PAGE + PAGE - 1 <= pmin)
-            block(std::true_type(), b, codes);
+          if (!hide && b * PAGE + PAGE - 1 <= pmin)
+            block(std::true_type(), b, hide, codes);
           else
-            block(std::false_type(), b, codes);
+            block(std::false_type(), b, hide, codes);
         }
       }
       if (b + 1 == blocks || (b + 1) % bpu == 0) {  // the unit ends
@@ -481,6 +485,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC <= 2 ? 2 : 1) void k_tree(AttnA
         ++u;
       }
       page = next;
+      hidden = hidden_next;
     }
     if (!SPLIT) {
 #pragma unroll

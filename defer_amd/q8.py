@@ -243,7 +243,7 @@ def kv_keep(pages: Pages, kv_len: torch.Tensor, row_start: Optional[torch.Tensor
 
 
 def log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0) -> LogProbs:
-    """Log probabilities under softmax(scale * logits) [rows, n] of ``target`` [rows] int32, and of the ``top`` <= 32
+    """Log probabilities under softmax(scale * logits) [rows, n], 1e-30 <= scale <= 1e30, of ``target`` [rows] int32, and of the ``top`` <= 32
     likeliest (the lower index first among equals). A target outside [0, n) has NaN and rank -1; a row with a NaN or
     +inf, or nothing over -inf, NaN and -1 throughout."""
     return LogProbs(*_native().log_probs(logits, target, top, scale))
