@@ -690,7 +690,10 @@ __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
 // 20 best of 2047 rows of 128,256: 21 us, of one row of 49,152: 5.8; without the best 4.7. Every
 // row's workgroup is on the chip at once: a chain of reads (maxima, then the groups') and of the
 // bound's and the ranking's serial steps.
-__global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) {
+template <class T, bool VEC>
+__global__ __launch_bounds__(256) void k_score_join(ScoreArgs a) {
+  constexpr uint32_t V = 16 / sizeof(T), NV = SCORE_EACH / V;
+  typedef T vt __attribute__((ext_vector_type(V)));
   constexpr uint32_t HELD = 4;  // groups' maxima that a thread keeps
   constexpr double LN2 = 0.69314718055994530942;
   __shared__ uint64_t s_key[SCORE_FEW], s_wave[4];
@@ -701,7 +704,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
   __shared__ float s_top;
   static_assert(MAX_SCORE / SCORE_CHUNK * SCORE_GROUPS <= 0x10000 && MAX_TOP <= WAVE, "a group's number in 16 bits");
   const uint32_t row = blockIdx.x, lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const int64_t x0 = (int64_t)row * a.xs;
+  const T* const x = static_cast<const T*>(a.x) + (int64_t)row * a.xs;
   const uint32_t groups = a.chunks * SCORE_GROUPS;
   const uint32_t* maxima = a.maxima + (size_t)row * groups;
   auto group_max = [&](uint32_t i) { return i < groups ? maxima[i] : 0u; };
@@ -748,7 +751,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
       const bool none = !(sum >= 1.0);  // a NaN, an infinity, or nothing over -inf: no distribution
       const bool has = target >= 0 && (uint32_t)target < a.n && !none;
       const double scale = (double)a.scale, log_sum = none ? (double)nan : log(sum);
-      a.log_p[row] = has ? (float)(scale * ((double)load_value(a.x, x0 + target, type) - (double)top) - log_sum) : nan;
+      a.log_p[row] = has ? (float)(scale * ((double)(float)x[target] - (double)top) - log_sum) : nan;
       a.entropy[row] = (float)(log_sum - moment / sum);
       a.rank[row] = has ? (int32_t)above : -1;
       s_sum = log_sum;
@@ -758,11 +761,6 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
   if (!a.top) return;
   __syncthreads();
   const uint32_t o = max(max(s_max[0][lane], s_max[1][lane]), max(s_max[2][lane], s_max[3][lane]));
-  // columns of a group: of each 16-byte vector of a thread's, a run
-  const uint32_t vector = type == DEFER_GPU_F32 ? 4 : 8, run = SCORE_GROUP * vector;
-  auto column = [&](uint32_t group, uint32_t e) {
-    return group / SCORE_GROUPS * SCORE_CHUNK + e / run * (WAVE * vector) + group % SCORE_GROUPS * run + e % run;
-  };
   // Keys of the logits that reach `from` (counts are 0); returns how many there are.
   auto gather = [&](uint32_t from) {
     auto list = [&](uint32_t i, uint32_t m) {
@@ -778,22 +776,30 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
     const uint32_t n = s_groups;
     if (n > SCORE_LIST) return SCORE_FEW + 1;
     for (uint32_t i = threadIdx.x / 16; i < n; i += 16) {  // 16 lanes a group
-      const uint32_t group = s_list[i];
-      constexpr uint32_t EACH = SCORE_GROUP * SCORE_EACH / 16;
-      float v[EACH];
+      const uint32_t group = s_list[i], l = lane % 16;
+      const uint32_t c0 = group / SCORE_GROUPS * SCORE_CHUNK + l / 8 * (WAVE * V) + (group % SCORE_GROUPS * SCORE_GROUP + l % 8) * V;
+      vt w[NV / 2];
 #pragma unroll
-      for (uint32_t s = 0; s < EACH; ++s) {
-        const uint32_t c = column(group, 16 * s + lane % 16);
-        v[s] = c < a.n ? load_value(a.x, x0 + c, type) : -INFINITY;
-      }
+      for (uint32_t v = 0; v < NV / 2; ++v) {
+        const uint32_t c = c0 + v * (2 * WAVE * V);
+        if (VEC && c + V <= a.n) {
+          w[v] = *reinterpret_cast<const vt*>(x + c);
+        } else {
 #pragma unroll
-      for (uint32_t s = 0; s < EACH; ++s) {
-        const uint32_t c = column(group, 16 * s + lane % 16);
-        if (c < a.n && score_order(v[s]) >= from) {
-          const uint32_t at = atomicAdd(&s_count, 1u);
-          if (at < SCORE_FEW) s_key[at] = score_key(v[s], c);
+          for (uint32_t e = 0; e < V; ++e) w[v][e] = c + e < a.n ? x[c + e] : (T)-INFINITY;
         }
       }
+#pragma unroll
+      for (uint32_t v = 0; v < NV / 2; ++v)
+#pragma unroll
+        for (uint32_t e = 0; e < V; ++e) {
+          const uint32_t c = c0 + v * (2 * WAVE * V) + e;
+          const float value = (float)w[v][e];
+          if (c < a.n && score_order(value) >= from) {
+            const uint32_t at = atomicAdd(&s_count, 1u);
+            if (at < SCORE_FEW) s_key[at] = score_key(value, c);
+          }
+        }
     }
     __syncthreads();
     return s_count;
@@ -812,7 +818,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
       if (wave == 0)
         for (uint32_t c0 = 0; c0 < a.n && count < a.top; c0 += WAVE) {
           const uint32_t c = c0 + lane;
-          const float v = c < a.n ? load_value(a.x, x0 + c, type) : 0.0f;
+          const float v = c < a.n ? (float)x[c] : 0.0f;
           const bool is = c < a.n && v == equal;
           const uint64_t mask = __ballot(is);
           const uint32_t at = count + (uint32_t)__popcll(mask & ((1ull << lane) - 1));
@@ -825,7 +831,7 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
       for (uint32_t t = 0; t < a.top; ++t) {
         uint64_t k = 0;
         for (uint32_t c = threadIdx.x; c < a.n; c += 256) {
-          const uint64_t key = score_key(load_value(a.x, x0 + c, type), c);
+          const uint64_t key = score_key((float)x[c], c);
           k = key < last && key > k ? key : k;
         }
         for (int s = 32; s > 0; s >>= 1) {
@@ -861,7 +867,8 @@ __global__ __launch_bounds__(256) void k_score_join(ScoreArgs a, uint32_t type) 
 template <class T>
 int score_launch(const ScoreArgs& a, bool vec, hipStream_t s) {
   const uint32_t blocks = (a.rows * a.chunks + SCORE_WAVES - 1) / SCORE_WAVES;
-  return launch(vec ? k_score<T, true> : k_score<T, false>, blocks, SCORE_THREADS, 0, s, a);
+  const int rc = launch(vec ? k_score<T, true> : k_score<T, false>, blocks, SCORE_THREADS, 0, s, a);
+  return rc ? rc : launch(vec ? k_score_join<T, true> : k_score_join<T, false>, a.rows, 256, 0, s, a);
 }
 
 uint32_t score_chunks(uint32_t n) { return (n + SCORE_CHUNK - 1) / SCORE_CHUNK; }
@@ -1012,8 +1019,7 @@ extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_st
   a.maxima = reinterpret_cast<uint32_t*>(a.part + (size_t)rows * a.chunks);
   const bool vec = ((uintptr_t)x | (uintptr_t)(x_stride * (int64_t)value_size(type))) % 16 == 0;
   const hipStream_t s = (hipStream_t)stream;
-  const int e = type == DEFER_GPU_F32    ? score_launch<float>(a, vec, s)
-                : type == DEFER_GPU_BF16 ? score_launch<__bf16>(a, vec, s)
-                                         : score_launch<_Float16>(a, vec, s);
-  return e ? e : launch(k_score_join, rows, 256, 0, s, a, type);
+  return type == DEFER_GPU_F32    ? score_launch<float>(a, vec, s)
+         : type == DEFER_GPU_BF16 ? score_launch<__bf16>(a, vec, s)
+                                  : score_launch<_Float16>(a, vec, s);
 }
