@@ -154,7 +154,7 @@ struct Codes {
 //
 // y = x w / sqrt(mean(x^2) + eps), or x; a pair (a, b) at an angle t becomes factor (a cos t - b
 // sin t, b cos t + a sin t). Every value is read once, but for the half layout's pairs, which lie
-// 8 lanes off and come from L1: cheaper than through LDS or the lanes.
+// 8 lanes off and come from L1 the second time.
 //
 // One row, 9 + 3 heads of 64, f32: 4.4 us, the chain of lengths, page, values and a launch. 64 such
 // rows of 32 + 8 heads 6.1. 2000 rows of 32 + 8 bf16 heads of 128, 45 MB: 21 us, 2.2 TB/s, where

@@ -103,8 +103,8 @@ def test_keep_refuses():
 def test_log_probs_refuses():
     ok = [0, P, 100, 4, 100, P, 1.0, 5, P, P, P, P, P, P, 1 << 20, None]
     for i, bad in ((0, 3), (1, None), (1, P + 2), (2, 99), (4, 0), (4, (1 << 20) + 1), (5, P + 2), (6, 0.0), (6, -1.0), (6, math.nan),
-                   (6, math.inf), (6, 9e-31), (6, 2e30), (7, 33), (7, 101), (8, None), (9, None), (10, None), (11, None), (12, None), (8, P + 1), (11, P + 2),
-                   (13, None), (13, P + 8), (14, 10)):
+                   (6, math.inf), (6, 9e-31), (6, 2e30), (7, 33), (7, 101), (8, None), (9, None), (10, None), (11, None), (12, None),
+                   (8, P + 1), (11, P + 2), (13, None), (13, P + 8), (14, 10)):
         refused("log_probs", *[bad if j == i else a for j, a in enumerate(ok)])
     assert "too many" in refused("log_probs", 0, P, 1 << 20, 70000, 1 << 20, None, 1.0, 0, P, P, P, None, None, P, 1 << 40, None)
     assert call("log_probs", 0, None, 100, 0, 100, None, 1.0, 5, None, None, None, None, None, None, 0, None) == G.OK
