@@ -907,8 +907,15 @@ extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const def
   Q8_REQUIRE(fabsf(rotary->factor) < INFINITY, "factor %g", (double)rotary->factor);
   const int64_t vs = (int64_t)value_size(type), row = nq * vs;
   Q8_REQUIRE(!overlap(out, out_stride * vs, r.rows, q, q_stride * vs, r.rows, row), "out overlaps q");
-  Q8_REQUIRE(!overlap(out, out_stride * vs, r.rows, row, k, k_stride * vs, r.rows, nkv * vs), "out overlaps k");
-  Q8_REQUIRE(!overlap(out, out_stride * vs, r.rows, row, v, v_stride * vs, r.rows, nkv * vs), "out overlaps v");
+  // Of q a workgroup reads what it writes itself; all else is read by others while this one writes.
+  auto shares = [&](const void* in, int64_t stride, uint32_t n, int64_t bytes) {
+    return in && share(out, out_stride * vs, r.rows, row, in, stride, n, bytes);
+  };
+  Q8_REQUIRE(!shares(k, k_stride * vs, r.rows, nkv * vs), "out overlaps k");
+  Q8_REQUIRE(!shares(v, v_stride * vs, r.rows, nkv * vs), "out overlaps v");
+  Q8_REQUIRE(!shares(rotary->q_norm, 0, 1, hd * vs) && !shares(rotary->k_norm, 0, 1, hd * vs), "out overlaps a norm's weight");
+  Q8_REQUIRE(!shares(rotary->position, 0, 1, (int64_t)r.rows * 4), "out overlaps position");
+  Q8_REQUIRE(!rotary->rotated || !shares(rotary->freq, 0, 1, rotary->rotated * 4), "out overlaps freq");
   if (!r.rows) return DEFER_GPU_OK;
   const hipStream_t s = (hipStream_t)stream;
   if (!r.sequences || !r.most_rows)

@@ -63,16 +63,14 @@ Q8_HD int most_units(int64_t len) {
   return n < 1 ? 1 : n > MAX_UNITS ? MAX_UNITS : (int)n;
 }
 
-// Whether two sets of rows share memory other than row by row, each row the
-// same in both: rows of ar and br bytes from a and b on, as and bs bytes apart
-// (at least their length; any number where there is one row).
-inline bool overlap(const void* a, int64_t as, uint32_t a_rows, int64_t ar, const void* b, int64_t bs, uint32_t b_rows, int64_t br) {
+// Whether two sets of rows share a byte: rows of ar and br bytes from a and b on,
+// as and bs bytes apart (at least their length; any number where there is one row).
+inline bool share(const void* a, int64_t as, uint32_t a_rows, int64_t ar, const void* b, int64_t bs, uint32_t b_rows, int64_t br) {
   const int64_t x = (int64_t)(uintptr_t)a, y = (int64_t)(uintptr_t)b;
   const int64_t na = a_rows, nb = b_rows;
   if (!na || !nb) return false;
   if (na == 1) as = ar;
   if (nb == 1) bs = br;
-  if (x == y && na == nb && as == bs && ar == br) return false;
   if (x + (na - 1) * as + ar <= y || y + (nb - 1) * bs + br <= x) return false;
   if (as == bs) {  // columns of one matrix: the later one's first row lies between two of the other's
     const int64_t d = x < y ? y - x : x - y, n = x < y ? na : nb, k = d / as, left = d % as;
@@ -89,6 +87,11 @@ inline bool overlap(const void* a, int64_t as, uint32_t a_rows, int64_t ar, cons
       return true;
   }
   return false;
+}
+// ... other than row by row, each row the same in both.
+inline bool overlap(const void* a, int64_t as, uint32_t a_rows, int64_t ar, const void* b, int64_t bs, uint32_t b_rows, int64_t br) {
+  const bool same = a == b && a_rows == b_rows && ar == br && (as == bs || a_rows == 1);
+  return !same && share(a, as, a_rows, ar, b, bs, b_rows, br);
 }
 inline bool overlap(const void* a, int64_t as, uint32_t a_rows, const void* b, int64_t bs, uint32_t b_rows, int64_t row) {
   return overlap(a, as, a_rows, row, b, bs, b_rows, row);

@@ -116,11 +116,13 @@ int64_t row_stride(const Tensor& t, const char* what, at::Device dev, ScalarType
   return t.stride(0);
 }
 
-// Rows that a call writes lie apart from those it reads, or are the same rows.
-void apart(const Tensor& out, int64_t os, const Tensor& in, int64_t is, const char* what) {
+// Rows that a call writes lie apart from those it reads, or (own) are the same rows.
+void apart(const Tensor& out, int64_t os, const Tensor& in, int64_t is, const char* what, bool own = true) {
   const int64_t rows = out.size(0), v = out.element_size();
   const int64_t n = rows ? out.numel() / rows * v : 0, m = rows ? in.numel() / rows * v : 0;
-  if (rows <= 0xffffffffll && q8::overlap(out.data_ptr(), os * v, (uint32_t)rows, n, in.data_ptr(), is * v, (uint32_t)rows, m))
+  const void *const o = out.data_ptr(), *const i = in.data_ptr();
+  const uint32_t r = (uint32_t)rows;
+  if (rows <= 0xffffffffll && (own ? q8::overlap(o, os * v, r, n, i, is * v, r, m) : q8::share(o, os * v, r, n, i, is * v, r, m)))
     throw Refused(std::string("out overlaps ") + what);
 }
 
@@ -431,8 +433,8 @@ PyObject* kv_append(PyObject* const* a) {
     out = tensor(a[14], "out");
     os = row_stride(out, "out", dev, type, q.sizes());
     apart(out, os, q, qs, "q");
-    apart(out, os, k, ks, "k");
-    apart(out, os, v, vs, "v");
+    apart(out, os, k, ks, "k", false);
+    apart(out, os, v, vs, "v", false);
   }
   call(dev, [&](void* s) {
     return lib.kv_append(&c.p, &c.r, ty, &t, q.data_ptr(), qs, heads, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,

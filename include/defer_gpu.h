@@ -387,8 +387,8 @@ typedef struct defer_gpu_q8_rotary {
 
 /* out = q [rows, q_heads, head_dim] turned and rounded to its type; k, turned,
  * and v [rows, heads, head_dim] quantised into the cache as defer_gpu_q8_kv_write
- * does. out may be q itself; it shares no memory with k and v. Rows before position
- * 0 have an out, too. clear != 0: out is zeros for rows of no sequence. */
+ * does. out may be q itself; it shares no memory with k, v and what rotary names. Rows
+ * before position 0 have an out, too. clear != 0: out is zeros for rows of no sequence. */
 int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows, uint32_t type,
                            const defer_gpu_q8_rotary* rotary, const void* q, int64_t q_stride,
                            uint32_t q_heads, const void* k, int64_t k_stride, const void* v,
