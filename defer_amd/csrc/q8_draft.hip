@@ -410,9 +410,8 @@ struct KeepArgs {
 __global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
   const uint32_t g = blockIdx.x % a.p.heads, seq = blockIdx.x / a.p.heads;
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
-  const int n = min(max(a.kept[seq], 0), sp.n);  // rows that stay
-  if (g == 0 && threadIdx.x == 0) a.kv_len_out[seq] = (int32_t)max(sp.pos(n), (int64_t)INT32_MIN);
-  const int move = min(n, (int)a.r.most_rows);
+  const int move = min(min(max(a.kept[seq], 0), sp.n), (int)a.r.most_rows);  // rows that stay
+  if (g == 0 && threadIdx.x == 0) a.kv_len_out[seq] = (int32_t)max(sp.pos(move), (int64_t)INT32_MIN);
   __shared__ __align__(16) int8_t keys[MAX_TREE * 256], values[MAX_TREE * 256];
   __shared__ float scales[2][MAX_TREE];
   __shared__ int64_t from[MAX_TREE], to[MAX_TREE];  // places: page * 64 + position, or -1

@@ -227,10 +227,16 @@ struct Cache {
     r.rows = u32(n, "rows");
     r.most_rows = (uint32_t)most;
   }
-  // ... of which a sequence has at most 64: without most_rows, no more of them
+  // ... of which a sequence has at most 64. Without most_rows there are no more rows than
+  // the sequences may have: else one has too many, or some are of no sequence, which a call has to say.
   void drafted(PyObject* kv_len, PyObject* row_start, int64_t n, PyObject* most_rows, at::Device dev) {
     rows(kv_len, row_start, n, most_rows, dev);
-    if (most_rows == Py_None) r.most_rows = std::min(r.most_rows, q8::MAX_TREE);
+    if (most_rows == Py_None) {
+      if (r.sequences && n > (int64_t)q8::MAX_TREE * r.sequences)
+        throw Refused(std::to_string(n) + " rows of " + std::to_string(r.sequences) + " sequences without most_rows: at most " +
+                      std::to_string(q8::MAX_TREE) + " drafted rows of a sequence");
+      r.most_rows = std::min(r.most_rows, q8::MAX_TREE);
+    }
     if (r.most_rows > q8::MAX_TREE)
       throw Refused("most_rows " + std::to_string(r.most_rows) + ": at most " + std::to_string(q8::MAX_TREE) + " drafted rows of a sequence");
   }

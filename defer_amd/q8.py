@@ -230,7 +230,8 @@ def tree_attention(q: torch.Tensor, pages: Pages, parent: torch.Tensor, kv_len: 
     """attention of rows that are nodes of a tree, at most 64 a sequence: ``parent`` [rows] int32 is the number of a row's
     parent among its sequence's rows, a lower one than its own, or -1: it follows the history. A row sees the history,
     the rows above it and itself, with the bits of attention over a cache that holds this path alone. kv_len counts all
-    of a sequence's rows; ``hidden`` goes by places, as written."""
+    of a sequence's rows; ``hidden`` goes by places, as written. ``most_rows``: 64 without, where there are no more than
+    64 rows a sequence (more, rows of no sequence among them, want it given); rows behind it are as rows of no sequence."""
     return _native().tree_attention(parent, q, pages, kv_len, row_start, most_rows, most_len, scale, hidden, out)
 
 
@@ -238,7 +239,8 @@ def kv_keep(pages: Pages, kv_len: torch.Tensor, row_start: Optional[torch.Tensor
             most_rows: Optional[int] = None) -> torch.Tensor:
     """Moves drafted rows (at most 64 a sequence) together: the keep[row_start[i] + t]-th row of sequence i to the place
     of its t-th, for t < kept[i], and returns the lengths that the sequences then have (int32): the rest is as if it
-    had never been written. ``keep`` [rows] and ``kept`` [sequences] int32."""
+    had never been written. ``keep`` [rows] and ``kept`` [sequences] int32. ``most_rows`` as for tree_attention: no more
+    rows of a sequence are kept."""
     return _native().kv_keep(pages, kv_len, row_start, keep, kept, most_rows)
 
 

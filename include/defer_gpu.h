@@ -402,7 +402,8 @@ int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const defer_gpu_q8_r
  * history, the rows above it and itself, at the positions that they would have
  * in a cache with this path alone, and has the bits of attention over that. hidden
  * goes by places, as written. A sequence of fewer positions than rows attends to
- * nothing. */
+ * nothing. Where a sequence has more rows than most_rows all the same, those behind
+ * are as rows of no sequence. */
 size_t defer_gpu_q8_tree_attention_workspace(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
                                              uint32_t q_heads, uint32_t most_len);
 int defer_gpu_q8_tree_attention(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
@@ -415,7 +416,7 @@ int defer_gpu_q8_tree_attention(const defer_gpu_q8_pages* pages, const defer_gpu
 /* Moves rows of each sequence together: of its n rows (at most 64) the keep[row_start[i] + t]-th,
  * for t < kept[i], to the place of the t-th, as if the others had never been written.
  * An entry outside [0, n) leaves its place as it is. kv_len_out[i] = kv_len[i] - n +
- * min(kept[i], n), apart from all inputs. No two sequences of a call have a page
+ * min(kept[i], n, most_rows), apart from all inputs. No two sequences of a call have a page
  * of these rows in common. */
 int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
                          const int32_t* keep, const int32_t* kept, int32_t* kv_len_out, void* stream);
