@@ -1015,7 +1015,7 @@ extern "C" int defer_gpu_q8_log_probs(uint32_t type, const void* x, int64_t x_st
   Q8_REQUIRE(aligned_to(target, 4) && aligned_to(log_p, 4) && aligned_to(entropy, 4) && aligned_to(rank, 4) &&
                  aligned_to(top_index, 4) && aligned_to(top_log_p, 4),
              "an array is not aligned to its type");
-  Q8_REQUIRE((uint64_t)rows * score_chunks(n) <= MAX_THREADS / WAVE, "too many rows for one call");
+  Q8_REQUIRE((uint64_t)rows * score_chunks(n) <= MAX_THREADS / SCORE_THREADS * SCORE_WAVES, "too many rows for one call");
   if (!rows) return DEFER_GPU_OK;
   const size_t need = defer_gpu_q8_log_probs_workspace(rows, n, top);
   Q8_REQUIRE(workspace && workspace_bytes >= need, "log_probs needs a workspace of %zu bytes, got %zu", need,
