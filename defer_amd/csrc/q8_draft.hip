@@ -61,8 +61,8 @@ __device__ __forceinline__ double row_sum64(double v) {
 
 // (cos, sin) of position times frequency, in 64 bits: as turns, of which the
 // whole ones go, then the quarters; what is left is within an eighth of a turn,
-// where the series to x^14 and x^15 are off by less than 2^-44. The turns are
-// products in two parts each, so that no position is too far.
+// where the series to x^15 and x^16 are off by less than 2^-54 (their next terms,
+// x^17 / 17! and x^18 / 18!). The turns are products in two parts each, so that no position is too far.
 __device__ __forceinline__ double2 turn(int pos, double freq) {
   constexpr double PER = 0.15915494309189533577, LEFT = -9.839338337591251e-18;  // 1 / (2 pi) in two parts
   const double p = (double)pos, f = freq * PER, fl = fma(freq, PER, -f) + freq * LEFT;
@@ -70,7 +70,9 @@ __device__ __forceinline__ double2 turn(int pos, double freq) {
   double t = (h - rint(h)) + (fma(p, f, -h) + p * fl);
   t -= rint(t);
   const double quarter = rint(4.0 * t), x = (t - 0.25 * quarter) * 6.28318530717958647693, x2 = x * x;
-  double s = 1.0 / 6227020800.0, c = -1.0 / 87178291200.0;
+  double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;
+  s = fma(s, x2, 1.0 / 6227020800.0);
+  c = fma(c, x2, -1.0 / 87178291200.0);
   s = fma(s, x2, -1.0 / 39916800.0);
   s = fma(s, x2, 1.0 / 362880.0);
   s = fma(s, x2, -1.0 / 5040.0);
