@@ -120,7 +120,7 @@ __global__ __launch_bounds__(64 * TREE_WAVES, KC == 1 ? 3 : KC == 2 ? 2 : 1) voi
   }
   const Span sp = span_of(a.r.row_start, a.r.kv_len, seq, a.r.rows);
   const int rows = min(sp.n, (int)a.r.most_rows);  // (at most MAX_TREE)
-  if (a.clear && item == 0)  // rows behind the most are as rows of no sequence
+  if (__builtin_expect(sp.n > rows, 0) && a.clear && item == 0)  // rows behind the most are as rows of no sequence
     for (int j = rows + (int)wave; j < sp.n; j += TREE_WAVES)
       for (uint32_t d = lane; d < a.group * a.hd; d += WAVE)
         store_value(a.out, (int64_t)(sp.start + j) * a.os + (int64_t)g * a.group * a.hd + d, a.type, 0.0f);
