@@ -87,10 +87,11 @@ __device__ __forceinline__ float scale_of(double top, bool nan) {
   const float s = top < TINY ? 0.0f : (float)(top / 127.0);
   return nan || !(s < INFINITY) ? __builtin_nanf("") : s;
 }
-// The code of x at a scale, rint(x / s) with ties to even. x and s are 24-bit
-// values: what the product with 1 / s leaves is exact in 64 bits and says
-// where the quotient is on the wrong side of a half (a division takes three
-// times the instructions). `scale` is 0 or NaN for a row of zeros.
+// The code of x, of 64 bits, at a scale s of 32: rint(x / s) with ties to even. The
+// code times s is exact in 64 bits and, but for code 0, within a factor of two
+// of x, so what it leaves of x is exact, too, and says where the product with
+// 1 / s is on the wrong side of a half (a division takes three times the
+// instructions). `scale` is 0 or NaN for a row of zeros.
 struct Coder {
   double s, r;
   __device__ __forceinline__ explicit Coder(float scale) : s(scale > 0.0f ? (double)scale : 0.0), r(s > 0.0 ? 1.0 / s : 0.0) {}

@@ -159,10 +159,11 @@ struct Codes {
 // 8 lanes off and come from L1 the second time.
 //
 // One row, 9 + 3 heads of 64, f32: 4.4 us, the chain of lengths, page, values and a launch. 64 such
-// rows of 32 + 8 heads 6.1. 2000 rows of 32 + 8 bf16 heads of 128, 45 MB: 21 us, 2.2 TB/s, where
-// a copy of the queries and a cache write alone take 7.9 + 9.1: bound by vector instructions, the
-// 64-bit rotation and codes (without rotation 17.5), at four waves a SIMD. Two items on their way
-// instead of one cost registers (27 us), angles formed anew by each lane 48.
+// rows of 32 + 8 heads 6.2. 2000 rows of 32 + 8 bf16 heads of 128, 45 MB: 21.6 us, 2.1 TB/s, where
+// a copy of the queries and a cache write alone take 7.9 + 9.1. The rotation is about 4 of them (without
+// it 17.5); what bounds the rest is not measured. The half layout reads every rotated value twice,
+// and the queries' workgroups hold the registers of the codes' path, four waves a SIMD. Two items on their
+// way instead of one cost registers (27 us), angles formed anew by each lane 48.
 template <class T, bool VEC, bool WIDE>
 __global__ __launch_bounds__(256) void k_append(AppendArgs a) {
   typedef typename Eight<T>::type t8;
@@ -407,7 +408,7 @@ struct KeepArgs {
 // One workgroup for a sequence and head: its kept rows' codes and scales all
 // come into LDS, then go to their new places, so that the order of rows and
 // places that are both does not matter. A chain of dependent reads (lengths, entry, page,
-// codes) bounds it: 4.0 us for one sequence of 3 heads of 64, 7.4 for 64 of 8 heads of 128, of
+// codes) bounds it: 4.1 us for one sequence of 3 heads of 64, 7.2 for 64 of 8 heads of 128, of
 // whose values each byte lies in a line of its own.
 __global__ __launch_bounds__(256) void k_keep(KeepArgs a) {
   const uint32_t g = blockIdx.x % a.p.heads, seq = blockIdx.x / a.p.heads;
@@ -613,7 +614,9 @@ __device__ __forceinline__ float sum_of_wave(float v) { return add_step<0x143, 0
 // NaN), x - m comes first.
 //
 // 2047 rows of 128,256 bf16: 92 us, 5.7 TB/s, where a plain read takes 84; with the best's maxima
-// and targets 96; f32 178 of 169. Bound by memory and, nearly as much, by vector instructions (about 150 a
+// and targets 98; f32 178 of 169. Rows that are not aligned to 16 bytes are read by the logit, each lane's
+// 16 bytes from the next one's (61 of 128,256 f32, 31 MB: 11.2). A chunk with a logit of -inf, or with the
+// row's end in it, is summed twice. Bound by memory and, nearly as much, by vector instructions (about 150 a
 // wave's 1,024 logits). Workgroups of 8 waves joined through LDS took 117 with more instructions
 // and 130 with fewer, waiting at their barrier; 32 logits a lane 94, and 30 more in the join, whose
 // groups are larger then; workgroups that stay and fetch the next chunk ahead 137.
@@ -686,7 +689,10 @@ __global__ __launch_bounds__(SCORE_THREADS, 8) void k_score(ScoreArgs a) {
 // from the groups of logits whose maximum reaches a bound that `top` groups' maxima reach (the
 // top-th of 64 maxima of groups), read again. Where more than LDS takes reach it, because
 // many are equal to it: those over it, and of the equal ones the first in the row.
-// Where those over it are too many still, one after the other.
+// Where those over it are too many still, one after the other, each by a pass over the row: where
+// the best lie side by side, so that few groups hold more of them than LDS takes, or where a row of more logits
+// than that has fewer groups than `top`. The 32 best of one row of 128,256 logits in order: 2.0 ms, of
+// 1,024 such rows 8.1, the same where all but a run of 2,500 logits are -inf; of one row of 2,500 62 us.
 //
 // 20 best of 2047 rows of 128,256 bf16: 16 us (21 with the groups read by the value), of one row of
 // 49,152: 5.7; without the best 4.7. Every
@@ -946,8 +952,8 @@ extern "C" int defer_gpu_q8_kv_append(const defer_gpu_q8_pages* pages, const def
   // it 4 rounds and one of the cache's heads 2 (keys, values); fewer rows take more heads, so
   // that the lanes have work. Where those would be more workgroups than the chip holds at once
   // (4 on a CU), each takes twice as many heads and forms the rows' angles for all of them:
-  // 2000 rows of 32 + 8 heads of 128 in 21 us rather than 25 (4 times as many: 23), but 11 x 33
-  // normed rows of 24 + 4 heads of 96, too few for that, in 11.2 rather than 8.8.
+  // 2000 rows of 32 + 8 heads of 128 in 21.6 us rather than 25 (4 times as many: 23), but 11 x 33
+  // normed rows of 24 + 4 heads of 96, too few for that, in 11.2 rather than 8.9.
   const uint32_t most = std::min(r.most_rows, (uint32_t)KV_RUN);
   auto power = [&](uint32_t n, uint32_t heads) {  // the largest one up to n, no more than heads need
     uint32_t s = 0;

@@ -88,13 +88,13 @@ struct Stage {
 //
 // SPLIT: a workgroup takes per_wave units, left in the workspace for k_tree_join.
 //
-// 7 x 25 rows over 6000 positions, 32 heads on 8 of 128: 162 to 167 us, of which the digits' products
+// 7 x 25 rows over 6000 positions, 32 heads on 8 of 128: 165 us, of which the digits' products
 // are 34 at the matrix cores' rate and the codes 15 (154 without copying them); bound by the chain of a
-// block, 188 vector and 16 matrix instructions with three passes through LDS in 1.7 us, at one or two
-// waves a SIMD (392 workgroups on 256 CUs). 32 x 12 rows over 384, 32 heads on 8 of 64, some places
-// hidden: 23 us, three workgroups a CU that each go through seven blocks (26 with each lane reading its
-// four places' marks when it needs them). 7 rows at 203, 9 heads on 3 of 64: 8.1 to 9.7, a chain of reads
-// and four blocks one after the other. With each wave loading the codes of its own tile, as k_attn does,
+// block, 1.7 us: 188 vector and 16 matrix instructions, about 0.4 us of issue, and the waits between
+// them (copies, three passes through LDS), which one or two waves a SIMD do not cover (392 workgroups on
+// 256 CUs). 32 x 12 rows over 384, 32 heads on 8 of 64, some places hidden: 23 us, three workgroups a
+// CU that each go through seven blocks (26 with each lane reading its four places' marks when it
+// needs them). 7 rows at 203, 9 heads on 3 of 64: 9.2, a chain of reads and four blocks one after the other. With each wave loading the codes of its own tile, as k_attn does,
 // the first two took 541 and 59 us; three blocks in LDS instead of two gave nothing, for one workgroup
 // less a CU.
 template <int KC, int R, bool SPLIT>

@@ -240,7 +240,7 @@ def kv_keep(pages: Pages, kv_len: torch.Tensor, row_start: Optional[torch.Tensor
     """Moves drafted rows (at most 64 a sequence) together: the keep[row_start[i] + t]-th row of sequence i to the place
     of its t-th, for t < kept[i], and returns the lengths that the sequences then have (int32): the rest is as if it
     had never been written. ``keep`` [rows] and ``kept`` [sequences] int32. ``most_rows`` as for tree_attention: no more
-    rows of a sequence are kept."""
+    rows of a sequence are kept. Marks of ``hidden`` places are the caller's to move, too."""
     return _native().kv_keep(pages, kv_len, row_start, keep, kept, most_rows)
 
 

@@ -417,7 +417,7 @@ int defer_gpu_q8_tree_attention(const defer_gpu_q8_pages* pages, const defer_gpu
  * for t < kept[i], to the place of the t-th, as if the others had never been written.
  * An entry outside [0, n) leaves its place as it is. kv_len_out[i] = kv_len[i] - n +
  * min(kept[i], n, most_rows), apart from all inputs. No two sequences of a call have a page
- * of these rows in common. */
+ * of these rows in common. Marks of hidden places are the caller's to move, too. */
 int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer_gpu_q8_rows* rows,
                          const int32_t* keep, const int32_t* kept, int32_t* kv_len_out, void* stream);
 
@@ -427,7 +427,9 @@ int defer_gpu_q8_kv_keep(const defer_gpu_q8_pages* pages, const defer_gpu_q8_row
  * [rows, top]: the top <= 32 largest, the lower index first among equals. A target
  * outside [0, n) (or target NULL) has log_p NaN and rank -1. A logit of -inf has
  * probability 0. A row with a NaN or +inf, or with nothing over -inf, has no
- * distribution: NaN throughout, ranks and indexes -1. `workspace` (16-byte
+ * distribution: NaN throughout, ranks and indexes -1. Rows whose best lie side by side (logits
+ * in order, or a few thousand allowed ones in a run) can take a hundred times as long as others,
+ * where top is 17 or more. `workspace` (16-byte
  * aligned) is scratch of the size that defer_gpu_q8_log_probs_workspace gives, one
  * for each call that may overlap. */
 size_t defer_gpu_q8_log_probs_workspace(uint32_t rows, uint32_t n, uint32_t top);
