@@ -71,6 +71,27 @@ def test_rows_behind_the_most_attend_to_nothing(counts, most, history, nh, nkv, 
     assert not out[at:].any() and (into[at:] == 3).all()
 
 
+def test_rows_behind_the_most_in_calls_of_many_workgroups():
+    """Where a wave takes two tiles of rows."""
+    seqs, nh, nkv, hd, most = 40, 64, 8, 64, 17
+    counts = [(20, 17, 3, 64, 18)[i % 5] for i in range(seqs)]
+    assert seqs * nkv * -(-most * nh // nkv // 16) >= 2048
+    lens = [50 + n for n in counts]
+    pages = make_cache(lens, nkv, hd)
+    fill(pages, lens, nkv, hd)
+    q = rnd(sum(counts), nh, hd, seed=3).to(DEV)
+    trees = [random_tree(n, i) for i, n in enumerate(counts)]
+    torch.full_like(q, math.nan)  # what a fresh tensor may hold
+    out = q8.tree_attention(q, pages, i32(sum(trees, [])), i32(lens), starts(counts), most)
+    at = 0
+    for i, n in enumerate(counts):
+        m = min(n, most)
+        one = pages._replace(table=pages.table[i:i + 1].contiguous())
+        want = q8.tree_attention(q[at:at + m], one, i32(trees[i][:m]), i32([50 + m]), starts([m]))
+        assert torch.equal(out[at:at + m], want) and not out[at + m:at + n].any(), i
+        at += n
+
+
 @pytest.mark.parametrize("counts,kept,most", [([100, 10], [80, 4], None), ([100, 10], [64, 10], None), ([100, 10], [65, 0], None),
                                               ([9, 2, 0, 7], [7, 2, 3, 6], 5), ([5], [5], 0)])
 def test_rows_behind_the_most_are_not_kept(counts, kept, most):
